@@ -1,0 +1,1048 @@
+// Key-value cache in the pages of an array, of the C-ABI: appending keys and values (with norms of queries and keys and the
+// position rotation on the way), reading rows back, and attention of the newest tokens over what the cache holds.
+//
+// The cache is cut into blocks of T tokens.  A block has two pages for each key-value head: one of keys and one of values, T the largest power of
+// two for which T rows of `dim` 16-bit numbers fit a page.  Within a page the numbers lie in pieces of 16 bytes, in the order in
+// which the matrix instructions take them:
+//   keys    piece (c, t) at (c * T + t) * 16: numbers 8c .. 8c+7 of token t             c < dim / 8
+//   values  piece (t, d) at (t * dim + d) * 16: number d of tokens 8t .. 8t+7           t < T / 8
+// so sixteen neighbouring lanes of a wave load 256 neighbouring bytes, and what they load is an operand as it stands: with the
+// scores taken as S^T = K Q^T and the output as O^T = V^T P^T, a lane's accumulators of the scores are its part of P^T.
+#include "bam_capi_internal.h"
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// what a kernel knows about the cache: the range's tables do not move while the array is there
+struct kv_geom {
+    range_d_t<uint64_t>* r;
+    data_page_t* pages;
+    uint8_t* base;
+    uint64_t first_page, n_blocks;
+    uint32_t heads, dim, tokens, tokens_log, page_log;
+};
+struct bam_kv {
+    bam_array_t* a;
+    kv_geom g;
+    int f16;
+    uint64_t cache_pages;
+    bool unheld;                        /* reads of resident pages without a reference are switched on */
+};
+
+namespace {
+
+struct kv_seqs {
+    const int32_t* starts;              /* [n + 1] first row of each sequence's new tokens; NULL: one new token each */
+    const int32_t* lens;                /* [n] tokens of each sequence, the new ones among them */
+    const int32_t* table;               /* [n][width] blocks */
+    int64_t stride;
+    uint32_t n, rows, width;
+};
+
+// sequence of row i
+__device__ __forceinline__ uint32_t seq_of(const kv_seqs& s, const uint32_t i)
+{
+    if (!s.starts) return i;
+    uint32_t lo = 0, hi = s.n;          /* the last sequence that starts at or before row i */
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (s.starts[mid] <= (int32_t)i) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+// a row's place: sequence, position, rows of its sequence from it on; false where the row has none (no such sequence, before the first position, past the table)
+struct kv_place { uint32_t seq, pos, rest, first; };
+__device__ __forceinline__ bool place_of(const kv_seqs& s, const kv_geom& g, const uint32_t i, kv_place& p)
+{
+    p.seq = seq_of(s, i);
+    if (p.seq >= s.n) return false;
+    const int32_t end = s.starts ? s.starts[p.seq + 1] : (int32_t)i + 1, begin = s.starts ? s.starts[p.seq] : (int32_t)i;
+    const int64_t len = s.lens[p.seq], pos = len - (end - (int64_t)i);
+    if ((int32_t)i < begin || (int64_t)i >= end || pos < 0 || (pos >> g.tokens_log) >= s.width) return false;
+    p.pos = (uint32_t)pos;
+    p.rest = (uint32_t)(end - (int64_t)i);
+    const int64_t first = len - ((int64_t)end - begin);
+    p.first = first < 0 ? 0u : (uint32_t)first;
+    return true;
+}
+// the page of keys of a block (the page of values is the next one), or false: no such block
+__device__ __forceinline__ bool page_of_block(const kv_geom& g, const kv_seqs& s, const uint32_t seq, const uint32_t i, const uint32_t head, uint64_t& page)
+{
+    if (i >= s.width) return false;
+    const int32_t b = s.table[(int64_t)seq * s.stride + i];
+    if (b < 0 || (uint64_t)b >= g.n_blocks) return false;
+    page = g.first_page + ((uint64_t)b * g.heads + head) * 2u;
+    return true;
+}
+
+template <int F16> __device__ __forceinline__ float from16(const uint32_t x)
+{
+    if constexpr (F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)x);
+    else return __builtin_bit_cast(float, x << 16);
+}
+template <int F16> __device__ __forceinline__ uint32_t to16(const float lo, const float hi)
+{
+    if constexpr (F16) {
+        const _Float16 a = (_Float16)lo, b = (_Float16)hi;
+        return (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
+    } else {
+        const __bf16 a = (__bf16)lo, b = (__bf16)hi;
+        return (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
+    }
+}
+__device__ __forceinline__ u32x4 load_piece(const uint16_t* p, const bool aligned)
+{
+    if (aligned) return *(const u32x4*)p;
+    u32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    return x;
+}
+
+// ---------------------------------------------------------------------------
+// pages held for the length of a visit
+// ---------------------------------------------------------------------------
+#define KV_PASS_FRESH 512u
+#define KV_PASS_CLEARED 1024u
+__attribute__((noinline)) __device__ bam_pass_t kv_pass(range_d_t<uint64_t>* r, const uint64_t pg, const uint32_t queue, uint64_t sv, const uint32_t in)
+{
+    bool hit = false, progressed = false, wants = false;
+    uint32_t slot = 0;
+    const bool resolved = r->template slow_step<true>(pg, (in & BAM_PASS_WRITE) != 0, queue, sv, slot, hit, progressed, (in & BAM_PASS_TAKE_PART) != 0, true, &wants, BAM_PLACE_NORMAL,
+                                                      (in & KV_PASS_FRESH) != 0, (in & KV_PASS_CLEARED) != 0);
+    bam_pass_t out;
+    out.sv = sv;
+    out.slot = slot;
+    out.flags = (resolved ? BAM_PASS_RESOLVED : 0u) | (hit ? BAM_PASS_HIT : 0u) | (progressed ? BAM_PASS_PROGRESSED : 0u);
+    return out;
+}
+
+/*
+ * use(address of the slot) for the lanes with `take`, each with its page held: as range_view::acquire_helped, the lanes of resident pages first and
+ * nothing held while the others' pages are fetched, with what a writer of rows can say besides (`fresh`, `cleared`: range_d_t::slow_step).
+ * `use` stores past the caches (st16_sys and the like), so a wait for the wave's own stores is all that giving a page back needs: the write-back of the
+ * cluster's cache that a release costs would come once per wave.  All lanes of the wave call.
+ */
+template <bool WRITE, typename F>
+__device__ __forceinline__ void visit(const kv_geom& g, const uint64_t page, const bool take, const bool fresh, const bool cleared, uint32_t& n_access, uint32_t& n_hit, F&& use)
+{
+    using namespace bam;
+    const uint32_t me = lane();
+    data_page_t* const dp = g.pages + (take ? page : 0);
+    const uint64_t eq = match_any(take ? (uint64_t)dp : 0ull);
+    const uint32_t master = first_lane(eq), count = popc(eq);
+    const bool lead = take && master == me;
+    uint64_t sv = 0, pack = 0;
+    uint32_t slot = 0;
+    if (lead) { const bool h = bam_try_hit(dp, count, WRITE, sv, slot); pack = (uint64_t)slot | ((uint64_t)h << 63); }
+    pack = shfl(pack, master);
+    bool done = !take;
+    if (take && (pack >> 63)) {
+        use(g.base + ((uint64_t)(uint32_t)pack << g.page_log));
+        done = true;
+        fence_meta();
+        if (lead) { __hip_atomic_fetch_add(&dp->state, 0u - count, __ATOMIC_RELAXED, BAM_AGENT); n_access += count; n_hit += count; }
+    }
+    if (__builtin_expect(ballot(!done) == 0, 1)) return;
+    const uint32_t queue = wave_slot_hash();
+    spin_t sp;
+    page_cache_d_t* const cache = &g.r->cache;
+    for (;;) {
+        const bool part = !done && lead;
+        const bam_pass_t ps = kv_pass(g.r, take ? page : 0, queue, sv, (WRITE ? BAM_PASS_WRITE : 0u) | (part ? BAM_PASS_TAKE_PART : 0u) | (fresh ? KV_PASS_FRESH : 0u) | (cleared ? KV_PASS_CLEARED : 0u));
+        const bool progressed = (ps.flags & BAM_PASS_PROGRESSED) != 0;
+        if (part) {
+            sv = ps.sv;
+            pack = (uint64_t)ps.slot | ((uint64_t)((ps.flags & BAM_PASS_HIT) != 0) << 63) | ((uint64_t)((ps.flags & BAM_PASS_RESOLVED) != 0) << 62);
+        }
+        const uint64_t got = shfl(pack, master);
+        if (!done && ((got >> 62) & 1)) {
+            use(g.base + ((uint64_t)(uint32_t)got << g.page_log));
+            done = true;
+            fence_meta();
+            if (lead) { __hip_atomic_fetch_add(&dp->state, 0u - count, __ATOMIC_RELAXED, BAM_AGENT); n_access += count; n_hit += (got >> 63) ? count : 0u; }
+        }
+        if (!ballot(!done)) break;
+        if (ballot(progressed)) sp = spin_t();
+        else if (cache->spin_giveup(sp)) {
+            if (!done && lead) __hip_atomic_fetch_add(&dp->state, 0u - count, __ATOMIC_RELAXED, BAM_AGENT);
+            break;
+        }
+    }
+}
+
+// the wave's accesses into the range's counters
+__device__ __forceinline__ void count_accesses(const kv_geom& g, const uint32_t n_access, const uint32_t n_hit)
+{
+    bam_stat_shard_t* const shard = g.r->shard();
+    bam::stat_add<32>(&shard->access_cnt, n_access);
+    bam::stat_add<32>(&shard->hit_cnt, n_hit);
+}
+
+// ---------------------------------------------------------------------------
+// rows into the cache and out of it
+// ---------------------------------------------------------------------------
+struct kv_rows {
+    const uint16_t *q, *k, *v;          /* rows of heads; k and v are where rows go to when the cache is read */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    uint16_t* q_out;
+    const uint16_t *q_norm, *k_norm;
+    const float *cos, *sin;
+    uint32_t positions, q_heads, rot, pairs, aligned;      /* aligned: q, k, v in whole pieces of 16 bytes */
+    float eps;
+    uint32_t v_rows;                    /* rows a wave of values looks after */
+    uint32_t q_waves, k_waves;
+};
+
+/*
+ * Eight neighbouring numbers of a row per lane, LPR lanes to a row: x * rsqrt(mean x^2 + eps) * w, then the rotation of the pairs (i, i + rot/2), or
+ * (2i, 2i+1), i < rot/2, by the angles of the row's position; in 32 bits, rounded once.  A position past the tables gives NaN.
+ */
+template <int LPR, int F16>
+__device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geom& g, u32x4 x, const uint16_t* norm, const uint32_t piece, const uint32_t pos)
+{
+    if (!norm && !io.rot) return x;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) { f[2 * i] = from16<F16>(x[i] & 0xffffu); f[2 * i + 1] = from16<F16>(x[i] >> 16); }
+    const bool in = piece * 8u < g.dim;
+    if (norm) {
+        float ss = 0;
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss += f[i] * f[i];
+        }
+#pragma unroll
+        for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
+        const float by = rsqrtf(ss / (float)g.dim + io.eps);
+        if (in) {
+            const u32x4 w = load_piece(norm + piece * 8u, true);
+#pragma unroll
+            for (int i = 0; i < 4; i++) { f[2 * i] *= by * from16<F16>(w[i] & 0xffffu); f[2 * i + 1] *= by * from16<F16>(w[i] >> 16); }
+        }
+    }
+    if (io.rot) {
+        const uint32_t half = io.rot / 2, pieces = io.rot / 8;
+        const bool turns = piece < pieces, known = pos < io.positions;
+        const float nan = __builtin_nanf("");
+        if (io.pairs) {
+            if (turns) {
+                const f32x4 c = known ? *(const f32x4*)(io.cos + (uint64_t)pos * half + piece * 4u) : f32x4{nan, nan, nan, nan};
+                const f32x4 s = known ? *(const f32x4*)(io.sin + (uint64_t)pos * half + piece * 4u) : f32x4{nan, nan, nan, nan};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float a = f[2 * i], b = f[2 * i + 1];
+                    f[2 * i] = a * c[i] - b * s[i];
+                    f[2 * i + 1] = b * c[i] + a * s[i];
+                }
+            }
+        } else {
+            const uint32_t hp = pieces / 2, mine = piece < hp ? piece : piece - hp;
+            const uint32_t from = (bam::lane() & ~(uint32_t)(LPR - 1)) + (turns ? (piece < hp ? piece + hp : piece - hp) : piece);
+            const float sign = piece < hp ? -1.0f : 1.0f;
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[i] = __shfl(f[i], (int)from);
+            if (turns) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const f32x4 c = known ? *(const f32x4*)(io.cos + (uint64_t)pos * half + mine * 8u + j * 4) : f32x4{nan, nan, nan, nan};
+                    const f32x4 s = known ? *(const f32x4*)(io.sin + (uint64_t)pos * half + mine * 8u + j * 4) : f32x4{nan, nan, nan, nan};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) f[4 * j + i] = f[4 * j + i] * c[i] + sign * o[4 * j + i] * s[i];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = to16<F16>(f[2 * i], f[2 * i + 1]);
+    return x;
+}
+
+/*
+ * A wave takes either 64 / LPR rows of queries, or the keys of as many rows of one head, or the values of io.v_rows rows of one head.  Values lie in the
+ * cache in pieces of eight tokens: whoever finds the first row of such a piece among its rows writes all rows of the piece.
+ */
+template <int LPR, int F16, bool WRITE>
+__global__ __launch_bounds__(256) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
+{
+    using namespace bam;
+    constexpr uint32_t RPW = 64 / LPR;
+    const uint32_t wave = blockIdx.x * 4u + threadIdx.x / 64u, lane = bam::lane();
+    const uint32_t piece = lane % LPR;
+    uint32_t n_access = 0, n_hit = 0;
+    if (wave < io.q_waves) {
+        const uint64_t j = (uint64_t)wave * RPW + lane / LPR;
+        const uint32_t i = (uint32_t)(j / io.q_heads), h = (uint32_t)(j % io.q_heads);
+        kv_place p{0, 0, 0, 0};
+        const bool has = i < s.rows && piece * 8u < g.dim;
+        const bool known = i < s.rows && place_of(s, g, i, p);
+        u32x4 x{0, 0, 0, 0};
+        if (has) x = load_piece(io.q + (int64_t)i * io.q_row + (int64_t)h * io.q_head + piece * 8u, io.aligned);
+        x = norm_and_rotate<LPR, F16>(io, g, x, io.q_norm, piece, known ? p.pos : 0xffffffffu);
+        if (has) *(u32x4*)(io.q_out + ((uint64_t)i * io.q_heads + h) * g.dim + piece * 8u) = x;
+        return;
+    }
+    if (wave < io.q_waves + io.k_waves) {
+        const uint32_t w = wave - io.q_waves, h = w % g.heads, i = w / g.heads * RPW + lane / LPR;
+        kv_place p{0, 0, 0, 0};
+        uint64_t page = 0;
+        const bool has = i < s.rows && piece * 8u < g.dim && place_of(s, g, i, p) && page_of_block(g, s, p.seq, p.pos >> g.tokens_log, h, page);
+        const uint32_t in_block = p.pos & (g.tokens - 1u), block_first = p.pos - in_block;
+        const uint64_t at = ((uint64_t)piece * g.tokens + in_block) * 16u;
+        if constexpr (WRITE) {
+            u32x4 x{0, 0, 0, 0};
+            if (has) x = load_piece(io.k + (int64_t)i * io.k_row + (int64_t)h * io.k_head + piece * 8u, io.aligned);
+            x = norm_and_rotate<LPR, F16>(io, g, x, io.k_norm, piece, p.pos);
+            /* a page that holds none but this call's tokens needs nothing from the store */
+            visit<true>(g, page, has, block_first >= p.first, block_first + g.tokens > p.pos + p.rest, n_access, n_hit, [&](uint8_t* slot) { st16_sys(slot + at, x); });
+        } else {
+            u32x4 x{0, 0, 0, 0};
+            visit<false>(g, page, has, false, false, n_access, n_hit, [&](uint8_t* slot) { x = ld_payload((const u32x4*)(slot + at)); });
+            if (i < s.rows && piece * 8u < g.dim) *(u32x4*)((uint16_t*)io.k + (int64_t)i * io.k_row + (int64_t)h * io.k_head + piece * 8u) = x;
+        }
+        count_accesses(g, n_access, n_hit);
+        return;
+    }
+    const uint32_t w = wave - io.q_waves - io.k_waves, h = w % g.heads;
+    const uint64_t first = (uint64_t)(w / g.heads) * io.v_rows;
+    if (first >= s.rows) return;
+    kv_place p{0, 0, 0, 0};
+    const uint32_t mine = (uint32_t)first + lane;
+    const bool has = lane < io.v_rows && mine < s.rows && place_of(s, g, mine, p);
+    /* rows that begin a piece: of theirs, and of nobody's where the row has no place */
+    const bool begins = has && ((p.pos & 7u) == 0 || p.pos == p.first || (s.starts && s.starts[p.seq] == (int32_t)mine));
+    if constexpr (!WRITE) {
+        /* rows without a place come out as zeros */
+        for (uint64_t m = ballot(lane < io.v_rows && mine < s.rows && !has); m; m &= m - 1)
+            for (uint32_t d = lane; d < g.dim; d += 64u) ((uint16_t*)io.v)[(int64_t)(first + first_lane(m)) * io.v_row + (int64_t)h * io.v_head + d] = 0;
+    }
+    for (uint64_t m = ballot(begins); m; m &= m - 1) {
+        const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), seq = bcast(p.seq, j), row = (uint32_t)first + j;
+        const uint32_t left = 8u - (pos & 7u), cnt = rest < left ? rest : left;
+        uint64_t page = 0;
+        const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, h, page);
+        const uint32_t in_block = pos & (g.tokens - 1u), block_first = pos - in_block;
+        uint16_t* const rows = (uint16_t*)io.v + (int64_t)row * io.v_row + (int64_t)h * io.v_head;
+        if constexpr (WRITE) {
+            if (!there) continue;
+            visit<true>(g, page + 1, true, block_first >= bcast(p.first, j), block_first + g.tokens > pos + rest, n_access, n_hit, [&](uint8_t* slot) {
+                for (uint32_t d = lane * 2u; d < g.dim; d += 128u) {
+                    uint8_t* const at = slot + ((uint64_t)(in_block >> 3) * g.dim + d) * 16u;
+                    uint32_t x[8];
+#pragma unroll
+                    for (uint32_t t = 0; t < 8; t++) {
+                        const uint16_t* const from = rows + (int64_t)(t < cnt ? t : 0) * io.v_row + d;
+                        x[t] = io.aligned ? *(const uint32_t*)from : (uint32_t)from[0] | ((uint32_t)from[1] << 16);
+                    }
+                    if (cnt == 8) {
+                        u32x4 lo, hi;
+#pragma unroll
+                        for (int t = 0; t < 4; t++) {
+                            lo[t] = (x[2 * t] & 0xffffu) | (x[2 * t + 1] << 16);
+                            hi[t] = (x[2 * t] >> 16) | (x[2 * t + 1] & 0xffff0000u);
+                        }
+                        st16_sys(at, lo);
+                        st16_sys(at + 16, hi);
+                    } else {
+#pragma unroll
+                        for (uint32_t t = 0; t < 8; t++)
+                            if (t < cnt) {
+                                uint16_t* const to = (uint16_t*)at + (pos & 7u) + t;
+                                __hip_atomic_store(to, (uint16_t)x[t], __ATOMIC_RELAXED, BAM_SYSTEM);
+                                __hip_atomic_store(to + 8, (uint16_t)(x[t] >> 16), __ATOMIC_RELAXED, BAM_SYSTEM);
+                            }
+                    }
+                }
+            });
+        } else {
+            visit<false>(g, page + 1, there, false, false, n_access, n_hit, [&](uint8_t* slot) {
+                for (uint32_t d = lane * 2u; d < g.dim; d += 128u) {
+                    const uint8_t* const at = slot + ((uint64_t)(in_block >> 3) * g.dim + d) * 16u;
+                    const u32x4 lo = ld_payload((const u32x4*)at), hi = ld_payload((const u32x4*)(at + 16));
+                    const uint32_t o = pos & 7u;
+#pragma unroll
+                    for (uint32_t t = 0; t < 8; t++)
+                        if (t >= o && t < o + cnt) {
+                            const uint32_t a = (t & 1) ? lo[t / 2] >> 16 : lo[t / 2] & 0xffffu, b = (t & 1) ? hi[t / 2] >> 16 : hi[t / 2] & 0xffffu;
+                            *(uint32_t*)(rows + (int64_t)(t - o) * io.v_row + d) = a | (b << 16);
+                        }
+                }
+            });
+            if (!there)
+                for (uint32_t t = 0; t < cnt; t++)
+                    for (uint32_t d = lane; d < g.dim; d += 64u) rows[(int64_t)t * io.v_row + d] = 0;
+        }
+    }
+    count_accesses(g, n_access, n_hit);
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+struct kv_att {
+    const uint16_t* q;
+    int64_t q_row, q_head;
+    uint32_t aligned, q_heads, group;   /* group: heads of queries to a head of keys */
+    float scale;                        /* times log2(e) */
+    uint32_t window, sinks;             /* window 0: none */
+    uint16_t* out;                      /* [rows][q_heads][dim] */
+    float* lse;                         /* [rows][q_heads] or NULL */
+    uint32_t tiles, splits, steps;      /* tiles of rows of a sequence, splits of its tokens, steps of 32 tokens to a split */
+    float* part;                        /* [item][rows of a tile][split][dim] sums, then their maxima and denominators [item][row][split] each */
+    float *part_m, *part_l;
+    uint8_t* left;                      /* [item][split] pages were missing */
+    uint32_t chunk;                     /* blocks whose pages a wave holds at a time when it holds them */
+    uint32_t items;
+};
+
+template <int F16> __device__ __forceinline__ f32x4 mma(const u32x4 a, const u32x4 b, const f32x4 c)
+{
+    if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+/*
+ * Over the four lanes 16 apart: the halves of the wave, then the rows of sixteen lanes of a half, exchanged between two registers that hold the same.  (Written in
+ * asm: from the builtins with the same value for both operands the compiler takes the two results to be the same too.  The two idle cycles are
+ * what the exchange needs behind a vector instruction that writes one of its registers.)
+ */
+__device__ __forceinline__ void swap_halves(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void swap_rows(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ float max_of_four(float a)
+{
+    float b = a;
+    swap_halves(a, b);
+    a = b = fmaxf(a, b);
+    swap_rows(a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_of_four(float a)
+{
+    float b = a;
+    swap_halves(a, b);
+    a = b = a + b;
+    swap_rows(a, b);
+    return a + b;
+}
+/* whether one of the two 16-bit numbers is an infinity or NaN */
+template <int F16> __device__ __forceinline__ bool odd16(const uint32_t x)
+{
+    constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+    return (x & e) == e || ((x >> 16) & e) == e;
+}
+__device__ __forceinline__ u32x4 load_once(const uint8_t* p) { return __builtin_nontemporal_load((const u32x4*)p); }
+
+/* which tokens a tile of rows sees, and the order in which they are gone through: steps of 32 tokens, first those that stay visible in front of the window */
+struct kv_span {
+    int32_t first_pos, last_pos;        /* positions of the tile's rows */
+    uint32_t len;                       /* tokens to look at: up to the last row's */
+    uint32_t low, front, base, n_steps; /* first token of the window; steps in front of it; first token of the step it begins in; steps */
+};
+__device__ __forceinline__ kv_span span_of(const kv_att& a, const int32_t len, const int32_t new_rows, const uint32_t r0, const uint32_t r1)
+{
+    kv_span s;
+    const int32_t p0 = len - new_rows;
+    s.first_pos = p0 + (int32_t)(r0 / a.group);
+    s.last_pos = p0 + (int32_t)((r1 - 1) / a.group);
+    s.len = s.last_pos < 0 ? 0u : (uint32_t)s.last_pos + 1u;
+    s.low = a.window && s.first_pos + 1 > (int64_t)a.window ? (uint32_t)(s.first_pos + 1) - a.window : 0u;
+    const uint32_t sinks = a.sinks < s.low ? a.sinks : s.low;
+    s.front = (sinks + 31u) / 32u;
+    s.base = s.low & ~31u;
+    if (s.front * 32u >= s.base) { s.front = 0; s.base = 0; }
+    s.n_steps = s.front + (s.len > s.base ? (s.len - s.base + 31u) / 32u : 0u);
+    return s;
+}
+
+/*
+ * One wave's share of a split: steps [v0, v1) for NT tiles of 16 rows.  Lane l: row l % 16, tokens 8 (l / 16) .. + 7 of each step.
+ * The largest score and the denominator (of this lane's tokens) and the sums of every row are carried over the steps in 32 bits; exp(score - max) is
+ * rounded to 16 bits for the product with the values, which the matrix unit takes in 16 bits; the denominator is the sum of what was not rounded.
+ *
+ * HELD false: pages are read without a reference, a chunk of 32 blocks at a time: one look at their descriptors, an acquire (a slot may have
+ * been refilled since this compute unit last read it), the reads, and a second look that has to find the same.  False if a page was missing or has gone.
+ * HELD true: the pages of a.chunk blocks at a time are held, and fetched where they are missing; `gone` is set where the wait was given up.
+ */
+template <int DP, int F16, int NT, bool HELD>
+__device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, const kv_att& a, const kv_span& sp, const uint32_t seq, const uint32_t head, const uint32_t v0, const uint32_t v1,
+                                         const u32x4 (&q)[NT][DP / 32], const int32_t (&pos)[NT], f32x4 (&o)[NT][DP / 16], float (&m)[NT], float (&l)[NT], bool& gone, uint32_t& n_access, uint32_t& n_hit)
+{
+    using namespace bam;
+    const uint32_t lane = bam::lane(), row = lane & 15u, grp = lane >> 4;
+    const uint32_t T = g.tokens, D = g.dim;
+    for (uint32_t v = v0; v < v1;) {
+        /* a run of neighbouring steps within one chunk of blocks */
+        const bool front = v < sp.front;
+        const uint32_t t_first = front ? v * 32u : sp.base + (v - sp.front) * 32u;
+        const uint32_t run = (front && sp.front < v1 ? sp.front : v1) - v;
+        const uint32_t b_first = t_first >> g.tokens_log, n_chunk = HELD ? a.chunk : 32u;
+        uint32_t t_end = (b_first + n_chunk) << g.tokens_log;
+        if (t_first + run * 32u < t_end) t_end = t_first + run * 32u;
+        const uint32_t t_seen = t_end < sp.len ? t_end : sp.len;                  /* tokens from here on are not looked at */
+        /* lanes 0..31: the pages of keys, 32..63: of values */
+        const uint32_t blk = b_first + (lane & 31u);
+        uint64_t page = 0;
+        const bool asked = (lane & 31u) < n_chunk && (blk << g.tokens_log) < t_seen;
+        const bool need = asked && page_of_block(g, s, seq, blk, head, page);
+        if (lane >= 32) page += 1;
+        const uint32_t holes = (uint32_t)ballot(asked && !need);                  /* blocks the table does not have: their tokens are not visible */
+        uint32_t slot = 0;
+        uint64_t seen = 0;
+        if constexpr (!HELD) {
+            if (need) seen = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
+            if (ballot(need && ((uint32_t)seen >> (CNT_SHIFT + 1)) != V_NB)) return false;
+            slot = need ? (uint32_t)(seen >> 32) & BAM_SLOT_MASK : 0u;
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+            n_access += need ? 1u : 0u;
+            n_hit += need ? 1u : 0u;
+        } else {
+            range_view<uint64_t> view;
+            view.load(g.r);
+            slot = BAM_NO_SLOT;
+            auto keep = [&](uint32_t s_) { slot = s_; return false; };
+            view.template acquire_helped<true>(page, need, false, keep, keep);
+            n_access += view.n_access;
+            n_hit += view.n_hit;
+            view.n_access = view.n_hit = 0;
+            if (ballot(need && slot == BAM_NO_SLOT)) gone = true;
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        }
+        const uint32_t where = slot == BAM_NO_SLOT ? 0u : slot;
+        for (uint32_t t0 = t_first; t0 < t_end; t0 += 32u) {
+            /* this lane's tokens as a row of K (8 (row / 4) + row % 4, and 4 further on) and as its part of V (8 grp .. + 7) lie in one block each */
+            const uint32_t kt = t0 + 8u * (row >> 2), vt = t0 + 8u * grp;
+            const uint32_t kb = (kt >> g.tokens_log) - b_first, vb = (vt >> g.tokens_log) - b_first;
+            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(where, kb) << g.page_log) + (((kt & (T - 1u)) + (row & 3u)) + grp * T) * 16u;
+            const uint8_t* vp = g.base + ((uint64_t)bam::shfl(where, 32u + vb) << g.page_log) + (((vt & (T - 1u)) >> 3) * D + row) * 16u;
+            u32x4 k0[DP / 32], k1[DP / 32], vv[DP / 16];
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++) {
+                k0[j] = k1[j] = u32x4{0, 0, 0, 0};
+                if ((4u * j + grp) * 8u < D) { k0[j] = load_once(kp + (uint64_t)j * 64u * T); k1[j] = load_once(kp + (uint64_t)j * 64u * T + 64u); }
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 16; i++) {
+                vv[i] = u32x4{0, 0, 0, 0};
+                if (16u * i + row < D) vv[i] = load_once(vp + i * 256u);
+            }
+            const bool whole = !holes && (int64_t)t0 + 31 <= sp.first_pos && (!a.window || (int64_t)sp.last_pos - t0 < a.window || t0 + 32u <= a.sinks);
+            bool slow = false;
+            if (!whole) {
+                /* values of tokens that no row sees may be anything: none of it may meet the zeros of P */
+                const bool hole = (holes >> vb) & 1u;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) {
+                    const int64_t t = vt + e;
+                    const bool none = hole || t > sp.last_pos || (a.window && t <= (int64_t)sp.first_pos - a.window && t >= a.sinks);
+                    const uint32_t keep = none ? ((e & 1) ? 0x0000ffffu : 0xffff0000u) : 0xffffffffu;
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++) vv[i][e / 2] &= keep;
+                }
+                if (sp.first_pos != sp.last_pos) {
+                    bool odd = false;
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) odd |= odd16<F16>(vv[i][e]);
+                    slow = ballot(odd) != 0;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                f32x4 s0{0, 0, 0, 0}, s1{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < DP / 32; j++) { s0 = mma<F16>(k0[j], q[n][j], s0); s1 = mma<F16>(k1[j], q[n][j], s1); }
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) { x[e] = s0[e] * a.scale; x[4 + e] = s1[e] * a.scale; }
+                uint32_t sees = 0xffu;
+                if (!whole) {
+                    const bool hole = (holes >> vb) & 1u;
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++) {
+                        const int64_t t = vt + e;
+                        const bool in = !hole && t <= pos[n] && (!a.window || pos[n] - t < a.window || t < a.sinks);
+                        if (!in) { x[e] = -INFINITY; sees &= ~(1u << e); }
+                    }
+                }
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                top = fmaxf(max_of_four(top), m[n]);
+                const float use = top == -INFINITY ? 0.0f : top;
+                if (ballot(top != m[n])) {
+                    const float by = __builtin_amdgcn_exp2f(m[n] - use);
+                    l[n] *= by;
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++) o[n][i] *= by;
+                    m[n] = top;
+                }
+                float sum = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) { x[e] = __builtin_amdgcn_exp2f(x[e] - use); sum += x[e]; }
+                l[n] += sum;
+                u32x4 p;
+#pragma unroll
+                for (int e = 0; e < 4; e++) p[e] = to16<F16>(x[2 * e], x[2 * e + 1]);
+                if (!slow) {
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++) o[n][i] = mma<F16>(vv[i], p, o[n][i]);
+                } else {
+                    /* an infinity or NaN among the values of tokens that some rows see and others do not: row by row, what the row does not see as zero */
+                    for (uint32_t c = 0; c < 16; c++) {
+                        const uint32_t sc = bam::shfl(sees, (lane & 48u) + c);
+#pragma unroll
+                        for (int i = 0; i < DP / 16; i++) {
+                            u32x4 z = vv[i];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) z[e] &= ((sc >> (2 * e)) & 1u ? 0xffffu : 0u) | ((sc >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+                            const f32x4 with = mma<F16>(z, p, o[n][i]);
+                            if (row == c) o[n][i] = with;
+                        }
+                    }
+                }
+            }
+        }
+        fence_meta();                                            /* what was read is here */
+        if constexpr (!HELD) {
+            uint64_t now = seen;
+            if (need) now = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
+            if (ballot(need && ((seen ^ now) & 0xFFFFFFFFC0000000ull) != 0)) return false;
+        } else if (need && slot != BAM_NO_SLOT) bam_release_refs(g.pages + page, 1, false);
+        v += (t_end - t_first) / 32u;
+    }
+    return true;
+}
+
+/* rows of an item: a head of keys, a tile of the rows (new token, head of queries) of a sequence */
+struct kv_item { uint32_t seq, head, tile, r0, r1; int32_t len, rows, start; };
+__device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, const uint32_t tile_rows, kv_item& it)
+{
+    it.head = item % g.heads;
+    it.tile = item / g.heads % a.tiles;
+    it.seq = item / g.heads / a.tiles;
+    it.start = s.starts ? s.starts[it.seq] : (int32_t)it.seq;
+    int32_t end = s.starts ? s.starts[it.seq + 1] : (int32_t)it.seq + 1;
+    if (it.start < 0) it.start = 0;
+    if (end > (int32_t)s.rows) end = (int32_t)s.rows;
+    it.rows = end - it.start;
+    it.len = s.lens[it.seq];
+    if (it.rows <= 0 || it.tile * (uint64_t)tile_rows >= (uint64_t)it.rows * a.group) return false;
+    const uint32_t all = (uint32_t)it.rows * a.group;
+    it.r0 = it.tile * tile_rows;
+    it.r1 = it.r0 + tile_rows < all ? it.r0 + tile_rows : all;
+    return true;
+}
+
+/* a workgroup's split of an item: its four waves a quarter of the steps each, joined over LDS; the sums to their rows where there is one split, else to a.part */
+template <int DP, int F16, int NT, bool HELD>
+__device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, const kv_item& it, const uint32_t split, float* lds, bool& gone)
+{
+    using namespace bam;
+    constexpr uint32_t R = 16 * NT;
+    const uint32_t lane = bam::lane(), wave = threadIdx.x / 64u, row = lane & 15u, grp = lane >> 4, D = g.dim;
+    const kv_span sp = span_of(a, it.len, it.rows, it.r0, it.r1);
+    uint32_t v0 = split * a.steps, v1 = v0 + a.steps;
+    if (v1 > sp.n_steps || split + 1 == a.splits) v1 = sp.n_steps;              /* the last takes what is beyond the length that was announced */
+    if (v0 > v1) v0 = v1;
+    const uint32_t each = (v1 - v0 + 3u) / 4u;
+    uint32_t w0 = v0 + wave * each, w1 = w0 + each;
+    if (w0 > v1) w0 = v1;
+    if (w1 > v1) w1 = v1;
+    u32x4 q[NT][DP / 32];
+    int32_t pos[NT];
+    f32x4 o[NT][DP / 16];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const uint32_t r = it.r0 + n * 16u + row;
+        const bool has = r < it.r1;
+        const uint32_t tok = has ? r / a.group : 0u, h = it.head * a.group + (has ? r % a.group : 0u);
+        pos[n] = has ? it.len - it.rows + (int32_t)tok : -1;
+        const uint16_t* const from = a.q + (int64_t)(it.start + (int32_t)tok) * a.q_row + (int64_t)h * a.q_head;
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++) {
+            q[n][j] = u32x4{0, 0, 0, 0};
+            if (has && (4u * j + grp) * 8u < D) q[n][j] = load_piece(from + (4u * j + grp) * 8u, a.aligned);
+        }
+        m[n] = -INFINITY;
+        l[n] = 0;
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) o[n][i] = f32x4{0, 0, 0, 0};
+    }
+    uint32_t n_access = 0, n_hit = 0;
+    const bool ok = kv_steps<DP, F16, NT, HELD>(g, s, a, sp, it.seq, it.head, w0, w1, q, pos, o, m, l, gone, n_access, n_hit);
+    /* [4][R] maxima, [4][R] denominators, [R][DP] sums */
+    float *const ms = lds, *const ls = lds + 4 * R, *const os = lds + 8 * R;
+    uint32_t* const flag = (uint32_t*)(lds + 8 * R + R * DP);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        l[n] = sum_of_four(l[n]);
+        if (grp == 0) { ms[wave * R + n * 16u + row] = m[n]; ls[wave * R + n * 16u + row] = l[n]; }
+    }
+    if (threadIdx.x == 0) *flag = 0;
+    __syncthreads();
+    if ((!ok || gone) && lane == 0) __hip_atomic_fetch_or(flag, (ok ? 0u : 1u) | (gone ? 2u : 0u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    float by[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const uint32_t r = n * 16u + row;
+        const float top = fmaxf(fmaxf(ms[r], ms[R + r]), fmaxf(ms[2 * R + r], ms[3 * R + r]));
+        by[n] = __builtin_amdgcn_exp2f(m[n] - (top == -INFINITY ? 0.0f : top));
+    }
+    /* a quarter of the columns each, by turns: the order in which a column's four parts are added does not depend on who comes first */
+    constexpr int QUARTER = DP / 64;
+#pragma unroll 1
+    for (uint32_t turn = 0; turn < 4; turn++) {
+        const uint32_t part = (wave + turn) & 3u;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < DP / 16; i++) {
+                if ((uint32_t)(i / QUARTER) != part) continue;
+                f32x4* const at = (f32x4*)(os + (n * 16u + row) * DP + i * 16 + grp * 4);
+                const f32x4 x = o[n][i] * by[n];
+                *at = turn ? *at + x : x;
+            }
+        __syncthreads();
+    }
+    const uint32_t bad = *flag;
+    gone = (bad & 2u) != 0;
+    count_accesses(g, n_access, n_hit);
+    if (!HELD && (bad & 1u)) return false;
+    const uint32_t n_rows = it.r1 - it.r0;
+    for (uint32_t x = threadIdx.x; x < n_rows * (DP / 8u); x += 256u) {
+        const uint32_t r = x / (DP / 8u), c = x % (DP / 8u) * 8u;
+        if (c >= D) continue;
+        const float top = fmaxf(fmaxf(ms[r], ms[R + r]), fmaxf(ms[2 * R + r], ms[3 * R + r])), use = top == -INFINITY ? 0.0f : top;
+        float den = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) den += ls[w * R + r] * __builtin_amdgcn_exp2f(ms[w * R + r] - use);
+        if (gone) den = __builtin_nanf("");
+        f32x4 lo = *(const f32x4*)(os + r * DP + c), hi = *(const f32x4*)(os + r * DP + c + 4);
+        if (a.splits > 1) {
+            const uint64_t at = ((uint64_t)item * R + r) * a.splits + split;
+            *(f32x4*)(a.part + at * D + c) = lo;
+            *(f32x4*)(a.part + at * D + c + 4) = hi;
+            if (c == 0) { a.part_m[at] = top; a.part_l[at] = den; }
+        } else {
+            /* a row that sees no token is zero */
+            const float inv = top == -INFINITY && !gone ? 0.0f : 1.0f / den;
+            const uint32_t rr = it.r0 + r, tok = (uint32_t)it.start + rr / a.group, h = it.head * a.group + rr % a.group;
+            const u32x4 y = {to16<F16>(lo[0] * inv, lo[1] * inv), to16<F16>(lo[2] * inv, lo[3] * inv), to16<F16>(hi[0] * inv, hi[1] * inv), to16<F16>(hi[2] * inv, hi[3] * inv)};
+            *(u32x4*)(a.out + ((uint64_t)tok * a.q_heads + h) * D + c) = y;
+            if (a.lse && c == 0) a.lse[(uint64_t)tok * a.q_heads + h] = (top + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
+        }
+    }
+    return true;
+}
+template <int DP, int NT> constexpr uint32_t split_lds() { return (8 * 16 * NT + 16 * NT * DP + 4) * 4; }
+
+template <int DP, int F16, int NT>
+__global__ __launch_bounds__(256) void k_kv_attend(const kv_geom g, const kv_seqs s, const kv_att a)
+{
+    extern __shared__ float lds[];
+    const uint32_t item = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    kv_item it;
+    bool gone = false, ok = true;
+    if (item_of(g, s, a, item, 16 * NT, it)) ok = kv_split<DP, F16, NT, false>(g, s, a, item, it, split, lds, gone);
+    if (threadIdx.x == 0) a.left[blockIdx.x] = ok ? 0 : 1;
+}
+
+/*
+ * What the first launch left, with its pages held, and the splits of an item joined: out = sum over splits of exp(m_s - m) O_s / sum of exp(m_s - m) l_s.
+ */
+template <int DP, int F16, int NT>
+__global__ __launch_bounds__(256) void k_kv_finish(const kv_geom g, const kv_seqs s, const kv_att a)
+{
+    extern __shared__ float lds[];
+    constexpr uint32_t R = 16 * NT;
+    const uint32_t D = g.dim;
+    for (uint32_t item = blockIdx.x; item < a.items; item += gridDim.x) {
+        bool mine = false;
+        for (uint32_t k = threadIdx.x; k < a.splits; k += 256u) mine |= a.left[(uint64_t)item * a.splits + k] != 0;
+        const bool any = __syncthreads_or(mine);
+        if (!any && a.splits == 1) continue;
+        kv_item it;
+        if (!item_of(g, s, a, item, R, it)) continue;
+        if (any) {
+            for (uint32_t k = 0; k < a.splits; k++)
+                if (a.left[(uint64_t)item * a.splits + k]) {
+                    bool gone = false;
+                    kv_split<DP, F16, NT, true>(g, s, a, item, it, k, lds, gone);
+                    __syncthreads();
+                }
+            __threadfence();
+            __syncthreads();
+        }
+        if (a.splits == 1) continue;
+        const uint32_t n_rows = it.r1 - it.r0;
+        for (uint32_t x = threadIdx.x; x < n_rows * (D / 4u); x += 256u) {
+            const uint32_t r = x / (D / 4u), c = x % (D / 4u) * 4u;
+            const uint64_t at = ((uint64_t)item * R + r) * a.splits;
+            float top = -INFINITY, den = 0;
+            for (uint32_t k = 0; k < a.splits; k++) top = fmaxf(top, a.part_m[at + k]);
+            const float use = top == -INFINITY ? 0.0f : top;
+            f32x4 sum{0, 0, 0, 0};
+            for (uint32_t k = 0; k < a.splits; k++) {
+                const float by = __builtin_amdgcn_exp2f(a.part_m[at + k] - use);
+                den += by * a.part_l[at + k];
+                sum += by * *(const f32x4*)(a.part + (at + k) * D + c);
+            }
+            const float inv = top == -INFINITY && den == 0 ? 0.0f : 1.0f / den;
+            const uint32_t rr = it.r0 + r, tok = (uint32_t)it.start + rr / a.group, h = it.head * a.group + rr % a.group;
+            uint32_t* const to = (uint32_t*)(a.out + ((uint64_t)tok * a.q_heads + h) * D + c);
+            to[0] = to16<F16>(sum[0] * inv, sum[1] * inv);
+            to[1] = to16<F16>(sum[2] * inv, sum[3] * inv);
+            if (a.lse && c == 0) a.lse[(uint64_t)tok * a.q_heads + h] = (top + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+struct kv_plan { uint32_t nt, tiles, splits, steps; uint64_t items, left_at, m_at, l_at, part_at, bytes; };
+
+/* steps of 32 tokens that a tile of `rows` rows can have to look at, of sequences of up to max_len tokens */
+uint64_t most_steps(const uint64_t max_len, const uint64_t new_tokens, const uint32_t window, const uint32_t sinks)
+{
+    const uint64_t all = (max_len + 31) / 32;
+    if (!window) return all;
+    const uint64_t seen = (window + new_tokens + 31) / 32 + 1 + (sinks + 31ull) / 32;
+    return seen < all ? seen : all;
+}
+
+kv_plan plan_of(const bam_kv_t* kv, const uint64_t n_seqs, const uint64_t max_new, const uint32_t q_heads, const uint64_t max_len, const uint32_t window, const uint32_t sinks)
+{
+    kv_plan p{};
+    const uint64_t group = q_heads / kv->g.heads, rows = max_new * group;
+    p.nt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const uint64_t R = 16ull * p.nt;
+    p.tiles = (uint32_t)((rows + R - 1) / R);
+    p.items = n_seqs * p.tiles * kv->g.heads;
+    const uint64_t steps = most_steps(max_len, (R + group - 1) / group + 1, window, sinks);
+    uint64_t splits = (1024 + p.items - 1) / p.items;                 /* four workgroups to a compute unit */
+    const uint64_t most = (steps + 15) / 16;                          /* no fewer than four steps to a wave */
+    if (splits > most) splits = most;
+    if (splits > 256) splits = 256;
+    if (splits < 1) splits = 1;
+    p.steps = (uint32_t)((steps + splits - 1) / splits + 3) & ~3u;
+    if (p.steps < 4) p.steps = 4;
+    p.splits = (uint32_t)((steps + p.steps - 1) / p.steps);
+    if (p.splits < 1) p.splits = 1;
+    auto place = [&](uint64_t bytes) { const uint64_t at = p.bytes; p.bytes += (bytes + 255) & ~255ull; return at; };
+    p.left_at = place(p.items * p.splits);
+    if (p.splits > 1) {
+        p.m_at = place(p.items * R * p.splits * 4);
+        p.l_at = place(p.items * R * p.splits * 4);
+        p.part_at = place(p.items * R * p.splits * kv->g.dim * 4);
+    }
+    return p;
+}
+
+/* a kernel and not a memset: the stream may be captured */
+__global__ void k_kv_all_left(uint8_t* left, const uint64_t n)
+{
+    const uint64_t i = blockIdx.x * 256ull + threadIdx.x;
+    if (i < n) left[i] = 1;
+}
+
+template <typename K> void allow_lds(K kernel, const uint32_t bytes)
+{
+    if (bytes > 65536) hip_err_chk(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+template <int DP, int F16, int NT>
+void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan& p, hipStream_t st)
+{
+    constexpr uint32_t lds = split_lds<DP, NT>();
+    static const bool once = [] { allow_lds(k_kv_attend<DP, F16, NT>, lds); allow_lds(k_kv_finish<DP, F16, NT>, lds); return true; }();
+    (void)once;
+    /* what all waves of the second launch hold at a time stays under half the cache, or they wait for each other's slots */
+    const uint32_t least = kv->g.tokens < 32 ? 32 / kv->g.tokens : 1;
+    const uint64_t half = kv->cache_pages / 2;
+    uint64_t groups = p.items < 2048 ? p.items : 2048;
+    if (groups * 4 * 2 * least > half) groups = half / (8 * least);
+    uint64_t chunk = half / (groups * 8) / least * least;
+    a.chunk = (uint32_t)(chunk > 32 ? 32 : chunk);
+    if (kv->unheld) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), dim3((uint32_t)(p.items * p.splits)), dim3(256), lds, st, kv->g, s, a);
+    else hipLaunchKernelGGL(k_kv_all_left, dim3((uint32_t)((p.items * p.splits + 255) / 256)), dim3(256), 0, st, a.left, p.items * p.splits);
+    hipLaunchKernelGGL((k_kv_finish<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
+}
+template <int DP, int F16>
+void launch_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st)
+{
+    if (p.nt == 1) launch_attend<DP, F16, 1>(kv, s, a, p, st);
+    else if (p.nt == 2) launch_attend<DP, F16, 2>(kv, s, a, p, st);
+    else launch_attend<DP, F16, 4>(kv, s, a, p, st);
+}
+template <int F16>
+void launch_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st)
+{
+    if (kv->g.dim <= 64) launch_attend<64, F16>(kv, s, a, p, st);
+    else if (kv->g.dim <= 128) launch_attend<128, F16>(kv, s, a, p, st);
+    else launch_attend<256, F16>(kv, s, a, p, st);
+}
+
+template <bool WRITE>
+void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t st)
+{
+    const uint32_t lpr = kv->g.dim <= 64 ? 8 : kv->g.dim <= 128 ? 16 : 32, rpw = 64 / lpr;
+    io.q_waves = io.q ? (uint32_t)(((uint64_t)s.rows * io.q_heads + rpw - 1) / rpw) : 0;
+    io.k_waves = (s.rows + rpw - 1) / rpw * kv->g.heads;
+    /* a wave that looks after eight rows goes through eight pages one after the other where each belongs to another sequence */
+    io.v_rows = (uint64_t)s.rows * kv->g.heads <= 8192 ? 1 : 8;
+    const uint64_t waves = (uint64_t)io.q_waves + io.k_waves + (uint64_t)(s.rows + io.v_rows - 1) / io.v_rows * kv->g.heads;
+    const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
+#define KV_ROWS(LPR) \
+    if (kv->f16) hipLaunchKernelGGL((k_kv_rows<LPR, 1, WRITE>), grid, block, 0, st, kv->g, s, io); \
+    else hipLaunchKernelGGL((k_kv_rows<LPR, 0, WRITE>), grid, block, 0, st, kv->g, s, io)
+    if (lpr == 8) { KV_ROWS(8); } else if (lpr == 16) { KV_ROWS(16); } else { KV_ROWS(32); }
+#undef KV_ROWS
+}
+
+int bad_seqs(const char* who, const bam_kv_t* kv, uint64_t n_seqs, uint64_t n_rows, const int32_t* starts, const int32_t* lens, const int32_t* table, int64_t stride, uint64_t width)
+{
+    if (!kv || (n_rows && (!lens || !table))) return fail(EINVAL, std::string(who) + ": null argument");
+    if (n_seqs > 0x7fffffffull || n_rows > 0x7fffffffull) return fail(EINVAL, std::string(who) + ": more rows or sequences than 31 bits count");
+    if (!starts && n_seqs != n_rows) return fail(EINVAL, std::string(who) + ": without starts every sequence has one new token");
+    if (!n_rows) return 0;
+    if (width == 0 || width > 0x7fffffffull || stride < 0) return fail(EINVAL, std::string(who) + ": table of no width, or with its rows in reverse");
+    if (width > 0x7fffffffull >> kv->g.tokens_log) return fail(EINVAL, std::string(who) + ": the table has room for more positions than 31 bits count");
+    return 0;
+}
+bool whole_pieces(const void* p, int64_t row, int64_t head) { return ((uintptr_t)p & 15) == 0 && row % 8 == 0 && head % 8 == 0; }
+
+} // namespace
+
+extern "C" {
+
+int bam_kv_create(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t n_blocks, uint32_t n_heads, uint32_t dim, int f16)
+{
+    if (!out || !a) return fail(EINVAL, "bam_kv_create: null argument");
+    *out = nullptr;
+    if (!n_heads || !n_blocks) return fail(EINVAL, "bam_kv_create: no heads or no blocks");
+    if (!dim || dim % 16 || dim > 256) return fail(EINVAL, "bam_kv_create: head dimension must be a multiple of 16, at most 256");
+    if (f16 != 0 && f16 != 1) return fail(EINVAL, "bam_kv_create: type must be 0 (bfloat16) or 1 (float16)");
+    if (a->a->adt.n_ranges != 1) return fail(EINVAL, "bam_kv_create: the array must have one range");
+    BAM_API_BEGIN
+    const range_d_t<uint64_t>& r = a->a->h_ranges[0];
+    if (r.page_start_offset) return fail(EINVAL, "bam_kv_create: the array's range must begin a page");
+    const uint64_t row = 2ull * dim;
+    if (r.page_size < 8 * row) return fail(EINVAL, "bam_kv_create: a page must hold eight rows of a head");
+    if (n_heads > 65535 || n_blocks > 0x7fffffffull || first_page > r.page_count || n_blocks * n_heads > (r.page_count - first_page) / 2)
+        return fail(EINVAL, "bam_kv_create: the blocks do not fit the array (two pages for each block and head)");
+    bam_kv_t* kv = new bam_kv();
+    kv->a = a;
+    kv->f16 = f16;
+    kv->cache_pages = r.cache.n_pages;
+    kv->unheld = r.cache.fast_reads != 0;
+    kv_geom& g = kv->g;
+    g.r = a->a->adt.d_ranges;
+    g.pages = r.pages;
+    g.base = r.cache.base_addr;
+    g.first_page = first_page;
+    g.n_blocks = n_blocks;
+    g.heads = n_heads;
+    g.dim = dim;
+    g.page_log = (uint32_t)r.cache.page_size_log;
+    for (g.tokens_log = 3; (row << (g.tokens_log + 1)) <= r.page_size; g.tokens_log++) {}
+    g.tokens = 1u << g.tokens_log;
+    if (kv->cache_pages < 16 * (g.tokens < 32 ? 32 / g.tokens : 1)) { delete kv; return fail(EINVAL, "bam_kv_create: the page cache must have 16 pages, 32 where a page holds 16 tokens, 64 where it holds 8"); }
+    *out = kv;
+    BAM_API_END
+}
+
+void bam_kv_destroy(bam_kv_t* kv) { delete kv; }
+
+int bam_kv_info(bam_kv_t* kv, uint64_t* out)
+{
+    if (!kv || !out) return fail(EINVAL, "bam_kv_info: null argument");
+    out[0] = kv->g.tokens; out[1] = kv->g.n_blocks; out[2] = 2ull * kv->g.heads; out[3] = 1ull << kv->g.page_log;
+    return 0;
+}
+
+int bam_kv_append(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
+                  const void* d_k, int64_t k_row, int64_t k_head, const void* d_v, int64_t v_row, int64_t v_head,
+                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, void* d_q_out, const void* d_q_norm, const void* d_k_norm, float eps,
+                  const float* d_cos, const float* d_sin, uint64_t n_positions, uint32_t rot, int pairs, void* stream)
+{
+    if (int e = bad_seqs("bam_kv_append", kv, n_seqs, n_rows, d_starts, d_lens, d_table, table_stride, table_width)) return e;
+    if (!n_rows) return 0;
+    if (!d_k || !d_v || (d_q && !d_q_out) || (d_q && !q_heads) || (rot && (!d_cos || !d_sin))) return fail(EINVAL, "bam_kv_append: null argument");
+    if (rot % 16 || rot > kv->g.dim) return fail(EINVAL, "bam_kv_append: the rotated part must be a multiple of 16, at most the head dimension");
+    if (((uintptr_t)d_q_norm | (uintptr_t)d_k_norm | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_q_out) & 15) return fail(EINVAL, "bam_kv_append: weights, tables and output must be aligned to 16 bytes");
+    if (n_positions > 0x7fffffffull) return fail(EINVAL, "bam_kv_append: more positions than 31 bits count");
+    BAM_API_BEGIN
+    kv_seqs s{d_starts, d_lens, d_table, table_stride, (uint32_t)n_seqs, (uint32_t)n_rows, (uint32_t)table_width};
+    kv_rows io{};
+    io.q = (const uint16_t*)d_q; io.k = (const uint16_t*)d_k; io.v = (const uint16_t*)d_v;
+    io.q_row = q_row; io.q_head = q_head; io.k_row = k_row; io.k_head = k_head; io.v_row = v_row; io.v_head = v_head;
+    io.q_out = (uint16_t*)d_q_out; io.q_norm = (const uint16_t*)d_q_norm; io.k_norm = (const uint16_t*)d_k_norm;
+    io.cos = d_cos; io.sin = d_sin; io.positions = (uint32_t)n_positions; io.q_heads = q_heads; io.rot = rot; io.pairs = pairs != 0; io.eps = eps;
+    io.aligned = whole_pieces(d_k, k_row, k_head) && whole_pieces(d_v, v_row, v_head) && (!d_q || whole_pieces(d_q, q_row, q_head));
+    launch_rows<true>(kv, s, io, (hipStream_t)stream);
+    hip_err_chk(hipGetLastError());
+    BAM_API_END
+}
+
+int bam_kv_read(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
+                void* d_k, void* d_v, void* stream)
+{
+    if (int e = bad_seqs("bam_kv_read", kv, n_seqs, n_rows, d_starts, d_lens, d_table, table_stride, table_width)) return e;
+    if (!n_rows) return 0;
+    if (!d_k || !d_v) return fail(EINVAL, "bam_kv_read: null argument");
+    if (((uintptr_t)d_k | (uintptr_t)d_v) & 15) return fail(EINVAL, "bam_kv_read: output must be aligned to 16 bytes");
+    BAM_API_BEGIN
+    kv_seqs s{d_starts, d_lens, d_table, table_stride, (uint32_t)n_seqs, (uint32_t)n_rows, (uint32_t)table_width};
+    kv_rows io{};
+    io.k = (const uint16_t*)d_k; io.v = (const uint16_t*)d_v;
+    io.k_row = io.v_row = (int64_t)kv->g.heads * kv->g.dim;
+    io.k_head = io.v_head = kv->g.dim;
+    io.aligned = 1;
+    launch_rows<false>(kv, s, io, (hipStream_t)stream);
+    hip_err_chk(hipGetLastError());
+    BAM_API_END
+}
+
+int bam_kv_attend_bytes(bam_kv_t* kv, uint64_t n_seqs, uint64_t max_new, uint32_t q_heads, uint64_t max_len, uint32_t window, uint32_t sinks, uint64_t* bytes)
+{
+    if (!kv || !bytes) return fail(EINVAL, "bam_kv_attend_bytes: null argument");
+    if (!q_heads || q_heads % kv->g.heads) return fail(EINVAL, "bam_kv_attend_bytes: heads of queries must be a multiple of the heads of keys");
+    *bytes = n_seqs && max_new ? plan_of(kv, n_seqs, max_new, q_heads, max_len, window, sinks).bytes : 0;
+    return 0;
+}
+
+int bam_kv_attend(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
+                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, uint64_t max_new, uint64_t max_len, float scale, uint32_t window, uint32_t sinks,
+                  void* d_out, float* d_lse, void* d_work, uint64_t work_bytes, void* stream)
+{
+    if (int e = bad_seqs("bam_kv_attend", kv, n_seqs, n_rows, d_starts, d_lens, d_table, table_stride, table_width)) return e;
+    if (!n_rows || !n_seqs) return 0;
+    if (!d_q || !d_out) return fail(EINVAL, "bam_kv_attend: null argument");
+    if (!q_heads || q_heads % kv->g.heads) return fail(EINVAL, "bam_kv_attend: heads of queries must be a multiple of the heads of keys");
+    if (!(scale == scale) || scale - scale != 0) return fail(EINVAL, "bam_kv_attend: scale must be finite");
+    if (window > 0x7fffffffu || sinks > 0x7fffffffu || max_len > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: window, sinks and lengths are 31-bit numbers");
+    if (((uintptr_t)d_out | (uintptr_t)d_work) & 15) return fail(EINVAL, "bam_kv_attend: output and workspace must be aligned to 16 bytes");
+    if (!d_starts) max_new = 1;
+    if (!max_new || max_new > n_rows) return fail(EINVAL, "bam_kv_attend: max_new must be at least 1 and at most the number of rows");
+    if (max_new * (q_heads / kv->g.heads) > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more rows than 31 bits count");
+    BAM_API_BEGIN
+    const kv_plan p = plan_of(kv, n_seqs, max_new, q_heads, max_len, window, sinks);
+    if (p.items * p.splits > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more workgroups than 31 bits count");
+    if (!d_work || work_bytes < p.bytes) return fail(EINVAL, "bam_kv_attend: the workspace is smaller than bam_kv_attend_bytes says");
+    kv_seqs s{d_starts, d_lens, d_table, table_stride, (uint32_t)n_seqs, (uint32_t)n_rows, (uint32_t)table_width};
+    kv_att a{};
+    a.q = (const uint16_t*)d_q; a.q_row = q_row; a.q_head = q_head; a.aligned = whole_pieces(d_q, q_row, q_head); a.q_heads = q_heads; a.group = q_heads / kv->g.heads;
+    a.scale = scale * 1.4426950408889634f; a.window = window; a.sinks = sinks; a.out = (uint16_t*)d_out; a.lse = d_lse;
+    a.tiles = p.tiles; a.splits = p.splits; a.steps = p.steps; a.items = (uint32_t)p.items;
+    uint8_t* const w = (uint8_t*)d_work;
+    a.left = w + p.left_at; a.part_m = (float*)(w + p.m_at); a.part_l = (float*)(w + p.l_at); a.part = (float*)(w + p.part_at);
+    if (kv->f16) launch_attend<1>(kv, s, a, p, (hipStream_t)stream);
+    else launch_attend<0>(kv, s, a, p, (hipStream_t)stream);
+    hip_err_chk(hipGetLastError());
+    BAM_API_END
+}
+
+} // extern "C"

@@ -1,0 +1,170 @@
+"""A key-value cache in the pages of an array: what attention layers keep of their tokens, behind the page cache.
+
+Keys and values that the page cache does not hold lie on the store and are fetched by the waves that want them, like any other element of an
+array.  The reference has no counterpart; the C-ABI is bam_kv_* of include/bam_amd.h.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .host import Array, BamError, PageCache, Range, _chk, _stream, c_u64, c_vp
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+class KVCache:
+    """Blocks of `block_tokens` tokens in the pages of `array` from `first_page` on, two pages to a block and head.
+
+    The calls below share how sequences are given, all on the device in int32: `lens[b]` counts the tokens of sequence b, the new ones among them;
+    `table[b, i]` is the block of its tokens i * block_tokens and on; rows starts[b] .. starts[b+1]-1 of the packed inputs are its newest tokens
+    (starts None: one new token each).  They are queued on the current stream.  A block number outside the cache is not read or written.
+    """
+
+    def __init__(self, array, n_heads, head_dim, dtype=torch.bfloat16, first_page=0, n_blocks=None, _owned=()):
+        self.L = _lib.load()
+        self.h = c_vp()
+        self._owned = list(_owned)
+        if dtype not in _TYPES:
+            raise BamError("KVCache: dtype must be torch.bfloat16 or torch.float16")
+        if n_blocks is None:
+            raise BamError("KVCache: n_blocks must be given")
+        self.array = array
+        self.device = torch.device("cuda", array.device)
+        self.n_heads, self.head_dim, self.dtype = n_heads, head_dim, dtype
+        _chk(self.L.bam_kv_create(ctypes.byref(self.h), array.h, first_page, n_blocks, n_heads, head_dim, _TYPES[dtype]), "bam_kv_create")
+        out = (c_u64 * 4)()
+        _chk(self.L.bam_kv_info(self.h, out), "bam_kv_info")
+        self.block_tokens, self.n_blocks, self.pages_per_block, self.page_size = list(out)
+        self._bytes = {}
+
+    # ---- checks ----
+
+    def _rows(self, t, what, heads=None):
+        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+            raise BamError(f"KVCache: {what} must be [rows, {'heads' if heads is None else heads}, {self.head_dim}] of {self.dtype} on {self.device}")
+        if t.stride(2) != 1:
+            raise BamError(f"KVCache: the numbers of a row of {what} must be next to each other")
+        return t
+
+    def _seqs(self, n_rows, lens, table, starts):
+        if lens.dtype != torch.int32 or lens.dim() != 1 or not lens.is_contiguous() or lens.device != self.device:
+            raise BamError(f"KVCache: lens must be a contiguous int32 tensor on {self.device}")
+        if table.dtype != torch.int32 or table.dim() != 2 or table.device != self.device or table.shape[0] != lens.shape[0] or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise BamError(f"KVCache: table must be [{lens.shape[0]}, blocks] in int32 on {self.device}, the blocks of a sequence next to each other")
+        if starts is None:
+            if lens.shape[0] != n_rows:
+                raise BamError("KVCache: without starts every sequence has one new row")
+        elif starts.dtype != torch.int32 or starts.dim() != 1 or not starts.is_contiguous() or starts.device != self.device or starts.shape[0] != lens.shape[0] + 1:
+            raise BamError(f"KVCache: starts must be {lens.shape[0] + 1} int32 numbers on {self.device}")
+        width = table.shape[1]
+        return (n_rows, lens.shape[0], None if starts is None else starts.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0), width)
+
+    def _weights(self, t, what):
+        if t is None:
+            return None
+        if t.dtype != self.dtype or t.shape != (self.head_dim,) or not t.is_contiguous() or t.device != self.device:
+            raise BamError(f"KVCache: {what} must be {self.head_dim} contiguous numbers of {self.dtype} on {self.device}")
+        return t.data_ptr()
+
+    # ---- calls ----
+
+    def append(self, k, v, lens, table, starts=None, q=None, q_norm=None, k_norm=None, eps=1e-6, cos=None, sin=None, rotary="half", out=None):
+        """Put the new rows into the cache.  Keys, and queries if there are any, are normed per head (x * rsqrt(mean x^2 + eps) * weight) where a weight is
+        given, and their first 2 * cos.shape[1] numbers are turned by the angles of their positions: pairs (i, i + half) with rotary="half",
+        neighbours with "pairs"; cos and sin are [positions, half] in float32.  Returns the queries (None without)."""
+        n = self._rows(k, "k", self.n_heads).shape[0]
+        if self._rows(v, "v", self.n_heads).shape[0] != n:
+            raise BamError("KVCache: k and v must have the same rows")
+        seqs = self._seqs(n, lens, table, starts)
+        q_args = (None, 0, 0, 0, None)
+        if q is not None:
+            if self._rows(q, "q").shape[0] != n or q.shape[1] == 0:
+                raise BamError("KVCache: q must have the rows of k and at least one head")
+            if out is None:
+                out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
+            elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous():
+                raise BamError("KVCache: out must be like q, and contiguous")
+            q_args = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], out.data_ptr())
+        elif q_norm is not None or out is not None:
+            raise BamError("KVCache: q_norm and out go with q")
+        rot = 0
+        if (cos is None) != (sin is None):
+            raise BamError("KVCache: cos and sin go together")
+        if rotary not in ("half", "pairs"):
+            raise BamError('KVCache: rotary must be "half" or "pairs"')
+        if cos is not None:
+            for t in (cos, sin):
+                if t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.device != self.device or t.shape != cos.shape:
+                    raise BamError(f"KVCache: cos and sin must be contiguous [positions, half] in float32 on {self.device}")
+            rot = 2 * cos.shape[1]
+        _chk(self.L.bam_kv_append(self.h, *seqs, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *q_args, self._weights(q_norm, "q_norm"),
+                                  self._weights(k_norm, "k_norm"), eps, cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, cos.shape[0] if rot else 0, rot,
+                                  int(rotary == "pairs"), _stream()), "bam_kv_append")
+        return out if q is not None else None
+
+    def read(self, n_rows, lens, table, starts=None):
+        """The newest rows as the cache has them: (keys, values), [n_rows, heads, head_dim] each."""
+        seqs = self._seqs(n_rows, lens, table, starts)
+        k = torch.empty(n_rows, self.n_heads, self.head_dim, dtype=self.dtype, device=self.device)
+        v = torch.empty_like(k)
+        _chk(self.L.bam_kv_read(self.h, *seqs, k.data_ptr(), v.data_ptr(), _stream()), "bam_kv_read")
+        return k, v
+
+    def attend(self, q, lens, table, starts=None, max_new=None, max_len=None, scale=None, window=0, sinks=0, out=None, return_lse=False):
+        """Attention of the newest tokens (their rows in q) over what the cache holds of their sequences: the token at position p sees t <= p and, with
+        a window, those with p - t < window or t < sinks.  scale: head_dim ** -0.5 unless given.  max_new: the most new rows a sequence has (all rows unless given);
+        max_len: about the longest sequence (the table's width unless given); they decide how the work is shared out.  Rows of no sequence are left as they are.
+        Returns the output, or with return_lse (output, logarithm of the sum of exponentials)."""
+        n, hq = self._rows(q, "q").shape[:2]
+        seqs = self._seqs(n, lens, table, starts)
+        if hq == 0 or hq % self.n_heads:
+            raise BamError(f"KVCache: the heads of q must be a multiple of {self.n_heads}")
+        if window < 0 or sinks < 0 or (max_new is not None and max_new < 1) or (max_len is not None and max_len < 1):
+            raise BamError("KVCache: window and sinks must not be negative, max_new and max_len at least 1")
+        if out is None:
+            out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous():
+            raise BamError("KVCache: out must be like q, and contiguous")
+        lse = torch.empty(n, hq, dtype=torch.float32, device=self.device) if return_lse else None
+        if n and seqs[1]:
+            max_new = 1 if starts is None else min(n if max_new is None else max_new, n)
+            max_len = seqs[6] * self.block_tokens if max_len is None else max_len
+            key = (seqs[1], max_new, hq, max_len, window, sinks)
+            need = self._bytes.get(key)
+            if need is None:
+                b = c_u64(0)
+                _chk(self.L.bam_kv_attend_bytes(self.h, *key, ctypes.byref(b)), "bam_kv_attend_bytes")
+                if len(self._bytes) > 4096:
+                    self._bytes.clear()
+                need = self._bytes[key] = b.value
+            # from torch's allocator, which keeps it for this stream, or for the graph that is being captured
+            work = torch.empty(need, dtype=torch.uint8, device=self.device)
+            _chk(self.L.bam_kv_attend(self.h, *seqs, q.data_ptr(), q.stride(0), q.stride(1), hq, max_new, max_len, self.head_dim ** -0.5 if scale is None else scale, window, sinks,
+                                      out.data_ptr(), None if lse is None else lse.data_ptr(), work.data_ptr(), need, _stream()), "bam_kv_attend")
+        return (out, lse) if return_lse else out
+
+    def close(self):
+        if self.h:
+            self.L.bam_kv_destroy(self.h)
+            self.h = c_vp()
+        for x in self._owned:
+            x.close()
+        self._owned = []
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def make_kv_cache(ctrl, n_blocks, n_heads, head_dim, page_size=4096, cache_pages=None, dtype=torch.bfloat16, device=0, disk_offset_bytes=0, max_range=64):
+    """Page cache + one range + array + key-value cache of n_blocks blocks, stored from byte disk_offset_bytes (page aligned).  cache_pages: slots of the page cache (all
+    pages of the blocks unless given)."""
+    n_pages = 2 * n_blocks * n_heads
+    pc = PageCache(page_size, max(64, n_pages if cache_pages is None else cache_pages), device, ctrl, max_range)
+    elems = n_pages * page_size // 8
+    r = Range(0, elems, disk_offset_bytes // page_size, n_pages, 0, page_size, pc, device)
+    a = Array(elems, disk_offset_bytes, [r], device)
+    return KVCache(a, n_heads, head_dim, dtype, 0, n_blocks, _owned=(a, r, pc))

@@ -24,6 +24,7 @@ typedef struct bam_range bam_range_t;         /* range_t<uint64_t> */
 typedef struct bam_array bam_array_t;         /* array_t<uint64_t> */
 typedef struct bam_range32 bam_range32_t;     /* range_t<uint32_t> */
 typedef struct bam_array32 bam_array32_t;     /* array_t<uint32_t> */
+typedef struct bam_kv bam_kv_t;               /* a key-value cache in the pages of an array */
 
 const char* bam_last_error(void);
 /* 1 when the library was built with the gfx950 device path and a HIP device is present */
@@ -423,6 +424,50 @@ void bam_event_destroy(void* ev);
 /* protocol ceiling of the target with plain host clients (nvmt_selftest_iops) */
 double bam_target_ceiling_iops(uint64_t ns_bytes, uint32_t lba_bytes, int backing, uint32_t n_io_threads, uint32_t n_clients,
                                uint32_t depth, uint64_t n_cmds, uint32_t req_bytes);
+
+/* ---- key-value cache in the pages of an array ----
+ * The keys and values of the attention layers of a language model, kept in an array's pages: what the page cache does not hold lies on the store and is
+ * fetched by the waves that want it.  (No counterpart in the reference.)
+ *
+ * The cache is n_blocks blocks of T tokens in the array's pages from first_page on, 2 * n_heads pages to a block: for each head a page of
+ * keys and a page of values of its T tokens, T the largest power of two for which T rows of `dim` 16-bit numbers fit a page.  Pages hold pieces of 16 bytes: of keys, piece
+ * c * T + t has numbers 8c .. 8c+7 of token t; of values, piece t * dim + d has number d of tokens 8t .. 8t+7.
+ *
+ * Sequences: d_lens[b] counts the tokens of sequence b, the new ones among them; d_table[b * table_stride + i] is the block of its tokens iT .. iT+T-1;
+ * rows d_starts[b] .. d_starts[b+1]-1 of the packed inputs and outputs are its newest tokens, in order (d_starts NULL: one each).  Blocks may be shared
+ * between sequences.  What the tables do not hold (a block number outside the cache, a position past the table's width or before the first)
+ * is neither read nor written: such tokens are not visible, and rows appended there are dropped.
+ *
+ * The calls are queued on `stream` and do not wait; they may be captured into a graph.  A handle keeps nothing from call to call.  The array outlives it. */
+int bam_kv_create(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t n_blocks, uint32_t n_heads, uint32_t dim /* a multiple of 16, at most 256 */,
+                  int f16 /* 0: bfloat16, 1: float16 */);
+void bam_kv_destroy(bam_kv_t* kv);
+/* out[0] tokens to a block, [1] blocks, [2] pages to a block, [3] bytes of a page */
+int bam_kv_info(bam_kv_t* kv, uint64_t* out);
+/*
+ * New rows into the cache: d_v as they are; d_k, and d_q into d_q_out ([n_rows][q_heads][dim]), with d_k_norm / d_q_norm (dim numbers, or NULL) as
+ * x * rsqrt(mean x^2 + eps) * w per head, then the first `rot` numbers turned by the angles of the row's position: pairs (i, i + rot/2), or with
+ * `pairs` (2i, 2i+1), by d_cos / d_sin[position * rot/2 + i] (n_positions rows; a position past them gives NaN; rot 0: none).  In 32 bits, rounded once.
+ * Strides are in elements; the numbers of a row are next to each other.  d_q may be NULL.
+ */
+int bam_kv_append(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
+                  const void* d_k, int64_t k_row, int64_t k_head, const void* d_v, int64_t v_row, int64_t v_head,
+                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, void* d_q_out, const void* d_q_norm, const void* d_k_norm, float eps,
+                  const float* d_cos, const float* d_sin, uint64_t n_positions, uint32_t rot, int pairs, void* stream);
+/* the rows that bam_kv_append with the same sequences writes, as the cache has them now: [n_rows][n_heads][dim] each; a row without a place comes out as zeros */
+int bam_kv_read(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
+                void* d_k, void* d_v, void* stream);
+/*
+ * Attention of the newest tokens over what the cache holds: row i at position p, head h, sees the tokens t <= p of its sequence, with a window (not 0) those with
+ * p - t < window or t < sinks; out = sum of softmax(scale * q.k_t) v_t, with the keys of head h / (q_heads / n_heads).  A row that sees nothing is zero.  What a
+ * row does not see has no part in it, infinities and NaN included.  d_lse (or NULL): log of the sum of exp(scale * q.k_t), [n_rows][q_heads].
+ * max_new: no sequence has more new rows (rows beyond are not written; ignored without d_starts); max_len: about how long sequences get (it decides how the
+ * work is shared out, not what is read).  d_work: bam_kv_attend_bytes(...) bytes for the length of the call.
+ */
+int bam_kv_attend_bytes(bam_kv_t* kv, uint64_t n_seqs, uint64_t max_new, uint32_t q_heads, uint64_t max_len, uint32_t window, uint32_t sinks, uint64_t* bytes);
+int bam_kv_attend(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
+                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, uint64_t max_new, uint64_t max_len, float scale, uint32_t window, uint32_t sinks,
+                  void* d_out, float* d_lse, void* d_work, uint64_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }

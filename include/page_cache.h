@@ -647,8 +647,9 @@ struct range_d_t {
     __forceinline__ __device__ uint64_t acquire_page(const size_t pg, const uint32_t count, const bool write, const uint32_t ctrl, const uint32_t queue);
     /* spread by workgroup so that no counter word is shared by more than a few waves at a time */
     __forceinline__ __device__ bam_stat_shard_t* shard() const { return stats + (((blockIdx.x + blockIdx.y * gridDim.x) * 0x9E3779B1u) >> 20) % BAM_STAT_SHARDS; }
+    template <bool FRESH = false>
     __forceinline__ __device__ bool slow_step(const size_t pg, const bool write, const uint32_t queue, uint64_t& sv, uint32_t& slot, bool& was_hit, bool& progressed, const bool take_part = true,
-                                              const bool may_load = true, bool* wants_load = nullptr, const uint32_t place = BAM_PLACE_NORMAL);
+                                              const bool may_load = true, bool* wants_load = nullptr, const uint32_t place = BAM_PLACE_NORMAL, const bool fresh = false, const bool cleared = false);
 };
 
 /*
@@ -750,11 +751,17 @@ __device__ __forceinline__ void stat_add(unsigned long long* ctr, uint32_t v)
  * Callers use a resolved page and drop its references before they make the
  * next pass for the lanes still waiting: a lane that sat on a resident page
  * while its siblings look for slots could pin the last evictable slot.
+ *
+ * FRESH, for writers: a lane with `fresh` set knows that nothing its page holds
+ * on the store is wanted; the page gets a slot and no read, and with `cleared`
+ * the slot is filled with zeros (for pages that are not written in full, so
+ * that nothing of the slot's last page is left in them).
  */
 template <typename T>
+template <bool FRESH>
 __forceinline__ __device__
 bool range_d_t<T>::slow_step(const size_t pg, const bool write, const uint32_t queue, uint64_t& sv, uint32_t& slot, bool& was_hit, bool& progressed, const bool take_part,
-                             const bool may_load, bool* wants_load, const uint32_t place)
+                             const bool may_load, bool* wants_load, const uint32_t place, const bool fresh, const bool cleared)
 {
     using namespace bam;
     data_page_t* dp = &pages[pg];
@@ -795,6 +802,8 @@ bool range_d_t<T>::slow_step(const size_t pg, const bool write, const uint32_t q
             /* no evictable slot right now: hand the page back; a later pass tries again */
             __hip_atomic_fetch_and(&dp->state, DISABLE_BUSY_MASK, __ATOMIC_RELAXED, BAM_AGENT);
             load_me = false;
+        } else if (FRESH && fresh) {
+            io_ok = true;
         } else {
             uint64_t c = get_backing_ctrl(pg);
             if (c == ALL_CTRLS) c = cache.n_ctrls == 1 ? 0 : cache.ctrl_counter->fetch_add(1, simt::memory_order_relaxed) % cache.n_ctrls;
@@ -826,6 +835,13 @@ bool range_d_t<T>::slow_step(const size_t pg, const bool write, const uint32_t q
 #ifdef BAM_PROFILE
     if (cache.prof && bam::ballot(load_me) && bam::lane() == bam::first_lane(bam::active_mask())) atomicAdd(&cache.prof[5], wall_clock64() - pc0);
 #endif
+    if constexpr (FRESH) {
+        for (uint64_t m = bam::ballot(load_me && fresh && cleared); m; m &= m - 1) {
+            uint8_t* const at = cache.base_addr + (uint64_t)bam::bcast(found, bam::first_lane(m)) * cache.page_size;
+            const uint64_t all = bam::active_mask();
+            for (uint64_t o = bam::rank_in(all) * 16ull; o < cache.page_size; o += bam::popc(all) * 16ull) bam::st16_sys(at + o, bam::u32x4_t{0, 0, 0, 0});
+        }
+    }
     if (load_me) {
         if (held) read_end(qp, cid);
         if (!io_ok) {
