@@ -12,6 +12,7 @@
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -395,7 +396,7 @@ struct kv_att {
     float *part_m, *part_l;
     uint8_t* left;                      /* [item][split] pages were missing */
     uint32_t chunk;                     /* blocks whose pages a wave holds at a time when it holds them */
-    uint32_t items;
+    uint32_t items, tile_rows;
 };
 
 template <int F16> __device__ __forceinline__ f32x4 mma(const u32x4 a, const u32x4 b, const f32x4 c)
@@ -434,19 +435,36 @@ template <int F16> __device__ __forceinline__ bool odd16(const uint32_t x)
 }
 __device__ __forceinline__ u32x4 load_once(const uint8_t* p) { return __builtin_nontemporal_load((const u32x4*)p); }
 
+/* of the eight tokens from t on, those up to `last` that are not before `low`, or are before `sinks` */
+__device__ __forceinline__ uint32_t seen_of_eight(const int32_t t, const int32_t last, const int32_t low, const int32_t sinks)
+{
+    auto below = [t](const int32_t end) { const int32_t n = end - t; return (1u << (n < 0 ? 0 : n > 8 ? 8 : n)) - 1u; };
+    return below(last + 1) & (~below(low) | below(sinks));
+}
+/* the first token that a row at `pos` sees through the window */
+__device__ __forceinline__ int32_t low_of(const kv_att& a, const int32_t pos) { return a.window && pos >= (int32_t)a.window ? pos - (int32_t)a.window + 1 : 0; }
+/* eight 16-bit numbers, those whose bit is not set as zero */
+__device__ __forceinline__ u32x4 only(u32x4 x, const uint32_t bits)
+{
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] &= ((bits >> (2 * e)) & 1u) * 0xffffu | ((bits >> (2 * e + 1)) & 1u) * 0xffff0000u;
+    return x;
+}
+
 /* which tokens a tile of rows sees, and the order in which they are gone through: steps of 32 tokens, first those that stay visible in front of the window */
 struct kv_span {
     int32_t first_pos, last_pos;        /* positions of the tile's rows */
     uint32_t len;                       /* tokens to look at: up to the last row's */
     uint32_t low, front, base, n_steps; /* first token of the window; steps in front of it; first token of the step it begins in; steps */
 };
-__device__ __forceinline__ kv_span span_of(const kv_att& a, const int32_t len, const int32_t new_rows, const uint32_t r0, const uint32_t r1)
+__device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most, const int32_t len, const int32_t new_rows, const uint32_t r0, const uint32_t r1)
 {
     kv_span s;
     const int32_t p0 = len - new_rows;
     s.first_pos = p0 + (int32_t)(r0 / a.group);
     s.last_pos = p0 + (int32_t)((r1 - 1) / a.group);
     s.len = s.last_pos < 0 ? 0u : (uint32_t)s.last_pos + 1u;
+    if (s.len > most) s.len = most;             /* what lies past the table is not visible */
     s.low = a.window && s.first_pos + 1 > (int64_t)a.window ? (uint32_t)(s.first_pos + 1) - a.window : 0u;
     const uint32_t sinks = a.sinks < s.low ? a.sinks : s.low;
     s.front = (sinks + 31u) / 32u;
@@ -528,18 +546,13 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                 if (16u * i + row < D) vv[i] = load_once(vp + i * 256u);
             }
             const bool whole = !holes && (int64_t)t0 + 31 <= sp.first_pos && (!a.window || (int64_t)sp.last_pos - t0 < a.window || t0 + 32u <= a.sinks);
+            const bool hole = (holes >> vb) & 1u;
             bool slow = false;
             if (!whole) {
                 /* values of tokens that no row sees may be anything: none of it may meet the zeros of P */
-                const bool hole = (holes >> vb) & 1u;
+                const uint32_t any = hole ? 0u : seen_of_eight((int32_t)vt, sp.last_pos, low_of(a, sp.first_pos), (int32_t)a.sinks);
 #pragma unroll
-                for (uint32_t e = 0; e < 8; e++) {
-                    const int64_t t = vt + e;
-                    const bool none = hole || t > sp.last_pos || (a.window && t <= (int64_t)sp.first_pos - a.window && t >= a.sinks);
-                    const uint32_t keep = none ? ((e & 1) ? 0x0000ffffu : 0xffff0000u) : 0xffffffffu;
-#pragma unroll
-                    for (int i = 0; i < DP / 16; i++) vv[i][e / 2] &= keep;
-                }
+                for (int i = 0; i < DP / 16; i++) vv[i] = only(vv[i], any);
                 if (sp.first_pos != sp.last_pos) {
                     bool odd = false;
 #pragma unroll
@@ -559,13 +572,9 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                 for (int e = 0; e < 4; e++) { x[e] = s0[e] * a.scale; x[4 + e] = s1[e] * a.scale; }
                 uint32_t sees = 0xffu;
                 if (!whole) {
-                    const bool hole = (holes >> vb) & 1u;
+                    sees = hole ? 0u : seen_of_eight((int32_t)vt, pos[n], low_of(a, pos[n]), (int32_t)a.sinks);
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; e++) {
-                        const int64_t t = vt + e;
-                        const bool in = !hole && t <= pos[n] && (!a.window || pos[n] - t < a.window || t < a.sinks);
-                        if (!in) { x[e] = -INFINITY; sees &= ~(1u << e); }
-                    }
+                    for (uint32_t e = 0; e < 8; e++) x[e] = (sees >> e) & 1u ? x[e] : -INFINITY;
                 }
                 float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
                 top = fmaxf(max_of_four(top), m[n]);
@@ -593,10 +602,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                         const uint32_t sc = bam::shfl(sees, (lane & 48u) + c);
 #pragma unroll
                         for (int i = 0; i < DP / 16; i++) {
-                            u32x4 z = vv[i];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) z[e] &= ((sc >> (2 * e)) & 1u ? 0xffffu : 0u) | ((sc >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
-                            const f32x4 with = mma<F16>(z, p, o[n][i]);
+                            const f32x4 with = mma<F16>(only(vv[i], sc), p, o[n][i]);
                             if (row == c) o[n][i] = with;
                         }
                     }
@@ -616,8 +622,9 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
 
 /* rows of an item: a head of keys, a tile of the rows (new token, head of queries) of a sequence */
 struct kv_item { uint32_t seq, head, tile, r0, r1; int32_t len, rows, start; };
-__device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, const uint32_t tile_rows, kv_item& it)
+__device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, kv_item& it)
 {
+    const uint32_t tile_rows = a.tile_rows;
     it.head = item % g.heads;
     it.tile = item / g.heads % a.tiles;
     it.seq = item / g.heads / a.tiles;
@@ -627,6 +634,7 @@ __device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, cons
     if (end > (int32_t)s.rows) end = (int32_t)s.rows;
     it.rows = end - it.start;
     it.len = s.lens[it.seq];
+    if (it.len < 0) it.len = 0;
     if (it.rows <= 0 || it.tile * (uint64_t)tile_rows >= (uint64_t)it.rows * a.group) return false;
     const uint32_t all = (uint32_t)it.rows * a.group;
     it.r0 = it.tile * tile_rows;
@@ -634,14 +642,17 @@ __device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, cons
     return true;
 }
 
-/* a workgroup's split of an item: its four waves a quarter of the steps each, joined over LDS; the sums to their rows where there is one split, else to a.part */
+/* a workgroup's split of an item, of its rows from s0 on: its four waves a quarter of the steps each, joined over LDS; the sums to their rows where there is one split, else to a.part */
 template <int DP, int F16, int NT, bool HELD>
-__device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, const kv_item& it, const uint32_t split, float* lds, bool& gone)
+__device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, const kv_item& it, const uint32_t s0, const uint32_t split, float* lds, bool& gone)
 {
     using namespace bam;
     constexpr uint32_t R = 16 * NT;
     const uint32_t lane = bam::lane(), wave = threadIdx.x / 64u, row = lane & 15u, grp = lane >> 4, D = g.dim;
-    const kv_span sp = span_of(a, it.len, it.rows, it.r0, it.r1);
+    const uint32_t s1 = s0 + R < it.r1 ? s0 + R : it.r1;
+    kv_span sp = span_of(a, s.width << g.tokens_log, it.len, it.rows, it.r0, it.r1);                     /* the item's splits, */
+    sp.first_pos = it.len - it.rows + (int32_t)(s0 / a.group);                  /* as these rows see them */
+    sp.last_pos = it.len - it.rows + (int32_t)((s1 - 1) / a.group);
     uint32_t v0 = split * a.steps, v1 = v0 + a.steps;
     if (v1 > sp.n_steps || split + 1 == a.splits) v1 = sp.n_steps;              /* the last takes what is beyond the length that was announced */
     if (v0 > v1) v0 = v1;
@@ -655,8 +666,8 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
     float m[NT], l[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const uint32_t r = it.r0 + n * 16u + row;
-        const bool has = r < it.r1;
+        const uint32_t r = s0 + n * 16u + row;
+        const bool has = r < s1;
         const uint32_t tok = has ? r / a.group : 0u, h = it.head * a.group + (has ? r % a.group : 0u);
         pos[n] = has ? it.len - it.rows + (int32_t)tok : -1;
         const uint16_t* const from = a.q + (int64_t)(it.start + (int32_t)tok) * a.q_row + (int64_t)h * a.q_head;
@@ -710,7 +721,7 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
     gone = (bad & 2u) != 0;
     count_accesses(g, n_access, n_hit);
     if (!HELD && (bad & 1u)) return false;
-    const uint32_t n_rows = it.r1 - it.r0;
+    const uint32_t n_rows = s1 - s0;
     for (uint32_t x = threadIdx.x; x < n_rows * (DP / 8u); x += 256u) {
         const uint32_t r = x / (DP / 8u), c = x % (DP / 8u) * 8u;
         if (c >= D) continue;
@@ -721,14 +732,14 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
         if (gone) den = __builtin_nanf("");
         f32x4 lo = *(const f32x4*)(os + r * DP + c), hi = *(const f32x4*)(os + r * DP + c + 4);
         if (a.splits > 1) {
-            const uint64_t at = ((uint64_t)item * R + r) * a.splits + split;
+            const uint64_t at = ((uint64_t)item * a.tile_rows + (s0 - it.r0) + r) * a.splits + split;
             *(f32x4*)(a.part + at * D + c) = lo;
             *(f32x4*)(a.part + at * D + c + 4) = hi;
             if (c == 0) { a.part_m[at] = top; a.part_l[at] = den; }
         } else {
             /* a row that sees no token is zero */
             const float inv = top == -INFINITY && !gone ? 0.0f : 1.0f / den;
-            const uint32_t rr = it.r0 + r, tok = (uint32_t)it.start + rr / a.group, h = it.head * a.group + rr % a.group;
+            const uint32_t rr = s0 + r, tok = (uint32_t)it.start + rr / a.group, h = it.head * a.group + rr % a.group;
             const u32x4 y = {to16<F16>(lo[0] * inv, lo[1] * inv), to16<F16>(lo[2] * inv, lo[3] * inv), to16<F16>(hi[0] * inv, hi[1] * inv), to16<F16>(hi[2] * inv, hi[3] * inv)};
             *(u32x4*)(a.out + ((uint64_t)tok * a.q_heads + h) * D + c) = y;
             if (a.lse && c == 0) a.lse[(uint64_t)tok * a.q_heads + h] = (top + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
@@ -745,8 +756,289 @@ __global__ __launch_bounds__(256) void k_kv_attend(const kv_geom g, const kv_seq
     const uint32_t item = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
     kv_item it;
     bool gone = false, ok = true;
-    if (item_of(g, s, a, item, 16 * NT, it)) ok = kv_split<DP, F16, NT, false>(g, s, a, item, it, split, lds, gone);
+    if (item_of(g, s, a, item, it)) ok = kv_split<DP, F16, NT, false>(g, s, a, item, it, it.r0, split, lds, gone);
     if (threadIdx.x == 0) a.left[blockIdx.x] = ok ? 0 : 1;
+}
+
+// ---- many rows: tiles of rows against tiles of tokens in LDS ----
+/* 16 bytes a lane from memory to LDS, to lds + 16 x lane; counted by the wave's memory counter, and by nobody else: wait for all of them before a barrier */
+__device__ __forceinline__ void to_lds(const uint8_t* from, const uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(from) : "memory");
+}
+template <int F16> __device__ __forceinline__ f32x16 mma32(const u32x4 a, const u32x4 b, const f32x16 c)
+{
+    if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <int DP> constexpr uint32_t tile_tokens() { return DP > 128 ? 32 : 64; }
+template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>() * DP * 2; }
+
+/*
+ * NW waves of 32 rows each, all against the same tokens, KT at a time, which the waves bring into LDS together while they work on the tile before (two
+ * buffers, one barrier to a tile).  Pages lie in LDS as they lie in the cache, piece by piece.  Lane l: row l % 32 of its wave, and of each 16 tokens
+ * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 32 blocks as in kv_steps; the next chunk's descriptors are looked at
+ * while this one is gone through.
+ */
+template <int DP, int F16, int NW>
+__global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, const kv_seqs s, const kv_att a)
+{
+    using namespace bam;
+    extern __shared__ float lds[];
+    constexpr uint32_t KT = tile_tokens<DP>(), HALF = KT * DP * 2, PIECES = KT * DP / 8;      /* bytes and pieces of a tile's keys, and of its values */
+    constexpr uint32_t INSTR = PIECES / 64;
+    const uint32_t lane = bam::lane(), wave = first(threadIdx.x / 64u), row = lane & 31u, half = lane >> 5, D = g.dim, T = g.tokens;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    /* the tiles with the most tokens to look at first */
+    const uint32_t per_seq = a.tiles * g.heads, work = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    const uint32_t item = work / per_seq * per_seq + (a.tiles - 1u - work % per_seq / g.heads) * g.heads + work % g.heads;
+    kv_item it;
+    if (!item_of(g, s, a, item, it)) { if (threadIdx.x == 0) a.left[(uint64_t)item * a.splits + split] = 0; return; }
+    const kv_span sp = span_of(a, s.width << g.tokens_log, it.len, it.rows, it.r0, it.r1);
+    uint32_t v0 = split * a.steps, v1 = v0 + a.steps;
+    if (v1 > sp.n_steps || split + 1 == a.splits) v1 = sp.n_steps;
+    if (v0 > v1) v0 = v1;
+    if (D < DP) {                                /* what no piece is loaded for is zero */
+        for (uint32_t x = threadIdx.x; x < tile_lds<DP>() / 16u; x += 64u * NW) ((u32x4*)lds)[x] = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    /* this lane's row, and the positions of the wave's rows */
+    const uint32_t w0 = it.r0 + wave * 32u, w1 = w0 + 32u < it.r1 ? w0 + 32u : it.r1;
+    const bool idle = w0 >= it.r1;
+    const uint32_t r = w0 + row;
+    const bool has = r < it.r1;
+    const uint32_t tok = has ? r / a.group : 0u, head = it.head * a.group + (has ? r % a.group : 0u);
+    const int32_t p0 = it.len - it.rows, pos = has ? p0 + (int32_t)tok : -1;
+    const int32_t first_pos = idle ? -1 : p0 + (int32_t)(w0 / a.group), last_pos = idle ? -1 : p0 + (int32_t)((w1 - 1) / a.group);
+    /* a negative scale goes into the sign of the queries: the largest score is then the largest product */
+    const float c = fmaxf(fabsf(a.scale), 1e-30f);
+    const uint32_t flip = a.scale < 0 ? 0x80008000u : 0u;
+    u32x4 q[DP / 16];
+    {
+        const uint16_t* const from = a.q + (int64_t)(it.start + (int32_t)tok) * a.q_row + (int64_t)head * a.q_head;
+#pragma unroll
+        for (uint32_t j = 0; j < DP / 16; j++) {
+            q[j] = u32x4{0, 0, 0, 0};
+            if (has && (2u * j + half) * 8u < D) q[j] = load_piece(from + (2u * j + half) * 8u, a.aligned) ^ flip;
+        }
+    }
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (uint32_t i = 0; i < DP / 32; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[i][e] = 0;
+    float m = -INFINITY, l = 0;
+    bool ok = true;
+    uint32_t n_access = 0;
+
+    /* the chunk that tiles are loaded from, and the one after it */
+    uint32_t b_first = 0, t_next = 0, t_end = 0, holes = 0, slot = 0, v = v0;
+    uint64_t page = 0, seen = 0;
+    bool need = false;
+    uint32_t nb_first = 0, nt_first = 0, nt_end = 0, nholes = 0;
+    uint64_t npage = 0, nseen = 0;
+    int32_t nblock = -1;
+    bool nasked = false, nneed = false;
+    uint32_t stage = 3;                          /* of the chunk after: 0 nothing, 1 its blocks, 2 its descriptors are on their way, 3 there is none */
+    auto next_blocks = [&]() {
+        if (v >= v1) { stage = 3; return; }
+        const bool front = v < sp.front;
+        nt_first = front ? v * 32u : sp.base + (v - sp.front) * 32u;
+        const uint32_t run = (front && sp.front < v1 ? sp.front : v1) - v;
+        nb_first = nt_first >> g.tokens_log;
+        nt_end = (nb_first + 32u) << g.tokens_log;
+        if (nt_first + run * 32u < nt_end) nt_end = nt_first + run * 32u;
+        const uint32_t blk = nb_first + (lane & 31u);
+        nasked = (blk << g.tokens_log) < (nt_end < sp.len ? nt_end : sp.len);
+        nblock = nasked && blk < s.width ? s.table[(int64_t)it.seq * s.stride + blk] : -1;
+        v += (nt_end - nt_first) / 32u;
+        stage = 1;
+    };
+    auto next_looks = [&]() {
+        nneed = nblock >= 0 && (uint64_t)nblock < g.n_blocks;
+        npage = g.first_page + ((uint64_t)(uint32_t)nblock * g.heads + it.head) * 2u + half;
+        if (nneed) nseen = __hip_atomic_load((const uint64_t*)(g.pages + npage), __ATOMIC_RELAXED, BAM_AGENT);
+        stage = 2;
+    };
+    auto look_again = [&]() {
+        uint64_t now = seen;
+        if (need) now = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
+        if (ballot(need && ((seen ^ now) & 0xFFFFFFFFC0000000ull) != 0)) ok = false;
+    };
+    auto enter_next = [&]() {
+        b_first = nb_first; t_next = nt_first; t_end = nt_end; need = nneed; page = npage; seen = nseen;
+        holes = (uint32_t)ballot(nasked && !nneed);
+        if (ballot(need && ((uint32_t)seen >> (CNT_SHIFT + 1)) != V_NB)) ok = false;
+        slot = need ? (uint32_t)(seen >> 32) & BAM_SLOT_MASK : 0u;
+        n_access += popc(ballot(need));
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        stage = 0;
+    };
+    /* the tile from t_next on into a buffer */
+    uint32_t at_first = 0, at_end = 0, at_holes = 0, at_block = 0;          /* of the tile that is on its way */
+    auto load_tile = [&](const uint32_t buf) {
+        const uint32_t to = lds0 + buf * 2u * HALF;
+#pragma unroll
+        for (uint32_t x = 0; x < (INSTR + NW - 1) / NW; x++) {
+            const uint32_t n = x * NW + wave;
+            if (INSTR % NW && n >= INSTR) break;
+            const uint32_t piece = n * 64u + lane;
+            {
+                const uint32_t t = t_next + piece % KT, ch = piece / KT, b = (t >> g.tokens_log) - b_first;
+                const uint32_t sl = bam::shfl(slot, b & 31u);
+                if (ch * 8u < D) to_lds(g.base + ((uint64_t)sl << g.page_log) + ((uint64_t)ch * T + (t & (T - 1u))) * 16u, to + n * 1024u);
+            }
+            {
+                const uint32_t d = piece % DP, t = t_next + piece / DP * 8u, b = (t >> g.tokens_log) - b_first;
+                const uint32_t sl = bam::shfl(slot, 32u + (b & 31u));
+                if (d < D) to_lds(g.base + ((uint64_t)sl << g.page_log) + ((uint64_t)((t & (T - 1u)) >> 3) * D + d) * 16u, to + HALF + n * 1024u);
+            }
+        }
+        at_first = t_next; at_end = t_end; at_holes = holes; at_block = b_first;
+        t_next += KT;
+    };
+    next_blocks();
+    bool more = stage == 1;
+    if (more) { next_looks(); enter_next(); load_tile(0); }
+    /* K's row of this lane: of the 32 tokens, the one that puts the scores of tokens 8 half .. + 7 of each 16 into its accumulators */
+    const uint32_t k_row = (row & 0x13u) | ((row & 4u) << 1) | ((row & 8u) >> 1);
+    for (uint32_t buf = 0; more; buf ^= 1u) {
+        fence_meta();                            /* this wave's part of the tile is in LDS, */
+        __syncthreads();                         /* and everybody's; and everybody has done with the buffer that is loaded next */
+        const uint32_t t0 = at_first, t_lim = at_end, t_holes = at_holes, t_block = at_block;
+        if (stage == 1) next_looks();
+        else if (stage == 0) next_blocks();
+        more = true;
+        if (t_next >= t_end) {
+            if (stage == 1) next_looks();
+            if (stage == 2) { look_again(); enter_next(); }
+            else more = false;
+        }
+        if (more) load_tile(buf ^ 1u);
+        if (idle || (int64_t)t0 > last_pos) continue;
+        const uint8_t* const keys = (const uint8_t*)lds + buf * 2u * HALF;
+        const uint8_t* const values = keys + HALF;
+        f32x16 x[KT / 32];
+#pragma unroll
+        for (uint32_t mt = 0; mt < KT / 32; mt++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[mt][e] = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < DP / 16; j++)
+#pragma unroll
+            for (uint32_t mt = 0; mt < KT / 32; mt++) x[mt] = mma32<F16>(*(const u32x4*)(keys + ((2u * j + half) * KT + 32u * mt + k_row) * 16u), q[j], x[mt]);
+        const bool whole = !t_holes && (int64_t)t0 + KT - 1 <= first_pos && t0 + KT <= t_lim && (!a.window || (int64_t)last_pos - t0 < a.window || t0 + KT <= a.sinks);
+        uint32_t sees = 0xffffffffu;             /* of each 16 tokens, which of its eight the row sees */
+        if (!whole) {
+            const int32_t lim = (int32_t)t_lim - 1;
+            sees = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < KT / 16; k++) {
+                const uint32_t tt = t0 + k * 16u + half * 8u;
+                if ((t_holes >> (((tt >> g.tokens_log) - t_block) & 31u)) & 1u) continue;
+                sees |= seen_of_eight((int32_t)tt, pos < lim ? pos : lim, low_of(a, pos), (int32_t)a.sinks) << (8u * k);
+            }
+#pragma unroll
+            for (uint32_t mt = 0; mt < KT / 32; mt++)
+#pragma unroll
+                for (uint32_t e = 0; e < 16; e++) x[mt][e] = (sees >> (16u * mt + e)) & 1u ? x[mt][e] : -INFINITY;
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (uint32_t mt = 0; mt < KT / 32; mt++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = fmaxf(top, x[mt][e]);
+        {
+            float other = top;
+            swap_halves(top, other);
+            top = fmaxf(top, other);
+        }
+        /* the sums are moved to a larger maximum only where it is larger by 2^8 or more: weights of up to 2^8 lose nothing */
+        if (ballot((top - m) * c > 8.0f || m == -INFINITY && top != -INFINITY)) {
+            const float larger = fmaxf(top, m);
+            const float by = larger == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - larger) * c);
+            l *= by;
+#pragma unroll
+            for (uint32_t i = 0; i < DP / 32; i++) o[i] *= by;
+            m = larger;
+        }
+        const float mc = m == -INFINITY ? 0.0f : -m * c;
+        u32x4 p[KT / 16];
+#pragma unroll
+        for (uint32_t k = 0; k < KT / 16; k++)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 1][(k & 1u) * 8u + 2u * e], c, mc)), y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 1][(k & 1u) * 8u + 2u * e + 1u], c, mc));
+                l += y0 + y1;
+                p[k][e] = to16<F16>(y0, y1);
+            }
+        /* values of tokens that a row does not see meet zeros of P: that leaves them out unless there is an infinity or NaN among them */
+        bool odd = false;
+        if (!whole) {
+#pragma unroll 1
+            for (uint32_t n = lane; n < PIECES; n += 64u) {
+                const u32x4 z = *(const u32x4*)(values + n * 16u);
+                odd |= odd16<F16>(z[0]) || odd16<F16>(z[1]) || odd16<F16>(z[2]) || odd16<F16>(z[3]);
+            }
+        }
+        if (__builtin_expect(ballot(odd) == 0, 1)) {
+#pragma unroll
+            for (uint32_t k = 0; k < KT / 16; k++)
+#pragma unroll
+                for (uint32_t i = 0; i < DP / 32; i++) o[i] = mma32<F16>(*(const u32x4*)(values + ((2u * k + half) * DP + 32u * i + row) * 16u), p[k], o[i]);
+        } else {
+            /* row by row, the values that the row does not see as zeros */
+#pragma unroll 1
+            for (uint32_t n = 0; n < 32; n++) {
+                const uint32_t sn = bam::shfl(sees, (lane & 32u) + n);
+#pragma unroll
+                for (uint32_t k = 0; k < KT / 16; k++) {
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (uint32_t i = 0; i < DP / 32; i++) {
+                        const f32x16 with = mma32<F16>(only(*(const u32x4*)(values + ((2u * k + half) * DP + 32u * i + row) * 16u), sn >> (8u * k)), p[k], o[i]);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[i][e] = row == n ? with[e] : o[i][e];
+                    }
+                }
+            }
+        }
+    }
+    fence_meta();
+    look_again();
+    if (__syncthreads_or(!ok)) { if (threadIdx.x == 0) a.left[(uint64_t)item * a.splits + split] = 1; return; }
+    if (threadIdx.x == 0) a.left[(uint64_t)item * a.splits + split] = 0;
+    if (wave == 0) count_accesses(g, lane == 0 ? n_access : 0u, lane == 0 ? n_access : 0u);
+    {
+        float other = l;
+        swap_halves(l, other);
+        l += other;
+    }
+    if (!has) return;
+    /* lane: numbers 8i + 4 half .. + 3 of its row */
+    if (a.splits > 1) {
+        const uint64_t at = ((uint64_t)item * a.tile_rows + (r - it.r0)) * a.splits + split;
+#pragma unroll
+        for (uint32_t i = 0; i < DP / 8; i++) {
+            const uint32_t d = 8u * i + 4u * half;
+            if (d < D) *(f32x4*)(a.part + at * D + d) = f32x4{o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2], o[i / 4][i % 4 * 4 + 3]};
+        }
+        if (half == 0) { a.part_m[at] = m * c; a.part_l[at] = l; }
+        return;
+    }
+    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    uint16_t* const to = a.out + ((uint64_t)(it.start + (int32_t)tok) * a.q_heads + head) * D;
+#pragma unroll
+    for (uint32_t i = 0; i < DP / 8; i++) {
+        const uint32_t d = 8u * i + 4u * half;
+        if (d < D) {
+            uint2 y;
+            y.x = to16<F16>(o[i / 4][i % 4 * 4] * inv, o[i / 4][i % 4 * 4 + 1] * inv);
+            y.y = to16<F16>(o[i / 4][i % 4 * 4 + 2] * inv, o[i / 4][i % 4 * 4 + 3] * inv);
+            *(uint2*)(to + d) = y;
+        }
+    }
+    if (a.lse && half == 0) a.lse[(uint64_t)(it.start + (int32_t)tok) * a.q_heads + head] = (m * c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 /*
@@ -764,14 +1056,15 @@ __global__ __launch_bounds__(256) void k_kv_finish(const kv_geom g, const kv_seq
         const bool any = __syncthreads_or(mine);
         if (!any && a.splits == 1) continue;
         kv_item it;
-        if (!item_of(g, s, a, item, R, it)) continue;
+        if (!item_of(g, s, a, item, it)) continue;
         if (any) {
             for (uint32_t k = 0; k < a.splits; k++)
-                if (a.left[(uint64_t)item * a.splits + k]) {
-                    bool gone = false;
-                    kv_split<DP, F16, NT, true>(g, s, a, item, it, k, lds, gone);
-                    __syncthreads();
-                }
+                if (a.left[(uint64_t)item * a.splits + k])
+                    for (uint32_t s0 = it.r0; s0 < it.r1; s0 += R) {
+                        bool gone = false;
+                        kv_split<DP, F16, NT, true>(g, s, a, item, it, s0, k, lds, gone);
+                        __syncthreads();
+                    }
             __threadfence();
             __syncthreads();
         }
@@ -779,7 +1072,7 @@ __global__ __launch_bounds__(256) void k_kv_finish(const kv_geom g, const kv_seq
         const uint32_t n_rows = it.r1 - it.r0;
         for (uint32_t x = threadIdx.x; x < n_rows * (D / 4u); x += 256u) {
             const uint32_t r = x / (D / 4u), c = x % (D / 4u) * 4u;
-            const uint64_t at = ((uint64_t)item * R + r) * a.splits;
+            const uint64_t at = ((uint64_t)item * a.tile_rows + r) * a.splits;
             float top = -INFINITY, den = 0;
             for (uint32_t k = 0; k < a.splits; k++) top = fmaxf(top, a.part_m[at + k]);
             const float use = top == -INFINITY ? 0.0f : top;
@@ -802,7 +1095,7 @@ __global__ __launch_bounds__(256) void k_kv_finish(const kv_geom g, const kv_seq
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-struct kv_plan { uint32_t nt, tiles, splits, steps; uint64_t items, left_at, m_at, l_at, part_at, bytes; };
+struct kv_plan { uint32_t nt, waves, rows, tiles, splits, steps; uint64_t items, left_at, m_at, l_at, part_at, bytes; };
 
 /* steps of 32 tokens that a tile of `rows` rows can have to look at, of sequences of up to max_len tokens */
 uint64_t most_steps(const uint64_t max_len, const uint64_t new_tokens, const uint32_t window, const uint32_t sinks)
@@ -817,12 +1110,14 @@ kv_plan plan_of(const bam_kv_t* kv, const uint64_t n_seqs, const uint64_t max_ne
 {
     kv_plan p{};
     const uint64_t group = q_heads / kv->g.heads, rows = max_new * group;
-    p.nt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const uint64_t R = 16ull * p.nt;
+    p.nt = rows <= 16 ? 1 : 2;
+    p.waves = rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 128 || kv->g.dim > 128 ? 4 : 8;
+    p.rows = p.waves ? 32 * p.waves : 16 * p.nt;
+    const uint64_t R = p.rows;
     p.tiles = (uint32_t)((rows + R - 1) / R);
     p.items = n_seqs * p.tiles * kv->g.heads;
     const uint64_t steps = most_steps(max_len, (R + group - 1) / group + 1, window, sinks);
-    uint64_t splits = (1024 + p.items - 1) / p.items;                 /* four workgroups to a compute unit */
+    uint64_t splits = p.waves ? 4096 / p.waves / p.items : (1024 + p.items - 1) / p.items;
     const uint64_t most = (steps + 15) / 16;                          /* no fewer than four steps to a wave */
     if (splits > most) splits = most;
     if (splits > 256) splits = 256;
@@ -856,8 +1151,14 @@ template <typename K> void allow_lds(K kernel, const uint32_t bytes)
 template <int DP, int F16, int NT>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan& p, hipStream_t st)
 {
-    constexpr uint32_t lds = split_lds<DP, NT>();
-    static const bool once = [] { allow_lds(k_kv_attend<DP, F16, NT>, lds); allow_lds(k_kv_finish<DP, F16, NT>, lds); return true; }();
+    constexpr uint32_t lds = split_lds<DP, NT>(), lds_tiles = tile_lds<DP>();
+    constexpr int MOST = DP > 128 ? 4 : 8;
+    static const bool once = [] {
+        allow_lds(k_kv_attend<DP, F16, NT>, lds);
+        allow_lds(k_kv_finish<DP, F16, NT>, lds);
+        if constexpr (NT == 2) { allow_lds(k_kv_attend_tiles<DP, F16, 2>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, MOST>, lds_tiles); }
+        return true;
+    }();
     (void)once;
     /* what all waves of the second launch hold at a time stays under half the cache, or they wait for each other's slots */
     const uint32_t least = kv->g.tokens < 32 ? 32 / kv->g.tokens : 1;
@@ -866,16 +1167,22 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     if (groups * 4 * 2 * least > half) groups = half / (8 * least);
     uint64_t chunk = half / (groups * 8) / least * least;
     a.chunk = (uint32_t)(chunk > 32 ? 32 : chunk);
-    if (kv->unheld) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), dim3((uint32_t)(p.items * p.splits)), dim3(256), lds, st, kv->g, s, a);
-    else hipLaunchKernelGGL(k_kv_all_left, dim3((uint32_t)((p.items * p.splits + 255) / 256)), dim3(256), 0, st, a.left, p.items * p.splits);
+    a.tile_rows = p.rows;
+    const dim3 grid((uint32_t)(p.items * p.splits));
+    if (!kv->unheld) hipLaunchKernelGGL(k_kv_all_left, dim3((uint32_t)((p.items * p.splits + 255) / 256)), dim3(256), 0, st, a.left, p.items * p.splits);
+    else if (!p.waves) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
+    else if constexpr (NT == 2) {
+        if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
+        else if (p.waves == 4) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+        else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, MOST>), grid, dim3(64 * MOST), lds_tiles, st, kv->g, s, a);
+    }
     hipLaunchKernelGGL((k_kv_finish<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
 }
 template <int DP, int F16>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st)
 {
     if (p.nt == 1) launch_attend<DP, F16, 1>(kv, s, a, p, st);
-    else if (p.nt == 2) launch_attend<DP, F16, 2>(kv, s, a, p, st);
-    else launch_attend<DP, F16, 4>(kv, s, a, p, st);
+    else launch_attend<DP, F16, 2>(kv, s, a, p, st);
 }
 template <int F16>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st)
@@ -909,7 +1216,7 @@ int bad_seqs(const char* who, const bam_kv_t* kv, uint64_t n_seqs, uint64_t n_ro
     if (!starts && n_seqs != n_rows) return fail(EINVAL, std::string(who) + ": without starts every sequence has one new token");
     if (!n_rows) return 0;
     if (width == 0 || width > 0x7fffffffull || stride < 0) return fail(EINVAL, std::string(who) + ": table of no width, or with its rows in reverse");
-    if (width > 0x7fffffffull >> kv->g.tokens_log) return fail(EINVAL, std::string(who) + ": the table has room for more positions than 31 bits count");
+    if (width > 0x7ffffc00ull >> kv->g.tokens_log) return fail(EINVAL, std::string(who) + ": the table has room for more positions than 31 bits count");
     return 0;
 }
 bool whole_pieces(const void* p, int64_t row, int64_t head) { return ((uintptr_t)p & 15) == 0 && row % 8 == 0 && head % 8 == 0; }
