@@ -85,13 +85,9 @@ template <int F16> __device__ __forceinline__ float from16(const uint32_t x)
 }
 template <int F16> __device__ __forceinline__ uint32_t to16(const float lo, const float hi)
 {
-    if constexpr (F16) {
-        const _Float16 a = (_Float16)lo, b = (_Float16)hi;
-        return (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
-    } else {
-        const __bf16 a = (__bf16)lo, b = (__bf16)hi;
-        return (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
-    }
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), _Float16 __attribute__((ext_vector_type(2)))));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), __bf16 __attribute__((ext_vector_type(2)))));
 }
 __device__ __forceinline__ u32x4 load_piece(const uint16_t* p, const bool aligned)
 {
@@ -827,7 +823,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
     for (uint32_t i = 0; i < DP / 32; i++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[i][e] = 0;
-    float m = -INFINITY, l = 0;
+    float m = -INFINITY, l = 0, l1 = 0;
     bool ok = true;
     uint32_t n_access = 0;
 
@@ -918,20 +914,44 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
         if (idle || (int64_t)t0 > last_pos) continue;
         const uint8_t* const keys = (const uint8_t*)lds + buf * 2u * HALF;
         const uint8_t* const values = keys + HALF;
+        /*
+         * The operands from LDS are read eight ahead of the products that take them, and the order is held (sched_barrier): left to itself the compiler reads each right before
+         * its product and waits for it, a hundred cycles for every 32 of the matrix unit.
+         */
+        constexpr uint32_t NK = DP / 16 * (KT / 32), NV = DP / 32 * (KT / 16);
+        auto key_piece = [&](const uint32_t n) { return *(const u32x4*)(keys + ((2u * (n / (KT / 32)) + half) * KT + 32u * (n % (KT / 32)) + k_row) * 16u); };
+        auto value_piece = [&](const uint32_t n) { return *(const u32x4*)(values + ((2u * (n / (DP / 32)) + half) * DP + 32u * (n % (DP / 32)) + row) * 16u); };
         f32x16 x[KT / 32];
 #pragma unroll
         for (uint32_t mt = 0; mt < KT / 32; mt++)
 #pragma unroll
             for (int e = 0; e < 16; e++) x[mt][e] = 0;
+        u32x4 f[8];
 #pragma unroll
-        for (uint32_t j = 0; j < DP / 16; j++)
+        for (uint32_t n = 0; n < 8; n++) f[n] = key_piece(n);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (uint32_t mt = 0; mt < KT / 32; mt++) x[mt] = mma32<F16>(*(const u32x4*)(keys + ((2u * j + half) * KT + 32u * mt + k_row) * 16u), q[j], x[mt]);
+        for (uint32_t n = 0; n < NK; n += 4) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) x[(n + e) % (KT / 32)] = mma32<F16>(f[(n + e) % 8], q[(n + e) / (KT / 32)], x[(n + e) % (KT / 32)]);
+            /* behind the last keys, the first values */
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) f[(n + e) % 8] = n + 8 < NK ? key_piece(n + 8 + e) : value_piece(n + 8 + e - NK);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         const bool whole = !t_holes && (int64_t)t0 + KT - 1 <= first_pos && t0 + KT <= t_lim && (!a.window || (int64_t)last_pos - t0 < a.window || t0 + KT <= a.sinks);
-        uint32_t sees = 0xffffffffu;             /* of each 16 tokens, which of its eight the row sees */
         if (!whole) {
+            /* values of tokens that a row does not see meet zeros of P.  That leaves them out unless there is an infinity or NaN among them: then
+             * the split is left to the launch that takes the rows one by one there (kv_steps) */
+            bool odd = false;
+#pragma unroll 1
+            for (uint32_t n = lane; n < PIECES; n += 64u) {
+                const u32x4 z = *(const u32x4*)(values + n * 16u);
+                odd |= odd16<F16>(z[0]) || odd16<F16>(z[1]) || odd16<F16>(z[2]) || odd16<F16>(z[3]);
+            }
+            if (ballot(odd)) ok = false;
+            uint32_t sees = 0;                   /* of each 16 tokens, which of its eight the row sees */
             const int32_t lim = (int32_t)t_lim - 1;
-            sees = 0;
 #pragma unroll
             for (uint32_t k = 0; k < KT / 16; k++) {
                 const uint32_t tt = t0 + k * 16u + half * 8u;
@@ -958,6 +978,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
             const float larger = fmaxf(top, m);
             const float by = larger == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - larger) * c);
             l *= by;
+            l1 *= by;
 #pragma unroll
             for (uint32_t i = 0; i < DP / 32; i++) o[i] *= by;
             m = larger;
@@ -965,43 +986,22 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
         const float mc = m == -INFINITY ? 0.0f : -m * c;
         u32x4 p[KT / 16];
 #pragma unroll
-        for (uint32_t k = 0; k < KT / 16; k++)
+        for (uint32_t k = 0; k < KT / 16; k++) {
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) {
                 const float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 1][(k & 1u) * 8u + 2u * e], c, mc)), y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[k >> 1][(k & 1u) * 8u + 2u * e + 1u], c, mc));
-                l += y0 + y1;
+                l += y0;
+                l1 += y1;
                 p[k][e] = to16<F16>(y0, y1);
             }
-        /* values of tokens that a row does not see meet zeros of P: that leaves them out unless there is an infinity or NaN among them */
-        bool odd = false;
-        if (!whole) {
-#pragma unroll 1
-            for (uint32_t n = lane; n < PIECES; n += 64u) {
-                const u32x4 z = *(const u32x4*)(values + n * 16u);
-                odd |= odd16<F16>(z[0]) || odd16<F16>(z[1]) || odd16<F16>(z[2]) || odd16<F16>(z[3]);
+            /* the weights of the next sixteen tokens are worked out while the matrix unit has these */
+#pragma unroll
+            for (uint32_t i = 0; i < DP / 32; i++) {
+                const uint32_t n = k * (DP / 32) + i;
+                o[i] = mma32<F16>(f[n % 8], p[k], o[i]);
+                if (n + 8 < NV) f[n % 8] = value_piece(n + 8);
             }
-        }
-        if (__builtin_expect(ballot(odd) == 0, 1)) {
-#pragma unroll
-            for (uint32_t k = 0; k < KT / 16; k++)
-#pragma unroll
-                for (uint32_t i = 0; i < DP / 32; i++) o[i] = mma32<F16>(*(const u32x4*)(values + ((2u * k + half) * DP + 32u * i + row) * 16u), p[k], o[i]);
-        } else {
-            /* row by row, the values that the row does not see as zeros */
-#pragma unroll 1
-            for (uint32_t n = 0; n < 32; n++) {
-                const uint32_t sn = bam::shfl(sees, (lane & 32u) + n);
-#pragma unroll
-                for (uint32_t k = 0; k < KT / 16; k++) {
-                    asm volatile("" ::: "memory");
-#pragma unroll
-                    for (uint32_t i = 0; i < DP / 32; i++) {
-                        const f32x16 with = mma32<F16>(only(*(const u32x4*)(values + ((2u * k + half) * DP + 32u * i + row) * 16u), sn >> (8u * k)), p[k], o[i]);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) o[i][e] = row == n ? with[e] : o[i][e];
-                    }
-                }
-            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     fence_meta();
@@ -1010,6 +1010,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
     if (threadIdx.x == 0) a.left[(uint64_t)item * a.splits + split] = 0;
     if (wave == 0) count_accesses(g, lane == 0 ? n_access : 0u, lane == 0 ? n_access : 0u);
     {
+        l += l1;
         float other = l;
         swap_halves(l, other);
         l += other;
