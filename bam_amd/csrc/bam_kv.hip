@@ -400,13 +400,22 @@ template <int F16> __device__ __forceinline__ f32x4 mma(const u32x4 a, const u32
     if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-/*
- * Over the four lanes 16 apart: the halves of the wave, then the rows of sixteen lanes of a half, exchanged between two registers that hold the same.  (Written in
- * asm: from the builtins with the same value for both operands the compiler takes the two results to be the same too.  The two idle cycles are
- * what the exchange needs behind a vector instruction that writes one of its registers.)
- */
-__device__ __forceinline__ void swap_halves(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
-__device__ __forceinline__ void swap_rows(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b)); }
+/* the halves of the wave, or the rows of sixteen lanes of each half, exchanged between two registers that hold the same: then one of them has a lane's own, the other
+ * its partner's.  (The results go through scalars: a bit cast of a vector's element takes its first one, whichever is named.) */
+__device__ __forceinline__ void swap_halves(float& a, float& b)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t x = r[0], y = r[1];
+    a = __builtin_bit_cast(float, x);
+    b = __builtin_bit_cast(float, y);
+}
+__device__ __forceinline__ void swap_rows(float& a, float& b)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    const uint32_t x = r[0], y = r[1];
+    a = __builtin_bit_cast(float, x);
+    b = __builtin_bit_cast(float, y);
+}
 __device__ __forceinline__ float max_of_four(float a)
 {
     float b = a;
@@ -757,10 +766,10 @@ __global__ __launch_bounds__(256) void k_kv_attend(const kv_geom g, const kv_seq
 }
 
 // ---- many rows: tiles of rows against tiles of tokens in LDS ----
-/* 16 bytes a lane from memory to LDS, to lds + 16 x lane; counted by the wave's memory counter, and by nobody else: wait for all of them before a barrier */
-__device__ __forceinline__ void to_lds(const uint8_t* from, const uint32_t lds)
+/* 16 bytes a lane from memory to LDS, from base + at to lds + 16 x lane; counted by the wave's memory counter, and by nobody else: wait for all of them before a barrier */
+__device__ __forceinline__ void to_lds(const uint8_t* base, const uint32_t at, const uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(at), "s"(base) : "memory");
 }
 template <int F16> __device__ __forceinline__ f32x16 mma32(const u32x4 a, const u32x4 b, const f32x16 c)
 {
@@ -777,12 +786,13 @@ template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>
  * while this one is gone through.
  */
 template <int DP, int F16, int NW>
-__global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, const kv_seqs s, const kv_att a)
+__global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(const kv_geom g, const kv_seqs s, const kv_att a)
 {
     using namespace bam;
     extern __shared__ float lds[];
     constexpr uint32_t KT = tile_tokens<DP>(), HALF = KT * DP * 2, PIECES = KT * DP / 8;      /* bytes and pieces of a tile's keys, and of its values */
-    constexpr uint32_t INSTR = PIECES / 64;
+    constexpr uint32_t UNITS = KT / 8 / NW;      /* of eight tokens, that a wave brings in: their keys, then their values, as they lie in their pages */
+    static_assert(UNITS >= 1, "a unit to a wave");
     const uint32_t lane = bam::lane(), wave = first(threadIdx.x / 64u), row = lane & 31u, half = lane >> 5, D = g.dim, T = g.tokens;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     /* the tiles with the most tokens to look at first */
@@ -872,22 +882,20 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
     };
     /* the tile from t_next on into a buffer */
     uint32_t at_first = 0, at_end = 0, at_holes = 0, at_block = 0;          /* of the tile that is on its way */
+    const uint32_t k_lane0 = (lane & 7u) * 16u + (lane >> 3) * T * 16u, k_lane1 = (lane & 7u) * 16u + (lane >> 3 ^ 1u) * T * 16u;
     auto load_tile = [&](const uint32_t buf) {
         const uint32_t to = lds0 + buf * 2u * HALF;
 #pragma unroll
-        for (uint32_t x = 0; x < (INSTR + NW - 1) / NW; x++) {
-            const uint32_t n = x * NW + wave;
-            if (INSTR % NW && n >= INSTR) break;
-            const uint32_t piece = n * 64u + lane;
-            {
-                const uint32_t t = t_next + piece % KT, ch = piece / KT, b = (t >> g.tokens_log) - b_first;
-                const uint32_t sl = bam::shfl(slot, b & 31u);
-                if (ch * 8u < D) to_lds(g.base + ((uint64_t)sl << g.page_log) + ((uint64_t)ch * T + (t & (T - 1u))) * 16u, to + n * 1024u);
-            }
-            {
-                const uint32_t d = piece % DP, t = t_next + piece / DP * 8u, b = (t >> g.tokens_log) - b_first;
-                const uint32_t sl = bam::shfl(slot, 32u + (b & 31u));
-                if (d < D) to_lds(g.base + ((uint64_t)sl << g.page_log) + ((uint64_t)((t & (T - 1u)) >> 3) * D + d) * 16u, to + HALF + n * 1024u);
+        for (uint32_t x = 0; x < UNITS; x++) {
+            const uint32_t u = wave * UNITS + x, t = t_next + 8u * u, b = ((t >> g.tokens_log) - b_first) & 31u, in = t & (T - 1u);
+            const uint8_t* const k_at = g.base + ((uint64_t)bcast(slot, b) << g.page_log) + in * 16u;
+            const uint8_t* const v_at = g.base + ((uint64_t)bcast(slot, 32u + b) << g.page_log) + (in >> 3) * D * 16u;
+#pragma unroll
+            for (uint32_t i = 0; i < DP / 64; i++) {
+                /* odd units with neighbouring pieces exchanged: read by sixteen lanes from two units, they lie in different banks */
+                const uint32_t odd = UNITS % 2 ? u & 1u : x & 1u;
+                if (D == DP || (8u * i + (lane >> 3 ^ odd)) * 8u < D) to_lds(k_at, (odd ? k_lane1 : k_lane0) + i * 128u * T, to + u * DP * 16u + i * 1024u);
+                if (D == DP || 64u * i + lane < D) to_lds(v_at, (64u * i + lane) * 16u, to + HALF + u * DP * 16u + i * 1024u);
             }
         }
         at_first = t_next; at_end = t_end; at_holes = holes; at_block = b_first;
@@ -898,6 +906,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
     if (more) { next_looks(); enter_next(); load_tile(0); }
     /* K's row of this lane: of the 32 tokens, the one that puts the scores of tokens 8 half .. + 7 of each 16 into its accumulators */
     const uint32_t k_row = (row & 0x13u) | ((row & 4u) << 1) | ((row & 8u) >> 1);
+    const uint32_t k_read = (k_row >> 3) * DP * 16u + (k_row & 7u) * 16u + (half ^ (k_row >> 3 & 1u)) * 128u;
     for (uint32_t buf = 0; more; buf ^= 1u) {
         fence_meta();                            /* this wave's part of the tile is in LDS, */
         __syncthreads();                         /* and everybody's; and everybody has done with the buffer that is loaded next */
@@ -911,7 +920,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
             else more = false;
         }
         if (more) load_tile(buf ^ 1u);
-        if (idle || (int64_t)t0 > last_pos) continue;
+        if (idle || (int32_t)t0 > last_pos) continue;
         const uint8_t* const keys = (const uint8_t*)lds + buf * 2u * HALF;
         const uint8_t* const values = keys + HALF;
         /*
@@ -919,7 +928,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
          * its product and waits for it, a hundred cycles for every 32 of the matrix unit.
          */
         constexpr uint32_t NK = DP / 16 * (KT / 32), NV = DP / 32 * (KT / 16);
-        auto key_piece = [&](const uint32_t n) { return *(const u32x4*)(keys + ((2u * (n / (KT / 32)) + half) * KT + 32u * (n % (KT / 32)) + k_row) * 16u); };
+        auto key_piece = [&](const uint32_t n) { return *(const u32x4*)(keys + (n / (KT / 32)) * 256u + (n % (KT / 32)) * (DP * 64u) + k_read); };
         auto value_piece = [&](const uint32_t n) { return *(const u32x4*)(values + ((2u * (n / (DP / 32)) + half) * DP + 32u * (n % (DP / 32)) + row) * 16u); };
         f32x16 x[KT / 32];
 #pragma unroll
@@ -939,7 +948,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
             for (uint32_t e = 0; e < 4; e++) f[(n + e) % 8] = n + 8 < NK ? key_piece(n + 8 + e) : value_piece(n + 8 + e - NK);
             __builtin_amdgcn_sched_barrier(0);
         }
-        const bool whole = !t_holes && (int64_t)t0 + KT - 1 <= first_pos && t0 + KT <= t_lim && (!a.window || (int64_t)last_pos - t0 < a.window || t0 + KT <= a.sinks);
+        const bool whole = !t_holes && (int32_t)(t0 + KT) - 1 <= first_pos && t0 + KT <= t_lim && (!a.window || last_pos - (int32_t)t0 < (int32_t)a.window || t0 + KT <= a.sinks);
         if (!whole) {
             /* values of tokens that a row does not see meet zeros of P.  That leaves them out unless there is an infinity or NaN among them: then
              * the split is left to the launch that takes the rows one by one there (kv_steps) */
@@ -967,7 +976,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv_attend_tiles(const kv_geom g, co
 #pragma unroll
         for (uint32_t mt = 0; mt < KT / 32; mt++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) top = fmaxf(top, x[mt][e]);
+            for (int e = 0; e < 16; e++) top = __builtin_elementwise_maximum(top, x[mt][e]);      /* three operands to an instruction, and no quieting of each */
         {
             float other = top;
             swap_halves(top, other);
@@ -1112,7 +1121,7 @@ kv_plan plan_of(const bam_kv_t* kv, const uint64_t n_seqs, const uint64_t max_ne
     kv_plan p{};
     const uint64_t group = q_heads / kv->g.heads, rows = max_new * group;
     p.nt = rows <= 16 ? 1 : 2;
-    p.waves = rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 128 || kv->g.dim > 128 ? 4 : 8;
+    p.waves = rows <= 32 ? 0 : rows <= 64 ? 2 : 4;
     p.rows = p.waves ? 32 * p.waves : 16 * p.nt;
     const uint64_t R = p.rows;
     p.tiles = (uint32_t)((rows + R - 1) / R);
@@ -1153,11 +1162,10 @@ template <int DP, int F16, int NT>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan& p, hipStream_t st)
 {
     constexpr uint32_t lds = split_lds<DP, NT>(), lds_tiles = tile_lds<DP>();
-    constexpr int MOST = DP > 128 ? 4 : 8;
     static const bool once = [] {
         allow_lds(k_kv_attend<DP, F16, NT>, lds);
         allow_lds(k_kv_finish<DP, F16, NT>, lds);
-        if constexpr (NT == 2) { allow_lds(k_kv_attend_tiles<DP, F16, 2>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, MOST>, lds_tiles); }
+        if constexpr (NT == 2) { allow_lds(k_kv_attend_tiles<DP, F16, 2>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4>, lds_tiles); }
         return true;
     }();
     (void)once;
@@ -1174,8 +1182,7 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     else if (!p.waves) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
     else if constexpr (NT == 2) {
         if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
-        else if (p.waves == 4) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
-        else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, MOST>), grid, dim3(64 * MOST), lds_tiles, st, kv->g, s, a);
+        else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
     }
     hipLaunchKernelGGL((k_kv_finish<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
 }
