@@ -782,10 +782,9 @@ template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>
 /*
  * NW waves of 32 rows each, all against the same tokens, KT at a time, which the waves bring into LDS together while they work on the tile before (two
  * buffers, one barrier to a tile).  Pages lie in LDS as they lie in the cache, piece by piece.  Lane l: row l % 32 of its wave, and of each 16 tokens
- * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 32 blocks as in kv_steps; the next chunk's descriptors are looked at
- * while this one is gone through.
+ * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 64 blocks, as in kv_steps.
  */
-template <int DP, int F16, int NW>
+template <int DP, int F16, int NW, bool EXACT>
 __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(const kv_geom g, const kv_seqs s, const kv_att a)
 {
     using namespace bam;
@@ -793,7 +792,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     constexpr uint32_t KT = tile_tokens<DP>(), HALF = KT * DP * 2, PIECES = KT * DP / 8;      /* bytes and pieces of a tile's keys, and of its values */
     constexpr uint32_t UNITS = KT / 8 / NW;      /* of eight tokens, that a wave brings in: their keys, then their values, as they lie in their pages */
     static_assert(UNITS >= 1, "a unit to a wave");
-    const uint32_t lane = bam::lane(), wave = first(threadIdx.x / 64u), row = lane & 31u, half = lane >> 5, D = g.dim, T = g.tokens;
+    const uint32_t lane = bam::lane(), wave = first(threadIdx.x / 64u), row = lane & 31u, half = lane >> 5, D = EXACT ? DP : g.dim, T = g.tokens;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     /* the tiles with the most tokens to look at first */
     const uint32_t per_seq = a.tiles * g.heads, work = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
@@ -804,7 +803,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     uint32_t v0 = split * a.steps, v1 = v0 + a.steps;
     if (v1 > sp.n_steps || split + 1 == a.splits) v1 = sp.n_steps;
     if (v0 > v1) v0 = v1;
-    if (D < DP) {                                /* what no piece is loaded for is zero */
+    if (!EXACT) {                                /* what no piece is loaded for is zero */
         for (uint32_t x = threadIdx.x; x < tile_lds<DP>() / 16u; x += 64u * NW) ((u32x4*)lds)[x] = u32x4{0, 0, 0, 0};
         __syncthreads();
     }
@@ -837,87 +836,93 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     bool ok = true;
     uint32_t n_access = 0;
 
-    /* the chunk that tiles are loaded from, and the one after it */
-    uint32_t b_first = 0, t_next = 0, t_end = 0, holes = 0, slot = 0, v = v0;
-    uint64_t page = 0, seen = 0;
-    bool need = false;
-    uint32_t nb_first = 0, nt_first = 0, nt_end = 0, nholes = 0;
-    uint64_t npage = 0, nseen = 0;
+    /*
+     * The chunk that tiles are loaded from, a block to a lane, and the blocks of the one after it.  What is loaded here has arrived before the next tile is asked for: the
+     * compiler waits for its own loads by waiting for all that are on their way.
+     */
+    uint32_t b_first = 0, t_next = 0, t_end = 0, k_slot = 0, v_slot = 0, v = v0, nb_first = 0, nt_first = 0, nt_end = 0;
+    uint64_t holes = 0, page = 0, k_seen = 0, v_seen = 0;
     int32_t nblock = -1;
-    bool nasked = false, nneed = false;
-    uint32_t stage = 3;                          /* of the chunk after: 0 nothing, 1 its blocks, 2 its descriptors are on their way, 3 there is none */
+    bool need = false, nasked = false, there = false;      /* there: nblock and the like are those of a chunk to come */
     auto next_blocks = [&]() {
-        if (v >= v1) { stage = 3; return; }
+        there = v < v1;
+        if (!there) return;
         const bool front = v < sp.front;
         nt_first = front ? v * 32u : sp.base + (v - sp.front) * 32u;
         const uint32_t run = (front && sp.front < v1 ? sp.front : v1) - v;
         nb_first = nt_first >> g.tokens_log;
-        nt_end = (nb_first + 32u) << g.tokens_log;
+        nt_end = (nb_first + 64u) << g.tokens_log;
         if (nt_first + run * 32u < nt_end) nt_end = nt_first + run * 32u;
-        const uint32_t blk = nb_first + (lane & 31u);
+        const uint32_t blk = nb_first + lane;
         nasked = (blk << g.tokens_log) < (nt_end < sp.len ? nt_end : sp.len);
-        nblock = nasked && blk < s.width ? s.table[(int64_t)it.seq * s.stride + blk] : -1;
+        nblock = -1;
+        if (nasked && blk < s.width) nblock = s.table[(int64_t)it.seq * s.stride + blk];
+        asm volatile("" : "+v"(nblock));
         v += (nt_end - nt_first) / 32u;
-        stage = 1;
     };
-    auto next_looks = [&]() {
-        nneed = nblock >= 0 && (uint64_t)nblock < g.n_blocks;
-        npage = g.first_page + ((uint64_t)(uint32_t)nblock * g.heads + it.head) * 2u + half;
-        if (nneed) nseen = __hip_atomic_load((const uint64_t*)(g.pages + npage), __ATOMIC_RELAXED, BAM_AGENT);
-        stage = 2;
+    auto look = [&](uint64_t& k, uint64_t& v_) {
+        k = v_ = (uint64_t)VALID;
+        if (need) {
+            k = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
+            v_ = __hip_atomic_load((const uint64_t*)(g.pages + page + 1), __ATOMIC_RELAXED, BAM_AGENT);
+        }
+        asm volatile("" : "+v"(k), "+v"(v_));
     };
     auto look_again = [&]() {
-        uint64_t now = seen;
-        if (need) now = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
-        if (ballot(need && ((seen ^ now) & 0xFFFFFFFFC0000000ull) != 0)) ok = false;
+        uint64_t k, v_;
+        look(k, v_);
+        if (ballot(need && (((k_seen ^ k) | (v_seen ^ v_)) & 0xFFFFFFFFC0000000ull) != 0)) ok = false;
     };
     auto enter_next = [&]() {
-        b_first = nb_first; t_next = nt_first; t_end = nt_end; need = nneed; page = npage; seen = nseen;
-        holes = (uint32_t)ballot(nasked && !nneed);
-        if (ballot(need && ((uint32_t)seen >> (CNT_SHIFT + 1)) != V_NB)) ok = false;
-        slot = need ? (uint32_t)(seen >> 32) & BAM_SLOT_MASK : 0u;
-        n_access += popc(ballot(need));
+        b_first = nb_first; t_next = nt_first; t_end = nt_end;
+        need = nblock >= 0 && (uint64_t)nblock < g.n_blocks;
+        page = g.first_page + ((uint64_t)(uint32_t)nblock * g.heads + it.head) * 2u;
+        holes = ballot(nasked && !need);
+        look(k_seen, v_seen);
+        if (ballot(((uint32_t)k_seen >> (CNT_SHIFT + 1)) != V_NB || ((uint32_t)v_seen >> (CNT_SHIFT + 1)) != V_NB)) ok = false;
+        k_slot = (uint32_t)(k_seen >> 32) & BAM_SLOT_MASK;
+        v_slot = (uint32_t)(v_seen >> 32) & BAM_SLOT_MASK;
+        n_access += 2u * popc(ballot(need));
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        stage = 0;
+        next_blocks();
     };
     /* the tile from t_next on into a buffer */
-    uint32_t at_first = 0, at_end = 0, at_holes = 0, at_block = 0;          /* of the tile that is on its way */
+    uint32_t at_first = 0, at_end = 0, at_block = 0;          /* of the tile that is on its way */
+    uint64_t at_holes = 0;
     const uint32_t k_lane0 = (lane & 7u) * 16u + (lane >> 3) * T * 16u, k_lane1 = (lane & 7u) * 16u + (lane >> 3 ^ 1u) * T * 16u;
     auto load_tile = [&](const uint32_t buf) {
         const uint32_t to = lds0 + buf * 2u * HALF;
 #pragma unroll
         for (uint32_t x = 0; x < UNITS; x++) {
-            const uint32_t u = wave * UNITS + x, t = t_next + 8u * u, b = ((t >> g.tokens_log) - b_first) & 31u, in = t & (T - 1u);
-            const uint8_t* const k_at = g.base + ((uint64_t)bcast(slot, b) << g.page_log) + in * 16u;
-            const uint8_t* const v_at = g.base + ((uint64_t)bcast(slot, 32u + b) << g.page_log) + (in >> 3) * D * 16u;
+            const uint32_t u = wave * UNITS + x, t = t_next + 8u * u, b = ((t >> g.tokens_log) - b_first) & 63u, in = t & (T - 1u);
+            const uint8_t* const k_at = g.base + ((uint64_t)bcast(k_slot, b) << g.page_log) + in * 16u;
+            const uint8_t* const v_at = g.base + ((uint64_t)bcast(v_slot, b) << g.page_log) + (in >> 3) * D * 16u;
 #pragma unroll
             for (uint32_t i = 0; i < DP / 64; i++) {
                 /* odd units with neighbouring pieces exchanged: read by sixteen lanes from two units, they lie in different banks */
                 const uint32_t odd = UNITS % 2 ? u & 1u : x & 1u;
-                if (D == DP || (8u * i + (lane >> 3 ^ odd)) * 8u < D) to_lds(k_at, (odd ? k_lane1 : k_lane0) + i * 128u * T, to + u * DP * 16u + i * 1024u);
-                if (D == DP || 64u * i + lane < D) to_lds(v_at, (64u * i + lane) * 16u, to + HALF + u * DP * 16u + i * 1024u);
+                if (EXACT || (8u * i + (lane >> 3 ^ odd)) * 8u < D) to_lds(k_at, (odd ? k_lane1 : k_lane0) + i * 128u * T, to + u * DP * 16u + i * 1024u);
+                if (EXACT || 64u * i + lane < D) to_lds(v_at, (64u * i + lane) * 16u, to + HALF + u * DP * 16u + i * 1024u);
             }
         }
         at_first = t_next; at_end = t_end; at_holes = holes; at_block = b_first;
         t_next += KT;
     };
     next_blocks();
-    bool more = stage == 1;
-    if (more) { next_looks(); enter_next(); load_tile(0); }
+    bool more = there;
+    if (more) { enter_next(); load_tile(0); }
     /* K's row of this lane: of the 32 tokens, the one that puts the scores of tokens 8 half .. + 7 of each 16 into its accumulators */
     const uint32_t k_row = (row & 0x13u) | ((row & 4u) << 1) | ((row & 8u) >> 1);
     const uint32_t k_read = (k_row >> 3) * DP * 16u + (k_row & 7u) * 16u + (half ^ (k_row >> 3 & 1u)) * 128u;
     for (uint32_t buf = 0; more; buf ^= 1u) {
         fence_meta();                            /* this wave's part of the tile is in LDS, */
         __syncthreads();                         /* and everybody's; and everybody has done with the buffer that is loaded next */
-        const uint32_t t0 = at_first, t_lim = at_end, t_holes = at_holes, t_block = at_block;
-        if (stage == 1) next_looks();
-        else if (stage == 0) next_blocks();
+        const uint32_t t0 = at_first, t_lim = at_end, t_block = at_block;
+        const uint64_t t_holes = at_holes;
         more = true;
         if (t_next >= t_end) {
-            if (stage == 1) next_looks();
-            if (stage == 2) { look_again(); enter_next(); }
-            else more = false;
+            more = there;
+            if (more) { look_again(); enter_next(); }
         }
         if (more) load_tile(buf ^ 1u);
         if (idle || (int32_t)t0 > last_pos) continue;
@@ -964,7 +969,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
 #pragma unroll
             for (uint32_t k = 0; k < KT / 16; k++) {
                 const uint32_t tt = t0 + k * 16u + half * 8u;
-                if ((t_holes >> (((tt >> g.tokens_log) - t_block) & 31u)) & 1u) continue;
+                if ((t_holes >> (((tt >> g.tokens_log) - t_block) & 63u)) & 1u) continue;
                 sees |= seen_of_eight((int32_t)tt, pos < lim ? pos : lim, low_of(a, pos), (int32_t)a.sinks) << (8u * k);
             }
 #pragma unroll
@@ -1165,7 +1170,10 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     static const bool once = [] {
         allow_lds(k_kv_attend<DP, F16, NT>, lds);
         allow_lds(k_kv_finish<DP, F16, NT>, lds);
-        if constexpr (NT == 2) { allow_lds(k_kv_attend_tiles<DP, F16, 2>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4>, lds_tiles); }
+        if constexpr (NT == 2) {
+            allow_lds(k_kv_attend_tiles<DP, F16, 2, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 2, false>, lds_tiles);
+            allow_lds(k_kv_attend_tiles<DP, F16, 4, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4, false>, lds_tiles);
+        }
         return true;
     }();
     (void)once;
@@ -1181,8 +1189,11 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     if (!kv->unheld) hipLaunchKernelGGL(k_kv_all_left, dim3((uint32_t)((p.items * p.splits + 255) / 256)), dim3(256), 0, st, a.left, p.items * p.splits);
     else if (!p.waves) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
     else if constexpr (NT == 2) {
-        if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
-        else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+        const bool exact = kv->g.dim == DP;
+        if (p.waves == 2 && exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, true>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
+        else if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, false>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
+        else if (exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, true>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+        else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, false>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
     }
     hipLaunchKernelGGL((k_kv_finish<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
 }
