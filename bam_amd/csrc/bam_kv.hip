@@ -815,6 +815,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     const uint32_t tok = has ? r / a.group : 0u, head = it.head * a.group + (has ? r % a.group : 0u);
     const int32_t p0 = it.len - it.rows, pos = has ? p0 + (int32_t)tok : -1;
     const int32_t first_pos = idle ? -1 : p0 + (int32_t)(w0 / a.group), last_pos = idle ? -1 : p0 + (int32_t)((w1 - 1) / a.group);
+    const int32_t first_of_all = sp.first_pos, last_of_all = sp.last_pos;
     /* a negative scale goes into the sign of the queries: the largest score is then the largest product */
     const float c = fmaxf(fabsf(a.scale), 1e-30f);
     const uint32_t flip = a.scale < 0 ? 0x80008000u : 0u;
@@ -925,9 +926,24 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             if (more) { look_again(); enter_next(); }
         }
         if (more) load_tile(buf ^ 1u);
-        if (idle || (int32_t)t0 > last_pos) continue;
         const uint8_t* const keys = (const uint8_t*)lds + buf * 2u * HALF;
         const uint8_t* const values = keys + HALF;
+        /* whether all rows from `from` to `to` see all of the tile */
+        auto all_seen = [&](const int32_t from, const int32_t to) {
+            return !t_holes && (int32_t)(t0 + KT) - 1 <= from && t0 + KT <= t_lim && (!a.window || to - (int32_t)t0 < (int32_t)a.window || t0 + KT <= a.sinks);
+        };
+        if (!all_seen(first_of_all, last_of_all)) {
+            /* values of tokens that a row does not see meet zeros of P.  That leaves them out unless there is an infinity or NaN among them: then
+             * the split is left to the launch that takes the rows one by one there (kv_steps).  Each wave looks at a part of the values. */
+            bool odd = false;
+#pragma unroll
+            for (uint32_t n = 0; n < PIECES / (64u * NW); n++) {
+                const u32x4 z = *(const u32x4*)(values + (n * 64u * NW + threadIdx.x) * 16u);
+                odd |= odd16<F16>(z[0]) || odd16<F16>(z[1]) || odd16<F16>(z[2]) || odd16<F16>(z[3]);
+            }
+            if (ballot(odd)) ok = false;
+        }
+        if (idle || (int32_t)t0 > last_pos) continue;
         /*
          * The operands from LDS are read eight ahead of the products that take them, and the order is held (sched_barrier): left to itself the compiler reads each right before
          * its product and waits for it, a hundred cycles for every 32 of the matrix unit.
@@ -953,17 +969,8 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             for (uint32_t e = 0; e < 4; e++) f[(n + e) % 8] = n + 8 < NK ? key_piece(n + 8 + e) : value_piece(n + 8 + e - NK);
             __builtin_amdgcn_sched_barrier(0);
         }
-        const bool whole = !t_holes && (int32_t)(t0 + KT) - 1 <= first_pos && t0 + KT <= t_lim && (!a.window || last_pos - (int32_t)t0 < (int32_t)a.window || t0 + KT <= a.sinks);
+        const bool whole = all_seen(first_pos, last_pos);
         if (!whole) {
-            /* values of tokens that a row does not see meet zeros of P.  That leaves them out unless there is an infinity or NaN among them: then
-             * the split is left to the launch that takes the rows one by one there (kv_steps) */
-            bool odd = false;
-#pragma unroll 1
-            for (uint32_t n = lane; n < PIECES; n += 64u) {
-                const u32x4 z = *(const u32x4*)(values + n * 16u);
-                odd |= odd16<F16>(z[0]) || odd16<F16>(z[1]) || odd16<F16>(z[2]) || odd16<F16>(z[3]);
-            }
-            if (ballot(odd)) ok = false;
             uint32_t sees = 0;                   /* of each 16 tokens, which of its eight the row sees */
             const int32_t lim = (int32_t)t_lim - 1;
 #pragma unroll
@@ -1056,55 +1063,88 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     if (a.lse && half == 0) a.lse[(uint64_t)(it.start + (int32_t)tok) * a.q_heads + head] = (m * c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
-/*
- * What the first launch left, with its pages held, and the splits of an item joined: out = sum over splits of exp(m_s - m) O_s / sum of exp(m_s - m) l_s.
- */
+/* what the first launch left, with its pages held; ends at once where that is nothing */
 template <int DP, int F16, int NT>
-__global__ __launch_bounds__(256) void k_kv_finish(const kv_geom g, const kv_seqs s, const kv_att a)
+__global__ __launch_bounds__(256) void k_kv_rest(const kv_geom g, const kv_seqs s, const kv_att a)
 {
     extern __shared__ float lds[];
-    constexpr uint32_t R = 16 * NT;
-    const uint32_t D = g.dim;
-    for (uint32_t item = blockIdx.x; item < a.items; item += gridDim.x) {
-        bool mine = false;
-        for (uint32_t k = threadIdx.x; k < a.splits; k += 256u) mine |= a.left[(uint64_t)item * a.splits + k] != 0;
-        const bool any = __syncthreads_or(mine);
-        if (!any && a.splits == 1) continue;
+    const uint32_t each = (a.items + gridDim.x - 1) / gridDim.x, first = blockIdx.x * each, last = first + each < a.items ? first + each : a.items;
+    bool mine = false;
+    for (uint64_t k = (uint64_t)first * a.splits + threadIdx.x; k < (uint64_t)last * a.splits; k += 256u) mine |= a.left[k] != 0;
+    if (!__syncthreads_or(mine)) return;
+    for (uint64_t x = (uint64_t)first * a.splits; x < (uint64_t)last * a.splits; x++) {
         kv_item it;
-        if (!item_of(g, s, a, item, it)) continue;
-        if (any) {
-            for (uint32_t k = 0; k < a.splits; k++)
-                if (a.left[(uint64_t)item * a.splits + k])
-                    for (uint32_t s0 = it.r0; s0 < it.r1; s0 += R) {
-                        bool gone = false;
-                        kv_split<DP, F16, NT, true>(g, s, a, item, it, s0, k, lds, gone);
-                        __syncthreads();
-                    }
-            __threadfence();
+        if (!a.left[x] || !item_of(g, s, a, (uint32_t)(x / a.splits), it)) continue;
+        for (uint32_t s0 = it.r0; s0 < it.r1; s0 += 16u * NT) {
+            bool gone = false;
+            kv_split<DP, F16, NT, true>(g, s, a, (uint32_t)(x / a.splits), it, s0, (uint32_t)(x % a.splits), lds, gone);
             __syncthreads();
         }
-        if (a.splits == 1) continue;
-        const uint32_t n_rows = it.r1 - it.r0;
-        for (uint32_t x = threadIdx.x; x < n_rows * (D / 4u); x += 256u) {
-            const uint32_t r = x / (D / 4u), c = x % (D / 4u) * 4u;
-            const uint64_t at = ((uint64_t)item * a.tile_rows + r) * a.splits;
-            float top = -INFINITY, den = 0;
-            for (uint32_t k = 0; k < a.splits; k++) top = fmaxf(top, a.part_m[at + k]);
-            const float use = top == -INFINITY ? 0.0f : top;
-            f32x4 sum{0, 0, 0, 0};
-            for (uint32_t k = 0; k < a.splits; k++) {
-                const float by = __builtin_amdgcn_exp2f(a.part_m[at + k] - use);
-                den += by * a.part_l[at + k];
-                sum += by * *(const f32x4*)(a.part + (at + k) * D + c);
-            }
-            const float inv = top == -INFINITY && den == 0 ? 0.0f : 1.0f / den;
-            const uint32_t rr = it.r0 + r, tok = (uint32_t)it.start + rr / a.group, h = it.head * a.group + rr % a.group;
-            uint32_t* const to = (uint32_t*)(a.out + ((uint64_t)tok * a.q_heads + h) * D + c);
-            to[0] = to16<F16>(sum[0] * inv, sum[1] * inv);
-            to[1] = to16<F16>(sum[2] * inv, sum[3] * inv);
-            if (a.lse && c == 0) a.lse[(uint64_t)tok * a.q_heads + h] = (top + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
+    }
+}
+
+/*
+ * The splits of a row joined: out = sum over splits of exp(m_s - m) O_s / sum of exp(m_s - m) l_s.  LPR lanes to a row, four numbers to a lane; WIDE: the four waves of a
+ * workgroup share the splits of a row (64 of 128 splits of 32 rows: 42 us by a workgroup for all rows of a head of keys), else they have rows of their own.
+ */
+template <int LPR, int F16, bool WIDE>
+__global__ __launch_bounds__(256) void k_kv_join(const kv_geom g, const kv_seqs s, const kv_att a)
+{
+    __shared__ f32x4 sums[WIDE ? 256 : 1];
+    __shared__ float tops[WIDE ? 256 : 1], dens[WIDE ? 256 : 1];
+    constexpr uint32_t RPW = 64 / LPR;
+    const uint32_t lane = bam::lane(), wave = threadIdx.x / 64u, c = lane % LPR * 4u, D = g.dim;
+    const uint64_t x = (uint64_t)(WIDE ? blockIdx.x : blockIdx.x * 4u + wave) * RPW + lane / LPR;
+    const uint32_t item = (uint32_t)(x / a.tile_rows), r = (uint32_t)(x % a.tile_rows);
+    kv_item it;
+    const bool has = item < a.items && item_of(g, s, a, item, it) && it.r0 + r < it.r1 && c < D;
+    float top = -INFINITY, den = 0;
+    f32x4 sum{0, 0, 0, 0};
+    if (has) {
+        const uint64_t at = ((uint64_t)item * a.tile_rows + r) * a.splits;
+        auto take = [&](const float m, const float l, const f32x4 o) {
+            const float larger = fmaxf(top, m), use = larger == -INFINITY ? 0.0f : larger;
+            const float mine = __builtin_amdgcn_exp2f(top - use), by = __builtin_amdgcn_exp2f(m - use);
+            den = den * mine + l * by;
+            sum = sum * mine + o * by;
+            top = larger;
+        };
+        const uint32_t step = WIDE ? 4u : 1u;
+        uint32_t k = WIDE ? wave : 0u;
+        for (; k + 3u * step < a.splits; k += 4u * step) {
+            float m[4], l[4];
+            f32x4 o[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) { m[i] = a.part_m[at + k + i * step]; l[i] = a.part_l[at + k + i * step]; o[i] = *(const f32x4*)(a.part + (at + k + i * step) * D + c); }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) take(m[i], l[i], o[i]);
+        }
+        for (; k < a.splits; k += step) take(a.part_m[at + k], a.part_l[at + k], *(const f32x4*)(a.part + (at + k) * D + c));
+        if constexpr (WIDE) { sums[threadIdx.x] = sum; tops[threadIdx.x] = top; dens[threadIdx.x] = den; }
+    }
+    if constexpr (WIDE) {
+        __syncthreads();
+        if (wave) return;
+        if (has) {
+            auto take = [&](const float m, const float l, const f32x4 o) {
+                const float larger = fmaxf(top, m), use = larger == -INFINITY ? 0.0f : larger;
+                const float mine = __builtin_amdgcn_exp2f(top - use), by = __builtin_amdgcn_exp2f(m - use);
+                den = den * mine + l * by;
+                sum = sum * mine + o * by;
+                top = larger;
+            };
+#pragma unroll
+            for (uint32_t w = 1; w < 4; w++) take(tops[w * 64u + lane], dens[w * 64u + lane], sums[w * 64u + lane]);
         }
     }
+    if (!has) return;
+    const float inv = top == -INFINITY && den == 0 ? 0.0f : 1.0f / den;
+    const uint32_t rr = it.r0 + r, tok = (uint32_t)it.start + rr / a.group, h = it.head * a.group + rr % a.group;
+    uint2 y;
+    y.x = to16<F16>(sum[0] * inv, sum[1] * inv);
+    y.y = to16<F16>(sum[2] * inv, sum[3] * inv);
+    *(uint2*)(a.out + ((uint64_t)tok * a.q_heads + h) * D + c) = y;
+    if (a.lse && c == 0) a.lse[(uint64_t)tok * a.q_heads + h] = (top + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------
@@ -1169,7 +1209,7 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     constexpr uint32_t lds = split_lds<DP, NT>(), lds_tiles = tile_lds<DP>();
     static const bool once = [] {
         allow_lds(k_kv_attend<DP, F16, NT>, lds);
-        allow_lds(k_kv_finish<DP, F16, NT>, lds);
+        allow_lds(k_kv_rest<DP, F16, NT>, lds);
         if constexpr (NT == 2) {
             allow_lds(k_kv_attend_tiles<DP, F16, 2, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 2, false>, lds_tiles);
             allow_lds(k_kv_attend_tiles<DP, F16, 4, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4, false>, lds_tiles);
@@ -1180,7 +1220,7 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     /* what all waves of the second launch hold at a time stays under half the cache, or they wait for each other's slots */
     const uint32_t least = kv->g.tokens < 32 ? 32 / kv->g.tokens : 1;
     const uint64_t half = kv->cache_pages / 2;
-    uint64_t groups = p.items < 2048 ? p.items : 2048;
+    uint64_t groups = p.items < 512 ? p.items : 512;
     if (groups * 4 * 2 * least > half) groups = half / (8 * least);
     uint64_t chunk = half / (groups * 8) / least * least;
     a.chunk = (uint32_t)(chunk > 32 ? 32 : chunk);
@@ -1195,7 +1235,12 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
         else if (exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, true>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
         else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, false>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
     }
-    hipLaunchKernelGGL((k_kv_finish<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
+    hipLaunchKernelGGL((k_kv_rest<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
+    if (p.splits == 1) return;
+    constexpr int LPR = DP / 4;
+    const uint64_t rows = p.items * p.rows, rpw = 64 / LPR;
+    if (p.splits >= 16) hipLaunchKernelGGL((k_kv_join<LPR, F16, true>), dim3((uint32_t)((rows + rpw - 1) / rpw)), dim3(256), 0, st, kv->g, s, a);
+    else hipLaunchKernelGGL((k_kv_join<LPR, F16, false>), dim3((uint32_t)((rows + 4 * rpw - 1) / (4 * rpw))), dim3(256), 0, st, kv->g, s, a);
 }
 template <int DP, int F16>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st)
