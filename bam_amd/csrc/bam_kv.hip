@@ -89,9 +89,9 @@ template <int F16> __device__ __forceinline__ uint32_t to16(const float lo, cons
     if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), _Float16 __attribute__((ext_vector_type(2)))));
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), __bf16 __attribute__((ext_vector_type(2)))));
 }
-__device__ __forceinline__ u32x4 load_piece(const uint16_t* p, const bool aligned)
+template <bool ALIGNED> __device__ __forceinline__ u32x4 load_piece(const uint16_t* p)
 {
-    if (aligned) return *(const u32x4*)p;
+    if constexpr (ALIGNED) return *(const u32x4*)p;
     u32x4 x;
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
@@ -117,56 +117,47 @@ __attribute__((noinline)) __device__ bam_pass_t kv_pass(range_d_t<uint64_t>* r, 
 }
 
 /*
- * use(address of the slot) for the lanes with `take`, each with its page held: as range_view::acquire_helped, the lanes of resident pages first and
- * nothing held while the others' pages are fetched, with what a writer of rows can say besides (`fresh`, `cleared`: range_d_t::slow_step).
- * `use` stores past the caches (st16_sys and the like), so a wait for the wave's own stores is all that giving a page back needs: the write-back of the
- * cluster's cache that a release costs would come once per wave.  All lanes of the wave call.
+ * use(address of the slot of the keys or NULL, and of the values) by the whole wave, with those pages held: two neighbouring pages, as range_view::acquire_helped would
+ * have them, what is resident first and nothing held while the other is fetched, with what a writer of rows can say besides (`fresh`, `cleared`:
+ * range_d_t::slow_step).  It stores past the caches (st16_sys and the like), so a wait for the wave's own stores is all that giving a page back needs: the
+ * write-back of the cluster's cache that a release costs would come once per wave.  The miss path is a call: what the rows need is loaded in `use`, behind it (loaded
+ * before, it would be kept across the call, in so many registers that one wave is left to a SIMD).
  */
 template <bool WRITE, typename F>
-__device__ __forceinline__ void visit(const kv_geom& g, const uint64_t page, const bool take, const bool fresh, const bool cleared, uint32_t& n_access, uint32_t& n_hit, F&& use)
+__device__ __forceinline__ void visit(const kv_geom& g, const uint64_t page, const bool fresh, const bool cleared, F&& use)
 {
     using namespace bam;
     const uint32_t me = lane();
-    data_page_t* const dp = g.pages + (take ? page : 0);
-    const uint64_t eq = match_any(take ? (uint64_t)dp : 0ull);
-    const uint32_t master = first_lane(eq), count = popc(eq);
-    const bool lead = take && master == me;
-    uint64_t sv = 0, pack = 0;
-    uint32_t slot = 0;
-    if (lead) { const bool h = bam_try_hit(dp, count, WRITE, sv, slot); pack = (uint64_t)slot | ((uint64_t)h << 63); }
-    pack = shfl(pack, master);
-    bool done = !take;
-    if (take && (pack >> 63)) {
-        use(g.base + ((uint64_t)(uint32_t)pack << g.page_log));
-        done = true;
-        fence_meta();
-        if (lead) { __hip_atomic_fetch_add(&dp->state, 0u - count, __ATOMIC_RELAXED, BAM_AGENT); n_access += count; n_hit += count; }
-    }
-    if (__builtin_expect(ballot(!done) == 0, 1)) return;
-    const uint32_t queue = wave_slot_hash();
+    data_page_t* const dp = g.pages + page + (me & 1u);
+    uint64_t sv = 0;
+    uint32_t slot = 0, n_hit = 0;
+    bool open = me < 2, in = false;
+    if (open) in = bam_try_hit(dp, 1, WRITE, sv, slot);
+    uint32_t todo = 3;
     spin_t sp;
-    page_cache_d_t* const cache = &g.r->cache;
-    for (;;) {
-        const bool part = !done && lead;
-        const bam_pass_t ps = kv_pass(g.r, take ? page : 0, queue, sv, (WRITE ? BAM_PASS_WRITE : 0u) | (part ? BAM_PASS_TAKE_PART : 0u) | (fresh ? KV_PASS_FRESH : 0u) | (cleared ? KV_PASS_CLEARED : 0u));
-        const bool progressed = (ps.flags & BAM_PASS_PROGRESSED) != 0;
-        if (part) {
-            sv = ps.sv;
-            pack = (uint64_t)ps.slot | ((uint64_t)((ps.flags & BAM_PASS_HIT) != 0) << 63) | ((uint64_t)((ps.flags & BAM_PASS_RESOLVED) != 0) << 62);
-        }
-        const uint64_t got = shfl(pack, master);
-        if (!done && ((got >> 62) & 1)) {
-            use(g.base + ((uint64_t)(uint32_t)got << g.page_log));
-            done = true;
+    const uint32_t queue = wave_slot_hash();
+    for (bool again = false;; again = true) {
+        uint32_t got = (uint32_t)ballot(in && open);
+        if (!again) n_hit = popc(got);
+        if (got) {
+            use(got & 1u ? g.base + ((uint64_t)bcast(slot, 0) << g.page_log) : nullptr, got & 2u ? g.base + ((uint64_t)bcast(slot, 1) << g.page_log) : nullptr);
             fence_meta();
-            if (lead) { __hip_atomic_fetch_add(&dp->state, 0u - count, __ATOMIC_RELAXED, BAM_AGENT); n_access += count; n_hit += (got >> 63) ? count : 0u; }
+            if (in && open) { __hip_atomic_fetch_add(&dp->state, 0u - 1u, __ATOMIC_RELAXED, BAM_AGENT); open = false; }
+            todo &= ~got;
         }
-        if (!ballot(!done)) break;
-        if (ballot(progressed)) sp = spin_t();
-        else if (cache->spin_giveup(sp)) {
-            if (!done && lead) __hip_atomic_fetch_add(&dp->state, 0u - count, __ATOMIC_RELAXED, BAM_AGENT);
+        if (__builtin_expect(todo == 0, 1)) break;
+        const bam_pass_t ps = kv_pass(g.r, page + (me & 1u), queue, sv, (WRITE ? BAM_PASS_WRITE : 0u) | (open ? BAM_PASS_TAKE_PART : 0u) | (fresh ? KV_PASS_FRESH : 0u) | (cleared ? KV_PASS_CLEARED : 0u));
+        if (open) { sv = ps.sv; slot = ps.slot; in = (ps.flags & BAM_PASS_RESOLVED) != 0; n_hit += in && (ps.flags & BAM_PASS_HIT) ? 1u : 0u; }
+        if (ballot((ps.flags & BAM_PASS_PROGRESSED) != 0)) sp = spin_t();
+        else if (!ballot(in && open) && g.r->cache.spin_giveup(sp)) {
+            if (open) __hip_atomic_fetch_add(&dp->state, 0u - 1u, __ATOMIC_RELAXED, BAM_AGENT);
             break;
         }
+    }
+    if (me == 0) {
+        bam_stat_shard_t* const shard = g.r->shard();
+        __hip_atomic_fetch_add(&shard->access_cnt, 2ull, __ATOMIC_RELAXED, BAM_AGENT);
+        if (n_hit) __hip_atomic_fetch_add(&shard->hit_cnt, (unsigned long long)n_hit, __ATOMIC_RELAXED, BAM_AGENT);
     }
 }
 
@@ -189,54 +180,69 @@ struct kv_rows {
     const float *cos, *sin;
     uint32_t positions, q_heads, rot, pairs, aligned;      /* aligned: q, k, v in whole pieces of 16 bytes */
     float eps;
-    uint32_t v_rows;                    /* rows a wave of values looks after */
-    uint32_t q_waves, k_waves;
+    uint32_t window, run;               /* rows that a wave looks for beginnings of runs among, and the most rows of a run */
+    uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes */
 };
+
+/* the angles of eight neighbouring numbers of a row; lanes whose numbers are not turned load some, and do not use them */
+struct kv_turn { f32x4 c[2], s[2]; };
+__device__ __forceinline__ kv_turn turn_of(const kv_rows& io, const uint32_t piece, const uint32_t pos)
+{
+    kv_turn t;
+    if (!io.rot) return t;
+    const uint32_t half = io.rot / 2, hp = io.rot / 16;
+    const bool known = pos < io.positions;
+    const uint64_t row = (uint64_t)(known ? pos : 0u) * half;
+    if (io.pairs) {
+        const uint64_t at = row + (piece < 2u * hp ? piece : 0u) * 4u;
+        t.c[0] = *(const f32x4*)(io.cos + at);
+        t.s[0] = *(const f32x4*)(io.sin + at);
+    } else {
+        const uint64_t at = row + (piece < hp ? piece : piece < 2u * hp ? piece - hp : 0u) * 8u;
+        t.c[0] = *(const f32x4*)(io.cos + at); t.c[1] = *(const f32x4*)(io.cos + at + 4);
+        t.s[0] = *(const f32x4*)(io.sin + at); t.s[1] = *(const f32x4*)(io.sin + at + 4);
+    }
+    if (!known) {
+        const float nan = __builtin_nanf("");
+        t.c[0] = t.c[1] = t.s[0] = t.s[1] = f32x4{nan, nan, nan, nan};
+    }
+    return t;
+}
 
 /*
  * Eight neighbouring numbers of a row per lane, LPR lanes to a row: x * rsqrt(mean x^2 + eps) * w, then the rotation of the pairs (i, i + rot/2), or
  * (2i, 2i+1), i < rot/2, by the angles of the row's position; in 32 bits, rounded once.  A position past the tables gives NaN.
  */
 template <int LPR, int F16>
-__device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geom& g, u32x4 x, const uint16_t* norm, const uint32_t piece, const uint32_t pos)
+__device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geom& g, u32x4 x, const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
 {
     if (!norm && !io.rot) return x;
     float f[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) { f[2 * i] = from16<F16>(x[i] & 0xffffu); f[2 * i + 1] = from16<F16>(x[i] >> 16); }
-    const bool in = piece * 8u < g.dim;
+    for (int i = 0; i < 4; i++) { const uint32_t y = x[i]; f[2 * i] = from16<F16>(y & 0xffffu); f[2 * i + 1] = from16<F16>(y >> 16); }
     if (norm) {
-        float ss = 0;
-        if (in) {
+        float ss = 0;                            /* (pieces past the row's end are zero) */
 #pragma unroll
-            for (int i = 0; i < 8; i++) ss += f[i] * f[i];
-        }
+        for (int i = 0; i < 8; i++) ss += f[i] * f[i];
 #pragma unroll
         for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
         const float by = rsqrtf(ss / (float)g.dim + io.eps);
-        if (in) {
-            const u32x4 w = load_piece(norm + piece * 8u, true);
 #pragma unroll
-            for (int i = 0; i < 4; i++) { f[2 * i] *= by * from16<F16>(w[i] & 0xffffu); f[2 * i + 1] *= by * from16<F16>(w[i] >> 16); }
-        }
+        for (int i = 0; i < 4; i++) { const uint32_t y = w[i]; f[2 * i] *= by * from16<F16>(y & 0xffffu); f[2 * i + 1] *= by * from16<F16>(y >> 16); }
     }
     if (io.rot) {
-        const uint32_t half = io.rot / 2, pieces = io.rot / 8;
-        const bool turns = piece < pieces, known = pos < io.positions;
-        const float nan = __builtin_nanf("");
+        const uint32_t pieces = io.rot / 8, hp = pieces / 2;
+        const bool turns = piece < pieces;
         if (io.pairs) {
             if (turns) {
-                const f32x4 c = known ? *(const f32x4*)(io.cos + (uint64_t)pos * half + piece * 4u) : f32x4{nan, nan, nan, nan};
-                const f32x4 s = known ? *(const f32x4*)(io.sin + (uint64_t)pos * half + piece * 4u) : f32x4{nan, nan, nan, nan};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float a = f[2 * i], b = f[2 * i + 1];
-                    f[2 * i] = a * c[i] - b * s[i];
-                    f[2 * i + 1] = b * c[i] + a * s[i];
+                    f[2 * i] = a * t.c[0][i] - b * t.s[0][i];
+                    f[2 * i + 1] = b * t.c[0][i] + a * t.s[0][i];
                 }
             }
         } else {
-            const uint32_t hp = pieces / 2, mine = piece < hp ? piece : piece - hp;
             const uint32_t from = (bam::lane() & ~(uint32_t)(LPR - 1)) + (turns ? (piece < hp ? piece + hp : piece - hp) : piece);
             const float sign = piece < hp ? -1.0f : 1.0f;
             float o[8];
@@ -244,12 +250,7 @@ __device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geo
             for (int i = 0; i < 8; i++) o[i] = __shfl(f[i], (int)from);
             if (turns) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const f32x4 c = known ? *(const f32x4*)(io.cos + (uint64_t)pos * half + mine * 8u + j * 4) : f32x4{nan, nan, nan, nan};
-                    const f32x4 s = known ? *(const f32x4*)(io.sin + (uint64_t)pos * half + mine * 8u + j * 4) : f32x4{nan, nan, nan, nan};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) f[4 * j + i] = f[4 * j + i] * c[i] + sign * o[4 * j + i] * s[i];
-                }
+                for (int i = 0; i < 8; i++) f[i] = f[i] * t.c[i / 4][i % 4] + sign * o[i] * t.s[i / 4][i % 4];
             }
         }
     }
@@ -259,121 +260,150 @@ __device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geo
 }
 
 /*
- * A wave takes either 64 / LPR rows of queries, or the keys of as many rows of one head, or the values of io.v_rows rows of one head.  Values lie in the
- * cache in pieces of eight tokens: whoever finds the first row of such a piece among its rows writes all rows of the piece.
+ * A wave takes some heads of queries of one row, or one head's keys and values of the runs of rows that begin among io.window rows: a run is the new rows of
+ * a sequence within io.run tokens of one block, eight or sixteen that begin at a multiple of that.
  */
-template <int LPR, int F16, bool WRITE>
-__global__ __launch_bounds__(256) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
+template <int LPR, int F16, bool WRITE, bool ALIGNED>
+__global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
 {
     using namespace bam;
-    constexpr uint32_t RPW = 64 / LPR;
-    const uint32_t wave = blockIdx.x * 4u + threadIdx.x / 64u, lane = bam::lane();
-    const uint32_t piece = lane % LPR;
-    uint32_t n_access = 0, n_hit = 0;
-    if (wave < io.q_waves) {
-        const uint64_t j = (uint64_t)wave * RPW + lane / LPR;
-        const uint32_t i = (uint32_t)(j / io.q_heads), h = (uint32_t)(j % io.q_heads);
+    constexpr uint32_t RPW = 64 / LPR, TRIPS = 16 / RPW, DT = LPR / 8;           /* trips of a run's keys; of its values: a trip is 64 times two numbers of eight tokens */
+    const uint32_t wave = first(blockIdx.x * 4u + threadIdx.x / 64u), lane = bam::lane();
+    const uint32_t sub = lane / LPR, piece = lane % LPR;
+    const bool in_row = piece * 8u < g.dim;
+    const uint32_t col = in_row ? piece * 8u : 0u;           /* lanes past the row's end load its beginning, and count as zeros */
+    if (WRITE && wave < io.q_waves) {
+        const uint32_t per = (io.q_heads + io.q_heads_each - 1) / io.q_heads_each, i = wave / per, h0 = wave % per * io.q_heads_each;
+        const uint32_t h1 = h0 + io.q_heads_each < io.q_heads ? h0 + io.q_heads_each : io.q_heads;
         kv_place p{0, 0, 0, 0};
-        const bool has = i < s.rows && piece * 8u < g.dim;
-        const bool known = i < s.rows && place_of(s, g, i, p);
-        u32x4 x{0, 0, 0, 0};
-        if (has) x = load_piece(io.q + (int64_t)i * io.q_row + (int64_t)h * io.q_head + piece * 8u, io.aligned);
-        x = norm_and_rotate<LPR, F16>(io, g, x, io.q_norm, piece, known ? p.pos : 0xffffffffu);
-        if (has) *(u32x4*)(io.q_out + ((uint64_t)i * io.q_heads + h) * g.dim + piece * 8u) = x;
-        return;
-    }
-    if (wave < io.q_waves + io.k_waves) {
-        const uint32_t w = wave - io.q_waves, h = w % g.heads, i = w / g.heads * RPW + lane / LPR;
-        kv_place p{0, 0, 0, 0};
-        uint64_t page = 0;
-        const bool has = i < s.rows && piece * 8u < g.dim && place_of(s, g, i, p) && page_of_block(g, s, p.seq, p.pos >> g.tokens_log, h, page);
-        const uint32_t in_block = p.pos & (g.tokens - 1u), block_first = p.pos - in_block;
-        const uint64_t at = ((uint64_t)piece * g.tokens + in_block) * 16u;
-        if constexpr (WRITE) {
-            u32x4 x{0, 0, 0, 0};
-            if (has) x = load_piece(io.k + (int64_t)i * io.k_row + (int64_t)h * io.k_head + piece * 8u, io.aligned);
-            x = norm_and_rotate<LPR, F16>(io, g, x, io.k_norm, piece, p.pos);
-            /* a page that holds none but this call's tokens needs nothing from the store */
-            visit<true>(g, page, has, block_first >= p.first, block_first + g.tokens > p.pos + p.rest, n_access, n_hit, [&](uint8_t* slot) { st16_sys(slot + at, x); });
-        } else {
-            u32x4 x{0, 0, 0, 0};
-            visit<false>(g, page, has, false, false, n_access, n_hit, [&](uint8_t* slot) { x = ld_payload((const u32x4*)(slot + at)); });
-            if (i < s.rows && piece * 8u < g.dim) *(u32x4*)((uint16_t*)io.k + (int64_t)i * io.k_row + (int64_t)h * io.k_head + piece * 8u) = x;
+        const bool known = place_of(s, g, i, p);
+        const kv_turn t = turn_of(io, piece, known ? p.pos : 0xffffffffu);
+        u32x4 w{0, 0, 0, 0};
+        if (io.q_norm) w = load_piece<true>(io.q_norm + col);
+        const uint16_t* const from = io.q + (int64_t)i * io.q_row + col;
+        uint16_t* const to = io.q_out + (uint64_t)i * io.q_heads * g.dim + col;
+        for (uint32_t h = h0; h < h1; h += 4u * RPW) {
+            u32x4 x[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t hh = h + e * RPW + sub;
+                x[e] = load_piece<ALIGNED>(from + (int64_t)(hh < h1 ? hh : h0) * io.q_head);
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t hh = h + e * RPW + sub;
+                if (h + e * RPW >= h1) break;
+                x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.q_norm != nullptr, w, t, piece);
+                if (hh < h1 && in_row) *(u32x4*)(to + hh * g.dim) = x[e];
+            }
         }
-        count_accesses(g, n_access, n_hit);
         return;
     }
-    const uint32_t w = wave - io.q_waves - io.k_waves, h = w % g.heads;
-    const uint64_t first = (uint64_t)(w / g.heads) * io.v_rows;
-    if (first >= s.rows) return;
+    const uint32_t n = wave - (WRITE ? io.q_waves : 0u), head = n % g.heads;
+    const uint64_t first_row = (uint64_t)(n / g.heads) * io.window;
+    if (first_row >= s.rows) return;
     kv_place p{0, 0, 0, 0};
-    const uint32_t mine = (uint32_t)first + lane;
-    const bool has = lane < io.v_rows && mine < s.rows && place_of(s, g, mine, p);
-    /* rows that begin a piece: of theirs, and of nobody's where the row has no place */
-    const bool begins = has && ((p.pos & 7u) == 0 || p.pos == p.first || (s.starts && s.starts[p.seq] == (int32_t)mine));
+    const uint32_t mine = (uint32_t)first_row + lane;
+    const bool has = lane < io.window && mine < s.rows && place_of(s, g, mine, p);
+    const bool begins = has && ((p.pos & (io.run - 1u)) == 0 || p.pos == p.first || (s.starts && s.starts[p.seq] == (int32_t)mine));
     if constexpr (!WRITE) {
         /* rows without a place come out as zeros */
-        for (uint64_t m = ballot(lane < io.v_rows && mine < s.rows && !has); m; m &= m - 1)
-            for (uint32_t d = lane; d < g.dim; d += 64u) ((uint16_t*)io.v)[(int64_t)(first + first_lane(m)) * io.v_row + (int64_t)h * io.v_head + d] = 0;
+        for (uint64_t m = ballot(lane < io.window && mine < s.rows && !has); m; m &= m - 1)
+            for (uint32_t d = lane; d < g.dim; d += 64u) {
+                ((uint16_t*)io.k)[(int64_t)(first_row + first_lane(m)) * io.k_row + (int64_t)head * io.k_head + d] = 0;
+                ((uint16_t*)io.v)[(int64_t)(first_row + first_lane(m)) * io.v_row + (int64_t)head * io.v_head + d] = 0;
+            }
     }
     for (uint64_t m = ballot(begins); m; m &= m - 1) {
-        const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), seq = bcast(p.seq, j), row = (uint32_t)first + j;
-        const uint32_t left = 8u - (pos & 7u), cnt = rest < left ? rest : left;
+        const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), seq = bcast(p.seq, j), row = (uint32_t)first_row + j;
+        const uint32_t left = io.run - (pos & (io.run - 1u)), cnt = rest < left ? rest : left;
         uint64_t page = 0;
-        const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, h, page);
+        const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, head, page);
         const uint32_t in_block = pos & (g.tokens - 1u), block_first = pos - in_block;
-        uint16_t* const rows = (uint16_t*)io.v + (int64_t)row * io.v_row + (int64_t)h * io.v_head;
-        if constexpr (WRITE) {
-            if (!there) continue;
-            visit<true>(g, page + 1, true, block_first >= bcast(p.first, j), block_first + g.tokens > pos + rest, n_access, n_hit, [&](uint8_t* slot) {
-                for (uint32_t d = lane * 2u; d < g.dim; d += 128u) {
-                    uint8_t* const at = slot + ((uint64_t)(in_block >> 3) * g.dim + d) * 16u;
-                    uint32_t x[8];
+        uint16_t* const k_rows = (uint16_t*)io.k + (int64_t)row * io.k_row + (int64_t)head * io.k_head;
+        uint16_t* const v_rows = (uint16_t*)io.v + (int64_t)row * io.v_row + (int64_t)head * io.v_head;
+        /* of the values, a lane takes numbers d and d + 1 of the eight tokens from `tok` on, counted from the run's first row */
+        const int32_t run_first = (int32_t)(in_block & (io.run - 1u));
+        const uint32_t groups = io.run / 8u, pairs = g.dim / 2u;
+        auto use = [&](uint8_t* const keys, uint8_t* const values, const bool no_page) {
+            /* what is worked out from the lane's number is worked out here, not kept across the miss path */
+            uint32_t l = lane;
+            asm volatile("" : "+v"(l));
+            if (keys || no_page) {
+                u32x4 x[TRIPS];
+                const uint32_t r0 = l / LPR;
+                uint8_t* const at = keys + ((uint64_t)(col / 8u) * g.tokens + in_block) * 16u;
 #pragma unroll
-                    for (uint32_t t = 0; t < 8; t++) {
-                        const uint16_t* const from = rows + (int64_t)(t < cnt ? t : 0) * io.v_row + d;
-                        x[t] = io.aligned ? *(const uint32_t*)from : (uint32_t)from[0] | ((uint32_t)from[1] << 16);
-                    }
-                    if (cnt == 8) {
-                        u32x4 lo, hi;
+                for (uint32_t e = 0; e < TRIPS; e++) {
+                    const uint32_t r = r0 + e * RPW < cnt ? r0 + e * RPW : 0u;
+                    if constexpr (WRITE) x[e] = load_piece<ALIGNED>(k_rows + (int64_t)r * io.k_row + col);
+                    else x[e] = no_page ? u32x4{0, 0, 0, 0} : ld_payload((const u32x4*)(at + r * 16u));
+                }
+                u32x4 w{0, 0, 0, 0};
+                if (WRITE && io.k_norm) w = load_piece<true>(io.k_norm + col);
 #pragma unroll
-                        for (int t = 0; t < 4; t++) {
-                            lo[t] = (x[2 * t] & 0xffffu) | (x[2 * t + 1] << 16);
-                            hi[t] = (x[2 * t] >> 16) | (x[2 * t + 1] & 0xffff0000u);
+                for (uint32_t e = 0; e < TRIPS; e++) {
+                    if (e * RPW >= cnt) break;
+                    const uint32_t r = r0 + e * RPW;
+                    if constexpr (WRITE) {
+                        const kv_turn t = turn_of(io, piece, pos + (r < cnt ? r : 0u));
+                        x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.k_norm != nullptr, w, t, piece);
+                        if (r < cnt && in_row) st16_sys(at + r * 16u, x[e]);
+                    } else if (r < cnt && in_row) *(u32x4*)(k_rows + (int64_t)r * io.k_row + col) = x[e];
+                }
+            }
+            if (values || no_page) {
+#pragma unroll
+                for (uint32_t e = 0; e < DT; e++) {
+                    const uint32_t y = e * 64u + l, group = y / pairs, d = y % pairs * 2u;
+                    const int32_t tok = (int32_t)(group * 8u) - run_first;
+                    if (group >= groups || tok + 8 <= 0 || tok >= (int32_t)cnt) continue;
+                    uint8_t* const at = values + ((uint64_t)((in_block + tok) >> 3) * g.dim + d) * 16u;
+                    uint16_t* const rows = v_rows + d;
+                    const bool full = tok >= 0 && tok + 8 <= (int32_t)cnt;
+                    if constexpr (WRITE) {
+                        uint32_t z[8];
+#pragma unroll
+                        for (int32_t t = 0; t < 8; t++) {
+                            const int32_t r = tok + t < 0 ? 0 : tok + t < (int32_t)cnt ? tok + t : (int32_t)cnt - 1;
+                            const uint16_t* const from = rows + r * io.v_row;
+                            z[t] = ALIGNED ? *(const uint32_t*)from : (uint32_t)from[0] | ((uint32_t)from[1] << 16);
                         }
-                        st16_sys(at, lo);
-                        st16_sys(at + 16, hi);
-                    } else {
+                        if (full) {
+                            u32x4 lo, hi;
 #pragma unroll
-                        for (uint32_t t = 0; t < 8; t++)
-                            if (t < cnt) {
-                                uint16_t* const to = (uint16_t*)at + (pos & 7u) + t;
-                                __hip_atomic_store(to, (uint16_t)x[t], __ATOMIC_RELAXED, BAM_SYSTEM);
-                                __hip_atomic_store(to + 8, (uint16_t)(x[t] >> 16), __ATOMIC_RELAXED, BAM_SYSTEM);
+                            for (int t = 0; t < 4; t++) {
+                                lo[t] = (z[2 * t] & 0xffffu) | (z[2 * t + 1] << 16);
+                                hi[t] = (z[2 * t] >> 16) | (z[2 * t + 1] & 0xffff0000u);
+                            }
+                            st16_sys(at, lo);
+                            st16_sys(at + 16, hi);
+                        } else {
+#pragma unroll
+                            for (int32_t t = 0; t < 8; t++)
+                                if (tok + t >= 0 && tok + t < (int32_t)cnt) {
+                                    __hip_atomic_store((uint16_t*)at + t, (uint16_t)z[t], __ATOMIC_RELAXED, BAM_SYSTEM);
+                                    __hip_atomic_store((uint16_t*)at + 8 + t, (uint16_t)(z[t] >> 16), __ATOMIC_RELAXED, BAM_SYSTEM);
+                                }
+                        }
+                    } else {
+                        u32x4 lo{0, 0, 0, 0}, hi{0, 0, 0, 0};
+                        if (!no_page) { lo = ld_payload((const u32x4*)at); hi = ld_payload((const u32x4*)(at + 16)); }
+#pragma unroll
+                        for (int32_t t = 0; t < 8; t++)
+                            if (full || (tok + t >= 0 && tok + t < (int32_t)cnt)) {
+                                const uint32_t a = lo[t / 2], b = hi[t / 2];
+                                *(uint32_t*)(rows + (tok + t) * io.v_row) = (t & 1) ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
                             }
                     }
                 }
-            });
-        } else {
-            visit<false>(g, page + 1, there, false, false, n_access, n_hit, [&](uint8_t* slot) {
-                for (uint32_t d = lane * 2u; d < g.dim; d += 128u) {
-                    const uint8_t* const at = slot + ((uint64_t)(in_block >> 3) * g.dim + d) * 16u;
-                    const u32x4 lo = ld_payload((const u32x4*)at), hi = ld_payload((const u32x4*)(at + 16));
-                    const uint32_t o = pos & 7u;
-#pragma unroll
-                    for (uint32_t t = 0; t < 8; t++)
-                        if (t >= o && t < o + cnt) {
-                            const uint32_t a = (t & 1) ? lo[t / 2] >> 16 : lo[t / 2] & 0xffffu, b = (t & 1) ? hi[t / 2] >> 16 : hi[t / 2] & 0xffffu;
-                            *(uint32_t*)(rows + (int64_t)(t - o) * io.v_row + d) = a | (b << 16);
-                        }
-                }
-            });
-            if (!there)
-                for (uint32_t t = 0; t < cnt; t++)
-                    for (uint32_t d = lane; d < g.dim; d += 64u) rows[(int64_t)t * io.v_row + d] = 0;
-        }
+            }
+        };
+        if (there) {
+            /* a page that holds none but this call's tokens needs nothing from the store */
+            visit<WRITE>(g, page, WRITE && block_first >= bcast(p.first, j), WRITE && block_first + g.tokens > pos + rest, [&](uint8_t* keys, uint8_t* values) { use(keys, values, false); });
+        } else if constexpr (!WRITE) use(nullptr, nullptr, true);
     }
-    count_accesses(g, n_access, n_hit);
 }
 
 // ---------------------------------------------------------------------------
@@ -679,7 +709,7 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
 #pragma unroll
         for (int j = 0; j < DP / 32; j++) {
             q[n][j] = u32x4{0, 0, 0, 0};
-            if (has && (4u * j + grp) * 8u < D) q[n][j] = load_piece(from + (4u * j + grp) * 8u, a.aligned);
+            if (has && (4u * j + grp) * 8u < D) q[n][j] = a.aligned ? load_piece<true>(from + (4u * j + grp) * 8u) : load_piece<false>(from + (4u * j + grp) * 8u);
         }
         m[n] = -INFINITY;
         l[n] = 0;
@@ -825,7 +855,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
 #pragma unroll
         for (uint32_t j = 0; j < DP / 16; j++) {
             q[j] = u32x4{0, 0, 0, 0};
-            if (has && (2u * j + half) * 8u < D) q[j] = load_piece(from + (2u * j + half) * 8u, a.aligned) ^ flip;
+            if (has && (2u * j + half) * 8u < D) q[j] = (a.aligned ? load_piece<true>(from + (2u * j + half) * 8u) : load_piece<false>(from + (2u * j + half) * 8u)) ^ flip;
         }
     }
     f32x16 o[DP / 32];
@@ -1260,16 +1290,19 @@ template <bool WRITE>
 void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t st)
 {
     const uint32_t lpr = kv->g.dim <= 64 ? 8 : kv->g.dim <= 128 ? 16 : 32, rpw = 64 / lpr;
-    io.q_waves = io.q ? (uint32_t)(((uint64_t)s.rows * io.q_heads + rpw - 1) / rpw) : 0;
-    io.k_waves = (s.rows + rpw - 1) / rpw * kv->g.heads;
-    /* a wave that looks after eight rows goes through eight pages one after the other where each belongs to another sequence */
-    io.v_rows = (uint64_t)s.rows * kv->g.heads <= 8192 ? 1 : 8;
-    const uint64_t waves = (uint64_t)io.q_waves + io.k_waves + (uint64_t)(s.rows + io.v_rows - 1) / io.v_rows * kv->g.heads;
+    /* few rows: a trip of heads to a wave, a row to a wave; many: eight trips, and the runs that begin among sixteen rows */
+    io.q_heads_each = io.q && (uint64_t)s.rows * io.q_heads > 16384 ? 8 * rpw : rpw;
+    io.q_waves = io.q ? (uint32_t)((io.q_heads + io.q_heads_each - 1) / io.q_heads_each * s.rows) : 0;
+    io.run = kv->g.tokens < 16 ? 8 : 16;
+    io.window = s.starts && s.rows / s.n >= 8 ? io.run : 1;
+    const uint64_t waves = (uint64_t)io.q_waves + (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads;
+    if (waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
     const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
-#define KV_ROWS(LPR) \
-    if (kv->f16) hipLaunchKernelGGL((k_kv_rows<LPR, 1, WRITE>), grid, block, 0, st, kv->g, s, io); \
-    else hipLaunchKernelGGL((k_kv_rows<LPR, 0, WRITE>), grid, block, 0, st, kv->g, s, io)
-    if (lpr == 8) { KV_ROWS(8); } else if (lpr == 16) { KV_ROWS(16); } else { KV_ROWS(32); }
+#define KV_ROWS(LPR, AL) \
+    if (kv->f16) hipLaunchKernelGGL((k_kv_rows<LPR, 1, WRITE, AL>), grid, block, 0, st, kv->g, s, io); \
+    else hipLaunchKernelGGL((k_kv_rows<LPR, 0, WRITE, AL>), grid, block, 0, st, kv->g, s, io)
+    if (WRITE && !io.aligned) { if (lpr == 8) { KV_ROWS(8, !WRITE); } else if (lpr == 16) { KV_ROWS(16, !WRITE); } else { KV_ROWS(32, !WRITE); } }
+    else if (lpr == 8) { KV_ROWS(8, true); } else if (lpr == 16) { KV_ROWS(16, true); } else { KV_ROWS(32, true); }
 #undef KV_ROWS
 }
 
