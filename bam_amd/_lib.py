@@ -6,7 +6,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = None
 _HOST = None
 
-c_u64, c_u32, c_i64, c_int, c_vp = ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p
+c_u64, c_u32, c_int, c_vp = ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c_void_p
 P = ctypes.POINTER
 
 
@@ -78,11 +78,10 @@ SIGNATURES = {
     "bam_kv_create": (c_int, [P(c_vp), c_vp, c_u64, c_u64, c_u32, c_u32, c_int]),
     "bam_kv_destroy": (None, [c_vp]),
     "bam_kv_info": (c_int, [c_vp, P(c_u64)]),
-    "bam_kv_append": (c_int, [c_vp, c_u64, c_u64, c_vp, c_vp, c_vp, c_i64, c_u64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_u32, c_vp, c_vp, c_vp,
-                              ctypes.c_float, c_vp, c_vp, c_u64, c_u32, c_int, c_vp]),
-    "bam_kv_read": (c_int, [c_vp, c_u64, c_u64, c_vp, c_vp, c_vp, c_i64, c_u64, c_vp, c_vp, c_vp]),
+    "bam_kv_append": (c_int, [c_vp, c_vp, c_vp]),
+    "bam_kv_read": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp]),
     "bam_kv_attend_bytes": (c_int, [c_vp, c_u64, c_u64, c_u32, c_u64, c_u32, c_u32, P(c_u64)]),
-    "bam_kv_attend": (c_int, [c_vp, c_u64, c_u64, c_vp, c_vp, c_vp, c_i64, c_u64, c_vp, c_i64, c_i64, c_u32, c_u64, c_u64, ctypes.c_float, c_u32, c_u32, c_vp, c_vp, c_vp, c_u64, c_vp]),
+    "bam_kv_attend": (c_int, [c_vp, c_vp, c_vp]),
     "bam_bfs_frontier": (c_int, [c_vp, c_vp, c_u64, c_u64, c_vp, P(c_u32), c_vp]),
     "bam_gen_words": (c_int, [c_u64, c_u64, c_u64, c_vp, c_vp]),
     "bam_gen_mod": (c_int, [c_u64, c_u64, c_u64, c_u64, c_u64, c_vp, c_vp]),

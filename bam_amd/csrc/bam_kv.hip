@@ -1306,16 +1306,18 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
 #undef KV_ROWS
 }
 
-int bad_seqs(const char* who, const bam_kv_t* kv, uint64_t n_seqs, uint64_t n_rows, const int32_t* starts, const int32_t* lens, const int32_t* table, int64_t stride, uint64_t width)
+int bad_seqs(const char* who, const bam_kv_t* kv, const bam_kv_seqs_t& s)
 {
-    if (!kv || (n_rows && (!lens || !table))) return fail(EINVAL, std::string(who) + ": null argument");
-    if (n_seqs > 0x7fffffffull || n_rows > 0x7fffffffull) return fail(EINVAL, std::string(who) + ": more rows or sequences than 31 bits count");
-    if (!starts && n_seqs != n_rows) return fail(EINVAL, std::string(who) + ": without starts every sequence has one new token");
-    if (!n_rows) return 0;
-    if (width == 0 || width > 0x7fffffffull || stride < 0) return fail(EINVAL, std::string(who) + ": table of no width, or with its rows in reverse");
-    if (width > 0x7ffffc00ull >> kv->g.tokens_log) return fail(EINVAL, std::string(who) + ": the table has room for more positions than 31 bits count");
+    if (!kv || (s.n_rows && (!s.d_lens || !s.d_table))) return fail(EINVAL, std::string(who) + ": null argument");
+    if (s.n_seqs > 0x7fffffffull || s.n_rows > 0x7fffffffull) return fail(EINVAL, std::string(who) + ": more rows or sequences than 31 bits count");
+    if (!s.d_starts && s.n_seqs != s.n_rows) return fail(EINVAL, std::string(who) + ": without starts every sequence has one new token");
+    if (!s.n_rows) return 0;
+    if (!s.n_seqs) return fail(EINVAL, std::string(who) + ": rows and no sequences");
+    if (s.table_width == 0 || s.table_width > 0x7fffffffull || s.table_stride < 0) return fail(EINVAL, std::string(who) + ": table of no width, or with its rows in reverse");
+    if (s.table_width > 0x7ffffc00ull >> kv->g.tokens_log) return fail(EINVAL, std::string(who) + ": the table has room for more positions than 31 bits count");
     return 0;
 }
+kv_seqs seqs_of(const bam_kv_seqs_t& s) { return kv_seqs{s.d_starts, s.d_lens, s.d_table, s.table_stride, (uint32_t)s.n_seqs, (uint32_t)s.n_rows, (uint32_t)s.table_width}; }
 bool whole_pieces(const void* p, int64_t row, int64_t head) { return ((uintptr_t)p & 15) == 0 && row % 8 == 0 && head % 8 == 0; }
 
 } // namespace
@@ -1367,45 +1369,42 @@ int bam_kv_info(bam_kv_t* kv, uint64_t* out)
     return 0;
 }
 
-int bam_kv_append(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
-                  const void* d_k, int64_t k_row, int64_t k_head, const void* d_v, int64_t v_row, int64_t v_head,
-                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, void* d_q_out, const void* d_q_norm, const void* d_k_norm, float eps,
-                  const float* d_cos, const float* d_sin, uint64_t n_positions, uint32_t rot, int pairs, void* stream)
+int bam_kv_append(bam_kv_t* kv, const bam_kv_append_t* what, void* stream)
 {
-    if (int e = bad_seqs("bam_kv_append", kv, n_seqs, n_rows, d_starts, d_lens, d_table, table_stride, table_width)) return e;
-    if (!n_rows) return 0;
-    if (!d_k || !d_v || (d_q && !d_q_out) || (d_q && !q_heads) || (rot && (!d_cos || !d_sin))) return fail(EINVAL, "bam_kv_append: null argument");
-    if (rot % 16 || rot > kv->g.dim) return fail(EINVAL, "bam_kv_append: the rotated part must be a multiple of 16, at most the head dimension");
-    if (((uintptr_t)d_q_norm | (uintptr_t)d_k_norm | (uintptr_t)d_cos | (uintptr_t)d_sin | (uintptr_t)d_q_out) & 15) return fail(EINVAL, "bam_kv_append: weights, tables and output must be aligned to 16 bytes");
-    if (n_positions > 0x7fffffffull) return fail(EINVAL, "bam_kv_append: more positions than 31 bits count");
+    if (!kv || !what) return fail(EINVAL, "bam_kv_append: null argument");
+    const bam_kv_append_t& w = *what;
+    if (int e = bad_seqs("bam_kv_append", kv, w.seqs)) return e;
+    if (!w.seqs.n_rows) return 0;
+    if (!w.d_k || !w.d_v || (w.d_q && (!w.d_q_out || !w.q_heads)) || (w.rot && (!w.d_cos || !w.d_sin))) return fail(EINVAL, "bam_kv_append: null argument");
+    if (w.rot % 16 || w.rot > kv->g.dim) return fail(EINVAL, "bam_kv_append: the rotated part must be a multiple of 16, at most the head dimension");
+    if (((uintptr_t)w.d_q_norm | (uintptr_t)w.d_k_norm | (uintptr_t)w.d_cos | (uintptr_t)w.d_sin | (uintptr_t)w.d_q_out) & 15) return fail(EINVAL, "bam_kv_append: weights, tables and output must be aligned to 16 bytes");
+    if (w.n_positions > 0x7fffffffull || (w.rot && !w.n_positions)) return fail(EINVAL, "bam_kv_append: no positions, or more than 31 bits count");
     BAM_API_BEGIN
-    kv_seqs s{d_starts, d_lens, d_table, table_stride, (uint32_t)n_seqs, (uint32_t)n_rows, (uint32_t)table_width};
     kv_rows io{};
-    io.q = (const uint16_t*)d_q; io.k = (const uint16_t*)d_k; io.v = (const uint16_t*)d_v;
-    io.q_row = q_row; io.q_head = q_head; io.k_row = k_row; io.k_head = k_head; io.v_row = v_row; io.v_head = v_head;
-    io.q_out = (uint16_t*)d_q_out; io.q_norm = (const uint16_t*)d_q_norm; io.k_norm = (const uint16_t*)d_k_norm;
-    io.cos = d_cos; io.sin = d_sin; io.positions = (uint32_t)n_positions; io.q_heads = q_heads; io.rot = rot; io.pairs = pairs != 0; io.eps = eps;
-    io.aligned = whole_pieces(d_k, k_row, k_head) && whole_pieces(d_v, v_row, v_head) && (!d_q || whole_pieces(d_q, q_row, q_head));
-    launch_rows<true>(kv, s, io, (hipStream_t)stream);
+    io.q = (const uint16_t*)w.d_q; io.k = (const uint16_t*)w.d_k; io.v = (const uint16_t*)w.d_v;
+    io.q_row = w.q_row; io.q_head = w.q_head; io.k_row = w.k_row; io.k_head = w.k_head; io.v_row = w.v_row; io.v_head = w.v_head;
+    io.q_out = (uint16_t*)w.d_q_out; io.q_norm = (const uint16_t*)w.d_q_norm; io.k_norm = (const uint16_t*)w.d_k_norm;
+    io.cos = w.d_cos; io.sin = w.d_sin; io.positions = (uint32_t)w.n_positions; io.q_heads = w.q_heads; io.rot = w.rot; io.pairs = w.pairs != 0; io.eps = w.eps;
+    io.aligned = whole_pieces(w.d_k, w.k_row, w.k_head) && whole_pieces(w.d_v, w.v_row, w.v_head) && (!w.d_q || whole_pieces(w.d_q, w.q_row, w.q_head));
+    launch_rows<true>(kv, seqs_of(w.seqs), io, (hipStream_t)stream);
     hip_err_chk(hipGetLastError());
     BAM_API_END
 }
 
-int bam_kv_read(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
-                void* d_k, void* d_v, void* stream)
+int bam_kv_read(bam_kv_t* kv, const bam_kv_seqs_t* seqs, void* d_k, void* d_v, void* stream)
 {
-    if (int e = bad_seqs("bam_kv_read", kv, n_seqs, n_rows, d_starts, d_lens, d_table, table_stride, table_width)) return e;
-    if (!n_rows) return 0;
+    if (!kv || !seqs) return fail(EINVAL, "bam_kv_read: null argument");
+    if (int e = bad_seqs("bam_kv_read", kv, *seqs)) return e;
+    if (!seqs->n_rows) return 0;
     if (!d_k || !d_v) return fail(EINVAL, "bam_kv_read: null argument");
     if (((uintptr_t)d_k | (uintptr_t)d_v) & 15) return fail(EINVAL, "bam_kv_read: output must be aligned to 16 bytes");
     BAM_API_BEGIN
-    kv_seqs s{d_starts, d_lens, d_table, table_stride, (uint32_t)n_seqs, (uint32_t)n_rows, (uint32_t)table_width};
     kv_rows io{};
     io.k = (const uint16_t*)d_k; io.v = (const uint16_t*)d_v;
     io.k_row = io.v_row = (int64_t)kv->g.heads * kv->g.dim;
     io.k_head = io.v_head = kv->g.dim;
     io.aligned = 1;
-    launch_rows<false>(kv, s, io, (hipStream_t)stream);
+    launch_rows<false>(kv, seqs_of(*seqs), io, (hipStream_t)stream);
     hip_err_chk(hipGetLastError());
     BAM_API_END
 }
@@ -1418,33 +1417,32 @@ int bam_kv_attend_bytes(bam_kv_t* kv, uint64_t n_seqs, uint64_t max_new, uint32_
     return 0;
 }
 
-int bam_kv_attend(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
-                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, uint64_t max_new, uint64_t max_len, float scale, uint32_t window, uint32_t sinks,
-                  void* d_out, float* d_lse, void* d_work, uint64_t work_bytes, void* stream)
+int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream)
 {
-    if (int e = bad_seqs("bam_kv_attend", kv, n_seqs, n_rows, d_starts, d_lens, d_table, table_stride, table_width)) return e;
-    if (!n_rows || !n_seqs) return 0;
-    if (!d_q || !d_out) return fail(EINVAL, "bam_kv_attend: null argument");
-    if (!q_heads || q_heads % kv->g.heads) return fail(EINVAL, "bam_kv_attend: heads of queries must be a multiple of the heads of keys");
-    if (!(scale == scale) || scale - scale != 0) return fail(EINVAL, "bam_kv_attend: scale must be finite");
-    if (window > 0x7fffffffu || sinks > 0x7fffffffu || max_len > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: window, sinks and lengths are 31-bit numbers");
-    if (((uintptr_t)d_out | (uintptr_t)d_work) & 15) return fail(EINVAL, "bam_kv_attend: output and workspace must be aligned to 16 bytes");
-    if (!d_starts) max_new = 1;
-    if (!max_new || max_new > n_rows) return fail(EINVAL, "bam_kv_attend: max_new must be at least 1 and at most the number of rows");
-    if (max_new * (q_heads / kv->g.heads) > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more rows than 31 bits count");
+    if (!kv || !what) return fail(EINVAL, "bam_kv_attend: null argument");
+    const bam_kv_attend_t& w = *what;
+    if (int e = bad_seqs("bam_kv_attend", kv, w.seqs)) return e;
+    if (!w.q_heads || w.q_heads % kv->g.heads) return fail(EINVAL, "bam_kv_attend: heads of queries must be a multiple of the heads of keys");
+    if (!(w.scale == w.scale) || w.scale - w.scale != 0) return fail(EINVAL, "bam_kv_attend: scale must be finite");
+    if (w.window > 0x7fffffffu || w.sinks > 0x7fffffffu || w.max_len > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: window, sinks and lengths are 31-bit numbers");
+    if (!w.seqs.n_rows) return 0;
+    if (!w.d_q || !w.d_out || !w.d_work) return fail(EINVAL, "bam_kv_attend: null argument");
+    if (((uintptr_t)w.d_out | (uintptr_t)w.d_work) & 15) return fail(EINVAL, "bam_kv_attend: output and workspace must be aligned to 16 bytes");
+    const uint64_t max_new = w.seqs.d_starts ? w.max_new : 1;
+    if (!max_new || max_new > w.seqs.n_rows) return fail(EINVAL, "bam_kv_attend: max_new must be at least 1 and at most the number of rows");
+    if (max_new * (w.q_heads / kv->g.heads) > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more rows than 31 bits count");
     BAM_API_BEGIN
-    const kv_plan p = plan_of(kv, n_seqs, max_new, q_heads, max_len, window, sinks);
-    if (p.items * p.splits > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more workgroups than 31 bits count");
-    if (!d_work || work_bytes < p.bytes) return fail(EINVAL, "bam_kv_attend: the workspace is smaller than bam_kv_attend_bytes says");
-    kv_seqs s{d_starts, d_lens, d_table, table_stride, (uint32_t)n_seqs, (uint32_t)n_rows, (uint32_t)table_width};
+    const kv_plan p = plan_of(kv, w.seqs.n_seqs, max_new, w.q_heads, w.max_len, w.window, w.sinks);
+    if (p.items * p.splits > 0x7fffffffull || p.items * p.rows > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more workgroups than 31 bits count");
+    if (w.work_bytes < p.bytes) return fail(EINVAL, "bam_kv_attend: the workspace is smaller than bam_kv_attend_bytes says");
     kv_att a{};
-    a.q = (const uint16_t*)d_q; a.q_row = q_row; a.q_head = q_head; a.aligned = whole_pieces(d_q, q_row, q_head); a.q_heads = q_heads; a.group = q_heads / kv->g.heads;
-    a.scale = scale * 1.4426950408889634f; a.window = window; a.sinks = sinks; a.out = (uint16_t*)d_out; a.lse = d_lse;
+    a.q = (const uint16_t*)w.d_q; a.q_row = w.q_row; a.q_head = w.q_head; a.aligned = whole_pieces(w.d_q, w.q_row, w.q_head); a.q_heads = w.q_heads; a.group = w.q_heads / kv->g.heads;
+    a.scale = w.scale * 1.4426950408889634f; a.window = w.window; a.sinks = w.sinks; a.out = (uint16_t*)w.d_out; a.lse = w.d_lse;
     a.tiles = p.tiles; a.splits = p.splits; a.steps = p.steps; a.items = (uint32_t)p.items;
-    uint8_t* const w = (uint8_t*)d_work;
-    a.left = w + p.left_at; a.part_m = (float*)(w + p.m_at); a.part_l = (float*)(w + p.l_at); a.part = (float*)(w + p.part_at);
-    if (kv->f16) launch_attend<1>(kv, s, a, p, (hipStream_t)stream);
-    else launch_attend<0>(kv, s, a, p, (hipStream_t)stream);
+    uint8_t* const at = (uint8_t*)w.d_work;
+    a.left = at + p.left_at; a.part_m = (float*)(at + p.m_at); a.part_l = (float*)(at + p.l_at); a.part = (float*)(at + p.part_at);
+    if (kv->f16) launch_attend<1>(kv, seqs_of(w.seqs), a, p, (hipStream_t)stream);
+    else launch_attend<0>(kv, seqs_of(w.seqs), a, p, (hipStream_t)stream);
     hip_err_chk(hipGetLastError());
     BAM_API_END
 }

@@ -4,6 +4,7 @@ Keys and values that the page cache does not hold lie on the store and are fetch
 array.  The reference has no counterpart; the C-ABI is bam_kv_* of include/bam_amd.h.
 """
 import ctypes
+import struct
 
 import torch
 
@@ -11,6 +12,12 @@ from . import _lib
 from .host import Array, BamError, PageCache, Range, _chk, _stream, c_u64, c_vp
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+# the structs of include/bam_amd.h, packed at once: a call takes 3 us less than with a ctypes argument for each field
+_SEQS = "QQPPPqQ"
+_READ = struct.Struct("@" + _SEQS)
+_APPEND = struct.Struct("@" + _SEQS + "Pqq" * 3 + "PPPPPQIIfi")
+_ATTEND = struct.Struct("@" + _SEQS + "PqqPPPQQQIIIf")
 
 
 class KVCache:
@@ -30,6 +37,7 @@ class KVCache:
         if n_blocks is None:
             raise BamError("KVCache: n_blocks must be given")
         self.array = array
+        self._index = array.device
         self.device = torch.device("cuda", array.device)
         self.n_heads, self.head_dim, self.dtype = n_heads, head_dim, dtype
         _chk(self.L.bam_kv_create(ctypes.byref(self.h), array.h, first_page, n_blocks, n_heads, head_dim, _TYPES[dtype]), "bam_kv_create")
@@ -38,34 +46,51 @@ class KVCache:
         self.block_tokens, self.n_blocks, self.pages_per_block, self.page_size = list(out)
         self._bytes = {}
 
-    # ---- checks ----
+    # ---- checks: each property of a tensor is asked for once, they are what a small call takes on the host ----
 
     def _rows(self, t, what, heads=None):
-        if t.dim() != 3 or t.dtype != self.dtype or t.device != self.device or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+        """(rows, heads, row stride, head stride) of a tensor of rows"""
+        shape = t.shape
+        if len(shape) != 3 or t.dtype is not self.dtype or t.get_device() != self._index or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             raise BamError(f"KVCache: {what} must be [rows, {'heads' if heads is None else heads}, {self.head_dim}] of {self.dtype} on {self.device}")
-        if t.stride(2) != 1:
+        row, head, one = t.stride()
+        if one != 1:
             raise BamError(f"KVCache: the numbers of a row of {what} must be next to each other")
-        return t
+        return shape[0], shape[1], row, head
 
     def _seqs(self, n_rows, lens, table, starts):
-        if lens.dtype != torch.int32 or lens.dim() != 1 or not lens.is_contiguous() or lens.device != self.device:
+        shape, width = lens.shape, table.shape
+        if len(shape) != 1 or lens.dtype is not torch.int32 or lens.get_device() != self._index or (shape[0] > 1 and lens.stride()[0] != 1):
             raise BamError(f"KVCache: lens must be a contiguous int32 tensor on {self.device}")
-        if table.dtype != torch.int32 or table.dim() != 2 or table.device != self.device or table.shape[0] != lens.shape[0] or (table.shape[1] > 1 and table.stride(1) != 1):
-            raise BamError(f"KVCache: table must be [{lens.shape[0]}, blocks] in int32 on {self.device}, the blocks of a sequence next to each other")
+        n = shape[0]
+        if len(width) != 2 or table.dtype is not torch.int32 or table.get_device() != self._index or width[0] != n:
+            raise BamError(f"KVCache: table must be [{n}, blocks] in int32 on {self.device}")
+        stride, one = table.stride()
+        if one != 1 and width[1] > 1:
+            raise BamError("KVCache: the blocks of a sequence must be next to each other in the table")
         if starts is None:
-            if lens.shape[0] != n_rows:
+            if n != n_rows:
                 raise BamError("KVCache: without starts every sequence has one new row")
-        elif starts.dtype != torch.int32 or starts.dim() != 1 or not starts.is_contiguous() or starts.device != self.device or starts.shape[0] != lens.shape[0] + 1:
-            raise BamError(f"KVCache: starts must be {lens.shape[0] + 1} int32 numbers on {self.device}")
-        width = table.shape[1]
-        return (n_rows, lens.shape[0], None if starts is None else starts.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0), width)
+            at = 0
+        else:
+            if starts.shape != (n + 1,) or starts.dtype is not torch.int32 or starts.get_device() != self._index or (n and starts.stride()[0] != 1):
+                raise BamError(f"KVCache: starts must be {n + 1} contiguous int32 numbers on {self.device}")
+            at = starts.data_ptr()
+        return n_rows, n, at, lens.data_ptr(), table.data_ptr(), stride, width[1]
 
     def _weights(self, t, what):
         if t is None:
-            return None
-        if t.dtype != self.dtype or t.shape != (self.head_dim,) or not t.is_contiguous() or t.device != self.device:
+            return 0
+        if t.dtype is not self.dtype or t.shape != (self.head_dim,) or t.stride()[0] != 1 or t.get_device() != self._index:
             raise BamError(f"KVCache: {what} must be {self.head_dim} contiguous numbers of {self.dtype} on {self.device}")
         return t.data_ptr()
+
+    def _out(self, out, like):
+        if out is None:
+            return torch.empty(like.shape, dtype=self.dtype, device=self.device)
+        if out.shape != like.shape or out.dtype is not self.dtype or out.get_device() != self._index or not out.is_contiguous():
+            raise BamError("KVCache: out must be like q, and contiguous")
+        return out
 
     # ---- calls ----
 
@@ -73,34 +98,35 @@ class KVCache:
         """Put the new rows into the cache.  Keys, and queries if there are any, are normed per head (x * rsqrt(mean x^2 + eps) * weight) where a weight is
         given, and their first 2 * cos.shape[1] numbers are turned by the angles of their positions: pairs (i, i + half) with rotary="half",
         neighbours with "pairs"; cos and sin are [positions, half] in float32.  Returns the queries (None without)."""
-        n = self._rows(k, "k", self.n_heads).shape[0]
-        if self._rows(v, "v", self.n_heads).shape[0] != n:
+        n, _, *k_strides = self._rows(k, "k", self.n_heads)
+        v_rows, _, *v_strides = self._rows(v, "v", self.n_heads)
+        if v_rows != n:
             raise BamError("KVCache: k and v must have the same rows")
         seqs = self._seqs(n, lens, table, starts)
-        q_args = (None, 0, 0, 0, None)
         if q is not None:
-            if self._rows(q, "q").shape[0] != n or q.shape[1] == 0:
+            q_rows, q_heads, *q_strides = self._rows(q, "q")
+            if q_rows != n or q_heads == 0:
                 raise BamError("KVCache: q must have the rows of k and at least one head")
-            if out is None:
-                out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-            elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous():
-                raise BamError("KVCache: out must be like q, and contiguous")
-            q_args = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1], out.data_ptr())
+            out = self._out(out, q)
+            q_args = (q.data_ptr(), *q_strides, out.data_ptr())
         elif q_norm is not None or out is not None:
             raise BamError("KVCache: q_norm and out go with q")
-        rot = 0
-        if (cos is None) != (sin is None):
-            raise BamError("KVCache: cos and sin go together")
-        if rotary not in ("half", "pairs"):
+        else:
+            q_heads, q_args = 0, (0, 0, 0, 0)
+        if rotary != "half" and rotary != "pairs":
             raise BamError('KVCache: rotary must be "half" or "pairs"')
-        if cos is not None:
+        angles, rot = (0, 0, 0), 0
+        if cos is not None and sin is not None:
+            shape = cos.shape
             for t in (cos, sin):
-                if t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() or t.device != self.device or t.shape != cos.shape:
+                if len(shape) != 2 or t.shape != shape or t.dtype is not torch.float32 or t.get_device() != self._index or not t.is_contiguous():
                     raise BamError(f"KVCache: cos and sin must be contiguous [positions, half] in float32 on {self.device}")
-            rot = 2 * cos.shape[1]
-        _chk(self.L.bam_kv_append(self.h, *seqs, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *q_args, self._weights(q_norm, "q_norm"),
-                                  self._weights(k_norm, "k_norm"), eps, cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, cos.shape[0] if rot else 0, rot,
-                                  int(rotary == "pairs"), _stream()), "bam_kv_append")
+            angles, rot = (cos.data_ptr(), sin.data_ptr(), shape[0]), 2 * shape[1]
+        elif cos is not None or sin is not None:
+            raise BamError("KVCache: cos and sin go together")
+        what = _APPEND.pack(*seqs, k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, *q_args, self._weights(q_norm, "q_norm"), self._weights(k_norm, "k_norm"),
+                            *angles, q_heads, rot, eps, rotary == "pairs")
+        _chk(self.L.bam_kv_append(self.h, what, _stream()), "bam_kv_append")
         return out if q is not None else None
 
     def read(self, n_rows, lens, table, starts=None):
@@ -108,7 +134,7 @@ class KVCache:
         seqs = self._seqs(n_rows, lens, table, starts)
         k = torch.empty(n_rows, self.n_heads, self.head_dim, dtype=self.dtype, device=self.device)
         v = torch.empty_like(k)
-        _chk(self.L.bam_kv_read(self.h, *seqs, k.data_ptr(), v.data_ptr(), _stream()), "bam_kv_read")
+        _chk(self.L.bam_kv_read(self.h, _READ.pack(*seqs), k.data_ptr(), v.data_ptr(), _stream()), "bam_kv_read")
         return k, v
 
     def attend(self, q, lens, table, starts=None, max_new=None, max_len=None, scale=None, window=0, sinks=0, out=None, return_lse=False):
@@ -116,16 +142,13 @@ class KVCache:
         a window, those with p - t < window or t < sinks.  scale: head_dim ** -0.5 unless given.  max_new: the most new rows a sequence has (all rows unless given);
         max_len: about the longest sequence (the table's width unless given); they decide how the work is shared out.  Rows of no sequence are left as they are.
         Returns the output, or with return_lse (output, logarithm of the sum of exponentials)."""
-        n, hq = self._rows(q, "q").shape[:2]
+        n, hq, row, head = self._rows(q, "q")
         seqs = self._seqs(n, lens, table, starts)
         if hq == 0 or hq % self.n_heads:
             raise BamError(f"KVCache: the heads of q must be a multiple of {self.n_heads}")
         if window < 0 or sinks < 0 or (max_new is not None and max_new < 1) or (max_len is not None and max_len < 1):
             raise BamError("KVCache: window and sinks must not be negative, max_new and max_len at least 1")
-        if out is None:
-            out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != self.dtype or out.device != self.device or not out.is_contiguous():
-            raise BamError("KVCache: out must be like q, and contiguous")
+        out = self._out(out, q)
         lse = torch.empty(n, hq, dtype=torch.float32, device=self.device) if return_lse else None
         if n and seqs[1]:
             max_new = 1 if starts is None else min(n if max_new is None else max_new, n)
@@ -140,8 +163,9 @@ class KVCache:
                 need = self._bytes[key] = b.value
             # from torch's allocator, which keeps it for this stream, or for the graph that is being captured
             work = torch.empty(need, dtype=torch.uint8, device=self.device)
-            _chk(self.L.bam_kv_attend(self.h, *seqs, q.data_ptr(), q.stride(0), q.stride(1), hq, max_new, max_len, self.head_dim ** -0.5 if scale is None else scale, window, sinks,
-                                      out.data_ptr(), None if lse is None else lse.data_ptr(), work.data_ptr(), need, _stream()), "bam_kv_attend")
+            what = _ATTEND.pack(*seqs, q.data_ptr(), row, head, out.data_ptr(), 0 if lse is None else lse.data_ptr(), work.data_ptr(), need, max_new, max_len,
+                                hq, window, sinks, self.head_dim ** -0.5 if scale is None else scale)
+            _chk(self.L.bam_kv_attend(self.h, what, _stream()), "bam_kv_attend")
         return (out, lse) if return_lse else out
 
     def close(self):

@@ -444,19 +444,35 @@ int bam_kv_create(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t 
 void bam_kv_destroy(bam_kv_t* kv);
 /* out[0] tokens to a block, [1] blocks, [2] pages to a block, [3] bytes of a page */
 int bam_kv_info(bam_kv_t* kv, uint64_t* out);
+/* how sequences are given, first in the structs of the calls below */
+typedef struct bam_kv_seqs {
+    uint64_t n_rows, n_seqs;
+    const int32_t *d_starts, *d_lens, *d_table;
+    int64_t table_stride;
+    uint64_t table_width;
+} bam_kv_seqs_t;
 /*
  * New rows into the cache: d_v as they are; d_k, and d_q into d_q_out ([n_rows][q_heads][dim]), with d_k_norm / d_q_norm (dim numbers, or NULL) as
  * x * rsqrt(mean x^2 + eps) * w per head, then the first `rot` numbers turned by the angles of the row's position: pairs (i, i + rot/2), or with
  * `pairs` (2i, 2i+1), by d_cos / d_sin[position * rot/2 + i] (n_positions rows; a position past them gives NaN; rot 0: none).  In 32 bits, rounded once.
- * Strides are in elements; the numbers of a row are next to each other.  d_q may be NULL.
+ * Strides are in elements; the numbers of a row are next to each other.  d_q may be NULL.  A page that holds none but new rows is not read from the store.
  */
-int bam_kv_append(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
-                  const void* d_k, int64_t k_row, int64_t k_head, const void* d_v, int64_t v_row, int64_t v_head,
-                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, void* d_q_out, const void* d_q_norm, const void* d_k_norm, float eps,
-                  const float* d_cos, const float* d_sin, uint64_t n_positions, uint32_t rot, int pairs, void* stream);
+typedef struct bam_kv_append {
+    bam_kv_seqs_t seqs;
+    const void* d_k; int64_t k_row, k_head;
+    const void* d_v; int64_t v_row, v_head;
+    const void* d_q; int64_t q_row, q_head;
+    void* d_q_out;
+    const void *d_q_norm, *d_k_norm;
+    const float *d_cos, *d_sin;
+    uint64_t n_positions;
+    uint32_t q_heads, rot;
+    float eps;
+    int32_t pairs;
+} bam_kv_append_t;
+int bam_kv_append(bam_kv_t* kv, const bam_kv_append_t* what, void* stream);
 /* the rows that bam_kv_append with the same sequences writes, as the cache has them now: [n_rows][n_heads][dim] each; a row without a place comes out as zeros */
-int bam_kv_read(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
-                void* d_k, void* d_v, void* stream);
+int bam_kv_read(bam_kv_t* kv, const bam_kv_seqs_t* seqs, void* d_k, void* d_v, void* stream);
 /*
  * Attention of the newest tokens over what the cache holds: row i at position p, head h, sees the tokens t <= p of its sequence, with a window (not 0) those with
  * p - t < window or t < sinks; out = sum of softmax(scale * q.k_t) v_t, with the keys of head h / (q_heads / n_heads).  A row that sees nothing is zero.  What a
@@ -464,10 +480,18 @@ int bam_kv_read(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d
  * max_new: no sequence has more new rows (rows beyond are not written; ignored without d_starts); max_len: about how long sequences get (it decides how the
  * work is shared out, not what is read).  d_work: bam_kv_attend_bytes(...) bytes for the length of the call.
  */
+typedef struct bam_kv_attend {
+    bam_kv_seqs_t seqs;
+    const void* d_q; int64_t q_row, q_head;
+    void* d_out;
+    float* d_lse;
+    void* d_work;
+    uint64_t work_bytes, max_new, max_len;
+    uint32_t q_heads, window, sinks;
+    float scale;
+} bam_kv_attend_t;
 int bam_kv_attend_bytes(bam_kv_t* kv, uint64_t n_seqs, uint64_t max_new, uint32_t q_heads, uint64_t max_len, uint32_t window, uint32_t sinks, uint64_t* bytes);
-int bam_kv_attend(bam_kv_t* kv, uint64_t n_rows, uint64_t n_seqs, const int32_t* d_starts, const int32_t* d_lens, const int32_t* d_table, int64_t table_stride, uint64_t table_width,
-                  const void* d_q, int64_t q_row, int64_t q_head, uint32_t q_heads, uint64_t max_new, uint64_t max_len, float scale, uint32_t window, uint32_t sinks,
-                  void* d_out, float* d_lse, void* d_work, uint64_t work_bytes, void* stream);
+int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream);
 
 #ifdef __cplusplus
 }
