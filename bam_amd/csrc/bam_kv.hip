@@ -4,10 +4,11 @@
 // The cache is cut into blocks of T tokens.  A block has two pages for each key-value head: one of keys and one of values, T the largest power of
 // two for which T rows of `dim` 16-bit numbers fit a page.  Within a page the numbers lie in pieces of 16 bytes, in the order in
 // which the matrix instructions take them:
-//   keys    piece (c, t) at (c * T + t) * 16: numbers 8c .. 8c+7 of token t             c < dim / 8
+//   keys    piece (c, t) at (c * T + place(t)) * 16: numbers 8c .. 8c+7 of token t             c < dim / 8
 //   values  piece (t, d) at (t * dim + d) * 16: number d of tokens 8t .. 8t+7           t < T / 8
-// so sixteen neighbouring lanes of a wave load 256 neighbouring bytes, and what they load is an operand as it stands: with the
-// scores taken as S^T = K Q^T and the output as O^T = V^T P^T, a lane's accumulators of the scores are its part of P^T.
+// place(t) is t with its bits 2 and 3 exchanged (t itself where a page holds eight tokens).  What neighbouring lanes of a wave load lies next to each other, and
+// is an operand as it stands: with the scores taken as S^T = K Q^T and the output as O^T = V^T P^T, a lane's accumulators of the scores are its
+// part of P^T if the rows of K come in that order.
 #include "bam_capi_internal.h"
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -77,6 +78,9 @@ __device__ __forceinline__ bool page_of_block(const kv_geom& g, const kv_seqs& s
     page = g.first_page + ((uint64_t)b * g.heads + head) * 2u;
     return true;
 }
+
+/* where a token of a block lies among its block's keys */
+__device__ __forceinline__ uint32_t place_in(const kv_geom& g, const uint32_t t) { return g.tokens < 16 ? t : (t & ~12u) | (t & 4u) << 1 | (t & 8u) >> 1; }
 
 template <int F16> __device__ __forceinline__ float from16(const uint32_t x)
 {
@@ -332,12 +336,12 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
             if (keys || no_page) {
                 u32x4 x[TRIPS];
                 const uint32_t r0 = l / LPR;
-                uint8_t* const at = keys + ((uint64_t)(col / 8u) * g.tokens + in_block) * 16u;
+                uint8_t* const at = keys + (uint64_t)(col / 8u) * g.tokens * 16u;
 #pragma unroll
                 for (uint32_t e = 0; e < TRIPS; e++) {
                     const uint32_t r = r0 + e * RPW < cnt ? r0 + e * RPW : 0u;
                     if constexpr (WRITE) x[e] = load_piece<ALIGNED>(k_rows + (int64_t)r * io.k_row + col);
-                    else x[e] = no_page ? u32x4{0, 0, 0, 0} : ld_payload((const u32x4*)(at + r * 16u));
+                    else x[e] = no_page ? u32x4{0, 0, 0, 0} : ld_payload((const u32x4*)(at + place_in(g, in_block + r) * 16u));
                 }
                 u32x4 w{0, 0, 0, 0};
                 if (WRITE && io.k_norm) w = load_piece<true>(io.k_norm + col);
@@ -348,7 +352,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                     if constexpr (WRITE) {
                         const kv_turn t = turn_of(io, piece, pos + (r < cnt ? r : 0u));
                         x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.k_norm != nullptr, w, t, piece);
-                        if (r < cnt && in_row) st16_sys(at + r * 16u, x[e]);
+                        if (r < cnt && in_row) st16_sys(at + place_in(g, in_block + r) * 16u, x[e]);
                     } else if (r < cnt && in_row) *(u32x4*)(k_rows + (int64_t)r * io.k_row + col) = x[e];
                 }
             }
@@ -565,15 +569,15 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
         const uint32_t where = slot == BAM_NO_SLOT ? 0u : slot;
         for (uint32_t t0 = t_first; t0 < t_end; t0 += 32u) {
             /* this lane's tokens as a row of K (8 (row / 4) + row % 4, and 4 further on) and as its part of V (8 grp .. + 7) lie in one block each */
-            const uint32_t kt = t0 + 8u * (row >> 2), vt = t0 + 8u * grp;
+            const uint32_t kt = T < 16 ? t0 + 8u * (row >> 2) : t0 + 16u * (row >> 3), vt = t0 + 8u * grp;
             const uint32_t kb = (kt >> g.tokens_log) - b_first, vb = (vt >> g.tokens_log) - b_first;
-            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(where, kb) << g.page_log) + (((kt & (T - 1u)) + (row & 3u)) + grp * T) * 16u;
+            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(where, kb) << g.page_log) + ((kt & (T - 1u)) + (T < 16 ? row & 3u : row & 7u) + grp * T) * 16u;
             const uint8_t* vp = g.base + ((uint64_t)bam::shfl(where, 32u + vb) << g.page_log) + (((vt & (T - 1u)) >> 3) * D + row) * 16u;
             u32x4 k0[DP / 32], k1[DP / 32], vv[DP / 16];
 #pragma unroll
             for (int j = 0; j < DP / 32; j++) {
                 k0[j] = k1[j] = u32x4{0, 0, 0, 0};
-                if ((4u * j + grp) * 8u < D) { k0[j] = load_once(kp + (uint64_t)j * 64u * T); k1[j] = load_once(kp + (uint64_t)j * 64u * T + 64u); }
+                if ((4u * j + grp) * 8u < D) { k0[j] = load_once(kp + (uint64_t)j * 64u * T); k1[j] = load_once(kp + (uint64_t)j * 64u * T + (T < 16 ? 64u : 128u)); }
             }
 #pragma unroll
             for (int i = 0; i < DP / 16; i++) {
@@ -942,8 +946,8 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     next_blocks();
     bool more = there;
     if (more) { enter_next(); load_tile(0); }
-    /* K's row of this lane: of the 32 tokens, the one that puts the scores of tokens 8 half .. + 7 of each 16 into its accumulators */
-    const uint32_t k_row = (row & 0x13u) | ((row & 4u) << 1) | ((row & 8u) >> 1);
+    /* the lane's row of K among the places of 32 tokens: the one that puts the scores of tokens 8 half .. + 7 of each 16 into its accumulators */
+    const uint32_t k_row = T < 16 ? (row & 0x13u) | ((row & 4u) << 1) | ((row & 8u) >> 1) : row;
     const uint32_t k_read = (k_row >> 3) * DP * 16u + (k_row & 7u) * 16u + (half ^ (k_row >> 3 & 1u)) * 128u;
     for (uint32_t buf = 0; more; buf ^= 1u) {
         fence_meta();                            /* this wave's part of the tile is in LDS, */
@@ -1202,8 +1206,20 @@ kv_plan plan_of(const bam_kv_t* kv, const uint64_t n_seqs, const uint64_t max_ne
     p.tiles = (uint32_t)((rows + R - 1) / R);
     p.items = n_seqs * p.tiles * kv->g.heads;
     const uint64_t steps = most_steps(max_len, (R + group - 1) / group + 1, window, sinks);
-    uint64_t splits = p.waves ? 4096 / p.waves / p.items : (1024 + p.items - 1) / p.items;
-    const uint64_t most = (steps + 15) / 16;                          /* no fewer than four steps to a wave */
+    /*
+     * Workgroups of four waves: as many as keep the memory busy, and no more, since each has its latencies before its first token and behind its last, and its split is
+     * written and read again.  One to a compute unit where a step of 32 tokens is 16 KiB, two where it is 8.  32 heads on 8 of 128 numbers, one token each, with a workgroup for
+     * 1024 / 512 / 256 of the device: 8 sequences of up to 8000 tokens 71 / 61 / 56 us, 64 of up to 4099 177 / 150 / 149, one of 262121 193 / 183 / 176;
+     * heads of 64 numbers, 32 sequences of up to 4000: 67 / 51 / 61.
+     */
+    uint64_t splits = (kv->g.dim <= 64 ? 512 : 256) / p.items, least = 16;             /* no fewer than four steps to a wave */
+    /*
+     * Tiles of rows: two workgroups of four waves to a compute unit, but no splits where there is one to each already, and a split no shorter than 1024 tokens.  The same heads, with
+     * splits for 1024 / 512 / 256 workgroups whatever there is: 1000 new tokens (256 tiles) 51 / 52 / 37 us, 500 after 32500 (128 tiles) 366 / 343 / 388,
+     * 64 after 16000 (16 tiles, splits of 512 / 512 / 1024 tokens) 53 / 53 / 45.
+     */
+    if (p.waves) { splits = p.items >= 256 ? 1 : 2048 / p.waves / p.items; least = 32; }
+    const uint64_t most = (steps + least - 1) / least;
     if (splits > most) splits = most;
     if (splits > 256) splits = 256;
     if (splits < 1) splits = 1;

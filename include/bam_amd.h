@@ -431,7 +431,8 @@ double bam_target_ceiling_iops(uint64_t ns_bytes, uint32_t lba_bytes, int backin
  *
  * The cache is n_blocks blocks of T tokens in the array's pages from first_page on, 2 * n_heads pages to a block: for each head a page of
  * keys and a page of values of its T tokens, T the largest power of two for which T rows of `dim` 16-bit numbers fit a page.  Pages hold pieces of 16 bytes: of keys, piece
- * c * T + t has numbers 8c .. 8c+7 of token t; of values, piece t * dim + d has number d of tokens 8t .. 8t+7.
+ * c * T + place(t) has numbers 8c .. 8c+7 of token t, place(t) being t with bits 2 and 3 exchanged (t where T is 8); of values, piece t * dim + d has
+ * number d of tokens 8t .. 8t+7.
  *
  * Sequences: d_lens[b] counts the tokens of sequence b, the new ones among them; d_table[b * table_stride + i] is the block of its tokens iT .. iT+T-1;
  * rows d_starts[b] .. d_starts[b+1]-1 of the packed inputs and outputs are its newest tokens, in order (d_starts NULL: one each).  Blocks may be shared

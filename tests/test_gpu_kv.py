@@ -425,9 +425,10 @@ def test_a_cache_smaller_than_what_is_kept(bam, dim, page, heads, cache_pages, n
         words = c.rig.backing(2 * n_blocks * heads * page // 8).view(np.int16).reshape(n_blocks, heads, 2, page // 2)
         for b, n in enumerate(lens):
             for p in (0, n // 2, n - 1):
-                block = int(table[b, p // t])
+                block, x = int(table[b, p // t]), p % t
+                place = x if t == 8 else (x & ~12) | (x & 4) << 1 | (x & 8) >> 1
                 for h in range(heads):
-                    keys = words[block, h, 0, :t * dim].reshape(dim // 8, t, 8)[:, p % t].reshape(-1)
+                    keys = words[block, h, 0, :t * dim].reshape(dim // 8, t, 8)[:, place].reshape(-1)
                     values = words[block, h, 1, :t * dim].reshape(t // 8, dim, 8)[p % t // 8, :, p % 8]
                     assert np.array_equal(keys, c.k[block, h, p % t].view(torch.int16).numpy())
                     assert np.array_equal(values, c.v[block, h, p % t].view(torch.int16).numpy())
