@@ -579,12 +579,25 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                 k0[j] = k1[j] = u32x4{0, 0, 0, 0};
                 if ((4u * j + grp) * 8u < D) { k0[j] = load_once(kp + (uint64_t)j * 64u * T); k1[j] = load_once(kp + (uint64_t)j * 64u * T + (T < 16 ? 64u : 128u)); }
             }
+            /* (wide heads: the values behind the scores, for which they would not leave registers) */
+            constexpr bool LATE = DP > 128;
+            auto load_values = [&]() {
 #pragma unroll
-            for (int i = 0; i < DP / 16; i++) {
-                vv[i] = u32x4{0, 0, 0, 0};
-                if (16u * i + row < D) vv[i] = load_once(vp + i * 256u);
-            }
+                for (int i = 0; i < DP / 16; i++) {
+                    vv[i] = u32x4{0, 0, 0, 0};
+                    if (16u * i + row < D) vv[i] = load_once(vp + i * 256u);
+                }
+            };
+            if constexpr (!LATE) load_values();
             const bool whole = !holes && (int64_t)t0 + 31 <= sp.first_pos && (!a.window || (int64_t)sp.last_pos - t0 < a.window || t0 + 32u <= a.sinks);
+            f32x4 s0[NT], s1[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                s0[n] = s1[n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < DP / 32; j++) { s0[n] = mma<F16>(k0[j], q[n][j], s0[n]); s1[n] = mma<F16>(k1[j], q[n][j], s1[n]); }
+            }
+            if constexpr (LATE) { __builtin_amdgcn_sched_barrier(0); load_values(); }
             const bool hole = (holes >> vb) & 1u;
             bool slow = false;
             if (!whole) {
@@ -599,16 +612,14 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
 #pragma unroll
                         for (int e = 0; e < 4; e++) odd |= odd16<F16>(vv[i][e]);
                     slow = ballot(odd) != 0;
+                    if (!HELD && slow) return false;             /* row by row, in the launch that holds its pages: the sums of this one stay where they are */
                 }
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                f32x4 s0{0, 0, 0, 0}, s1{0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < DP / 32; j++) { s0 = mma<F16>(k0[j], q[n][j], s0); s1 = mma<F16>(k1[j], q[n][j], s1); }
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 4; e++) { x[e] = s0[e] * a.scale; x[4 + e] = s1[e] * a.scale; }
+                for (int e = 0; e < 4; e++) { x[e] = s0[n][e] * a.scale; x[4 + e] = s1[n][e] * a.scale; }
                 uint32_t sees = 0xffu;
                 if (!whole) {
                     sees = hole ? 0u : seen_of_eight((int32_t)vt, pos[n], low_of(a, pos[n]), (int32_t)a.sinks);
@@ -632,7 +643,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                 u32x4 p;
 #pragma unroll
                 for (int e = 0; e < 4; e++) p[e] = to16<F16>(x[2 * e], x[2 * e + 1]);
-                if (!slow) {
+                if (!HELD || !slow) {
 #pragma unroll
                     for (int i = 0; i < DP / 16; i++) o[n][i] = mma<F16>(vv[i], p, o[n][i]);
                 } else {
