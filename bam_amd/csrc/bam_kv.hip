@@ -184,7 +184,7 @@ struct kv_rows {
     const float *cos, *sin;
     uint32_t positions, q_heads, rot, pairs, aligned;      /* aligned: q, k, v in whole pieces of 16 bytes */
     float eps;
-    uint32_t window, run;               /* rows that a wave looks for beginnings of runs among, and the most rows of a run */
+    uint32_t window, piece;             /* rows that a wave looks for beginnings of runs among, and the most rows it takes at a time */
     uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes */
 };
 
@@ -265,13 +265,14 @@ __device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geo
 
 /*
  * A wave takes some heads of queries of one row, or one head's keys and values of the runs of rows that begin among io.window rows: a run is the new rows of
- * a sequence within io.run tokens of one block, eight or sixteen that begin at a multiple of that.
+ * a sequence in one block, gone through in pieces of up to io.piece tokens (eight or sixteen that begin at a multiple of that).  A page's rows all belong to one
+ * wave: a page that holds new rows only is not read, and one that a second wave found gone again would come without the rows of the first.
  */
 template <int LPR, int F16, bool WRITE, bool ALIGNED>
 __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
 {
     using namespace bam;
-    constexpr uint32_t RPW = 64 / LPR, TRIPS = 16 / RPW, DT = LPR / 8;           /* trips of a run's keys; of its values: a trip is 64 times two numbers of eight tokens */
+    constexpr uint32_t RPW = 64 / LPR, TRIPS = 16 / RPW, DT = LPR / 8;           /* trips of a piece's keys; of its values: a trip is 64 times two numbers of eight tokens */
     const uint32_t wave = first(blockIdx.x * 4u + threadIdx.x / 64u), lane = bam::lane();
     const uint32_t sub = lane / LPR, piece = lane % LPR;
     const bool in_row = piece * 8u < g.dim;
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
     kv_place p{0, 0, 0, 0};
     const uint32_t mine = (uint32_t)first_row + lane;
     const bool has = lane < io.window && mine < s.rows && place_of(s, g, mine, p);
-    const bool begins = has && ((p.pos & (io.run - 1u)) == 0 || p.pos == p.first || (s.starts && s.starts[p.seq] == (int32_t)mine));
+    const bool begins = has && ((p.pos & (g.tokens - 1u)) == 0 || p.pos == p.first || (s.starts && s.starts[p.seq] == (int32_t)mine));
     if constexpr (!WRITE) {
         /* rows without a place come out as zeros */
         for (uint64_t m = ballot(lane < io.window && mine < s.rows && !has); m; m &= m - 1)
@@ -320,16 +321,17 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
     }
     for (uint64_t m = ballot(begins); m; m &= m - 1) {
         const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), seq = bcast(p.seq, j), row = (uint32_t)first_row + j;
-        const uint32_t left = io.run - (pos & (io.run - 1u)), cnt = rest < left ? rest : left;
         uint64_t page = 0;
         const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, head, page);
-        const uint32_t in_block = pos & (g.tokens - 1u), block_first = pos - in_block;
-        uint16_t* const k_rows = (uint16_t*)io.k + (int64_t)row * io.k_row + (int64_t)head * io.k_head;
-        uint16_t* const v_rows = (uint16_t*)io.v + (int64_t)row * io.v_row + (int64_t)head * io.v_head;
-        /* of the values, a lane takes numbers d and d + 1 of the eight tokens from `tok` on, counted from the run's first row */
-        const int32_t run_first = (int32_t)(in_block & (io.run - 1u));
-        const uint32_t groups = io.run / 8u, pairs = g.dim / 2u;
-        auto use = [&](uint8_t* const keys, uint8_t* const values, const bool no_page) {
+        const uint32_t run_first = pos & (g.tokens - 1u), block_first = pos - run_first, run_end = rest < g.tokens - run_first ? run_first + rest : g.tokens;
+        const uint32_t groups = io.piece / 8u, pairs = g.dim / 2u;
+        /* a piece: `cnt` tokens from `in_block` of the block on */
+        auto use_piece = [&](uint8_t* const keys, uint8_t* const values, const bool no_page, const uint32_t in_block, const uint32_t cnt) {
+            const uint32_t off = in_block - run_first;
+            uint16_t* const k_rows = (uint16_t*)io.k + (int64_t)(row + off) * io.k_row + (int64_t)head * io.k_head;
+            uint16_t* const v_rows = (uint16_t*)io.v + (int64_t)(row + off) * io.v_row + (int64_t)head * io.v_head;
+            /* of the values, a lane takes numbers d and d + 1 of the eight tokens from `tok` on, counted from the piece's first row */
+            const int32_t piece_first = (int32_t)(in_block & (io.piece - 1u));
             /* what is worked out from the lane's number is worked out here, not kept across the miss path */
             uint32_t l = lane;
             asm volatile("" : "+v"(l));
@@ -350,7 +352,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                     if (e * RPW >= cnt) break;
                     const uint32_t r = r0 + e * RPW;
                     if constexpr (WRITE) {
-                        const kv_turn t = turn_of(io, piece, pos + (r < cnt ? r : 0u));
+                        const kv_turn t = turn_of(io, piece, pos + off + (r < cnt ? r : 0u));
                         x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.k_norm != nullptr, w, t, piece);
                         if (r < cnt && in_row) st16_sys(at + place_in(g, in_block + r) * 16u, x[e]);
                     } else if (r < cnt && in_row) *(u32x4*)(k_rows + (int64_t)r * io.k_row + col) = x[e];
@@ -360,7 +362,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
 #pragma unroll
                 for (uint32_t e = 0; e < DT; e++) {
                     const uint32_t y = e * 64u + l, group = y / pairs, d = y % pairs * 2u;
-                    const int32_t tok = (int32_t)(group * 8u) - run_first;
+                    const int32_t tok = (int32_t)(group * 8u) - piece_first;
                     if (group >= groups || tok + 8 <= 0 || tok >= (int32_t)cnt) continue;
                     uint8_t* const at = values + ((uint64_t)((in_block + tok) >> 3) * g.dim + d) * 16u;
                     uint16_t* const rows = v_rows + d;
@@ -401,6 +403,14 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                             }
                     }
                 }
+            }
+        };
+        auto use = [&](uint8_t* const keys, uint8_t* const values, const bool no_page) {
+            for (uint32_t at = run_first; at < run_end;) {
+                uint32_t end = (at | (io.piece - 1u)) + 1u;
+                if (end > run_end) end = run_end;
+                use_piece(keys, values, no_page, at, end - at);
+                at = end;
             }
         };
         if (there) {
@@ -1320,8 +1330,8 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
     /* few rows: a trip of heads to a wave, a row to a wave; many: eight trips, and the runs that begin among sixteen rows */
     io.q_heads_each = io.q && (uint64_t)s.rows * io.q_heads > 16384 ? 8 * rpw : rpw;
     io.q_waves = io.q ? (uint32_t)((io.q_heads + io.q_heads_each - 1) / io.q_heads_each * s.rows) : 0;
-    io.run = kv->g.tokens < 16 ? 8 : 16;
-    io.window = s.starts && s.rows / s.n >= 8 ? io.run : 1;
+    io.piece = kv->g.tokens < 16 ? 8 : 16;
+    io.window = s.starts && s.rows / s.n >= 8 ? (kv->g.tokens < 64 ? kv->g.tokens : 64) : 1;
     const uint64_t waves = (uint64_t)io.q_waves + (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads;
     if (waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
     const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);

@@ -435,6 +435,22 @@ def test_a_cache_smaller_than_what_is_kept(bam, dim, page, heads, cache_pages, n
         assert not c.rig.c.aborted()
 
 
+@pytest.mark.parametrize("dim,page", [(128, 4096), (64, 4096), (32, 4096), (64, 16384), (256, 4096)])
+@pytest.mark.parametrize("odd", [0, 5])
+def test_new_blocks_that_do_not_fit(bam, dim, page, odd):
+    """many blocks at once into a cache that holds a few of their pages: whoever writes a page, its rows are all there when it has gone to the store and come back"""
+    import torch
+    t = 1 << ((page // (2 * dim)).bit_length() - 1)
+    lens = [20 * t + odd, 15 * t - odd, 9 * t + odd]
+    with Cache(bam, 64, 2, dim, "f16", page, cache_pages=64 if t == 8 else 32, backing=True) as c:
+        table = _table(lens, c.t, 64)
+        for seed in (1, 2, 3):
+            k, v = c.fill(lens, table, seed=seed)
+            got_k, got_v = c.kv.read(sum(lens), _i32(lens), table.cuda(), starts=_starts(lens))
+            assert torch.equal(got_k.cpu(), k) and torch.equal(got_v.cpu(), v), seed
+        assert not c.rig.c.aborted()
+
+
 def test_new_blocks_are_not_read(bam):
     """a block whose tokens are all new needs nothing from the store; what is not written of its pages is zero"""
     import torch
