@@ -267,6 +267,8 @@ __device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geo
  * A wave takes some heads of queries of one row, or one head's keys and values of the runs of rows that begin among io.window rows: a run is the new rows of
  * a sequence in one block, gone through in pieces of up to io.piece tokens (eight or sixteen that begin at a multiple of that).  A page's rows all belong to one
  * wave: a page that holds new rows only is not read, and one that a second wave found gone again would come without the rows of the first.
+ *   Bound by memory where there are many rows: 19 459 rows of 32 heads on 8 of 128 numbers, normed and turned, 480 MB in 124 us (3.9 TB/s), 160 MB out again in 43; a wave for
+ * each four rows took 288 and 112 (each looked its sequence up for 1 KiB).  Few rows: the chain of looks, table, references, rows, 6 to 7 us.
  */
 template <int LPR, int F16, bool WRITE, bool ALIGNED>
 __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
@@ -531,6 +533,9 @@ __device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most,
  * HELD false: pages are read without a reference, a chunk of 32 blocks at a time: one look at their descriptors, an acquire (a slot may have
  * been refilled since this compute unit last read it), the reads, and a second look that has to find the same.  False if a page was missing or has gone.
  * HELD true: the pages of a.chunk blocks at a time are held, and fetched where they are missing; `gone` is set where the wait was given up.
+ *   Bound by the reads of keys and values, each once and marked as not to be kept (without the mark 10 % slower): a step's 16 KiB are on their way at once, the matrix unit is idle most of the
+ * time, and what is left of a tile of 16 rows by a group of four heads costs nothing.  128 sequences of up to 8192 tokens, 3.2 GB: 519 us, 6.2 TB/s (a copy
+ * reaches 4.9 on this card); 64 of up to 4099: 151 us, 5.3 TB/s, the longest sequence's workgroups last.  More waves to a SIMD (three, four) were slower: 564 us.
  */
 template <int DP, int F16, int NT, bool HELD>
 __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, const kv_att& a, const kv_span& sp, const uint32_t seq, const uint32_t head, const uint32_t v0, const uint32_t v1,
@@ -838,6 +843,9 @@ template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>
  * NW waves of 32 rows each, all against the same tokens, KT at a time, which the waves bring into LDS together while they work on the tile before (two
  * buffers, one barrier to a tile).  Pages lie in LDS as they lie in the cache, piece by piece.  Lane l: row l % 32 of its wave, and of each 16 tokens
  * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 64 blocks, as in kv_steps.
+ *   Bound by the matrix unit and by what its two waves to a SIMD cannot hide: 32 products of 32 cycles and some 200 other instructions, 32 of them exponentials of 16
+ * cycles, to a tile and wave.  A document of 16384 tokens, 32 heads on 8 of 128 numbers: 2.24 ms, 981 TFLOP/s of what is visible (a large product of the library's: 1218).  Rows of 32 to a
+ * wave read a tile's 32 KiB of LDS in as many cycles as its products take; eight waves to a workgroup, one to a compute unit, were a tenth slower than two of four.
  */
 template <int DP, int F16, int NW, bool EXACT>
 __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(const kv_geom g, const kv_seqs s, const kv_att a)
@@ -1140,7 +1148,8 @@ __global__ __launch_bounds__(256) void k_kv_rest(const kv_geom g, const kv_seqs 
 
 /*
  * The splits of a row joined: out = sum over splits of exp(m_s - m) O_s / sum of exp(m_s - m) l_s.  LPR lanes to a row, four numbers to a lane; WIDE: the four waves of a
- * workgroup share the splits of a row (64 of 128 splits of 32 rows: 42 us by a workgroup for all rows of a head of keys), else they have rows of their own.
+ * workgroup share the splits of a row, else they have rows of their own.  32 splits of 32 rows: 4.6 us, 4 splits of 16 000 rows 7.5 (by the workgroups that look after
+ * missing pages, an item each: 42 and 85 with 128 and 8 splits).
  */
 template <int LPR, int F16, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv_join(const kv_geom g, const kv_seqs s, const kv_att a)
