@@ -826,10 +826,10 @@ __global__ __launch_bounds__(256) void k_kv_attend(const kv_geom g, const kv_seq
 }
 
 // ---- many rows: tiles of rows against tiles of tokens in LDS ----
-/* 16 bytes a lane from memory to LDS, from base + at to lds + 16 x lane; counted by the wave's memory counter, and by nobody else: wait for all of them before a barrier */
+/* 16 bytes a lane from memory to LDS, from base + at to lds + 16 x lane, past the vector L1 as all payload is (ld_payload); counted by the wave's memory counter, and by nobody else: wait for all of them before a barrier */
 __device__ __forceinline__ void to_lds(const uint8_t* base, const uint32_t at, const uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(at), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 sc1" :: "s"(lds), "v"(at), "s"(base) : "memory");
 }
 template <int F16> __device__ __forceinline__ f32x16 mma32(const u32x4 a, const u32x4 b, const f32x16 c)
 {
@@ -842,7 +842,8 @@ template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>
 /*
  * NW waves of 32 rows each, all against the same tokens, KT at a time, which the waves bring into LDS together while they work on the tile before (two
  * buffers, one barrier to a tile).  Pages lie in LDS as they lie in the cache, piece by piece.  Lane l: row l % 32 of its wave, and of each 16 tokens
- * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 64 blocks, as in kv_steps.
+ * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 64 blocks, as in kv_steps (but past the L1, with no acquire: it invalidates more than
+ * that, and cost a tenth, and a quarter where there are 18 tiles to a workgroup).
  *   Bound by the matrix unit and by what its two waves to a SIMD cannot hide: 32 products of 32 cycles and some 200 other instructions, 32 of them exponentials of 16
  * cycles, to a tile and wave.  A document of 16384 tokens, 32 heads on 8 of 128 numbers: 2.24 ms, 981 TFLOP/s of what is visible (a large product of the library's: 1218).  Rows of 32 to a
  * wave read a tile's 32 KiB of LDS in as many cycles as its products take; eight waves to a workgroup, one to a compute unit, were a tenth slower than two of four.
@@ -947,7 +948,6 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
         k_slot = (uint32_t)(k_seen >> 32) & BAM_SLOT_MASK;
         v_slot = (uint32_t)(v_seen >> 32) & BAM_SLOT_MASK;
         n_access += 2u * popc(ballot(need));
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
         next_blocks();
     };
     /* the tile from t_next on into a buffer */
