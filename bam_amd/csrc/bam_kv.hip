@@ -484,7 +484,142 @@ template <int F16> __device__ __forceinline__ bool odd16(const uint32_t x)
     constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
     return (x & e) == e || ((x >> 16) & e) == e;
 }
-__device__ __forceinline__ u32x4 load_once(const uint8_t* p) { return __builtin_nontemporal_load((const u32x4*)p); }
+/*
+ * The pieces of a step, each at an address of the lane's own, loaded past the vector L1 like all payload and marked as not to be kept (bam_wave.h, ld_payload_nt): the
+ * keys of the two tiles of 16 tokens, and the values.  With their wait in one statement: the compiler does not count what an asm statement leaves in flight.  (Ordinary
+ * loads behind an acquire for each chunk overlap the scores with the wait for the values, and lost 3 to 30 % to what an acquire invalidates.)
+ * SECOND: from a token's keys to the second tile's, 128 bytes, or 64 where a block has eight tokens.
+ */
+template <int SECOND> __device__ __forceinline__ void load_step(const uint8_t* const (&k)[2], const uint8_t* const (&v)[4], u32x4 (&k0)[2], u32x4 (&k1)[2], u32x4 (&x)[4])
+{
+    if constexpr (SECOND == 64)
+        asm volatile("global_load_dwordx4 %0, %8, off sc1 nt\n\t"
+                     "global_load_dwordx4 %1, %9, off sc1 nt\n\t"
+                     "global_load_dwordx4 %2, %8, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %3, %9, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %4, %10, off sc1 nt\n\t"
+                     "global_load_dwordx4 %5, %11, off sc1 nt\n\t"
+                     "global_load_dwordx4 %6, %12, off sc1 nt\n\t"
+                     "global_load_dwordx4 %7, %13, off sc1 nt\n\t"
+                     "s_waitcnt vmcnt(0)"
+                     : "=&v"(k0[0]), "=&v"(k0[1]), "=&v"(k1[0]), "=&v"(k1[1]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+                     : "v"(k[0]), "v"(k[1]), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]) : "memory");
+    if constexpr (SECOND == 128)
+        asm volatile("global_load_dwordx4 %0, %8, off sc1 nt\n\t"
+                     "global_load_dwordx4 %1, %9, off sc1 nt\n\t"
+                     "global_load_dwordx4 %2, %8, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %3, %9, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %4, %10, off sc1 nt\n\t"
+                     "global_load_dwordx4 %5, %11, off sc1 nt\n\t"
+                     "global_load_dwordx4 %6, %12, off sc1 nt\n\t"
+                     "global_load_dwordx4 %7, %13, off sc1 nt\n\t"
+                     "s_waitcnt vmcnt(0)"
+                     : "=&v"(k0[0]), "=&v"(k0[1]), "=&v"(k1[0]), "=&v"(k1[1]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+                     : "v"(k[0]), "v"(k[1]), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]) : "memory");
+}
+template <int SECOND> __device__ __forceinline__ void load_step(const uint8_t* const (&k)[4], const uint8_t* const (&v)[8], u32x4 (&k0)[4], u32x4 (&k1)[4], u32x4 (&x)[8])
+{
+    if constexpr (SECOND == 64)
+        asm volatile("global_load_dwordx4 %0, %16, off sc1 nt\n\t"
+                     "global_load_dwordx4 %1, %17, off sc1 nt\n\t"
+                     "global_load_dwordx4 %2, %18, off sc1 nt\n\t"
+                     "global_load_dwordx4 %3, %19, off sc1 nt\n\t"
+                     "global_load_dwordx4 %4, %16, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %5, %17, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %6, %18, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %7, %19, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %8, %20, off sc1 nt\n\t"
+                     "global_load_dwordx4 %9, %21, off sc1 nt\n\t"
+                     "global_load_dwordx4 %10, %22, off sc1 nt\n\t"
+                     "global_load_dwordx4 %11, %23, off sc1 nt\n\t"
+                     "global_load_dwordx4 %12, %24, off sc1 nt\n\t"
+                     "global_load_dwordx4 %13, %25, off sc1 nt\n\t"
+                     "global_load_dwordx4 %14, %26, off sc1 nt\n\t"
+                     "global_load_dwordx4 %15, %27, off sc1 nt\n\t"
+                     "s_waitcnt vmcnt(0)"
+                     : "=&v"(k0[0]), "=&v"(k0[1]), "=&v"(k0[2]), "=&v"(k0[3]), "=&v"(k1[0]), "=&v"(k1[1]), "=&v"(k1[2]), "=&v"(k1[3]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+                     : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]) : "memory");
+    if constexpr (SECOND == 128)
+        asm volatile("global_load_dwordx4 %0, %16, off sc1 nt\n\t"
+                     "global_load_dwordx4 %1, %17, off sc1 nt\n\t"
+                     "global_load_dwordx4 %2, %18, off sc1 nt\n\t"
+                     "global_load_dwordx4 %3, %19, off sc1 nt\n\t"
+                     "global_load_dwordx4 %4, %16, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %5, %17, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %6, %18, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %7, %19, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %8, %20, off sc1 nt\n\t"
+                     "global_load_dwordx4 %9, %21, off sc1 nt\n\t"
+                     "global_load_dwordx4 %10, %22, off sc1 nt\n\t"
+                     "global_load_dwordx4 %11, %23, off sc1 nt\n\t"
+                     "global_load_dwordx4 %12, %24, off sc1 nt\n\t"
+                     "global_load_dwordx4 %13, %25, off sc1 nt\n\t"
+                     "global_load_dwordx4 %14, %26, off sc1 nt\n\t"
+                     "global_load_dwordx4 %15, %27, off sc1 nt\n\t"
+                     "s_waitcnt vmcnt(0)"
+                     : "=&v"(k0[0]), "=&v"(k0[1]), "=&v"(k0[2]), "=&v"(k0[3]), "=&v"(k1[0]), "=&v"(k1[1]), "=&v"(k1[2]), "=&v"(k1[3]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+                     : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]) : "memory");
+}
+template <int SECOND> __device__ __forceinline__ void load_keys(const uint8_t* const (&k)[8], u32x4 (&k0)[8], u32x4 (&k1)[8])
+{
+    if constexpr (SECOND == 64)
+        asm volatile("global_load_dwordx4 %0, %16, off sc1 nt\n\t"
+                     "global_load_dwordx4 %1, %17, off sc1 nt\n\t"
+                     "global_load_dwordx4 %2, %18, off sc1 nt\n\t"
+                     "global_load_dwordx4 %3, %19, off sc1 nt\n\t"
+                     "global_load_dwordx4 %4, %20, off sc1 nt\n\t"
+                     "global_load_dwordx4 %5, %21, off sc1 nt\n\t"
+                     "global_load_dwordx4 %6, %22, off sc1 nt\n\t"
+                     "global_load_dwordx4 %7, %23, off sc1 nt\n\t"
+                     "global_load_dwordx4 %8, %16, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %9, %17, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %10, %18, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %11, %19, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %12, %20, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %13, %21, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %14, %22, off offset:64 sc1 nt\n\t"
+                     "global_load_dwordx4 %15, %23, off offset:64 sc1 nt\n\t"
+                     "s_waitcnt vmcnt(0)"
+                     : "=&v"(k0[0]), "=&v"(k0[1]), "=&v"(k0[2]), "=&v"(k0[3]), "=&v"(k0[4]), "=&v"(k0[5]), "=&v"(k0[6]), "=&v"(k0[7]), "=&v"(k1[0]), "=&v"(k1[1]), "=&v"(k1[2]), "=&v"(k1[3]), "=&v"(k1[4]), "=&v"(k1[5]), "=&v"(k1[6]), "=&v"(k1[7])
+                     : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(k[4]), "v"(k[5]), "v"(k[6]), "v"(k[7]) : "memory");
+    if constexpr (SECOND == 128)
+        asm volatile("global_load_dwordx4 %0, %16, off sc1 nt\n\t"
+                     "global_load_dwordx4 %1, %17, off sc1 nt\n\t"
+                     "global_load_dwordx4 %2, %18, off sc1 nt\n\t"
+                     "global_load_dwordx4 %3, %19, off sc1 nt\n\t"
+                     "global_load_dwordx4 %4, %20, off sc1 nt\n\t"
+                     "global_load_dwordx4 %5, %21, off sc1 nt\n\t"
+                     "global_load_dwordx4 %6, %22, off sc1 nt\n\t"
+                     "global_load_dwordx4 %7, %23, off sc1 nt\n\t"
+                     "global_load_dwordx4 %8, %16, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %9, %17, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %10, %18, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %11, %19, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %12, %20, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %13, %21, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %14, %22, off offset:128 sc1 nt\n\t"
+                     "global_load_dwordx4 %15, %23, off offset:128 sc1 nt\n\t"
+                     "s_waitcnt vmcnt(0)"
+                     : "=&v"(k0[0]), "=&v"(k0[1]), "=&v"(k0[2]), "=&v"(k0[3]), "=&v"(k0[4]), "=&v"(k0[5]), "=&v"(k0[6]), "=&v"(k0[7]), "=&v"(k1[0]), "=&v"(k1[1]), "=&v"(k1[2]), "=&v"(k1[3]), "=&v"(k1[4]), "=&v"(k1[5]), "=&v"(k1[6]), "=&v"(k1[7])
+                     : "v"(k[0]), "v"(k[1]), "v"(k[2]), "v"(k[3]), "v"(k[4]), "v"(k[5]), "v"(k[6]), "v"(k[7]) : "memory");
+}
+__device__ __forceinline__ void load_pieces(const uint8_t* const (&v)[8], u32x4* x)
+{
+    u32x4 y[8];
+    asm volatile("global_load_dwordx4 %0, %8, off sc1 nt\n\t"
+                     "global_load_dwordx4 %1, %9, off sc1 nt\n\t"
+                     "global_load_dwordx4 %2, %10, off sc1 nt\n\t"
+                     "global_load_dwordx4 %3, %11, off sc1 nt\n\t"
+                     "global_load_dwordx4 %4, %12, off sc1 nt\n\t"
+                     "global_load_dwordx4 %5, %13, off sc1 nt\n\t"
+                     "global_load_dwordx4 %6, %14, off sc1 nt\n\t"
+                     "global_load_dwordx4 %7, %15, off sc1 nt\n\t"
+                     "s_waitcnt vmcnt(0)"
+                     : "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3]), "=&v"(y[4]), "=&v"(y[5]), "=&v"(y[6]), "=&v"(y[7])
+                     : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]) : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = y[i];
+}
 
 /* of the eight tokens from t on, those up to `last` that are not before `low`, or are before `sinks` */
 __device__ __forceinline__ uint32_t seen_of_eight(const int32_t t, const int32_t last, const int32_t low, const int32_t sinks)
@@ -530,8 +665,8 @@ __device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most,
  * The largest score and the denominator (of this lane's tokens) and the sums of every row are carried over the steps in 32 bits; exp(score - max) is
  * rounded to 16 bits for the product with the values, which the matrix unit takes in 16 bits; the denominator is the sum of what was not rounded.
  *
- * HELD false: pages are read without a reference, a chunk of 32 blocks at a time: one look at their descriptors, an acquire (a slot may have
- * been refilled since this compute unit last read it), the reads, and a second look that has to find the same.  False if a page was missing or has gone.
+ * HELD false: pages are read without a reference, a chunk of 32 blocks at a time: one look at their descriptors, the reads (past the L1: a slot may have
+ * been refilled since this compute unit last read it), and a second look that has to find the same.  False if a page was missing or has gone.
  * HELD true: the pages of a.chunk blocks at a time are held, and fetched where they are missing; `gone` is set where the wait was given up.
  *   Bound by the reads of keys and values, each once and marked as not to be kept (without the mark 10 % slower): a step's 16 KiB are on their way at once, the matrix unit is idle most of the
  * time, and what is left of a tile of 16 rows by a group of four heads costs nothing.  128 sequences of up to 8192 tokens, 3.2 GB: 519 us, 6.2 TB/s (a copy
@@ -566,7 +701,6 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             if (need) seen = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
             if (ballot(need && ((uint32_t)seen >> (CNT_SHIFT + 1)) != V_NB)) return false;
             slot = need ? (uint32_t)(seen >> 32) & BAM_SLOT_MASK : 0u;
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
             n_access += need ? 1u : 0u;
             n_hit += need ? 1u : 0u;
         } else {
@@ -579,31 +713,30 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             n_hit += view.n_hit;
             view.n_access = view.n_hit = 0;
             if (ballot(need && slot == BAM_NO_SLOT)) gone = true;
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
         }
         const uint32_t where = slot == BAM_NO_SLOT ? 0u : slot;
         for (uint32_t t0 = t_first; t0 < t_end; t0 += 32u) {
             /* this lane's tokens as a row of K (8 (row / 4) + row % 4, and 4 further on) and as its part of V (8 grp .. + 7) lie in one block each */
             const uint32_t kt = T < 16 ? t0 + 8u * (row >> 2) : t0 + 16u * (row >> 3), vt = t0 + 8u * grp;
             const uint32_t kb = (kt >> g.tokens_log) - b_first, vb = (vt >> g.tokens_log) - b_first;
-            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(where, kb) << g.page_log) + ((kt & (T - 1u)) + (T < 16 ? row & 3u : row & 7u) + grp * T) * 16u;
+            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(where, kb) << g.page_log) + ((kt & (T - 1u)) + (T < 16 ? row & 3u : row & 7u)) * 16u;
             const uint8_t* vp = g.base + ((uint64_t)bam::shfl(where, 32u + vb) << g.page_log) + (((vt & (T - 1u)) >> 3) * D + row) * 16u;
             u32x4 k0[DP / 32], k1[DP / 32], vv[DP / 16];
+            /* what lies past a row's end is not loaded: its place takes the row's beginning, zero among the keys, of no row among the values */
+            const uint8_t *k_at[DP / 32], *v_at[DP / 16];
 #pragma unroll
-            for (int j = 0; j < DP / 32; j++) {
-                k0[j] = k1[j] = u32x4{0, 0, 0, 0};
-                if ((4u * j + grp) * 8u < D) { k0[j] = load_once(kp + (uint64_t)j * 64u * T); k1[j] = load_once(kp + (uint64_t)j * 64u * T + (T < 16 ? 64u : 128u)); }
+            for (uint32_t j = 0; j < DP / 32; j++) k_at[j] = kp + ((4u * j + grp) * 8u < D ? (4u * j + grp) * T * 16u : 0u);
+#pragma unroll
+            for (uint32_t i = 0; i < DP / 16; i++) v_at[i] = 16u * i < D ? vp + i * 256u : vp;
+            if constexpr (DP <= 128) {
+                if (T < 16) load_step<64>(k_at, v_at, k0, k1, vv); else load_step<128>(k_at, v_at, k0, k1, vv);
+            } else {
+                if (T < 16) load_keys<64>(k_at, k0, k1); else load_keys<128>(k_at, k0, k1);
             }
-            /* (wide heads: the values behind the scores, for which they would not leave registers) */
-            constexpr bool LATE = DP > 128;
-            auto load_values = [&]() {
+            if (D < DP) {
 #pragma unroll
-                for (int i = 0; i < DP / 16; i++) {
-                    vv[i] = u32x4{0, 0, 0, 0};
-                    if (16u * i + row < D) vv[i] = load_once(vp + i * 256u);
-                }
-            };
-            if constexpr (!LATE) load_values();
+                for (uint32_t j = 0; j < DP / 32; j++) { const bool in = (4u * j + grp) * 8u < D; k0[j] = in ? k0[j] : u32x4{0, 0, 0, 0}; k1[j] = in ? k1[j] : u32x4{0, 0, 0, 0}; }
+            }
             const bool whole = !holes && (int64_t)t0 + 31 <= sp.first_pos && (!a.window || (int64_t)sp.last_pos - t0 < a.window || t0 + 32u <= a.sinks);
             f32x4 s0[NT], s1[NT];
 #pragma unroll
@@ -612,7 +745,15 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
 #pragma unroll
                 for (int j = 0; j < DP / 32; j++) { s0[n] = mma<F16>(k0[j], q[n][j], s0[n]); s1[n] = mma<F16>(k1[j], q[n][j], s1[n]); }
             }
-            if constexpr (LATE) { __builtin_amdgcn_sched_barrier(0); load_values(); }
+            if constexpr (DP > 128) {                /* wide heads: the values behind the scores, for which they would not leave registers */
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint8_t* at[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) at[i] = v_at[8 * h + i];
+                    load_pieces(at, vv + 8 * h);
+                }
+            }
             const bool hole = (holes >> vb) & 1u;
             bool slow = false;
             if (!whole) {
