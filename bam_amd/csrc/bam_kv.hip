@@ -1267,6 +1267,25 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     if (a.lse && half == 0) a.lse[(uint64_t)(it.start + (int32_t)tok) * a.q_heads + head] = (m * c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
+/*
+ * Both launches in one, where there are no more workgroups than compute units: the miss path beside the other wants all registers of a SIMD, which one workgroup to a compute
+ * unit has.  One token over 200, heads of 64: 7.4 and 4.5 us of two launches, 7.6 of this one (10.2 a pass for 12.6); over 8000, of 128: 18.5 a pass for 20.0; 7 sequences of 3000
+ * 22.2 for 23.9; 60000 and more: the same.  Heads of 256 would spill (5 % slower over 60000), and keep two launches.
+ */
+template <int DP, int F16, int NT>
+__global__ __launch_bounds__(256) void k_kv_attend_once(const kv_geom g, const kv_seqs s, const kv_att a)
+{
+    extern __shared__ float lds[];
+    const uint32_t item = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    kv_item it;
+    bool gone = false;
+    if (!item_of(g, s, a, item, it)) return;
+    if (kv_split<DP, F16, NT, false>(g, s, a, item, it, it.r0, split, lds, gone)) return;
+    __syncthreads();
+    gone = false;
+    kv_split<DP, F16, NT, true>(g, s, a, item, it, it.r0, split, lds, gone);
+}
+
 /* what the first launch left, with its pages held; ends at once where that is nothing */
 template <int DP, int F16, int NT>
 __global__ __launch_bounds__(256) void k_kv_rest(const kv_geom g, const kv_seqs s, const kv_att a)
@@ -1424,35 +1443,41 @@ template <int DP, int F16, int NT>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan& p, hipStream_t st)
 {
     constexpr uint32_t lds = split_lds<DP, NT>(), lds_tiles = tile_lds<DP>();
-    static const bool once = [] {
+    static const bool allowed = [] {
         allow_lds(k_kv_attend<DP, F16, NT>, lds);
         allow_lds(k_kv_rest<DP, F16, NT>, lds);
+        if constexpr (DP <= 128) allow_lds(k_kv_attend_once<DP, F16, NT>, lds);
         if constexpr (NT == 2) {
             allow_lds(k_kv_attend_tiles<DP, F16, 2, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 2, false>, lds_tiles);
             allow_lds(k_kv_attend_tiles<DP, F16, 4, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4, false>, lds_tiles);
         }
         return true;
     }();
-    (void)once;
-    /* what all waves of the second launch hold at a time stays under half the cache, or they wait for each other's slots */
+    (void)allowed;
+    /* what all waves that may hold pages hold at a time stays under half the cache, or they wait for each other's slots */
     const uint32_t least = kv->g.tokens < 32 ? 32 / kv->g.tokens : 1;
-    const uint64_t half = kv->cache_pages / 2;
-    uint64_t groups = p.items < 512 ? p.items : 512;
-    if (groups * 4 * 2 * least > half) groups = half / (8 * least);
+    const uint64_t half = kv->cache_pages / 2, all = p.items * p.splits;
+    const bool once = DP <= 128 && kv->unheld && !p.waves && all <= 256 && all * 8 * least <= half;
+    uint64_t groups = once ? all : p.items < 512 ? p.items : 512;
+    if (groups * 8 * least > half) groups = half / (8 * least);
     uint64_t chunk = half / (groups * 8) / least * least;
     a.chunk = (uint32_t)(chunk > 32 ? 32 : chunk);
     a.tile_rows = p.rows;
-    const dim3 grid((uint32_t)(p.items * p.splits));
-    if (!kv->unheld) hipLaunchKernelGGL(k_kv_all_left, dim3((uint32_t)((p.items * p.splits + 255) / 256)), dim3(256), 0, st, a.left, p.items * p.splits);
-    else if (!p.waves) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
-    else if constexpr (NT == 2) {
-        const bool exact = kv->g.dim == DP;
-        if (p.waves == 2 && exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, true>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
-        else if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, false>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
-        else if (exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, true>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
-        else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, false>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+    const dim3 grid((uint32_t)all);
+    if (once) {
+        if constexpr (DP <= 128) hipLaunchKernelGGL((k_kv_attend_once<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
+    } else {
+        if (!kv->unheld) hipLaunchKernelGGL(k_kv_all_left, dim3((uint32_t)((all + 255) / 256)), dim3(256), 0, st, a.left, all);
+        else if (!p.waves) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
+        else if constexpr (NT == 2) {
+            const bool exact = kv->g.dim == DP;
+            if (p.waves == 2 && exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, true>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
+            else if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, false>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
+            else if (exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, true>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+            else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, false>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+        }
+        hipLaunchKernelGGL((k_kv_rest<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
     }
-    hipLaunchKernelGGL((k_kv_rest<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
     if (p.splits == 1) return;
     constexpr int LPR = DP / 4;
     const uint64_t rows = p.items * p.rows, rpw = 64 / LPR;
