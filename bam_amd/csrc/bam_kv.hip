@@ -1397,19 +1397,26 @@ kv_plan plan_of(const bam_kv_t* kv, const uint64_t n_seqs, const uint64_t max_ne
     p.items = n_seqs * p.tiles * kv->g.heads;
     const uint64_t steps = most_steps(max_len, (R + group - 1) / group + 1, window, sinks);
     /*
-     * Workgroups of four waves: as many as keep the memory busy, and no more, since each has its latencies before its first token and behind its last, and its split is
-     * written and read again.  One to a compute unit where a step of 32 tokens is 16 KiB, two where it is 8.  32 heads on 8 of 128 numbers, one token each, with a workgroup for
-     * 1024 / 512 / 256 of the device: 8 sequences of up to 8000 tokens 71 / 61 / 56 us, 64 of up to 4099 177 / 150 / 149, one of 262121 193 / 183 / 176;
-     * heads of 64 numbers, 32 sequences of up to 4000: 67 / 51 / 61.
+     * Workgroups: as many as keep the memory busy, and no more, since each has its latencies before its first token and behind its last, and its split is written and
+     * read again.  Few rows, four waves: one to a compute unit where a step of 32 tokens is 16 KiB, two where it is 8.  32 heads on 8 of 128 numbers, one token each, with
+     * a workgroup for 512 / 256 of the device: 8 sequences of up to 8000 tokens 51 / 45 us, one of 262121 179 / 167; heads of 64 numbers, 32 sequences of
+     * up to 4000, 1024 / 512 / 256: 30 / 28 / 34.
      */
-    uint64_t splits = (kv->g.dim <= 64 ? 512 : 256) / p.items, least = 16;             /* no fewer than four steps to a wave */
+    uint64_t splits = (kv->g.dim <= 64 ? 512 : 256) / p.items;
     /*
-     * Tiles of rows: two workgroups of four waves to a compute unit, but no splits where there is one to each already, and a split no shorter than 1024 tokens.  The same heads, with
-     * splits for 1024 / 512 / 256 workgroups whatever there is: 1000 new tokens (256 tiles) 51 / 52 / 37 us, 500 after 32500 (128 tiles) 366 / 343 / 388,
-     * 64 after 16000 (16 tiles, splits of 512 / 512 / 1024 tokens) 53 / 53 / 45.
+     * Tiles of rows: as many workgroups as the LDS of the compute units has room for, but no splits where there is one to each already.  The same heads, with
+     * splits for 1024 / 512 / 256 workgroups whatever there is: 1000 new tokens (256 tiles) 41 / 40 / 32 us, 500 after 32500 (128 tiles) 325 / 309 / 377;
+     * 10 after 16000 of eight sequences (64 tiles of two waves) 99 / 94 / 101; heads of 64 numbers, the same 45 / 59.
      */
-    if (p.waves) { splits = p.items >= 256 ? 1 : 2048 / p.waves / p.items; least = 32; }
-    const uint64_t most = (steps + least - 1) / least;
+    if (p.waves) splits = p.items >= 256 ? 1 : (kv->g.dim <= 64 ? 2048 / p.waves : 512) / p.items;
+    /*
+     * The shortest split: 16 steps, and 8 where that makes no more than 32 splits, whose join is short; for few rows only above 1024 tokens, below them the join costs more than
+     * is gained, and 32 for tiles that half the compute units have one of.  At least 32 / 16 / 8 steps: 10 new tokens of 2000 34 / 24 / 19 us, of 16000
+     * 35 / 26 / 28 (63 splits), 500 of 600 (128 tiles) 24 / 27 / 31; one token of 600, heads of 64, - / 13 / 15, of 2500 - / 14 / 13, heads of 256 - / 31 / 24.
+     */
+    uint64_t most = (steps + 15) / 16;
+    if (p.waves && p.items >= 128) most = (steps + 31) / 32;
+    else if (most < 32 && (p.waves || steps > 32)) most = (steps + 7) / 8 < 32 ? (steps + 7) / 8 : 32;
     if (splits > most) splits = most;
     if (splits > 256) splits = 256;
     if (splits < 1) splits = 1;
