@@ -669,8 +669,9 @@ __device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most,
  * been refilled since this compute unit last read it), and a second look that has to find the same.  False if a page was missing or has gone.
  * HELD true: the pages of a.chunk blocks at a time are held, and fetched where they are missing; `gone` is set where the wait was given up.
  *   Bound by the reads of keys and values, each once and marked as not to be kept (without the mark 10 % slower): a step's 16 KiB are on their way at once, the matrix unit is idle most of the
- * time, and what is left of a tile of 16 rows by a group of four heads costs nothing.  128 sequences of up to 8192 tokens, 3.2 GB: 519 us, 6.2 TB/s (a copy
- * reaches 4.9 on this card); 64 of up to 4099: 151 us, 5.3 TB/s, the longest sequence's workgroups last.  More waves to a SIMD (three, four) were slower: 564 us.
+ * time, and what is left of a tile of 16 rows by a group of four heads costs nothing.  128 sequences of up to 8192 tokens, 3.2 GB: 530 us, 6.1 TB/s (a copy
+ * reaches 4.9 on this card); 64 of up to 4099: 141 us, 5.7 TB/s, the longest sequence's workgroups last; one of 262121: 165 us, 6.5 TB/s with the join.  More waves to
+ * a SIMD (three, four) were 9 % slower.
  */
 template <int DP, int F16, int NT, bool HELD>
 __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, const kv_att& a, const kv_span& sp, const uint32_t seq, const uint32_t head, const uint32_t v0, const uint32_t v1,
@@ -983,10 +984,10 @@ template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>
 /*
  * NW waves of 32 rows each, all against the same tokens, KT at a time, which the waves bring into LDS together while they work on the tile before (two
  * buffers, one barrier to a tile).  Pages lie in LDS as they lie in the cache, piece by piece.  Lane l: row l % 32 of its wave, and of each 16 tokens
- * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 64 blocks, as in kv_steps (but past the L1, with no acquire: it invalidates more than
- * that, and cost a tenth, and a quarter where there are 18 tiles to a workgroup).
+ * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 64 blocks, as in kv_steps (past the L1; an
+ * acquire behind each first look instead, which invalidates more than that, cost a tenth, and a quarter where there are 18 tiles to a workgroup).
  *   Bound by the matrix unit and by what its two waves to a SIMD cannot hide: 32 products of 32 cycles and some 200 other instructions, 32 of them exponentials of 16
- * cycles, to a tile and wave.  A document of 16384 tokens, 32 heads on 8 of 128 numbers: 2.24 ms, 981 TFLOP/s of what is visible (a large product of the library's: 1218).  Rows of 32 to a
+ * cycles, to a tile and wave.  A document of 16384 tokens, 32 heads on 8 of 128 numbers: 2.09 ms, 1050 TFLOP/s of what is visible (a large product of the library's: 1218).  Rows of 32 to a
  * wave read a tile's 32 KiB of LDS in as many cycles as its products take; eight waves to a workgroup, one to a compute unit, were a tenth slower than two of four.
  */
 template <int DP, int F16, int NW, bool EXACT>
