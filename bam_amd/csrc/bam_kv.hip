@@ -692,10 +692,11 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
         /* lanes 0..31: the pages of keys, 32..63: of values */
         const uint32_t blk = b_first + (lane & 31u);
         uint64_t page = 0;
-        const bool asked = (lane & 31u) < n_chunk && (blk << g.tokens_log) < t_seen;
+        const bool in_run = (lane & 31u) < n_chunk && (blk << g.tokens_log) < t_end, asked = in_run && (blk << g.tokens_log) < t_seen;
         const bool need = asked && page_of_block(g, s, seq, blk, head, page);
         if (lane >= 32) page += 1;
-        const uint32_t holes = (uint32_t)ballot(asked && !need);                  /* blocks the table does not have: their tokens are not visible */
+        /* blocks the table does not have, or that lie past its end (the last step may go on behind it): their tokens are not visible */
+        const uint32_t holes = (uint32_t)ballot((asked && !need) || (in_run && blk >= s.width));
         uint32_t slot = 0;
         uint64_t seen = 0;
         if constexpr (!HELD) {
@@ -715,7 +716,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             view.n_access = view.n_hit = 0;
             if (ballot(need && slot == BAM_NO_SLOT)) gone = true;
         }
-        const uint32_t where = slot == BAM_NO_SLOT ? 0u : slot;
+        const uint32_t where = slot == BAM_NO_SLOT ? 0u : slot, step_blocks = T < 32 ? (1u << (32u >> g.tokens_log)) - 1u : 1u;
         for (uint32_t t0 = t_first; t0 < t_end; t0 += 32u) {
             /* this lane's tokens as a row of K (8 (row / 4) + row % 4, and 4 further on) and as its part of V (8 grp .. + 7) lie in one block each */
             const uint32_t kt = T < 16 ? t0 + 8u * (row >> 2) : t0 + 16u * (row >> 3), vt = t0 + 8u * grp;
@@ -738,7 +739,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
 #pragma unroll
                 for (uint32_t j = 0; j < DP / 32; j++) { const bool in = (4u * j + grp) * 8u < D; k0[j] = in ? k0[j] : u32x4{0, 0, 0, 0}; k1[j] = in ? k1[j] : u32x4{0, 0, 0, 0}; }
             }
-            const bool whole = !holes && (int64_t)t0 + 31 <= sp.first_pos && (!a.window || (int64_t)sp.last_pos - t0 < a.window || t0 + 32u <= a.sinks);
+            const bool whole = !((holes >> ((t0 >> g.tokens_log) - b_first)) & step_blocks) && (int64_t)t0 + 31 <= sp.first_pos && (!a.window || (int64_t)sp.last_pos - t0 < a.window || t0 + 32u <= a.sinks);
             f32x4 s0[NT], s1[NT];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -1061,7 +1062,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
         nt_end = (nb_first + 64u) << g.tokens_log;
         if (nt_first + run * 32u < nt_end) nt_end = nt_first + run * 32u;
         const uint32_t blk = nb_first + lane;
-        nasked = (blk << g.tokens_log) < (nt_end < sp.len ? nt_end : sp.len);
+        nasked = (blk << g.tokens_log) < nt_end && ((blk << g.tokens_log) < sp.len || blk >= s.width);      /* past the table's end: a hole */
         nblock = -1;
         if (nasked && blk < s.width) nblock = s.table[(int64_t)it.seq * s.stride + blk];
         asm volatile("" : "+v"(nblock));
@@ -1094,7 +1095,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     };
     /* the tile from t_next on into a buffer */
     uint32_t at_first = 0, at_end = 0, at_block = 0;          /* of the tile that is on its way */
-    uint64_t at_holes = 0;
+    uint64_t at_holes = 0;                                    /* among its blocks, from at_block on */
     const uint32_t k_lane0 = (lane & 7u) * 16u + (lane >> 3) * T * 16u, k_lane1 = (lane & 7u) * 16u + (lane >> 3 ^ 1u) * T * 16u;
     auto load_tile = [&](const uint32_t buf) {
         const uint32_t to = lds0 + buf * 2u * HALF;
@@ -1111,7 +1112,9 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
                 if (EXACT || 64u * i + lane < D) to_lds(v_at, (64u * i + lane) * 16u, to + HALF + u * DP * 16u + i * 1024u);
             }
         }
-        at_first = t_next; at_end = t_end; at_holes = holes; at_block = b_first;
+        at_first = t_next; at_end = t_end;
+        at_block = t_next >> g.tokens_log;
+        at_holes = (holes >> (at_block - b_first)) & ((2ull << (((t_next + KT - 1u) >> g.tokens_log) - at_block)) - 1ull);
         t_next += KT;
     };
     next_blocks();
@@ -1181,7 +1184,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
 #pragma unroll
             for (uint32_t k = 0; k < KT / 16; k++) {
                 const uint32_t tt = t0 + k * 16u + half * 8u;
-                if ((t_holes >> (((tt >> g.tokens_log) - t_block) & 63u)) & 1u) continue;
+                if ((t_holes >> ((tt >> g.tokens_log) - t_block)) & 1u) continue;
                 sees |= seen_of_eight((int32_t)tt, pos < lim ? pos : lim, low_of(a, pos), (int32_t)a.sinks) << (8u * k);
             }
 #pragma unroll
