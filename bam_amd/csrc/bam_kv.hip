@@ -54,17 +54,20 @@ __device__ __forceinline__ uint32_t seq_of(const kv_seqs& s, const uint32_t i)
     }
     return lo;
 }
-// a row's place: sequence, position, rows of its sequence from it on; false where the row has none (no such sequence, before the first position, past the table)
+// a row's place: sequence, position, rows of its sequence from it on (those that there are: starts may say more than `rows`), position of its sequence's first new
+// row; false where the row has none (no such sequence, before the first position, past the table)
 struct kv_place { uint32_t seq, pos, rest, first; };
 __device__ __forceinline__ bool place_of(const kv_seqs& s, const kv_geom& g, const uint32_t i, kv_place& p)
 {
     p.seq = seq_of(s, i);
     if (p.seq >= s.n) return false;
-    const int32_t end = s.starts ? s.starts[p.seq + 1] : (int32_t)i + 1, begin = s.starts ? s.starts[p.seq] : (int32_t)i;
+    const int32_t end = s.starts ? s.starts[p.seq + 1] : (int32_t)i + 1;
+    int32_t begin = s.starts ? s.starts[p.seq] : (int32_t)i;
+    if (begin < 0) begin = 0;
     const int64_t len = s.lens[p.seq], pos = len - (end - (int64_t)i);
     if ((int32_t)i < begin || (int64_t)i >= end || pos < 0 || (pos >> g.tokens_log) >= s.width) return false;
     p.pos = (uint32_t)pos;
-    p.rest = (uint32_t)(end - (int64_t)i);
+    p.rest = ((uint32_t)end < s.rows ? (uint32_t)end : s.rows) - i;
     const int64_t first = len - ((int64_t)end - begin);
     p.first = first < 0 ? 0u : (uint32_t)first;
     return true;
@@ -643,10 +646,9 @@ struct kv_span {
     uint32_t len;                       /* tokens to look at: up to the last row's */
     uint32_t low, front, base, n_steps; /* first token of the window; steps in front of it; first token of the step it begins in; steps */
 };
-__device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most, const int32_t len, const int32_t new_rows, const uint32_t r0, const uint32_t r1)
+__device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most, const int32_t p0 /* position of the sequence's first new row */, const uint32_t r0, const uint32_t r1)
 {
     kv_span s;
-    const int32_t p0 = len - new_rows;
     s.first_pos = p0 + (int32_t)(r0 / a.group);
     s.last_pos = p0 + (int32_t)((r1 - 1) / a.group);
     s.len = s.last_pos < 0 ? 0u : (uint32_t)s.last_pos + 1u;
@@ -829,7 +831,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
 }
 
 /* rows of an item: a head of keys, a tile of the rows (new token, head of queries) of a sequence */
-struct kv_item { uint32_t seq, head, tile, r0, r1; int32_t len, rows, start; };
+struct kv_item { uint32_t seq, head, tile, r0, r1; int32_t pos0, start; };      /* pos0: position of row `start` */
 __device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, kv_item& it)
 {
     const uint32_t tile_rows = a.tile_rows;
@@ -837,14 +839,16 @@ __device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, cons
     it.tile = item / g.heads % a.tiles;
     it.seq = item / g.heads / a.tiles;
     it.start = s.starts ? s.starts[it.seq] : (int32_t)it.seq;
-    int32_t end = s.starts ? s.starts[it.seq + 1] : (int32_t)it.seq + 1;
+    const int32_t end = s.starts ? s.starts[it.seq + 1] : (int32_t)it.seq + 1;
     if (it.start < 0) it.start = 0;
-    if (end > (int32_t)s.rows) end = (int32_t)s.rows;
-    it.rows = end - it.start;
-    it.len = s.lens[it.seq];
-    if (it.len < 0) it.len = 0;
-    if (it.rows <= 0 || it.tile * (uint64_t)tile_rows >= (uint64_t)it.rows * a.group) return false;
-    const uint32_t all = (uint32_t)it.rows * a.group;
+    /* positions count from the end that `starts` says, rows end where the rows do */
+    const int32_t last = end < (int32_t)s.rows ? end : (int32_t)s.rows;
+    if (last <= it.start) return false;
+    int32_t len = s.lens[it.seq];
+    if (len < 0) len = 0;
+    it.pos0 = len - (end - it.start);
+    const uint32_t all = (uint32_t)(last - it.start) * a.group;
+    if (it.tile * (uint64_t)tile_rows >= all) return false;
     it.r0 = it.tile * tile_rows;
     it.r1 = it.r0 + tile_rows < all ? it.r0 + tile_rows : all;
     return true;
@@ -858,9 +862,9 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
     constexpr uint32_t R = 16 * NT;
     const uint32_t lane = bam::lane(), wave = threadIdx.x / 64u, row = lane & 15u, grp = lane >> 4, D = g.dim;
     const uint32_t s1 = s0 + R < it.r1 ? s0 + R : it.r1;
-    kv_span sp = span_of(a, s.width << g.tokens_log, it.len, it.rows, it.r0, it.r1);                     /* the item's splits, */
-    sp.first_pos = it.len - it.rows + (int32_t)(s0 / a.group);                  /* as these rows see them */
-    sp.last_pos = it.len - it.rows + (int32_t)((s1 - 1) / a.group);
+    kv_span sp = span_of(a, s.width << g.tokens_log, it.pos0, it.r0, it.r1);                     /* the item's splits, */
+    sp.first_pos = it.pos0 + (int32_t)(s0 / a.group);                           /* as these rows see them */
+    sp.last_pos = it.pos0 + (int32_t)((s1 - 1) / a.group);
     uint32_t v0 = split * a.steps, v1 = v0 + a.steps;
     if (v1 > sp.n_steps || split + 1 == a.splits) v1 = sp.n_steps;              /* the last takes what is beyond the length that was announced */
     if (v0 > v1) v0 = v1;
@@ -877,7 +881,7 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
         const uint32_t r = s0 + n * 16u + row;
         const bool has = r < s1;
         const uint32_t tok = has ? r / a.group : 0u, h = it.head * a.group + (has ? r % a.group : 0u);
-        pos[n] = has ? it.len - it.rows + (int32_t)tok : -1;
+        pos[n] = has ? it.pos0 + (int32_t)tok : -1;
         const uint16_t* const from = a.q + (int64_t)(it.start + (int32_t)tok) * a.q_row + (int64_t)h * a.q_head;
 #pragma unroll
         for (int j = 0; j < DP / 32; j++) {
@@ -1006,7 +1010,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     const uint32_t item = work / per_seq * per_seq + (a.tiles - 1u - work % per_seq / g.heads) * g.heads + work % g.heads;
     kv_item it;
     if (!item_of(g, s, a, item, it)) { if (threadIdx.x == 0) a.left[(uint64_t)item * a.splits + split] = 0; return; }
-    const kv_span sp = span_of(a, s.width << g.tokens_log, it.len, it.rows, it.r0, it.r1);
+    const kv_span sp = span_of(a, s.width << g.tokens_log, it.pos0, it.r0, it.r1);
     uint32_t v0 = split * a.steps, v1 = v0 + a.steps;
     if (v1 > sp.n_steps || split + 1 == a.splits) v1 = sp.n_steps;
     if (v0 > v1) v0 = v1;
@@ -1020,7 +1024,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     const uint32_t r = w0 + row;
     const bool has = r < it.r1;
     const uint32_t tok = has ? r / a.group : 0u, head = it.head * a.group + (has ? r % a.group : 0u);
-    const int32_t p0 = it.len - it.rows, pos = has ? p0 + (int32_t)tok : -1;
+    const int32_t p0 = it.pos0, pos = has ? p0 + (int32_t)tok : -1;
     const int32_t first_pos = idle ? -1 : p0 + (int32_t)(w0 / a.group), last_pos = idle ? -1 : p0 + (int32_t)((w1 - 1) / a.group);
     const int32_t first_of_all = sp.first_pos, last_of_all = sp.last_pos;
     /* a negative scale goes into the sign of the queries: the largest score is then the largest product */

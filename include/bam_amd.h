@@ -437,7 +437,8 @@ double bam_target_ceiling_iops(uint64_t ns_bytes, uint32_t lba_bytes, int backin
  * Sequences: d_lens[b] counts the tokens of sequence b, the new ones among them; d_table[b * table_stride + i] is the block of its tokens iT .. iT+T-1;
  * rows d_starts[b] .. d_starts[b+1]-1 of the packed inputs and outputs are its newest tokens, in order (d_starts NULL: one each).  Blocks may be shared
  * between sequences.  What the tables do not hold (a block number outside the cache, a position past the table's width or before the first)
- * is neither read nor written: such tokens are not visible, and rows appended there are dropped.
+ * is neither read nor written: such tokens are not visible, and rows appended there are dropped.  Rows are n_rows: where d_starts says more, those from n_rows
+ * on are not there, and the others have the positions that d_starts gives them.
  *
  * The calls are queued on `stream` and do not wait; they may be captured into a graph.  A handle keeps nothing from call to call.  The array outlives it. */
 int bam_kv_create(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t n_blocks, uint32_t n_heads, uint32_t dim /* a multiple of 16, at most 256 */,

@@ -34,3 +34,57 @@ def test_tokens_past_the_table_are_not_seen(bam, dtype, dim, page, width, new, w
         assert bool((got_lse.cpu()[none] == -np.inf).all())
         _near(got_lse.cpu()[~none], lse[~none], 2.0 ** -16 * (1 + lse[~none].abs()))
         assert not c.rig.c.aborted()
+
+
+# ---------------------------------------------------------------- starts that say more rows than there are
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("starts,rows", [([0, 9, 40], 23), ([0, 30, 77], 12), ([-5, 20, 2 ** 31 - 1], 60), ([2 ** 31 - 1, -2 ** 31, 50], 50), ([0, 70, 40], 40)])
+def test_no_more_rows_than_there_are(bam, dtype, dim, starts, rows):
+    """what lies behind the given rows is neither read nor written; the rows that are there have the places that starts gives them, in all three calls"""
+    import ctypes
+    import torch
+    heads, lens, behind = 2, [150, 160], 80
+    with Cache(bam, 64, heads, dim, dtype) as c:
+        table = _table([200, 200], c.t, 64)
+        c.fill([200, 200], table)
+        dl, dt, ds = _i32(lens), table.cuda(), _i32(starts)
+        # (sequence, position) of each row that has one
+        places = {}
+        for i in range(rows):
+            b = 1 if starts[1] <= i else 0
+            if max(starts[b], 0) <= i < starts[b + 1] and lens[b] - (starts[b + 1] - i) >= 0:
+                places[i] = (b, lens[b] - (starts[b + 1] - i))
+        k = torch.randn(rows + behind, heads, dim).to(c.dtype)
+        k[rows:] = float("nan")
+        v = k.flip(2).contiguous()
+        c.kv.append(k.cuda()[:rows], v.cuda()[:rows], dl, dt, starts=ds)
+        for i, (b, p) in places.items():
+            c.k[int(table[b, p // c.t]), :, p % c.t] = k[i]
+            c.v[int(table[b, p // c.t]), :, p % c.t] = v[i]
+        all_k, all_v = c.kv.read(400, _i32([200, 200]), dt, starts=_i32([0, 200, 400]))
+        at = [(int(table[b, p // c.t]), p % c.t) for b in range(2) for p in range(200)]
+        assert torch.equal(all_k.cpu(), torch.stack([c.k[b, :, x] for b, x in at])) and torch.equal(all_v.cpu(), torch.stack([c.v[b, :, x] for b, x in at]))
+        # rows out, with numbers behind the two outputs that have to stay
+        from bam_amd import kv as binding
+        out = torch.full((2, rows + behind, heads, dim), 7.0, dtype=c.dtype, device="cuda")
+        what = binding._READ.pack(rows, 2, ds.data_ptr(), dl.data_ptr(), dt.data_ptr(), dt.stride(0), dt.shape[1])
+        assert c.kv.L.bam_kv_read(c.kv.h, what, ctypes.c_void_p(out[0].data_ptr()), ctypes.c_void_p(out[1].data_ptr()), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        assert bool((out[:, rows:] == 7).all())
+        for i in range(rows):
+            x = out[:, i].cpu()
+            assert torch.equal(x[0], k[i]) and torch.equal(x[1], v[i]) if i in places else not bool(x.any()), i
+        # attention: rows of no sequence stay as they are
+        q = torch.randn(rows, 2 * heads, dim).to(c.dtype)
+        got = torch.full((rows + behind, 2 * heads, dim), 7.0, dtype=c.dtype, device="cuda")
+        c.kv.attend(q.cuda(), dl, dt, starts=ds, out=got[:rows])
+        assert bool((got[rows:] == 7).all())
+        for i in range(rows):
+            b = 1 if starts[1] <= i else 0
+            if i in places:
+                b, p = places[i]
+                want, tol, _ = c.want(q[i:i + 1], [p + 1, p + 1], [1 - b, b], table)
+                _near(got[i:i + 1], want, tol, i)
+            else:
+                assert bool((got[i] == (0 if max(starts[b], 0) <= i < starts[b + 1] else 7)).all()), i
+        assert not c.rig.c.aborted()
