@@ -440,7 +440,7 @@ struct kv_att {
     float* part;                        /* [item][rows of a tile][split][dim] sums, then their maxima and denominators [item][row][split] each */
     float *part_m, *part_l;
     uint8_t* left;                      /* [item][split] pages were missing */
-    uint32_t chunk;                     /* blocks whose pages a wave holds at a time when it holds them */
+    uint32_t chunk;                     /* blocks whose pages a wave asks for at a time when it holds them */
     uint32_t items, tile_rows;
 };
 
@@ -669,7 +669,9 @@ __device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most,
  *
  * HELD false: pages are read without a reference, a chunk of 32 blocks at a time: one look at their descriptors, the reads (past the L1: a slot may have
  * been refilled since this compute unit last read it), and a second look that has to find the same.  False if a page was missing or has gone.
- * HELD true: the pages of a.chunk blocks at a time are held, and fetched where they are missing; `gone` is set where the wait was given up.
+ * HELD true: the pages of a.chunk blocks at a time are asked for, and held together if they can be had without waiting while one is held; else each is brought in and given
+ * back, and they are asked for again.  If others have pushed some of them out by then, the pages of each step are loaded one by one, those of a step that came are loaded and given
+ * back before the next is waited for: no wave waits for a slot while it keeps another, however many calls share the page cache.  `gone` is set, and the rest left, where a wait was given up.
  *   Bound by the reads of keys and values, each once and marked as not to be kept (without the mark 10 % slower): a step's 16 KiB are on their way at once, the matrix unit is idle most of the
  * time, and what is left of a tile of 16 rows by a group of four heads costs nothing.  128 sequences of up to 8192 tokens, 3.2 GB: 530 us, 6.1 TB/s (a copy
  * reaches 4.9 on this card); 64 of up to 4099: 141 us, 5.7 TB/s, the longest sequence's workgroups last; one of 262121: 165 us, 6.5 TB/s with the join.  More waves to
@@ -707,24 +709,53 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             slot = need ? (uint32_t)(seen >> 32) & BAM_SLOT_MASK : 0u;
             n_access += need ? 1u : 0u;
             n_hit += need ? 1u : 0u;
-        } else {
-            range_view<uint64_t> view;
-            view.load(g.r);
-            slot = BAM_NO_SLOT;
-            auto keep = [&](uint32_t s_) { slot = s_; return false; };
-            view.template acquire_helped<true>(page, need, false, keep, keep);
-            n_access += view.n_access;
-            n_hit += view.n_hit;
-            view.n_access = view.n_hit = 0;
-            if (ballot(need && slot == BAM_NO_SLOT)) gone = true;
         }
-        const uint32_t where = slot == BAM_NO_SLOT ? 0u : slot, step_blocks = T < 32 ? (1u << (32u >> g.tokens_log)) - 1u : 1u;
+        [[maybe_unused]] range_view<uint64_t> view;
+        bool all = true;                                                          /* the chunk's pages are held (or read without a reference) */
+        if constexpr (HELD) {
+            view.load(g.r);
+            bool left = need;
+            while (ballot(left)) {
+                const bool in = view.template acquire_some<true>(page, left, slot);
+                if (!ballot(in)) { gone = true; break; }
+                all = !ballot(need && !in);                                       /* at the first go */
+                if (all) break;
+                if (in) bam_release_refs(g.pages + page, 1, false);
+                left = left && !in;
+            }
+            n_access += view.n_access;                                            /* a page of the chunk is one access, however often it is asked for */
+            n_hit += view.n_hit;
+            if (!all && !gone) {
+                const bool in = view.template acquire_some<true>(page, need, slot);
+                all = !ballot(need && !in);
+                if (in && !all) bam_release_refs(g.pages + page, 1, false);
+            }
+            view.n_access = view.n_hit = 0;
+            if (gone) return true;
+            if (!all) slot = 0;
+        }
+        const uint32_t n_blocks = T < 32 ? 32u >> g.tokens_log : 1u, step_blocks = (1u << n_blocks) - 1u;        /* of a step */
         for (uint32_t t0 = t_first; t0 < t_end; t0 += 32u) {
             /* this lane's tokens as a row of K (8 (row / 4) + row % 4, and 4 further on) and as its part of V (8 grp .. + 7) lie in one block each */
             const uint32_t kt = T < 16 ? t0 + 8u * (row >> 2) : t0 + 16u * (row >> 3), vt = t0 + 8u * grp;
             const uint32_t kb = (kt >> g.tokens_log) - b_first, vb = (vt >> g.tokens_log) - b_first;
-            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(where, kb) << g.page_log) + ((kt & (T - 1u)) + (T < 16 ? row & 3u : row & 7u)) * 16u;
-            const uint8_t* vp = g.base + ((uint64_t)bam::shfl(where, 32u + vb) << g.page_log) + (((vt & (T - 1u)) >> 3) * D + row) * 16u;
+            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(slot, kb) << g.page_log) + ((kt & (T - 1u)) + (T < 16 ? row & 3u : row & 7u)) * 16u;
+            const uint8_t* vp = g.base + ((uint64_t)bam::shfl(slot, 32u + vb) << g.page_log) + (((vt & (T - 1u)) >> 3) * D + row) * 16u;
+            /* keys (part 0) or values (part 32) of the step, page by page: `load` for the lanes whose block came, which is `mine` for this lane */
+            auto by_page = [&](const uint32_t part, const uint32_t mine, auto&& load) {
+                bool left = need && (lane & 32u) == part && (lane & 31u) - ((t0 >> g.tokens_log) - b_first) < n_blocks;
+                while (ballot(left)) {
+                    uint32_t at = 0;
+                    const bool in = view.template acquire_some<true>(page, left, at);
+                    const uint32_t came = (uint32_t)(ballot(in) >> part);
+                    if (!came) { gone = true; break; }
+                    const uint64_t by = (uint64_t)bam::shfl(at, part + mine) << g.page_log;
+                    if ((came >> mine) & 1u) load(by);
+                    if (in) bam_release_refs(g.pages + page, 1, false);          /* waits for what was loaded */
+                    left = left && !in;
+                }
+                view.n_access = view.n_hit = 0;
+            };
             u32x4 k0[DP / 32], k1[DP / 32], vv[DP / 16];
             /* what lies past a row's end is not loaded: its place takes the row's beginning, zero among the keys, of no row among the values */
             const uint8_t *k_at[DP / 32], *v_at[DP / 16];
@@ -732,7 +763,17 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             for (uint32_t j = 0; j < DP / 32; j++) k_at[j] = kp + ((4u * j + grp) * 8u < D ? (4u * j + grp) * T * 16u : 0u);
 #pragma unroll
             for (uint32_t i = 0; i < DP / 16; i++) v_at[i] = 16u * i < D ? vp + i * 256u : vp;
-            if constexpr (DP <= 128) {
+            if (HELD && !all) {
+#pragma unroll
+                for (int j = 0; j < DP / 32; j++) k0[j] = k1[j] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < DP / 16; i++) vv[i] = u32x4{0, 0, 0, 0};
+                by_page(0, kb, [&](const uint64_t by) {
+#pragma unroll
+                    for (int j = 0; j < DP / 32; j++) { k0[j] = ld_payload((const u32x4*)(k_at[j] + by)); k1[j] = ld_payload((const u32x4*)(k_at[j] + by + (T < 16 ? 64 : 128))); }
+                });
+                if (gone) return true;
+            } else if constexpr (DP <= 128) {
                 if (T < 16) load_step<64>(k_at, v_at, k0, k1, vv); else load_step<128>(k_at, v_at, k0, k1, vv);
             } else {
                 if (T < 16) load_keys<64>(k_at, k0, k1); else load_keys<128>(k_at, k0, k1);
@@ -749,7 +790,13 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
 #pragma unroll
                 for (int j = 0; j < DP / 32; j++) { s0[n] = mma<F16>(k0[j], q[n][j], s0[n]); s1[n] = mma<F16>(k1[j], q[n][j], s1[n]); }
             }
-            if constexpr (DP > 128) {                /* wide heads: the values behind the scores, for which they would not leave registers */
+            if (HELD && !all) {
+                by_page(32, vb, [&](const uint64_t by) {
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++) vv[i] = ld_payload((const u32x4*)(v_at[i] + by));
+                });
+                if (gone) return true;
+            } else if constexpr (DP > 128) {         /* wide heads: the values behind the scores, for which they would not leave registers */
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const uint8_t* at[8];
@@ -824,7 +871,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             uint64_t now = seen;
             if (need) now = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
             if (ballot(need && ((seen ^ now) & 0xFFFFFFFFC0000000ull) != 0)) return false;
-        } else if (need && slot != BAM_NO_SLOT) bam_release_refs(g.pages + page, 1, false);
+        } else if (need && all) bam_release_refs(g.pages + page, 1, false);
         v += (t_end - t_first) / 32u;
     }
     return true;
@@ -1469,7 +1516,7 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
         return true;
     }();
     (void)allowed;
-    /* what all waves that may hold pages hold at a time stays under half the cache, or they wait for each other's slots */
+    /* what all waves that may hold pages ask for at a time stays under half the cache, or they push each other's pages out */
     const uint32_t least = kv->g.tokens < 32 ? 32 / kv->g.tokens : 1;
     const uint64_t half = kv->cache_pages / 2, all = p.items * p.splits;
     const bool once = DP <= 128 && kv->unheld && !p.waves && all <= 256 && all * 8 * least <= half;

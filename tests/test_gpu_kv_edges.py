@@ -88,3 +88,69 @@ def test_no_more_rows_than_there_are(bam, dtype, dim, starts, rows):
             else:
                 assert bool((got[i] == (0 if max(starts[b], 0) <= i < starts[b + 1] else 7)).all()), i
         assert not c.rig.c.aborted()
+
+
+# ---------------------------------------------------------------- several calls over one small page cache
+
+CALLS = 6
+
+
+@pytest.mark.parametrize("dim,page,cache_pages", [(128, 4096, 32), (256, 4096, 64), (64, 16384, 16), (64, 4096, 40), (16, 512, 33)])
+@pytest.mark.parametrize("news", [[1, 1], [3, 5], [40, 70]])
+def test_six_calls_at_a_time(bam, dim, page, cache_pages, news):
+    """layers whose blocks lie in one array behind a page cache of a few pages, each on a stream of its own: no wave keeps a page while it waits for a slot, so none waits for what the
+    others have; appends and reads among the attentions"""
+    import threading
+    import torch
+    from bam_amd.host import make_array
+    from test_gpu_parity import Rig
+    t, heads = 1 << ((page // (2 * dim)).bit_length() - 1), 2
+    lens = [9 * t + 3, 6 * t + 1]
+    n_blocks = 17
+    pages = 2 * heads * n_blocks
+    with Rig(bam, CALLS * pages * page, backing=True, n_queues=16, depth=256, stage_bytes=max(4096, min(page, 8192))) as r:
+        pc, rg, array = make_array(r.c, CALLS * pages * page // 8, page, cache_pages)
+        layers = []
+        for j in range(CALLS):
+            c = Cache.__new__(Cache)          # what the layer should hold, without a store of its own
+            c.dtype, c.heads, c.dim, c.n_blocks, c.u, c.t = torch.bfloat16, heads, dim, n_blocks, 2.0 ** -8, t
+            c.k = torch.zeros(n_blocks, heads, t, dim, dtype=c.dtype)
+            c.v = torch.zeros_like(c.k)
+            c.kv = bam.KVCache(array, heads, dim, first_page=j * pages, n_blocks=n_blocks)
+            c.table = _table(lens, t, n_blocks, seed=j)
+            k, v = c.fill(lens, c.table, seed=j)
+            c.q = torch.randn(sum(news), 2 * heads, dim, generator=torch.Generator().manual_seed(j)).to(c.dtype)
+            c.args = [x.cuda() for x in (k, v, c.q, c.table)] + [_i32(lens), _starts(lens), _starts(news)]
+            c.want_out, c.tol, _ = c.want(c.q, lens, news, c.table)
+            layers.append(c)
+        torch.cuda.synchronize()
+        got, start = [[] for _ in layers], threading.Barrier(CALLS)
+
+        def work(j):
+            torch.cuda.set_device(0)
+            c = layers[j]
+            k, v, q, table, dl, all_starts, starts = c.args
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait(60)
+                for rep in range(3):
+                    out = c.kv.attend(q, dl, table, starts=starts, max_new=max(news))
+                    back = c.kv.read(sum(lens), dl, table, starts=all_starts) if j % 3 == rep else None
+                    if j % 3 != rep:
+                        c.kv.append(k, v, dl, table, starts=all_starts)
+                    torch.cuda.current_stream().synchronize()
+                    got[j].append((out, back))
+
+        threads = [threading.Thread(target=work, args=(j,)) for j in range(CALLS)]
+        for x in threads:
+            x.start()
+        for x in threads:
+            x.join()
+        assert not r.c.aborted()
+        for j, c in enumerate(layers):
+            assert len(got[j]) == 3, j
+            for out, back in got[j]:
+                _near(out, c.want_out, c.tol, j)
+                assert back is None or (torch.equal(back[0], c.args[0]) and torch.equal(back[1], c.args[1])), j
+            c.kv.close()
+        for x in (array, rg, pc):
+            x.close()
