@@ -128,10 +128,11 @@ __attribute__((noinline)) __device__ bam_pass_t kv_pass(range_d_t<uint64_t>* r, 
  * have them, what is resident first and nothing held while the other is fetched, with what a writer of rows can say besides (`fresh`, `cleared`:
  * range_d_t::slow_step).  It stores past the caches (st16_sys and the like), so a wait for the wave's own stores is all that giving a page back needs: the
  * write-back of the cluster's cache that a release costs would come once per wave.  The miss path is a call: what the rows need is loaded in `use`, behind it (loaded
- * before, it would be kept across the call, in so many registers that one wave is left to a SIMD).
+ * before, it would be kept across the call, in so many registers that one wave is left to a SIMD).  Returns the pages that were not visited since the wait was given up
+ * (1: keys, 2: values).
  */
 template <bool WRITE, typename F>
-__device__ __forceinline__ void visit(const kv_geom& g, const uint64_t page, const bool fresh, const bool cleared, F&& use)
+__device__ __forceinline__ uint32_t visit(const kv_geom& g, const uint64_t page, const bool fresh, const bool cleared, F&& use)
 {
     using namespace bam;
     const uint32_t me = lane();
@@ -166,6 +167,7 @@ __device__ __forceinline__ void visit(const kv_geom& g, const uint64_t page, con
         __hip_atomic_fetch_add(&shard->access_cnt, 2ull, __ATOMIC_RELAXED, BAM_AGENT);
         if (n_hit) __hip_atomic_fetch_add(&shard->hit_cnt, (unsigned long long)n_hit, __ATOMIC_RELAXED, BAM_AGENT);
     }
+    return todo;
 }
 
 // the wave's accesses into the range's counters
@@ -330,8 +332,8 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
         const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, head, page);
         const uint32_t run_first = pos & (g.tokens - 1u), block_first = pos - run_first, run_end = rest < g.tokens - run_first ? run_first + rest : g.tokens;
         const uint32_t groups = io.piece / 8u, pairs = g.dim / 2u;
-        /* a piece: `cnt` tokens from `in_block` of the block on */
-        auto use_piece = [&](uint8_t* const keys, uint8_t* const values, const bool no_page, const uint32_t in_block, const uint32_t cnt) {
+        /* a piece: `cnt` tokens from `in_block` of the block on; `none`: rows out are `fill` in place of keys (1), of values (2) */
+        auto use_piece = [&](uint8_t* const keys, uint8_t* const values, const uint32_t none, const uint32_t fill, const uint32_t in_block, const uint32_t cnt) {
             const uint32_t off = in_block - run_first;
             uint16_t* const k_rows = (uint16_t*)io.k + (int64_t)(row + off) * io.k_row + (int64_t)head * io.k_head;
             uint16_t* const v_rows = (uint16_t*)io.v + (int64_t)(row + off) * io.v_row + (int64_t)head * io.v_head;
@@ -340,7 +342,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
             /* what is worked out from the lane's number is worked out here, not kept across the miss path */
             uint32_t l = lane;
             asm volatile("" : "+v"(l));
-            if (keys || no_page) {
+            if (keys || (none & 1u)) {
                 u32x4 x[TRIPS];
                 const uint32_t r0 = l / LPR;
                 uint8_t* const at = keys + (uint64_t)(col / 8u) * g.tokens * 16u;
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                 for (uint32_t e = 0; e < TRIPS; e++) {
                     const uint32_t r = r0 + e * RPW < cnt ? r0 + e * RPW : 0u;
                     if constexpr (WRITE) x[e] = load_piece<ALIGNED>(k_rows + (int64_t)r * io.k_row + col);
-                    else x[e] = no_page ? u32x4{0, 0, 0, 0} : ld_payload((const u32x4*)(at + place_in(g, in_block + r) * 16u));
+                    else x[e] = none & 1u ? u32x4{fill, fill, fill, fill} : ld_payload((const u32x4*)(at + place_in(g, in_block + r) * 16u));
                 }
                 u32x4 w{0, 0, 0, 0};
                 if (WRITE && io.k_norm) w = load_piece<true>(io.k_norm + col);
@@ -363,7 +365,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                     } else if (r < cnt && in_row) *(u32x4*)(k_rows + (int64_t)r * io.k_row + col) = x[e];
                 }
             }
-            if (values || no_page) {
+            if (values || (none & 2u)) {
 #pragma unroll
                 for (uint32_t e = 0; e < DT; e++) {
                     const uint32_t y = e * 64u + l, group = y / pairs, d = y % pairs * 2u;
@@ -398,8 +400,8 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                                 }
                         }
                     } else {
-                        u32x4 lo{0, 0, 0, 0}, hi{0, 0, 0, 0};
-                        if (!no_page) { lo = ld_payload((const u32x4*)at); hi = ld_payload((const u32x4*)(at + 16)); }
+                        u32x4 lo{fill, fill, fill, fill}, hi = lo;
+                        if (!(none & 2u)) { lo = ld_payload((const u32x4*)at); hi = ld_payload((const u32x4*)(at + 16)); }
 #pragma unroll
                         for (int32_t t = 0; t < 8; t++)
                             if (full || (tok + t >= 0 && tok + t < (int32_t)cnt)) {
@@ -410,18 +412,21 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                 }
             }
         };
-        auto use = [&](uint8_t* const keys, uint8_t* const values, const bool no_page) {
+        auto use = [&](uint8_t* const keys, uint8_t* const values, const uint32_t none, const uint32_t fill) {
             for (uint32_t at = run_first; at < run_end;) {
                 uint32_t end = (at | (io.piece - 1u)) + 1u;
                 if (end > run_end) end = run_end;
-                use_piece(keys, values, no_page, at, end - at);
+                use_piece(keys, values, none, fill, at, end - at);
                 at = end;
             }
         };
+        uint32_t none = 3;                       /* rows without a block read as zeros, */
         if (there) {
             /* a page that holds none but this call's tokens needs nothing from the store */
-            visit<WRITE>(g, page, WRITE && block_first >= bcast(p.first, j), WRITE && block_first + g.tokens > pos + rest, [&](uint8_t* keys, uint8_t* values) { use(keys, values, false); });
-        } else if constexpr (!WRITE) use(nullptr, nullptr, true);
+            none = visit<WRITE>(g, page, WRITE && block_first >= bcast(p.first, j), WRITE && block_first + g.tokens > pos + rest, [&](uint8_t* keys, uint8_t* values) { use(keys, values, 0, 0); });
+        }
+        /* those whose page could not be had as NaN */
+        if constexpr (!WRITE) if (__builtin_expect(none != 0, 0)) use(nullptr, nullptr, none, !there ? 0u : F16 ? 0x7e007e00u : 0x7fc07fc0u);
     }
 }
 

@@ -440,6 +440,8 @@ double bam_target_ceiling_iops(uint64_t ns_bytes, uint32_t lba_bytes, int backin
  * is neither read nor written: such tokens are not visible, and rows appended there are dropped.  Rows are n_rows: where d_starts says more, those from n_rows
  * on are not there, and the others have the positions that d_starts gives them.
  *
+ * Where the wait for a page is given up (bam_ctrl_aborted says so), rows that needed it come out of a read or an attention as NaN, and rows that an append had for it are dropped.
+ *
  * The calls are queued on `stream` and do not wait; they may be captured into a graph.  A handle keeps nothing from call to call.  The array outlives it. */
 int bam_kv_create(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t n_blocks, uint32_t n_heads, uint32_t dim /* a multiple of 16, at most 256 */,
                   int f16 /* 0: bfloat16, 1: float16 */);

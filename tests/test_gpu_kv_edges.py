@@ -154,3 +154,27 @@ def test_six_calls_at_a_time(bam, dim, page, cache_pages, news):
             c.kv.close()
         for x in (array, rg, pc):
             x.close()
+
+
+# ---------------------------------------------------------------- pages that could not be had
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_rows_of_lost_pages_read_as_nan(bam, dtype):
+    """the target swallows every command: the waits are bounded, rows whose keys and values never came are NaN, and those that were there are as they were.  (One wave
+    waits, for two pages, in a queue that is never full.)"""
+    import torch
+    from test_gpu_parity import Rig
+    with Rig(bam, 1 << 20, backing=True, n_queues=1, depth=1024, drop_every=1, limit=100_000) as r:
+        kv = bam.KVCache(r.array(1 << 17, 4096, 64), 1, 128, {"bf16": torch.bfloat16, "f16": torch.float16}[dtype], n_blocks=64)
+        table = torch.tensor([[3, 7]], dtype=torch.int32, device="cuda")
+        k = torch.randn(16, 1, 128).to(kv.dtype).cuda()
+        v = k.flip(2).contiguous()
+        kv.append(k, v, _i32([16]), table, starts=_starts([16]))          # a block of new rows: nothing is read
+        torch.cuda.synchronize()
+        assert not r.c.aborted()
+        got_k, got_v = kv.read(25, _i32([25]), table, starts=_starts([25]))
+        torch.cuda.synchronize()
+        assert r.c.aborted() and r.t.stats()["dropped"] >= 1
+        assert torch.equal(got_k[:16], k) and torch.equal(got_v[:16], v)
+        assert bool(torch.isnan(got_k[16:]).all()) and bool(torch.isnan(got_v[16:]).all())
+        kv.close()
