@@ -486,6 +486,14 @@ __device__ __forceinline__ float sum_of_four(float a)
     swap_rows(a, b);
     return a + b;
 }
+/*
+ * Weights go to the product with the values in 16 bits: exp2(score - maximum + WEIGHT_SHIFT).  A float16 has full precision from 2^-14 on and nothing below 2^-25, and a
+ * quarter of a million tokens of 2^-25 of the largest weigh 2^-7 of it: they are scaled up by a power of two that the type has room for (2^16), and the sums with them.  In
+ * tiles, weights are up to 2^TILE_SLACK before the maximum is followed.  What falls below 2^-25 now is 2^-39 (2^-36 in tiles) of the largest.  A bfloat16 has a float's range.
+ */
+template <int F16> constexpr float WEIGHT_SHIFT = F16 ? 14.0f : 0.0f;
+template <int F16> constexpr float TILE_SLACK = F16 ? 4.0f : 8.0f;
+template <int F16> constexpr float TILE_SHIFT = F16 ? 11.0f : 0.0f;
 /* whether one of the two 16-bit numbers is an infinity or NaN */
 template <int F16> __device__ __forceinline__ bool odd16(const uint32_t x)
 {
@@ -850,7 +858,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                 }
                 float sum = 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) { x[e] = __builtin_amdgcn_exp2f(x[e] - use); sum += x[e]; }
+                for (int e = 0; e < 8; e++) { x[e] = __builtin_amdgcn_exp2f(x[e] - use + WEIGHT_SHIFT<F16>); sum += x[e]; }
                 l[n] += sum;
                 u32x4 p;
 #pragma unroll
@@ -963,7 +971,7 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
     for (int n = 0; n < NT; n++) {
         const uint32_t r = n * 16u + row;
         const float top = fmaxf(fmaxf(ms[r], ms[R + r]), fmaxf(ms[2 * R + r], ms[3 * R + r]));
-        by[n] = __builtin_amdgcn_exp2f(m[n] - (top == -INFINITY ? 0.0f : top));
+        by[n] = __builtin_amdgcn_exp2f(m[n] - (top == -INFINITY ? 0.0f : top) - WEIGHT_SHIFT<F16>);          /* and out of the sums again */
     }
     /* a quarter of the columns each, by turns: the order in which a column's four parts are added does not depend on who comes first */
     constexpr int QUARTER = DP / 64;
@@ -992,7 +1000,7 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
         const float top = fmaxf(fmaxf(ms[r], ms[R + r]), fmaxf(ms[2 * R + r], ms[3 * R + r])), use = top == -INFINITY ? 0.0f : top;
         float den = 0;
 #pragma unroll
-        for (int w = 0; w < 4; w++) den += ls[w * R + r] * __builtin_amdgcn_exp2f(ms[w * R + r] - use);
+        for (int w = 0; w < 4; w++) den += ls[w * R + r] * __builtin_amdgcn_exp2f(ms[w * R + r] - use - WEIGHT_SHIFT<F16>);
         if (gone) den = __builtin_nanf("");
         f32x4 lo = *(const f32x4*)(os + r * DP + c), hi = *(const f32x4*)(os + r * DP + c + 4);
         if (a.splits > 1) {
@@ -1258,8 +1266,8 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             swap_halves(top, other);
             top = fmaxf(top, other);
         }
-        /* the sums are moved to a larger maximum only where it is larger by 2^8 or more: weights of up to 2^8 lose nothing */
-        if (ballot((top - m) * c > 8.0f || m == -INFINITY && top != -INFINITY)) {
+        /* the sums are moved to a larger maximum only where its weight would be above 2^TILE_SLACK: up to there weights lose nothing */
+        if (ballot((top - m) * c > TILE_SLACK<F16> || m == -INFINITY && top != -INFINITY)) {
             const float larger = fmaxf(top, m);
             const float by = larger == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - larger) * c);
             l *= by;
@@ -1268,7 +1276,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             for (uint32_t i = 0; i < DP / 32; i++) o[i] *= by;
             m = larger;
         }
-        const float mc = m == -INFINITY ? 0.0f : -m * c;
+        const float mc = m == -INFINITY ? 0.0f : __builtin_fmaf(-m, c, TILE_SHIFT<F16>);
         u32x4 p[KT / 16];
 #pragma unroll
         for (uint32_t k = 0; k < KT / 16; k++) {
@@ -1301,6 +1309,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
         l += other;
     }
     if (!has) return;
+    const float at_one = m == -INFINITY ? -INFINITY : -__builtin_fmaf(-m, c, TILE_SHIFT<F16>);      /* the score whose weight in the sums is one */
     /* lane: numbers 8i + 4 half .. + 3 of its row */
     if (a.splits > 1) {
         const uint64_t at = ((uint64_t)item * a.tile_rows + (r - it.r0)) * a.splits + split;
@@ -1309,7 +1318,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             const uint32_t d = 8u * i + 4u * half;
             if (d < D) *(f32x4*)(a.part + at * D + d) = f32x4{o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2], o[i / 4][i % 4 * 4 + 3]};
         }
-        if (half == 0) { a.part_m[at] = m * c; a.part_l[at] = l; }
+        if (half == 0) { a.part_m[at] = at_one; a.part_l[at] = l; }
         return;
     }
     const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
@@ -1324,7 +1333,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             *(uint2*)(to + d) = y;
         }
     }
-    if (a.lse && half == 0) a.lse[(uint64_t)(it.start + (int32_t)tok) * a.q_heads + head] = (m * c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    if (a.lse && half == 0) a.lse[(uint64_t)(it.start + (int32_t)tok) * a.q_heads + head] = (at_one + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 /*

@@ -178,3 +178,40 @@ def test_rows_of_lost_pages_read_as_nan(bam, dtype):
         assert torch.equal(got_k[:16], k) and torch.equal(got_v[:16], v)
         assert bool(torch.isnan(got_k[16:]).all()) and bool(torch.isnan(got_v[16:]).all())
         kv.close()
+
+
+# ---------------------------------------------------------------- weights far below the largest
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("low", [12.5, 23.4, 25.0])
+@pytest.mark.parametrize("new,n", [(1, 1 << 19), (5, 1 << 19), (40, 1 << 17), (100, 1 << 17)])
+def test_one_peak_over_a_long_flat_tail(bam, dtype, low, new, n):
+    """one token above all others, of 2^-low of its weight each, which hold up to ninety times its share of the sum or a hundredth of it: their part is not lost in the weights'
+    rounding, wherever the peak is.  Bounds: weights and output are rounded to the type once (u each), scores are off by e as in test_gpu_kv, what rounds to nothing is below 2^-36 of the
+    largest, and sums in 32 bits are off by 2^-24 for each addition: one workgroup for all adds a weight at a time in tiles, n / 4 to a lane (sums of eight by four waves for few rows), and
+    16 weighted values at a time (32 by four waves)."""
+    import torch
+    dim, u = 64, {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype]
+    per = 16384 // (2 * dim)
+    adds, mixes = (n // 4, n // 16) if new * 2 > 32 else (n // 128 + 16, n // 128)
+    with Cache(bam, n // per, 1, dim, dtype, 16384) as c:
+        c.k = c.v = None
+        table = torch.arange(n // per, dtype=torch.int32).view(1, -1)
+        q = torch.zeros(new, 2, dim, dtype=c.dtype)
+        q[:, :, 0] = 8
+        for peak in (0, 70001, n - new):
+            k, v = torch.zeros(n, 1, dim, dtype=c.dtype, device="cuda"), torch.full((n, 1, dim), -1.0, dtype=c.dtype, device="cuda")
+            k[peak, 0, 0] = low * np.log(2)          # times 8 and a scale of an eighth
+            v[peak] = 1
+            c.kv.append(k, v, _i32([n]), table.cuda(), starts=_starts([n]))
+            x = float(k[peak, 0, 0])
+            tail = (torch.arange(n - new, n, dtype=torch.float64) * np.exp(-x))[:, None, None]          # of the peak's weight
+            want = (1 - tail) / (1 + tail)
+            e = 2 * dim * 2.0 ** -24 * x
+            tol = (1.01 * u + 2.0 ** -24 * adds) * want.abs() + 1.01 * u + 2.0 ** -24 * mixes + 2.0 ** -19 + e
+            sums = x + torch.log1p(tail[:, :, 0]).expand(new, 2)
+            for max_len in (n, 1):                   # split over the length, and by one workgroup
+                got, lse = c.kv.attend(q.cuda(), _i32([n]), table.cuda(), starts=_starts([new]), max_new=new, max_len=max_len, return_lse=True)
+                _near(got, want.expand(new, 2, dim), tol.expand(new, 2, dim), (peak, max_len))
+                _near(lse, sums, 2.0 ** -24 * adds + 2.0 ** -19 + e + 2.0 ** -22 * sums.abs(), (peak, max_len))
+        assert not c.rig.c.aborted()
