@@ -991,8 +991,8 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
     }
     const uint32_t bad = *flag;
     gone = (bad & 2u) != 0;
+    if (!HELD && (bad & 1u)) return false;              /* nothing of it counts: who does it again counts */
     count_accesses(g, n_access, n_hit);
-    if (!HELD && (bad & 1u)) return false;
     const uint32_t n_rows = s1 - s0;
     for (uint32_t x = threadIdx.x; x < n_rows * (DP / 8u); x += 256u) {
         const uint32_t r = x / (DP / 8u), c = x % (DP / 8u) * 8u;

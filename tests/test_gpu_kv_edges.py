@@ -215,3 +215,23 @@ def test_one_peak_over_a_long_flat_tail(bam, dtype, low, new, n):
                 _near(got, want.expand(new, 2, dim), tol.expand(new, 2, dim), (peak, max_len))
                 _near(lse, sums, 2.0 ** -24 * adds + 2.0 ** -19 + e + 2.0 ** -22 * sums.abs(), (peak, max_len))
         assert not c.rig.c.aborted()
+
+
+# ---------------------------------------------------------------- counters
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n_seqs", [1, 200])
+def test_a_split_that_is_done_again_counts_once(bam, dim, n_seqs):
+    """an infinity among values that some rows see and others do not leaves a split to be done row by row: its pages are counted by whoever does it"""
+    import torch
+    with Cache(bam, 32, 2, dim, "bf16") as c:
+        lens = [100]
+        table = _table(lens, c.t, 32)
+        v = torch.randn(100, 2, dim).to(c.dtype)
+        v[98] = float("inf")
+        c.fill(lens, table, v=v)
+        q = torch.randn(3 * n_seqs, 4, dim).to(c.dtype).cuda()
+        c.kv.array.stats()
+        c.kv.attend(q, _i32(lens * n_seqs), table.cuda().expand(n_seqs, -1), starts=_starts([3] * n_seqs), max_new=3)
+        st = c.kv.array.stats()
+        assert st["access_cnt"] == st["hit_cnt"] == n_seqs * 2 * 2 * -(-100 // c.t), st
