@@ -446,7 +446,7 @@ struct kv_att {
     float *part_m, *part_l;
     uint8_t* left;                      /* [item][split] pages were missing */
     uint32_t chunk;                     /* blocks whose pages a wave asks for at a time when it holds them */
-    uint32_t items, tile_rows;
+    uint32_t items, tile_rows, max_new;
 };
 
 template <int F16> __device__ __forceinline__ f32x4 mma(const u32x4 a, const u32x4 b, const f32x4 c)
@@ -907,7 +907,7 @@ __device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, cons
     int32_t len = s.lens[it.seq];
     if (len < 0) len = 0;
     it.pos0 = len - (end - it.start);
-    const uint32_t all = (uint32_t)(last - it.start) * a.group;
+    const uint32_t all = ((uint32_t)(last - it.start) < a.max_new ? (uint32_t)(last - it.start) : a.max_new) * a.group;
     if (it.tile * (uint64_t)tile_rows >= all) return false;
     it.r0 = it.tile * tile_rows;
     it.r1 = it.r0 + tile_rows < all ? it.r0 + tile_rows : all;
@@ -1726,7 +1726,7 @@ int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream)
     kv_att a{};
     a.q = (const uint16_t*)w.d_q; a.q_row = w.q_row; a.q_head = w.q_head; a.aligned = whole_pieces(w.d_q, w.q_row, w.q_head); a.q_heads = w.q_heads; a.group = w.q_heads / kv->g.heads;
     a.scale = w.scale * 1.4426950408889634f; a.window = w.window; a.sinks = w.sinks; a.out = (uint16_t*)w.d_out; a.lse = w.d_lse;
-    a.tiles = p.tiles; a.splits = p.splits; a.steps = p.steps; a.items = (uint32_t)p.items;
+    a.tiles = p.tiles; a.splits = p.splits; a.steps = p.steps; a.items = (uint32_t)p.items; a.max_new = (uint32_t)max_new;
     uint8_t* const at = (uint8_t*)w.d_work;
     a.left = at + p.left_at; a.part_m = (float*)(at + p.m_at); a.part_l = (float*)(at + p.l_at); a.part = (float*)(at + p.part_at);
     if (kv->f16) launch_attend<1>(kv, seqs_of(w.seqs), a, p, (hipStream_t)stream);

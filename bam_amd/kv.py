@@ -139,7 +139,8 @@ class KVCache:
 
     def attend(self, q, lens, table, starts=None, max_new=None, max_len=None, scale=None, window=0, sinks=0, out=None, return_lse=False):
         """Attention of the newest tokens (their rows in q) over what the cache holds of their sequences: the token at position p sees t <= p and, with
-        a window, those with p - t < window or t < sinks.  scale: head_dim ** -0.5 unless given.  max_new: the most new rows a sequence has (all rows unless given);
+        a window, those with p - t < window or t < sinks.  scale: head_dim ** -0.5 unless given.  max_new: the most new rows a sequence has (all rows unless given; those beyond
+        are left as they are);
         max_len: about the longest sequence (the table's width unless given); they decide how the work is shared out.  Rows of no sequence are left as they are.
         Returns the output, or with return_lse (output, logarithm of the sum of exponentials)."""
         n, hq, row, head = self._rows(q, "q")

@@ -481,7 +481,7 @@ int bam_kv_read(bam_kv_t* kv, const bam_kv_seqs_t* seqs, void* d_k, void* d_v, v
  * Attention of the newest tokens over what the cache holds: row i at position p, head h, sees the tokens t <= p of its sequence, with a window (not 0) those with
  * p - t < window or t < sinks; out = sum of softmax(scale * q.k_t) v_t, with the keys of head h / (q_heads / n_heads).  A row that sees nothing is zero.  What a
  * row does not see has no part in it, infinities and NaN included.  d_lse (or NULL): log of the sum of exp(scale * q.k_t), [n_rows][q_heads].
- * max_new: no sequence has more new rows (rows beyond are not written; ignored without d_starts); max_len: about how long sequences get (it decides how the
+ * max_new: no sequence has more new rows (of one that has, the first max_new are written; ignored without d_starts); max_len: about how long sequences get (it decides how the
  * work is shared out, not what is read).  d_work: bam_kv_attend_bytes(...) bytes for the length of the call.
  */
 typedef struct bam_kv_attend {

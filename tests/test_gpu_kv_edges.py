@@ -235,3 +235,25 @@ def test_a_split_that_is_done_again_counts_once(bam, dim, n_seqs):
         c.kv.attend(q, _i32(lens * n_seqs), table.cuda().expand(n_seqs, -1), starts=_starts([3] * n_seqs), max_new=3)
         st = c.kv.array.stats()
         assert st["access_cnt"] == st["hit_cnt"] == n_seqs * 2 * 2 * -(-100 // c.t), st
+
+
+# ---------------------------------------------------------------- more new rows than were announced
+
+@pytest.mark.parametrize("max_new", [1, 3, 20, 40, 70])
+def test_rows_beyond_max_new_are_left(bam, max_new):
+    """few rows, tiles of two and of four waves: of each sequence the first max_new rows are as without it, the others as the output was"""
+    import torch
+    lens, news = [150, 90, 130], [75, 2, 74]
+    with Cache(bam, 32, 1, 128, "bf16") as c:
+        table = _table(lens, c.t, 32)
+        c.fill(lens, table)
+        q = torch.randn(sum(news), 2, 128).to(c.dtype)
+        want, tol, _ = c.want(q, lens, news, table)
+        out = torch.full(q.shape, 7.0, dtype=c.dtype, device="cuda")
+        c.kv.attend(q.cuda(), _i32(lens), table.cuda(), starts=_starts(news), max_new=max_new, out=out)
+        at = 0
+        for n in news:
+            m = min(n, max_new)
+            _near(out[at:at + m], want[at:at + m], tol[at:at + m], at)
+            assert bool((out[at + m:at + n] == 7).all()), at
+            at += n
