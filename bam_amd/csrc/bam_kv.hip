@@ -1033,7 +1033,8 @@ __global__ __launch_bounds__(256) void k_kv_attend(const kv_geom g, const kv_seq
 }
 
 // ---- many rows: tiles of rows against tiles of tokens in LDS ----
-/* 16 bytes a lane from memory to LDS, from base + at to lds + 16 x lane, past the vector L1 as all payload is (ld_payload); counted by the wave's memory counter, and by nobody else: wait for all of them before a barrier */
+/* 16 bytes a lane from memory to LDS, from base + at to lds + 16 x lane, past the vector L1 as all payload is (ld_payload); counted by the wave's memory counter, and by nobody else: wait for all of them before a barrier.
+ * (m0 is one of the compiler's reserved registers: it keeps nothing there, and warns of a clobber list that names it.) */
 __device__ __forceinline__ void to_lds(const uint8_t* base, const uint32_t at, const uint32_t lds)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 sc1" :: "s"(lds), "v"(at), "s"(base) : "memory");
@@ -1510,26 +1511,11 @@ __global__ void k_kv_all_left(uint8_t* left, const uint64_t n)
     if (i < n) left[i] = 1;
 }
 
-template <typename K> void allow_lds(K kernel, const uint32_t bytes)
-{
-    if (bytes > 65536) hip_err_chk(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-}
-
 template <int DP, int F16, int NT>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan& p, hipStream_t st)
 {
     constexpr uint32_t lds = split_lds<DP, NT>(), lds_tiles = tile_lds<DP>();
-    static const bool allowed = [] {
-        allow_lds(k_kv_attend<DP, F16, NT>, lds);
-        allow_lds(k_kv_rest<DP, F16, NT>, lds);
-        if constexpr (DP <= 128) allow_lds(k_kv_attend_once<DP, F16, NT>, lds);
-        if constexpr (NT == 2) {
-            allow_lds(k_kv_attend_tiles<DP, F16, 2, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 2, false>, lds_tiles);
-            allow_lds(k_kv_attend_tiles<DP, F16, 4, true>, lds_tiles); allow_lds(k_kv_attend_tiles<DP, F16, 4, false>, lds_tiles);
-        }
-        return true;
-    }();
-    (void)allowed;
+    static_assert(lds <= 65536 && lds_tiles <= 65536, "more LDS than a launch has without asking for it");
     /* what all waves that may hold pages ask for at a time stays under half the cache, or they push each other's pages out */
     const uint32_t least = kv->g.tokens < 32 ? 32 / kv->g.tokens : 1;
     const uint64_t half = kv->cache_pages / 2, all = p.items * p.splits;
