@@ -25,7 +25,8 @@ class KVCache:
 
     The calls below share how sequences are given, all on the device in int32: `lens[b]` counts the tokens of sequence b, the new ones among them;
     `table[b, i]` is the block of its tokens i * block_tokens and on; rows starts[b] .. starts[b+1]-1 of the packed inputs are its newest tokens
-    (starts None: one new token each).  They are queued on the current stream.  A block number outside the cache is not read or written.
+    (starts None: one new token each).  They are queued on the current stream.  A block number outside the cache is not read or written.  There are no gradients: tensors
+    that require them are refused where gradients are being recorded.
     """
 
     def __init__(self, array, n_heads, head_dim, dtype=torch.bfloat16, first_page=0, n_blocks=None, _owned=()):
@@ -48,6 +49,10 @@ class KVCache:
 
     # ---- checks: each property of a tensor is asked for once, they are what a small call takes on the host ----
 
+    def _no_grad(self, t, what):
+        if t.requires_grad and torch.is_grad_enabled():
+            raise BamError(f"KVCache: {what} requires gradients and there are none: detach it, or call under torch.no_grad()")
+
     def _rows(self, t, what, heads=None):
         """(rows, heads, row stride, head stride) of a tensor of rows"""
         shape = t.shape
@@ -56,6 +61,7 @@ class KVCache:
         row, head, one = t.stride()
         if one != 1:
             raise BamError(f"KVCache: the numbers of a row of {what} must be next to each other")
+        self._no_grad(t, what)
         return shape[0], shape[1], row, head
 
     def _seqs(self, n_rows, lens, table, starts):
@@ -83,6 +89,7 @@ class KVCache:
             return 0
         if t.dtype is not self.dtype or t.shape != (self.head_dim,) or t.stride()[0] != 1 or t.get_device() != self._index:
             raise BamError(f"KVCache: {what} must be {self.head_dim} contiguous numbers of {self.dtype} on {self.device}")
+        self._no_grad(t, what)
         return t.data_ptr()
 
     def _out(self, out, like):
@@ -121,6 +128,7 @@ class KVCache:
             for t in (cos, sin):
                 if len(shape) != 2 or t.shape != shape or t.dtype is not torch.float32 or t.get_device() != self._index or not t.is_contiguous():
                     raise BamError(f"KVCache: cos and sin must be contiguous [positions, half] in float32 on {self.device}")
+                self._no_grad(t, "cos or sin")
             angles, rot = (cos.data_ptr(), sin.data_ptr(), shape[0]), 2 * shape[1]
         elif cos is not None or sin is not None:
             raise BamError("KVCache: cos and sin go together")

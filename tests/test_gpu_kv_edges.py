@@ -257,3 +257,25 @@ def test_rows_beyond_max_new_are_left(bam, max_new):
             _near(out[at:at + m], want[at:at + m], tol[at:at + m], at)
             assert bool((out[at + m:at + n] == 7).all()), at
             at += n
+
+
+# ---------------------------------------------------------------- gradients
+
+def test_tensors_that_require_gradients_are_refused(bam):
+    """outputs carry no graph: what would be lost without a word is refused, unless gradients are not being recorded"""
+    import torch
+    with Cache(bam, 4, 1, 64, "bf16") as c:
+        lens, table = _i32([1]), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+        x, w, angles = (torch.ones(*s, dtype=t, device="cuda") for s, t in (((1, 1, 64), c.dtype), ((64,), c.dtype), ((4, 32), torch.float32)))
+        good = {"k": x, "v": x, "q": x, "q_norm": w, "k_norm": w, "cos": angles, "sin": angles}
+        for name, t in good.items():
+            args = dict(good, **{name: t.clone().requires_grad_()})
+            k, v = args.pop("k"), args.pop("v")
+            with pytest.raises(bam.BamError, match="gradients"):
+                c.kv.append(k, v, lens, table, **args)
+            with torch.no_grad():
+                c.kv.append(k, v, lens, table, **args)
+        with pytest.raises(bam.BamError, match="gradients"):
+            c.kv.attend(x.clone().requires_grad_(), lens, table)
+        with torch.inference_mode():
+            assert not c.kv.attend(x.clone().requires_grad_(), lens, table).requires_grad
