@@ -422,7 +422,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
         };
         uint32_t none = 3;                       /* rows without a block read as zeros, */
         if (there) {
-            /* a page that holds none but this call's tokens needs nothing from the store */
+            /* a page whose first token is one of this call's holds nothing in front of them, and what was behind them is not kept: it needs nothing from the store */
             none = visit<WRITE>(g, page, WRITE && block_first >= bcast(p.first, j), WRITE && block_first + g.tokens > pos + rest, [&](uint8_t* keys, uint8_t* values) { use(keys, values, 0, 0); });
         }
         /* those whose page could not be had as NaN */

@@ -459,7 +459,9 @@ typedef struct bam_kv_seqs {
  * New rows into the cache: d_v as they are; d_k, and d_q into d_q_out ([n_rows][q_heads][dim]), with d_k_norm / d_q_norm (dim numbers, or NULL) as
  * x * rsqrt(mean x^2 + eps) * w per head, then the first `rot` numbers turned by the angles of the row's position: pairs (i, i + rot/2), or with
  * `pairs` (2i, 2i+1), by d_cos / d_sin[position * rot/2 + i] (n_positions rows; a position past them gives NaN; rot 0: none).  In 32 bits, rounded once.
- * Strides are in elements; the numbers of a row are next to each other.  d_q may be NULL.  A page that holds none but new rows is not read from the store.
+ * Strides are in elements; the numbers of a row are next to each other.  d_q may be NULL.  A block whose first token is one of the call's new ones
+ * belongs to that sequence from there on: its pages are not read from the store, and what they held behind the sequence's last token is not kept (zeros where they were not
+ * resident).  So blocks that several sequences share are not appended to except whole, or by the sequence that has the most tokens in them.
  */
 typedef struct bam_kv_append {
     bam_kv_seqs_t seqs;
@@ -479,7 +481,7 @@ int bam_kv_append(bam_kv_t* kv, const bam_kv_append_t* what, void* stream);
 int bam_kv_read(bam_kv_t* kv, const bam_kv_seqs_t* seqs, void* d_k, void* d_v, void* stream);
 /*
  * Attention of the newest tokens over what the cache holds: row i at position p, head h, sees the tokens t <= p of its sequence, with a window (not 0) those with
- * p - t < window or t < sinks; out = sum of softmax(scale * q.k_t) v_t, with the keys of head h / (q_heads / n_heads).  A row that sees nothing is zero.  What a
+ * p - t < window or t < sinks; out = sum of softmax(scale * q.k_t) v_t, with the keys of head h / (q_heads / n_heads).  A row that sees nothing, or whose scores are all minus infinity, is zero.  What a
  * row does not see has no part in it, infinities and NaN included.  d_lse (or NULL): log of the sum of exp(scale * q.k_t), [n_rows][q_heads].
  * max_new: no sequence has more new rows (of one that has, the first max_new are written; ignored without d_starts); max_len: about how long sequences get (it decides how the
  * work is shared out, not what is read).  d_work: bam_kv_attend_bytes(...) bytes for the length of the call.
