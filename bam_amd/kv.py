@@ -196,8 +196,15 @@ def make_kv_cache(ctrl, n_blocks, n_heads, head_dim, page_size=4096, cache_pages
     """Page cache + one range + array + key-value cache of n_blocks blocks, stored from byte disk_offset_bytes (page aligned).  cache_pages: slots of the page cache (all
     pages of the blocks unless given)."""
     n_pages = 2 * n_blocks * n_heads
-    pc = PageCache(page_size, max(64, n_pages if cache_pages is None else cache_pages), device, ctrl, max_range)
-    elems = n_pages * page_size // 8
-    r = Range(0, elems, disk_offset_bytes // page_size, n_pages, 0, page_size, pc, device)
-    a = Array(elems, disk_offset_bytes, [r], device)
-    return KVCache(a, n_heads, head_dim, dtype, 0, n_blocks, _owned=(a, r, pc))
+    made = []                # what there is so far, the last first
+    try:
+        made.insert(0, PageCache(page_size, max(64, n_pages if cache_pages is None else cache_pages), device, ctrl, max_range))
+        elems = n_pages * page_size // 8
+        made.insert(0, Range(0, elems, disk_offset_bytes // page_size, n_pages, 0, page_size, made[0], device))
+        made.insert(0, Array(elems, disk_offset_bytes, [made[0]], device))
+        return KVCache(made[0], n_heads, head_dim, dtype, 0, n_blocks, _owned=made)
+    except BaseException:
+        # not left to the collector: the error may be kept for longer than the controller lives
+        for x in made:
+            x.close()
+        raise

@@ -279,3 +279,26 @@ def test_tensors_that_require_gradients_are_refused(bam):
             c.kv.attend(x.clone().requires_grad_(), lens, table)
         with torch.inference_mode():
             assert not c.kv.attend(x.clone().requires_grad_(), lens, table).requires_grad
+
+
+# ---------------------------------------------------------------- refusals
+
+@pytest.mark.parametrize("wrong", [{"head_dim": 120}, {"head_dim": 48, "page_size": 512}, {"n_blocks": 0}, {"dtype": "float32"}, {"max_range": 0}])
+def test_a_refused_cache_leaves_nothing_open(bam, wrong):
+    """its page cache, range and array are closed when the error comes out, not when the error is let go of, which may be after the controller is gone"""
+    import gc
+    import torch
+    from test_gpu_parity import Rig
+    args = {"n_blocks": 4, "n_heads": 1, "head_dim": 64, "page_size": 4096, **wrong}
+    if "dtype" in args:
+        args["dtype"] = getattr(torch, args["dtype"])
+
+    def open_ones():
+        return {id(x): x for x in gc.get_objects() if type(x) in (bam.PageCache, bam.Range, bam.Array) and x.h}
+
+    with Rig(bam, 1 << 20) as r:
+        before = open_ones()
+        with pytest.raises(bam.BamError) as kept:
+            bam.make_kv_cache(r.c, **args)
+        assert not open_ones().keys() - before.keys()
+    assert "KVCache" in str(kept.value) or "bam_" in str(kept.value)
