@@ -302,3 +302,41 @@ def test_a_refused_cache_leaves_nothing_open(bam, wrong):
             bam.make_kv_cache(r.c, **args)
         assert not open_ones().keys() - before.keys()
     assert "KVCache" in str(kept.value) or "bam_" in str(kept.value)
+
+
+# ---------------------------------------------------------------- heads between the widths that kernels are built for
+
+@pytest.mark.parametrize("dtype,dim,page", [("bf16", 144, 4096), ("f16", 176, 8192), ("bf16", 192, 16384), ("f16", 240, 4096), ("bf16", 112, 4096), ("f16", 48, 1024), ("bf16", 256, 4096)])
+@pytest.mark.parametrize("group,news", [(1, [1, 1, 1]), (5, [4, 1, 3]), (2, [25, 3, 17]), (3, [30, 41, 2])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (37, 5)])
+def test_other_head_sizes(bam, dtype, dim, page, group, news, window, sinks):
+    """one row and few, tiles of two waves (33 to 64 rows of a head of keys) and of four; rows with norms and rotations into them and out"""
+    import torch
+    from test_gpu_kv import _rotated
+    lens, heads = [200, 133, 90], 2
+    gen = torch.Generator().manual_seed(dim)
+    with Cache(bam, 160, heads, dim, dtype, page) as c:
+        table = _table(lens, c.t, 160)
+        c.fill(lens, table)
+        n = sum(news)
+        rows = c.rows_of(lens, news)
+        x = torch.randn(3, n, heads * group, dim, generator=gen).to(c.dtype)
+        w = (1 + 0.2 * torch.randn(2, dim, generator=gen)).to(c.dtype)
+        rot = dim if group % 2 else dim // 32 * 16
+        angle = torch.rand(200, rot // 2, generator=gen) * 6.28
+        cos, sin, style = angle.cos(), angle.sin(), "half" if group > 1 else "pairs"
+        dev = [c_.cuda() for c_ in (x[0, :, :heads], x[1, :, :heads], x[2])]
+        q = c.kv.append(dev[0], dev[1], _i32(lens), table.cuda(), starts=_starts(news), q=dev[2], q_norm=w[0].cuda(), k_norm=w[1].cuda(), cos=cos.cuda(), sin=sin.cuda(), rotary=style)
+        got_k, got_v = (y.cpu() for y in c.kv.read(n, _i32(lens), table.cuda(), starts=_starts(news)))
+        assert torch.equal(got_v, x[1, :, :heads])
+        for i, (b, p) in enumerate(rows):
+            for h in range(heads):
+                for got, row, weight in ((q[i, h], x[2, i, h], w[0]), (got_k[i, h], x[0, i, h], w[1])):
+                    y, size = _rotated(row, weight, p, cos, sin, style, 1e-6)
+                    _near(got, y, 1.01 * c.u * y.abs() + 2.0 ** -18 * size + 2.0 ** -25, (i, h))
+        c.note(got_k, got_v, rows, table)
+        want, tol, lse = c.want(q.cpu(), lens, news, table, window, sinks)
+        got, got_lse = c.kv.attend(q, _i32(lens), table.cuda(), starts=_starts(news), max_new=max(news), window=window, sinks=sinks, return_lse=True)
+        _near(got, want, tol)
+        _near(got_lse, lse, 2.0 ** -16 * (1 + lse.abs()))
+        assert not c.rig.c.aborted()
