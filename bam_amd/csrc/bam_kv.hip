@@ -1652,6 +1652,7 @@ int bam_kv_append(bam_kv_t* kv, const bam_kv_append_t* what, void* stream)
     if (!w.d_k || !w.d_v || (w.d_q && (!w.d_q_out || !w.q_heads)) || (w.rot && (!w.d_cos || !w.d_sin))) return fail(EINVAL, "bam_kv_append: null argument");
     if (w.rot % 16 || w.rot > kv->g.dim) return fail(EINVAL, "bam_kv_append: the rotated part must be a multiple of 16, at most the head dimension");
     if (((uintptr_t)w.d_q_norm | (uintptr_t)w.d_k_norm | (uintptr_t)w.d_cos | (uintptr_t)w.d_sin | (uintptr_t)w.d_q_out) & 15) return fail(EINVAL, "bam_kv_append: weights, tables and output must be aligned to 16 bytes");
+    if ((w.d_q_norm || w.d_k_norm) && (!(w.eps >= 0) || w.eps - w.eps != 0)) return fail(EINVAL, "bam_kv_append: eps must be finite and not negative");
     if (w.n_positions > 0x7fffffffull || (w.rot && !w.n_positions)) return fail(EINVAL, "bam_kv_append: no positions, or more than 31 bits count");
     BAM_API_BEGIN
     kv_rows io{};
@@ -1707,7 +1708,7 @@ int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream)
     if (max_new * (w.q_heads / kv->g.heads) > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more rows than 31 bits count");
     BAM_API_BEGIN
     const kv_plan p = plan_of(kv, w.seqs.n_seqs, max_new, w.q_heads, w.max_len, w.window, w.sinks);
-    if (p.items * p.splits > 0x7fffffffull || p.items * p.rows > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more workgroups than 31 bits count");
+    if (p.tiles > 0x7fffffffull / kv->g.heads || w.seqs.n_seqs > 0x7fffffffull / ((uint64_t)p.tiles * kv->g.heads) || p.items * p.splits > 0x7fffffffull || p.items * p.rows > 0x7fffffffull) return fail(EINVAL, "bam_kv_attend: more workgroups than 31 bits count");
     if (w.work_bytes < p.bytes) return fail(EINVAL, "bam_kv_attend: the workspace is smaller than bam_kv_attend_bytes says");
     kv_att a{};
     a.q = (const uint16_t*)w.d_q; a.q_row = w.q_row; a.q_head = w.q_head; a.aligned = whole_pieces(w.d_q, w.q_row, w.q_head); a.q_heads = w.q_heads; a.group = w.q_heads / kv->g.heads;

@@ -20,6 +20,13 @@ _APPEND = struct.Struct("@" + _SEQS + "Pqq" * 3 + "PPPPPQIIfi")
 _ATTEND = struct.Struct("@" + _SEQS + "PqqPPPQQQIIIf")
 
 
+def _packed(layout, *fields):
+    try:
+        return layout.pack(*fields)
+    except (struct.error, OverflowError) as e:
+        raise BamError(f"KVCache: an argument is not a number that its field can hold ({e})") from None
+
+
 class KVCache:
     """Blocks of `block_tokens` tokens in the pages of `array` from `first_page` on, two pages to a block and head.
 
@@ -132,31 +139,32 @@ class KVCache:
             angles, rot = (cos.data_ptr(), sin.data_ptr(), shape[0]), 2 * shape[1]
         elif cos is not None or sin is not None:
             raise BamError("KVCache: cos and sin go together")
-        what = _APPEND.pack(*seqs, k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, *q_args, self._weights(q_norm, "q_norm"), self._weights(k_norm, "k_norm"),
-                            *angles, q_heads, rot, eps, rotary == "pairs")
+        what = _packed(_APPEND, *seqs, k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, *q_args, self._weights(q_norm, "q_norm"), self._weights(k_norm, "k_norm"),
+                       *angles, q_heads, rot, eps, rotary == "pairs")
         _chk(self.L.bam_kv_append(self.h, what, _stream()), "bam_kv_append")
         return out if q is not None else None
 
     def read(self, n_rows, lens, table, starts=None):
         """The newest rows as the cache has them: (keys, values), [n_rows, heads, head_dim] each."""
+        if n_rows < 0:
+            raise BamError("KVCache: n_rows must not be negative")
         seqs = self._seqs(n_rows, lens, table, starts)
         k = torch.empty(n_rows, self.n_heads, self.head_dim, dtype=self.dtype, device=self.device)
         v = torch.empty_like(k)
-        _chk(self.L.bam_kv_read(self.h, _READ.pack(*seqs), k.data_ptr(), v.data_ptr(), _stream()), "bam_kv_read")
+        _chk(self.L.bam_kv_read(self.h, _packed(_READ, *seqs), k.data_ptr(), v.data_ptr(), _stream()), "bam_kv_read")
         return k, v
 
     def attend(self, q, lens, table, starts=None, max_new=None, max_len=None, scale=None, window=0, sinks=0, out=None, return_lse=False):
         """Attention of the newest tokens (their rows in q) over what the cache holds of their sequences: the token at position p sees t <= p and, with
-        a window, those with p - t < window or t < sinks.  scale: head_dim ** -0.5 unless given.  max_new: the most new rows a sequence has (all rows unless given; those beyond
-        are left as they are);
+        a window, those with p - t < window or t < sinks.  scale: head_dim ** -0.5 unless given.  max_new: the most new rows a sequence has (all rows unless given; those beyond are left as they are);
         max_len: about the longest sequence (the table's width unless given); they decide how the work is shared out.  Rows of no sequence are left as they are.
         Returns the output, or with return_lse (output, logarithm of the sum of exponentials)."""
         n, hq, row, head = self._rows(q, "q")
         seqs = self._seqs(n, lens, table, starts)
         if hq == 0 or hq % self.n_heads:
             raise BamError(f"KVCache: the heads of q must be a multiple of {self.n_heads}")
-        if window < 0 or sinks < 0 or (max_new is not None and max_new < 1) or (max_len is not None and max_len < 1):
-            raise BamError("KVCache: window and sinks must not be negative, max_new and max_len at least 1")
+        if not 0 <= window <= 0x7fffffff or not 0 <= sinks <= 0x7fffffff or (max_new is not None and max_new < 1) or (max_len is not None and not 1 <= max_len <= 0x7fffffff):
+            raise BamError("KVCache: window and sinks must be 31-bit numbers, max_new and max_len at least 1, max_len a 31-bit number")
         out = self._out(out, q)
         lse = torch.empty(n, hq, dtype=torch.float32, device=self.device) if return_lse else None
         if n and seqs[1]:
@@ -172,8 +180,8 @@ class KVCache:
                 need = self._bytes[key] = b.value
             # from torch's allocator, which keeps it for this stream, or for the graph that is being captured
             work = torch.empty(need, dtype=torch.uint8, device=self.device)
-            what = _ATTEND.pack(*seqs, q.data_ptr(), row, head, out.data_ptr(), 0 if lse is None else lse.data_ptr(), work.data_ptr(), need, max_new, max_len,
-                                hq, window, sinks, self.head_dim ** -0.5 if scale is None else scale)
+            what = _packed(_ATTEND, *seqs, q.data_ptr(), row, head, out.data_ptr(), 0 if lse is None else lse.data_ptr(), work.data_ptr(), need, max_new, max_len,
+                           hq, window, sinks, self.head_dim ** -0.5 if scale is None else scale)
             _chk(self.L.bam_kv_attend(self.h, what, _stream()), "bam_kv_attend")
         return (out, lse) if return_lse else out
 
@@ -194,7 +202,9 @@ class KVCache:
 
 def make_kv_cache(ctrl, n_blocks, n_heads, head_dim, page_size=4096, cache_pages=None, dtype=torch.bfloat16, device=0, disk_offset_bytes=0, max_range=64):
     """Page cache + one range + array + key-value cache of n_blocks blocks, stored from byte disk_offset_bytes (page aligned).  cache_pages: slots of the page cache (all
-    pages of the blocks unless given)."""
+    pages of the blocks unless given, and 64 at least)."""
+    if disk_offset_bytes < 0 or page_size <= 0 or disk_offset_bytes % page_size:
+        raise BamError("make_kv_cache: disk_offset_bytes must be the beginning of a page")
     n_pages = 2 * n_blocks * n_heads
     made = []                # what there is so far, the last first
     try:

@@ -340,3 +340,24 @@ def test_other_head_sizes(bam, dtype, dim, page, group, news, window, sinks):
         _near(got, want, tol)
         _near(got_lse, lse, 2.0 ** -16 * (1 + lse.abs()))
         assert not c.rig.c.aborted()
+
+
+def test_arguments_out_of_range_are_refused(bam):
+    """numbers that do not fit the fields of a call, and a store offset inside a page, which was taken for the page's beginning"""
+    import torch
+    from test_gpu_parity import Rig
+    with Cache(bam, 4, 1, 64, "bf16") as c:
+        x, lens, table = torch.ones(1, 1, 64, dtype=c.dtype, device="cuda"), _i32([1]), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+        for kw in ({"window": 1 << 31}, {"window": (1 << 32) + 5}, {"sinks": 1 << 40}, {"max_len": 1 << 31}, {"scale": 1e39}, {"scale": "x"}):
+            with pytest.raises(bam.BamError):
+                c.kv.attend(x, lens, table, **kw)
+        for kw in ({"eps": 1e39, "k_norm": x[0, 0]}, {"eps": -1e-6, "k_norm": x[0, 0]}, {"eps": float("nan"), "q": x, "q_norm": x[0, 0]}, {"eps": None}):
+            with pytest.raises(bam.BamError):
+                c.kv.append(x, x, lens, table, **kw)
+        with pytest.raises(bam.BamError):
+            c.kv.read(-1, lens, table, starts=_starts([1]))
+    with Rig(bam, 1 << 20) as r:
+        for offset in (1, 4095, -4096):
+            with pytest.raises(bam.BamError):
+                bam.make_kv_cache(r.c, 4, 1, 64, disk_offset_bytes=offset)
+        bam.make_kv_cache(r.c, 4, 1, 64, disk_offset_bytes=8192).close()
