@@ -920,7 +920,7 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
 {
     using namespace bam;
     constexpr uint32_t R = 16 * NT;
-    const uint32_t lane = bam::lane(), wave = threadIdx.x / 64u, row = lane & 15u, grp = lane >> 4, D = g.dim;
+    const uint32_t lane = bam::lane(), wave = first(threadIdx.x / 64u), row = lane & 15u, grp = lane >> 4, D = g.dim;
     const uint32_t s1 = s0 + R < it.r1 ? s0 + R : it.r1;
     kv_span sp = span_of(a, s.width << g.tokens_log, it.pos0, it.r0, it.r1);                     /* the item's splits, */
     sp.first_pos = it.pos0 + (int32_t)(s0 / a.group);                           /* as these rows see them */
@@ -1127,7 +1127,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
         nt_end = (nb_first + 64u) << g.tokens_log;
         if (nt_first + run * 32u < nt_end) nt_end = nt_first + run * 32u;
         const uint32_t blk = nb_first + lane;
-        nasked = (blk << g.tokens_log) < nt_end && ((blk << g.tokens_log) < sp.len || blk >= s.width);      /* past the table's end: a hole */
+        nasked = (blk << g.tokens_log) < (nt_end < sp.len ? nt_end : sp.len);
         nblock = -1;
         if (nasked && blk < s.width) nblock = s.table[(int64_t)it.seq * s.stride + blk];
         asm volatile("" : "+v"(nblock));
@@ -1160,7 +1160,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     };
     /* the tile from t_next on into a buffer */
     uint32_t at_first = 0, at_end = 0, at_block = 0;          /* of the tile that is on its way */
-    uint64_t at_holes = 0;                                    /* among its blocks, from at_block on */
+    uint64_t at_holes = 0;
     const uint32_t k_lane0 = (lane & 7u) * 16u + (lane >> 3) * T * 16u, k_lane1 = (lane & 7u) * 16u + (lane >> 3 ^ 1u) * T * 16u;
     auto load_tile = [&](const uint32_t buf) {
         const uint32_t to = lds0 + buf * 2u * HALF;
@@ -1177,9 +1177,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
                 if (EXACT || 64u * i + lane < D) to_lds(v_at, (64u * i + lane) * 16u, to + HALF + u * DP * 16u + i * 1024u);
             }
         }
-        at_first = t_next; at_end = t_end;
-        at_block = t_next >> g.tokens_log;
-        at_holes = (holes >> (at_block - b_first)) & ((2ull << (((t_next + KT - 1u) >> g.tokens_log) - at_block)) - 1ull);
+        at_first = t_next; at_end = t_end < sp.len ? t_end : sp.len; at_holes = holes; at_block = b_first;          /* (the last step may go on behind the table's end) */
         t_next += KT;
     };
     next_blocks();
@@ -1249,7 +1247,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
 #pragma unroll
             for (uint32_t k = 0; k < KT / 16; k++) {
                 const uint32_t tt = t0 + k * 16u + half * 8u;
-                if ((t_holes >> ((tt >> g.tokens_log) - t_block)) & 1u) continue;
+                if ((t_holes >> (((tt >> g.tokens_log) - t_block) & 63u)) & 1u) continue;
                 sees |= seen_of_eight((int32_t)tt, pos < lim ? pos : lim, low_of(a, pos), (int32_t)a.sinks) << (8u * k);
             }
 #pragma unroll
