@@ -686,8 +686,8 @@ __device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most,
  * back, and they are asked for again.  If others have pushed some of them out by then, the pages of each step are loaded one by one, those of a step that came are loaded and given
  * back before the next is waited for: no wave waits for a slot while it keeps another, however many calls share the page cache.  `gone` is set, and the rest left, where a wait was given up.
  *   Bound by the reads of keys and values, each once and marked as not to be kept (without the mark 10 % slower): a step's 16 KiB are on their way at once, the matrix unit is idle most of the
- * time, and what is left of a tile of 16 rows by a group of four heads costs nothing.  128 sequences of up to 8192 tokens, 3.2 GB: 530 us, 6.1 TB/s (a copy
- * reaches 4.9 on this card); 64 of up to 4099: 141 us, 5.7 TB/s, the longest sequence's workgroups last; one of 262121: 165 us, 6.5 TB/s with the join.  More waves to
+ * time, and what is left of a tile of 16 rows by a group of four heads costs nothing.  128 sequences of up to 8192 tokens, 3.2 GB: 511 us, 6.3 TB/s (a copy
+ * reaches 4.9 on this card, a plain reader 7.2); 64 of up to 4099: 142 us, 5.6 TB/s, the longest sequence's workgroups last; one of 262121: 165 us, 6.5 TB/s with the join.  More waves to
  * a SIMD (three, four) were 9 % slower.
  */
 template <int DP, int F16, int NT, bool HELD>
@@ -1053,7 +1053,7 @@ template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>
  * those 8 (l / 32) .. + 7.  Pages are read without a reference, in chunks of 64 blocks, as in kv_steps (past the L1; an
  * acquire behind each first look instead, which invalidates more than that, cost a tenth, and a quarter where there are 18 tiles to a workgroup).
  *   Bound by the matrix unit and by what its two waves to a SIMD cannot hide: 32 products of 32 cycles and some 200 other instructions, 32 of them exponentials of 16
- * cycles, to a tile and wave.  A document of 16384 tokens, 32 heads on 8 of 128 numbers: 2.09 ms, 1050 TFLOP/s of what is visible (a large product of the library's: 1218).  Rows of 32 to a
+ * cycles, to a tile and wave.  A document of 16384 tokens, 32 heads on 8 of 128 numbers: 2.12 ms, 1040 TFLOP/s of what is visible (a large product of the library's: 1218).  Rows of 32 to a
  * wave read a tile's 32 KiB of LDS in as many cycles as its products take; eight waves to a workgroup, one to a compute unit, were a tenth slower than two of four.
  */
 template <int DP, int F16, int NW, bool EXACT>
@@ -1266,7 +1266,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             top = fmaxf(top, other);
         }
         /* the sums are moved to a larger maximum only where its weight would be above 2^TILE_SLACK: up to there weights lose nothing */
-        if (ballot((top - m) * c > TILE_SLACK<F16> || m == -INFINITY && top != -INFINITY)) {
+        if (ballot((top - m) * c > TILE_SLACK<F16> || (m == -INFINITY && top != -INFINITY))) {
             const float larger = fmaxf(top, m);
             const float by = larger == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - larger) * c);
             l *= by;
