@@ -1,0 +1,453 @@
+// The key-value cache in the pages of an array: the handle, where tokens lie, visits of pages, and rows into the cache and out of it.
+//
+// The cache is cut into blocks of T tokens.  A block has two pages for each key-value head: one of keys and one of values, T the largest power of
+// two for which T rows of `dim` 16-bit numbers fit a page.  Within a page the numbers lie in pieces of 16 bytes, in the order in
+// which the matrix instructions take them:
+//   keys    piece (c, t) at (c * T + place(t)) * 16: numbers 8c .. 8c+7 of token t             c < dim / 8
+//   values  piece (t, d) at (t * dim + d) * 16: number d of tokens 8t .. 8t+7           t < T / 8
+// place(t) is t with its bits 2 and 3 exchanged (t itself where a page holds eight tokens).  What neighbouring lanes of a wave load lies next to each other, and
+// is an operand as it stands: with the scores taken as S^T = K Q^T and the output as O^T = V^T P^T, a lane's accumulators of the scores are its
+// part of P^T if the rows of K come in that order.
+#ifndef __BAM_KV_CACHE_H__
+#define __BAM_KV_CACHE_H__
+#include "bam_capi_internal.h"
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// what a kernel knows about the cache: the range's tables do not move while the array is there
+struct kv_geom {
+    range_d_t<uint64_t>* r;
+    data_page_t* pages;
+    uint8_t* base;
+    uint64_t first_page, n_blocks;
+    uint32_t heads, dim, tokens, tokens_log, page_log;
+};
+struct bam_kv {
+    bam_array_t* a;
+    kv_geom g;
+    int f16;
+    uint64_t cache_pages;
+    bool unheld;                        /* reads of resident pages without a reference are switched on */
+};
+struct kv_seqs {
+    const int32_t* starts;              /* [n + 1] first row of each sequence's new tokens; NULL: one new token each */
+    const int32_t* lens;                /* [n] tokens of each sequence, the new ones among them */
+    const int32_t* table;               /* [n][width] blocks */
+    int64_t stride;
+    uint32_t n, rows, width;
+};
+struct kv_rows {
+    const uint16_t *q, *k, *v;          /* rows of heads; k and v are where rows go to when the cache is read */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    uint16_t* q_out;
+    const uint16_t *q_norm, *k_norm;
+    const float *cos, *sin;
+    uint32_t positions, q_heads, rot, pairs, aligned;      /* aligned: q, k, v in whole pieces of 16 bytes */
+    float eps;
+    uint32_t window, piece;             /* rows that a wave looks for beginnings of runs among, and the most rows it takes at a time */
+    uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes */
+};
+
+namespace {
+
+// sequence of row i
+__device__ __forceinline__ uint32_t seq_of(const kv_seqs& s, const uint32_t i)
+{
+    if (!s.starts) return i;
+    uint32_t lo = 0, hi = s.n;          /* the last sequence that starts at or before row i */
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (s.starts[mid] <= (int32_t)i) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+// a row's place: sequence, position, rows of its sequence from it on (those that there are: starts may say more than `rows`), position of its sequence's first new
+// row; false where the row has none (no such sequence, before the first position, past the table)
+struct kv_place { uint32_t seq, pos, rest, first; };
+__device__ __forceinline__ bool place_of(const kv_seqs& s, const kv_geom& g, const uint32_t i, kv_place& p)
+{
+    p.seq = seq_of(s, i);
+    if (p.seq >= s.n) return false;
+    const int32_t end = s.starts ? s.starts[p.seq + 1] : (int32_t)i + 1;
+    int32_t begin = s.starts ? s.starts[p.seq] : (int32_t)i;
+    if (begin < 0) begin = 0;
+    const int64_t len = s.lens[p.seq], pos = len - (end - (int64_t)i);
+    if ((int32_t)i < begin || (int64_t)i >= end || pos < 0 || (pos >> g.tokens_log) >= s.width) return false;
+    p.pos = (uint32_t)pos;
+    p.rest = ((uint32_t)end < s.rows ? (uint32_t)end : s.rows) - i;
+    const int64_t first = len - ((int64_t)end - begin);
+    p.first = first < 0 ? 0u : (uint32_t)first;
+    return true;
+}
+// the page of keys of a block (the page of values is the next one), or false: no such block
+__device__ __forceinline__ bool page_of_block(const kv_geom& g, const kv_seqs& s, const uint32_t seq, const uint32_t i, const uint32_t head, uint64_t& page)
+{
+    if (i >= s.width) return false;
+    const int32_t b = s.table[(int64_t)seq * s.stride + i];
+    if (b < 0 || (uint64_t)b >= g.n_blocks) return false;
+    page = g.first_page + ((uint64_t)b * g.heads + head) * 2u;
+    return true;
+}
+
+/* where a token of a block lies among its block's keys */
+__device__ __forceinline__ uint32_t place_in(const kv_geom& g, const uint32_t t) { return g.tokens < 16 ? t : (t & ~12u) | (t & 4u) << 1 | (t & 8u) >> 1; }
+
+template <int F16> __device__ __forceinline__ float from16(const uint32_t x)
+{
+    if constexpr (F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)x);
+    else return __builtin_bit_cast(float, x << 16);
+}
+template <int F16> __device__ __forceinline__ uint32_t to16(const float lo, const float hi)
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), _Float16 __attribute__((ext_vector_type(2)))));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), __bf16 __attribute__((ext_vector_type(2)))));
+}
+template <bool ALIGNED> __device__ __forceinline__ u32x4 load_piece(const uint16_t* p)
+{
+    if constexpr (ALIGNED) return *(const u32x4*)p;
+    u32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    return x;
+}
+
+// ---------------------------------------------------------------------------
+// pages held for the length of a visit
+// ---------------------------------------------------------------------------
+#define KV_PASS_FRESH 512u
+#define KV_PASS_CLEARED 1024u
+__attribute__((noinline)) __device__ bam_pass_t kv_pass(range_d_t<uint64_t>* r, const uint64_t pg, const uint32_t queue, uint64_t sv, const uint32_t in)
+{
+    bool hit = false, progressed = false, wants = false;
+    uint32_t slot = 0;
+    const bool resolved = r->template slow_step<true>(pg, (in & BAM_PASS_WRITE) != 0, queue, sv, slot, hit, progressed, (in & BAM_PASS_TAKE_PART) != 0, true, &wants, BAM_PLACE_NORMAL,
+                                                      (in & KV_PASS_FRESH) != 0, (in & KV_PASS_CLEARED) != 0);
+    bam_pass_t out;
+    out.sv = sv;
+    out.slot = slot;
+    out.flags = (resolved ? BAM_PASS_RESOLVED : 0u) | (hit ? BAM_PASS_HIT : 0u) | (progressed ? BAM_PASS_PROGRESSED : 0u);
+    return out;
+}
+
+/*
+ * use(address of the slot of the keys or NULL, and of the values) by the whole wave, with those pages held: two neighbouring pages, as range_view::acquire_helped would
+ * have them, what is resident first and nothing held while the other is fetched, with what a writer of rows can say besides (`fresh`, `cleared`:
+ * range_d_t::slow_step).  It stores past the caches (st16_sys and the like), so a wait for the wave's own stores is all that giving a page back needs: the
+ * write-back of the cluster's cache that a release costs would come once per wave.  The miss path is a call: what the rows need is loaded in `use`, behind it (loaded
+ * before, it would be kept across the call, in so many registers that one wave is left to a SIMD).  Returns the pages that were not visited since the wait was given up
+ * (1: keys, 2: values).
+ */
+template <bool WRITE, typename F>
+__device__ __forceinline__ uint32_t visit(const kv_geom& g, const uint64_t page, const bool fresh, const bool cleared, F&& use)
+{
+    using namespace bam;
+    const uint32_t me = lane();
+    data_page_t* const dp = g.pages + page + (me & 1u);
+    uint64_t sv = 0;
+    uint32_t slot = 0, n_hit = 0;
+    bool open = me < 2, in = false;
+    if (open) in = bam_try_hit(dp, 1, WRITE, sv, slot);
+    uint32_t todo = 3;
+    spin_t sp;
+    const uint32_t queue = wave_slot_hash();
+    for (bool again = false;; again = true) {
+        uint32_t got = (uint32_t)ballot(in && open);
+        if (!again) n_hit = popc(got);
+        if (got) {
+            use(got & 1u ? g.base + ((uint64_t)bcast(slot, 0) << g.page_log) : nullptr, got & 2u ? g.base + ((uint64_t)bcast(slot, 1) << g.page_log) : nullptr);
+            fence_meta();
+            if (in && open) { __hip_atomic_fetch_add(&dp->state, 0u - 1u, __ATOMIC_RELAXED, BAM_AGENT); open = false; }
+            todo &= ~got;
+        }
+        if (__builtin_expect(todo == 0, 1)) break;
+        const bam_pass_t ps = kv_pass(g.r, page + (me & 1u), queue, sv, (WRITE ? BAM_PASS_WRITE : 0u) | (open ? BAM_PASS_TAKE_PART : 0u) | (fresh ? KV_PASS_FRESH : 0u) | (cleared ? KV_PASS_CLEARED : 0u));
+        if (open) { sv = ps.sv; slot = ps.slot; in = (ps.flags & BAM_PASS_RESOLVED) != 0; n_hit += in && (ps.flags & BAM_PASS_HIT) ? 1u : 0u; }
+        if (ballot((ps.flags & BAM_PASS_PROGRESSED) != 0)) sp = spin_t();
+        else if (!ballot(in && open) && g.r->cache.spin_giveup(sp)) {
+            if (open) __hip_atomic_fetch_add(&dp->state, 0u - 1u, __ATOMIC_RELAXED, BAM_AGENT);
+            break;
+        }
+    }
+    if (me == 0) {
+        bam_stat_shard_t* const shard = g.r->shard();
+        __hip_atomic_fetch_add(&shard->access_cnt, 2ull, __ATOMIC_RELAXED, BAM_AGENT);
+        if (n_hit) __hip_atomic_fetch_add(&shard->hit_cnt, (unsigned long long)n_hit, __ATOMIC_RELAXED, BAM_AGENT);
+    }
+    return todo;
+}
+
+// the wave's accesses into the range's counters
+__device__ __forceinline__ void count_accesses(const kv_geom& g, const uint32_t n_access, const uint32_t n_hit)
+{
+    bam_stat_shard_t* const shard = g.r->shard();
+    bam::stat_add<32>(&shard->access_cnt, n_access);
+    bam::stat_add<32>(&shard->hit_cnt, n_hit);
+}
+
+// ---------------------------------------------------------------------------
+// rows into the cache and out of it// ---------------------------------------------------------------------------
+
+/* the angles of eight neighbouring numbers of a row; lanes whose numbers are not turned load some, and do not use them */
+struct kv_turn { f32x4 c[2], s[2]; };
+__device__ __forceinline__ kv_turn turn_of(const kv_rows& io, const uint32_t piece, const uint32_t pos)
+{
+    kv_turn t;
+    if (!io.rot) return t;
+    const uint32_t half = io.rot / 2, hp = io.rot / 16;
+    const bool known = pos < io.positions;
+    const uint64_t row = (uint64_t)(known ? pos : 0u) * half;
+    if (io.pairs) {
+        const uint64_t at = row + (piece < 2u * hp ? piece : 0u) * 4u;
+        t.c[0] = *(const f32x4*)(io.cos + at);
+        t.s[0] = *(const f32x4*)(io.sin + at);
+    } else {
+        const uint64_t at = row + (piece < hp ? piece : piece < 2u * hp ? piece - hp : 0u) * 8u;
+        t.c[0] = *(const f32x4*)(io.cos + at); t.c[1] = *(const f32x4*)(io.cos + at + 4);
+        t.s[0] = *(const f32x4*)(io.sin + at); t.s[1] = *(const f32x4*)(io.sin + at + 4);
+    }
+    if (!known) {
+        const float nan = __builtin_nanf("");
+        t.c[0] = t.c[1] = t.s[0] = t.s[1] = f32x4{nan, nan, nan, nan};
+    }
+    return t;
+}
+
+/*
+ * Eight neighbouring numbers of a row per lane, LPR lanes to a row: x * rsqrt(mean x^2 + eps) * w, then the rotation of the pairs (i, i + rot/2), or
+ * (2i, 2i+1), i < rot/2, by the angles of the row's position; in 32 bits, rounded once.  A position past the tables gives NaN.
+ */
+template <int LPR, int F16>
+__device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geom& g, u32x4 x, const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
+{
+    if (!norm && !io.rot) return x;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const uint32_t y = x[i]; f[2 * i] = from16<F16>(y & 0xffffu); f[2 * i + 1] = from16<F16>(y >> 16); }
+    if (norm) {
+        float ss = 0;                            /* (pieces past the row's end are zero) */
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss += f[i] * f[i];
+#pragma unroll
+        for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
+        const float by = rsqrtf(ss / (float)g.dim + io.eps);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { const uint32_t y = w[i]; f[2 * i] *= by * from16<F16>(y & 0xffffu); f[2 * i + 1] *= by * from16<F16>(y >> 16); }
+    }
+    if (io.rot) {
+        const uint32_t pieces = io.rot / 8, hp = pieces / 2;
+        const bool turns = piece < pieces;
+        if (io.pairs) {
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float a = f[2 * i], b = f[2 * i + 1];
+                    f[2 * i] = a * t.c[0][i] - b * t.s[0][i];
+                    f[2 * i + 1] = b * t.c[0][i] + a * t.s[0][i];
+                }
+            }
+        } else {
+            const uint32_t from = (bam::lane() & ~(uint32_t)(LPR - 1)) + (turns ? (piece < hp ? piece + hp : piece - hp) : piece);
+            const float sign = piece < hp ? -1.0f : 1.0f;
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[i] = __shfl(f[i], (int)from);
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) f[i] = f[i] * t.c[i / 4][i % 4] + sign * o[i] * t.s[i / 4][i % 4];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = to16<F16>(f[2 * i], f[2 * i + 1]);
+    return x;
+}
+
+/*
+ * A wave takes some heads of queries of one row, or one head's keys and values of the runs of rows that begin among io.window rows: a run is the new rows of
+ * a sequence in one block, gone through in pieces of up to io.piece tokens (eight or sixteen that begin at a multiple of that).  A page's rows all belong to one
+ * wave: a page that holds new rows only is not read, and one that a second wave found gone again would come without the rows of the first.
+ *   Bound by memory where there are many rows: 19 459 rows of 32 heads on 8 of 128 numbers, normed and turned, 480 MB in 124 us (3.9 TB/s), 160 MB out again in 43; a wave for
+ * each four rows took 288 and 112 (each looked its sequence up for 1 KiB).  Few rows: the chain of looks, table, references, rows, 6 to 7 us.
+ */
+template <int LPR, int F16, bool WRITE, bool ALIGNED>
+__global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
+{
+    using namespace bam;
+    constexpr uint32_t RPW = 64 / LPR, TRIPS = 16 / RPW, DT = LPR / 8;           /* trips of a piece's keys; of its values: a trip is 64 times two numbers of eight tokens */
+    const uint32_t wave = first(blockIdx.x * 4u + threadIdx.x / 64u), lane = bam::lane();
+    const uint32_t sub = lane / LPR, piece = lane % LPR;
+    const bool in_row = piece * 8u < g.dim;
+    const uint32_t col = in_row ? piece * 8u : 0u;           /* lanes past the row's end load its beginning, and count as zeros */
+    if (WRITE && wave < io.q_waves) {
+        const uint32_t per = (io.q_heads + io.q_heads_each - 1) / io.q_heads_each, i = wave / per, h0 = wave % per * io.q_heads_each;
+        const uint32_t h1 = h0 + io.q_heads_each < io.q_heads ? h0 + io.q_heads_each : io.q_heads;
+        kv_place p{0, 0, 0, 0};
+        const bool known = place_of(s, g, i, p);
+        const kv_turn t = turn_of(io, piece, known ? p.pos : 0xffffffffu);
+        u32x4 w{0, 0, 0, 0};
+        if (io.q_norm) w = load_piece<true>(io.q_norm + col);
+        const uint16_t* const from = io.q + (int64_t)i * io.q_row + col;
+        uint16_t* const to = io.q_out + (uint64_t)i * io.q_heads * g.dim + col;
+        for (uint32_t h = h0; h < h1; h += 4u * RPW) {
+            u32x4 x[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t hh = h + e * RPW + sub;
+                x[e] = load_piece<ALIGNED>(from + (int64_t)(hh < h1 ? hh : h0) * io.q_head);
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t hh = h + e * RPW + sub;
+                if (h + e * RPW >= h1) break;
+                x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.q_norm != nullptr, w, t, piece);
+                if (hh < h1 && in_row) *(u32x4*)(to + hh * g.dim) = x[e];
+            }
+        }
+        return;
+    }
+    const uint32_t n = wave - (WRITE ? io.q_waves : 0u), head = n % g.heads;
+    const uint64_t first_row = (uint64_t)(n / g.heads) * io.window;
+    if (first_row >= s.rows) return;
+    kv_place p{0, 0, 0, 0};
+    const uint32_t mine = (uint32_t)first_row + lane;
+    const bool has = lane < io.window && mine < s.rows && place_of(s, g, mine, p);
+    const bool begins = has && ((p.pos & (g.tokens - 1u)) == 0 || p.pos == p.first || (s.starts && s.starts[p.seq] == (int32_t)mine));
+    if constexpr (!WRITE) {
+        /* rows without a place come out as zeros */
+        for (uint64_t m = ballot(lane < io.window && mine < s.rows && !has); m; m &= m - 1)
+            for (uint32_t d = lane; d < g.dim; d += 64u) {
+                ((uint16_t*)io.k)[(int64_t)(first_row + first_lane(m)) * io.k_row + (int64_t)head * io.k_head + d] = 0;
+                ((uint16_t*)io.v)[(int64_t)(first_row + first_lane(m)) * io.v_row + (int64_t)head * io.v_head + d] = 0;
+            }
+    }
+    for (uint64_t m = ballot(begins); m; m &= m - 1) {
+        const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), seq = bcast(p.seq, j), row = (uint32_t)first_row + j;
+        uint64_t page = 0;
+        const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, head, page);
+        const uint32_t run_first = pos & (g.tokens - 1u), block_first = pos - run_first, run_end = rest < g.tokens - run_first ? run_first + rest : g.tokens;
+        const uint32_t groups = io.piece / 8u, pairs = g.dim / 2u;
+        /* a piece: `cnt` tokens from `in_block` of the block on; `none`: rows out are `fill` in place of keys (1), of values (2) */
+        auto use_piece = [&](uint8_t* const keys, uint8_t* const values, const uint32_t none, const uint32_t fill, const uint32_t in_block, const uint32_t cnt) {
+            const uint32_t off = in_block - run_first;
+            uint16_t* const k_rows = (uint16_t*)io.k + (int64_t)(row + off) * io.k_row + (int64_t)head * io.k_head;
+            uint16_t* const v_rows = (uint16_t*)io.v + (int64_t)(row + off) * io.v_row + (int64_t)head * io.v_head;
+            /* of the values, a lane takes numbers d and d + 1 of the eight tokens from `tok` on, counted from the piece's first row */
+            const int32_t piece_first = (int32_t)(in_block & (io.piece - 1u));
+            /* what is worked out from the lane's number is worked out here, not kept across the miss path */
+            uint32_t l = lane;
+            asm volatile("" : "+v"(l));
+            if (keys || (none & 1u)) {
+                u32x4 x[TRIPS];
+                const uint32_t r0 = l / LPR;
+                uint8_t* const at = keys + (uint64_t)(col / 8u) * g.tokens * 16u;
+#pragma unroll
+                for (uint32_t e = 0; e < TRIPS; e++) {
+                    const uint32_t r = r0 + e * RPW < cnt ? r0 + e * RPW : 0u;
+                    if constexpr (WRITE) x[e] = load_piece<ALIGNED>(k_rows + (int64_t)r * io.k_row + col);
+                    else x[e] = none & 1u ? u32x4{fill, fill, fill, fill} : ld_payload((const u32x4*)(at + place_in(g, in_block + r) * 16u));
+                }
+                u32x4 w{0, 0, 0, 0};
+                if (WRITE && io.k_norm) w = load_piece<true>(io.k_norm + col);
+#pragma unroll
+                for (uint32_t e = 0; e < TRIPS; e++) {
+                    if (e * RPW >= cnt) break;
+                    const uint32_t r = r0 + e * RPW;
+                    if constexpr (WRITE) {
+                        const kv_turn t = turn_of(io, piece, pos + off + (r < cnt ? r : 0u));
+                        x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.k_norm != nullptr, w, t, piece);
+                        if (r < cnt && in_row) st16_sys(at + place_in(g, in_block + r) * 16u, x[e]);
+                    } else if (r < cnt && in_row) *(u32x4*)(k_rows + (int64_t)r * io.k_row + col) = x[e];
+                }
+            }
+            if (values || (none & 2u)) {
+#pragma unroll
+                for (uint32_t e = 0; e < DT; e++) {
+                    const uint32_t y = e * 64u + l, group = y / pairs, d = y % pairs * 2u;
+                    const int32_t tok = (int32_t)(group * 8u) - piece_first;
+                    if (group >= groups || tok + 8 <= 0 || tok >= (int32_t)cnt) continue;
+                    uint8_t* const at = values + ((uint64_t)((in_block + tok) >> 3) * g.dim + d) * 16u;
+                    uint16_t* const rows = v_rows + d;
+                    const bool full = tok >= 0 && tok + 8 <= (int32_t)cnt;
+                    if constexpr (WRITE) {
+                        uint32_t z[8];
+#pragma unroll
+                        for (int32_t t = 0; t < 8; t++) {
+                            const int32_t r = tok + t < 0 ? 0 : tok + t < (int32_t)cnt ? tok + t : (int32_t)cnt - 1;
+                            const uint16_t* const from = rows + r * io.v_row;
+                            z[t] = ALIGNED ? *(const uint32_t*)from : (uint32_t)from[0] | ((uint32_t)from[1] << 16);
+                        }
+                        if (full) {
+                            u32x4 lo, hi;
+#pragma unroll
+                            for (int t = 0; t < 4; t++) {
+                                lo[t] = (z[2 * t] & 0xffffu) | (z[2 * t + 1] << 16);
+                                hi[t] = (z[2 * t] >> 16) | (z[2 * t + 1] & 0xffff0000u);
+                            }
+                            st16_sys(at, lo);
+                            st16_sys(at + 16, hi);
+                        } else {
+#pragma unroll
+                            for (int32_t t = 0; t < 8; t++)
+                                if (tok + t >= 0 && tok + t < (int32_t)cnt) {
+                                    __hip_atomic_store((uint16_t*)at + t, (uint16_t)z[t], __ATOMIC_RELAXED, BAM_SYSTEM);
+                                    __hip_atomic_store((uint16_t*)at + 8 + t, (uint16_t)(z[t] >> 16), __ATOMIC_RELAXED, BAM_SYSTEM);
+                                }
+                        }
+                    } else {
+                        u32x4 lo{fill, fill, fill, fill}, hi = lo;
+                        if (!(none & 2u)) { lo = ld_payload((const u32x4*)at); hi = ld_payload((const u32x4*)(at + 16)); }
+#pragma unroll
+                        for (int32_t t = 0; t < 8; t++)
+                            if (full || (tok + t >= 0 && tok + t < (int32_t)cnt)) {
+                                const uint32_t a = lo[t / 2], b = hi[t / 2];
+                                *(uint32_t*)(rows + (tok + t) * io.v_row) = (t & 1) ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
+                            }
+                    }
+                }
+            }
+        };
+        auto use = [&](uint8_t* const keys, uint8_t* const values, const uint32_t none, const uint32_t fill) {
+            for (uint32_t at = run_first; at < run_end;) {
+                uint32_t end = (at | (io.piece - 1u)) + 1u;
+                if (end > run_end) end = run_end;
+                use_piece(keys, values, none, fill, at, end - at);
+                at = end;
+            }
+        };
+        uint32_t none = 3;                       /* rows without a block read as zeros, */
+        if (there) {
+            /* a page whose first token is one of this call's holds nothing in front of them, and what was behind them is not kept: it needs nothing from the store */
+            none = visit<WRITE>(g, page, WRITE && block_first >= bcast(p.first, j), WRITE && block_first + g.tokens > pos + rest, [&](uint8_t* keys, uint8_t* values) { use(keys, values, 0, 0); });
+        }
+        /* those whose page could not be had as NaN */
+        if constexpr (!WRITE) if (__builtin_expect(none != 0, 0)) use(nullptr, nullptr, none, !there ? 0u : F16 ? 0x7e007e00u : 0x7fc07fc0u);
+    }
+}
+
+template <bool WRITE>
+void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t st)
+{
+    const uint32_t lpr = kv->g.dim <= 64 ? 8 : kv->g.dim <= 128 ? 16 : 32, rpw = 64 / lpr;
+    /* few rows: a trip of heads to a wave, a row to a wave; many: eight trips, and the runs that begin among sixteen rows */
+    io.q_heads_each = io.q && (uint64_t)s.rows * io.q_heads > 16384 ? 8 * rpw : rpw;
+    io.q_waves = io.q ? (uint32_t)((io.q_heads + io.q_heads_each - 1) / io.q_heads_each * s.rows) : 0;
+    io.piece = kv->g.tokens < 16 ? 8 : 16;
+    io.window = s.starts && s.rows / s.n >= 8 ? (kv->g.tokens < 64 ? kv->g.tokens : 64) : 1;
+    const uint64_t waves = (uint64_t)io.q_waves + (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads;
+    if (waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
+    const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
+#define KV_ROWS(LPR, AL) \
+    if (kv->f16) hipLaunchKernelGGL((k_kv_rows<LPR, 1, WRITE, AL>), grid, block, 0, st, kv->g, s, io); \
+    else hipLaunchKernelGGL((k_kv_rows<LPR, 0, WRITE, AL>), grid, block, 0, st, kv->g, s, io)
+    if (WRITE && !io.aligned) { if (lpr == 8) { KV_ROWS(8, !WRITE); } else if (lpr == 16) { KV_ROWS(16, !WRITE); } else { KV_ROWS(32, !WRITE); } }
+    else if (lpr == 8) { KV_ROWS(8, true); } else if (lpr == 16) { KV_ROWS(16, true); } else { KV_ROWS(32, true); }
+#undef KV_ROWS
+}
+
+} // namespace
+#endif /* __BAM_KV_CACHE_H__ */
