@@ -77,6 +77,7 @@ SIGNATURES = {
     "bam_sssp_float": (c_int, [c_vp, c_vp, c_vp, c_u64, c_u64, c_vp, P(c_u32), c_vp]),
     "bam_kv_create": (c_int, [P(c_vp), c_vp, c_u64, c_u64, c_u32, c_u32, c_int]),
     "bam_kv_destroy": (None, [c_vp]),
+    "bam_kv_create_e4m3": (c_int, [P(c_vp), c_vp, c_u64, c_u64, c_u32, c_u32, c_int, c_vp, c_u64]),
     "bam_kv_info": (c_int, [c_vp, P(c_u64)]),
     "bam_kv_append": (c_int, [c_vp, c_vp, c_vp]),
     "bam_kv_read": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp]),

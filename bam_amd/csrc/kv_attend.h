@@ -18,6 +18,10 @@ struct kv_att {
     uint32_t chunk;                     /* blocks whose pages a wave asks for at a time when it holds them */
     uint32_t items, tile_rows, max_new;
 };
+/* (bam_kv8.hip) */
+struct kv_plan;
+void kv8_rows(const bam_kv_t* kv, const kv_seqs& s, const kv_rows& io, bool write, hipStream_t st);
+void kv8_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st);
 struct kv_plan { uint32_t nt, waves, rows, tiles, splits, steps; uint64_t items, left_at, m_at, l_at, part_at, bytes; };
 
 namespace {
@@ -226,6 +230,24 @@ __device__ __forceinline__ u32x4 only(u32x4 x, const uint32_t bits)
     return x;
 }
 
+/* whether one of the four e4m3 numbers is NaN */
+__device__ __forceinline__ bool odd8(const uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+/* half a piece of keys in 8 bits: eight numbers of a token as an operand in 16 */
+template <int F16> __device__ __forceinline__ u32x4 keys_of(const uint32_t lo, const uint32_t hi, const float by)
+{
+    return u32x4{from8<F16, false>(lo, by), from8<F16, true>(lo, by), from8<F16, false>(hi, by), from8<F16, true>(hi, by)};
+}
+/* a piece of values in 8 bits: numbers 2x and 2x + 1 of eight tokens, each with its own power of two, as two operands in 16 */
+template <int F16> __device__ __forceinline__ void values_of(const u32x4 x, const float (&by)[8], u32x4& a, u32x4& b)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = x[i], y = from8<F16, false>(w, by[2 * i]), z = from8<F16, true>(w, by[2 * i + 1]);
+        a[i] = (y & 0xffffu) | (z << 16);
+        b[i] = (y >> 16) | (z & 0xffff0000u);
+    }
+}
+
 /* which tokens a tile of rows sees, and the order in which they are gone through: steps of 32 tokens, first those that stay visible in front of the window */
 struct kv_span {
     int32_t first_pos, last_pos;        /* positions of the tile's rows */
@@ -263,13 +285,15 @@ __device__ __forceinline__ kv_span span_of(const kv_att& a, const uint32_t most,
  * reaches 4.9 on this card, a plain reader 7.2); 64 of up to 4099: 142 us, 5.6 TB/s, the longest sequence's workgroups last; one of 262121: 165 us, 6.5 TB/s with the join.  More waves to
  * a SIMD (three, four) were 9 % slower.
  */
-template <int DP, int F16, int NT, bool HELD>
+template <int DP, int F16, int E8, int NT, bool HELD>
 __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, const kv_att& a, const kv_span& sp, const uint32_t seq, const uint32_t head, const uint32_t v0, const uint32_t v1,
                                          const u32x4 (&q)[NT][DP / 32], const int32_t (&pos)[NT], f32x4 (&o)[NT][DP / 16], float (&m)[NT], float (&l)[NT], bool& gone, uint32_t& n_access, uint32_t& n_hit)
 {
     using namespace bam;
     const uint32_t lane = bam::lane(), row = lane & 15u, grp = lane >> 4;
     const uint32_t T = g.tokens, D = g.dim;
+    /* 8 bits: half the bytes to a step of 32 tokens, so two steps at a time, or as little as before would be on its way */
+    constexpr int HALVES = E8 && DP <= 128 ? 2 : 1, KP = E8 ? DP / 64 : DP / 32, VP = E8 ? DP / 32 : DP / 16;      /* pieces of a token's keys, and of eight tokens' values, to a lane */
     for (uint32_t v = v0; v < v1;) {
         /* a run of neighbouring steps within one chunk of blocks */
         const bool front = v < sp.front;
@@ -288,6 +312,7 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
         /* blocks the table does not have, or that lie past its end (the last step may go on behind it): their tokens are not visible */
         const uint32_t holes = (uint32_t)ballot((asked && !need) || (in_run && blk >= s.width));
         uint32_t slot = 0;
+        [[maybe_unused]] const uint64_t powers_at = need ? page - g.first_page : 0u;      /* where a lane's page has its powers of two (a block that is not there: the first, which it does not use) */
         uint64_t seen = 0;
         if constexpr (!HELD) {
             if (need) seen = __hip_atomic_load((const uint64_t*)(g.pages + page), __ATOMIC_RELAXED, BAM_AGENT);
@@ -321,14 +346,43 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             if (!all) slot = 0;
         }
         const uint32_t n_blocks = T < 32 ? 32u >> g.tokens_log : 1u, step_blocks = (1u << n_blocks) - 1u;        /* of a step */
-        for (uint32_t t0 = t_first; t0 < t_end; t0 += 32u) {
+        for (uint32_t t_step = t_first; t_step < t_end; t_step += 32u * HALVES) {
+            u32x4 k0[HALVES * KP], k1[HALVES * KP], vv[HALVES * VP];
+            /* what lies past a row's end is not loaded: its place takes the row's beginning, zero among the keys, of no row among the values */
+            const uint8_t *k_at[HALVES * KP], *v_at[HALVES * VP];
+            [[maybe_unused]] float k_by[HALVES][2];
+            [[maybe_unused]] uint64_t v_by[HALVES];
             /* this lane's tokens as a row of K (8 (row / 4) + row % 4, and 4 further on) and as its part of V (8 grp .. + 7) lie in one block each */
-            const uint32_t kt = T < 16 ? t0 + 8u * (row >> 2) : t0 + 16u * (row >> 3), vt = t0 + 8u * grp;
-            const uint32_t kb = (kt >> g.tokens_log) - b_first, vb = (vt >> g.tokens_log) - b_first;
-            const uint8_t* kp = g.base + ((uint64_t)bam::shfl(slot, kb) << g.page_log) + ((kt & (T - 1u)) + (T < 16 ? row & 3u : row & 7u)) * 16u;
-            const uint8_t* vp = g.base + ((uint64_t)bam::shfl(slot, 32u + vb) << g.page_log) + (((vt & (T - 1u)) >> 3) * D + row) * 16u;
-            /* keys (part 0) or values (part 32) of the step, page by page: `load` for the lanes whose block came, which is `mine` for this lane */
-            auto by_page = [&](const uint32_t part, const uint32_t mine, auto&& load) {
+            uint32_t kbs[HALVES], vbs[HALVES], vts[HALVES];
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) {
+                /* where the run ends with one step the other is a second look at it, which counts for nothing */
+                const uint32_t t0 = t_step + 32u * h < t_end ? t_step + 32u * h : t_step;
+                const uint32_t kt = T < 16 ? t0 + 8u * (row >> 2) : t0 + 16u * (row >> 3), vt = t0 + 8u * grp;
+                const uint32_t kb = (kt >> g.tokens_log) - b_first, vb = (vt >> g.tokens_log) - b_first;
+                kbs[h] = kb; vbs[h] = vb; vts[h] = vt;
+                const uint8_t* kp = g.base + ((uint64_t)bam::shfl(slot, kb) << g.page_log) + ((kt & (T - 1u)) + (T < 16 ? row & 3u : row & 7u)) * 16u;
+                if constexpr (E8) {
+                    const uint8_t* vp = g.base + ((uint64_t)bam::shfl(slot, 32u + vb) << g.page_log) + ((vt & (T - 1u)) >> 3) * (D / 2u) * 16u;
+#pragma unroll
+                    for (uint32_t j = 0; j < KP; j++) k_at[h * KP + j] = kp + ((4u * j + grp) * 16u < D ? (4u * j + grp) * T * 16u : 0u);
+#pragma unroll
+                    for (uint32_t i = 0; i < VP; i++) v_at[h * VP + i] = vp + (32u * i + 2u * row < D ? (16u * i + row) * 16u : 0u);
+                    /* the powers of two of the tokens of the lane's rows of K (places row and row + 8 of sixteen), and of its part of V */
+                    const uint8_t* const kw = g.scales + (uint64_t)bam::shfl(powers_at, kb) * T + (kt & (T - 1u)) + ((row & 4u) << 1 | (row & 3u));
+                    k_by[h][0] = scale_of(kw[0]);
+                    k_by[h][1] = scale_of(kw[4]);
+                    v_by[h] = *(const uint64_t*)(g.scales + (uint64_t)bam::shfl(powers_at, 32u + vb) * T + (vt & (T - 1u)));
+                } else {
+                    const uint8_t* vp = g.base + ((uint64_t)bam::shfl(slot, 32u + vb) << g.page_log) + (((vt & (T - 1u)) >> 3) * D + row) * 16u;
+#pragma unroll
+                    for (uint32_t j = 0; j < KP; j++) k_at[j] = kp + ((4u * j + grp) * 8u < D ? (4u * j + grp) * T * 16u : 0u);
+#pragma unroll
+                    for (uint32_t i = 0; i < VP; i++) v_at[i] = 16u * i < D ? vp + i * 256u : vp;
+                }
+            }
+            /* keys (part 0) or values (part 32) of a step, page by page: `load` for the lanes whose block came, which is `mine` for this lane */
+            auto by_page = [&](const uint32_t t0, const uint32_t part, const uint32_t mine, auto&& load) {
                 bool left = need && (lane & 32u) == part && (lane & 31u) - ((t0 >> g.tokens_log) - b_first) < n_blocks;
                 while (ballot(left)) {
                     uint32_t at = 0;
@@ -342,31 +396,32 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                 }
                 view.n_access = view.n_hit = 0;
             };
-            u32x4 k0[DP / 32], k1[DP / 32], vv[DP / 16];
-            /* what lies past a row's end is not loaded: its place takes the row's beginning, zero among the keys, of no row among the values */
-            const uint8_t *k_at[DP / 32], *v_at[DP / 16];
-#pragma unroll
-            for (uint32_t j = 0; j < DP / 32; j++) k_at[j] = kp + ((4u * j + grp) * 8u < D ? (4u * j + grp) * T * 16u : 0u);
-#pragma unroll
-            for (uint32_t i = 0; i < DP / 16; i++) v_at[i] = 16u * i < D ? vp + i * 256u : vp;
             if (HELD && !all) {
 #pragma unroll
-                for (int j = 0; j < DP / 32; j++) k0[j] = k1[j] = u32x4{0, 0, 0, 0};
+                for (int j = 0; j < HALVES * KP; j++) k0[j] = k1[j] = u32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < DP / 16; i++) vv[i] = u32x4{0, 0, 0, 0};
-                by_page(0, kb, [&](const uint64_t by) {
+                for (int i = 0; i < HALVES * VP; i++) vv[i] = u32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int j = 0; j < DP / 32; j++) { k0[j] = ld_payload((const u32x4*)(k_at[j] + by)); k1[j] = ld_payload((const u32x4*)(k_at[j] + by + (T < 16 ? 64 : 128))); }
-                });
-                if (gone) return true;
-            } else if constexpr (DP <= 128) {
-                if (T < 16) load_step<64>(k_at, v_at, k0, k1, vv); else load_step<128>(k_at, v_at, k0, k1, vv);
+                for (int h = 0; h < HALVES; h++) {
+                    if (h && t_step + 32u * h >= t_end) break;
+                    by_page(t_step + 32u * h, 0, kbs[h], [&](const uint64_t by) {
+#pragma unroll
+                        for (int j = h * KP; j < (h + 1) * KP; j++) { k0[j] = ld_payload((const u32x4*)(k_at[j] + by)); k1[j] = ld_payload((const u32x4*)(k_at[j] + by + (T < 16 ? 64 : 128))); }
+                    });
+                    if (gone) return true;
+                }
+            } else if constexpr (DP <= 128 || E8) {
+                if (!E8 && T < 16) load_step<64>(k_at, v_at, k0, k1, vv); else load_step<128>(k_at, v_at, k0, k1, vv);
             } else {
                 if (T < 16) load_keys<64>(k_at, k0, k1); else load_keys<128>(k_at, k0, k1);
             }
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) {
+            const uint32_t t0 = t_step + 32u * h, vb = vbs[h], vt = vts[h];
+            if (h && t0 >= t_end) break;
             if (D < DP) {
 #pragma unroll
-                for (uint32_t j = 0; j < DP / 32; j++) { const bool in = (4u * j + grp) * 8u < D; k0[j] = in ? k0[j] : u32x4{0, 0, 0, 0}; k1[j] = in ? k1[j] : u32x4{0, 0, 0, 0}; }
+                for (uint32_t j = 0; j < KP; j++) { const bool in = (4u * j + grp) * (E8 ? 16u : 8u) < D; k0[h * KP + j] = in ? k0[h * KP + j] : u32x4{0, 0, 0, 0}; k1[h * KP + j] = in ? k1[h * KP + j] : u32x4{0, 0, 0, 0}; }
             }
             const bool whole = !((holes >> ((t0 >> g.tokens_log) - b_first)) & step_blocks) && (int64_t)t0 + 31 <= sp.first_pos && (!a.window || (int64_t)sp.last_pos - t0 < a.window || t0 + 32u <= a.sinks);
             f32x4 s0[NT], s1[NT];
@@ -374,39 +429,58 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             for (int n = 0; n < NT; n++) {
                 s0[n] = s1[n] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < DP / 32; j++) { s0[n] = mma<F16>(k0[j], q[n][j], s0[n]); s1[n] = mma<F16>(k1[j], q[n][j], s1[n]); }
+                for (int j = 0; j < DP / 32; j++) {
+                    if constexpr (E8) {
+                        const u32x4 x = k0[h * KP + j / 2], y = k1[h * KP + j / 2];
+                        s0[n] = mma<F16>(j & 1 ? keys_of<F16>(x[2], x[3], k_by[h][0]) : keys_of<F16>(x[0], x[1], k_by[h][0]), q[n][j], s0[n]);
+                        s1[n] = mma<F16>(j & 1 ? keys_of<F16>(y[2], y[3], k_by[h][1]) : keys_of<F16>(y[0], y[1], k_by[h][1]), q[n][j], s1[n]);
+                    } else { s0[n] = mma<F16>(k0[j], q[n][j], s0[n]); s1[n] = mma<F16>(k1[j], q[n][j], s1[n]); }
+                }
             }
             if (HELD && !all) {
-                by_page(32, vb, [&](const uint64_t by) {
+                by_page(t0, 32, vb, [&](const uint64_t by) {
 #pragma unroll
-                    for (int i = 0; i < DP / 16; i++) vv[i] = ld_payload((const u32x4*)(v_at[i] + by));
+                    for (int i = h * VP; i < (h + 1) * VP; i++) vv[i] = ld_payload((const u32x4*)(v_at[i] + by));
                 });
                 if (gone) return true;
-            } else if constexpr (DP > 128) {         /* wide heads: the values behind the scores, for which they would not leave registers */
+            } else if constexpr (DP > 128 && !E8) {         /* wide heads: the values behind the scores, for which they would not leave registers */
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int part = 0; part < 2; part++) {
                     const uint8_t* at[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) at[i] = v_at[8 * h + i];
-                    load_pieces(at, vv + 8 * h);
+                    for (int i = 0; i < 8; i++) at[i] = v_at[8 * part + i];
+                    load_pieces(at, vv + 8 * part);
                 }
             }
             const bool hole = (holes >> vb) & 1u;
             bool slow = false;
+            [[maybe_unused]] uint32_t any8 = 0xffu;
             if (!whole) {
                 /* values of tokens that no row sees may be anything: none of it may meet the zeros of P */
-                const uint32_t any = hole ? 0u : seen_of_eight((int32_t)vt, sp.last_pos, low_of(a, sp.first_pos), (int32_t)a.sinks);
+                const uint32_t any = any8 = hole ? 0u : seen_of_eight((int32_t)vt, sp.last_pos, low_of(a, sp.first_pos), (int32_t)a.sinks);
 #pragma unroll
-                for (int i = 0; i < DP / 16; i++) vv[i] = only(vv[i], any);
+                for (int i = h * VP; i < (h + 1) * VP; i++) vv[i] = only(vv[i], any);      /* (in 8 bits: the numbers of a token are 16 bits here too) */
                 if (sp.first_pos != sp.last_pos) {
                     bool odd = false;
 #pragma unroll
-                    for (int i = 0; i < DP / 16; i++)
+                    for (int i = h * VP; i < (h + 1) * VP; i++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) odd |= odd16<F16>(vv[i][e]);
+                        for (int e = 0; e < 4; e++) odd |= E8 ? odd8(vv[i][e]) : odd16<F16>(vv[i][e]);
                     slow = ballot(odd) != 0;
                     if (!HELD && slow) return false;             /* row by row, in the launch that holds its pages: the sums of this one stay where they are */
                 }
+            }
+            /* the values as operands: in 8 bits with each token's power of two, or with one where no row sees it (what stands there may be anything) */
+            u32x4 w[DP / 16];
+            if constexpr (E8) {
+                float by[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) by[e] = (any8 >> e) & 1u ? scale_of((uint32_t)(v_by[h] >> (8 * e)) & 0xffu) : 1.0f;
+#pragma unroll
+                for (int i = 0; i < VP; i++) values_of<F16>(vv[h * VP + i], by, w[2 * i], w[2 * i + 1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < DP / 16; i++) w[i] = vv[i];
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -438,18 +512,19 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                 for (int e = 0; e < 4; e++) p[e] = to16<F16>(x[2 * e], x[2 * e + 1]);
                 if (!HELD || !slow) {
 #pragma unroll
-                    for (int i = 0; i < DP / 16; i++) o[n][i] = mma<F16>(vv[i], p, o[n][i]);
+                    for (int i = 0; i < DP / 16; i++) o[n][i] = mma<F16>(w[i], p, o[n][i]);
                 } else {
                     /* an infinity or NaN among the values of tokens that some rows see and others do not: row by row, what the row does not see as zero */
                     for (uint32_t c = 0; c < 16; c++) {
                         const uint32_t sc = bam::shfl(sees, (lane & 48u) + c);
 #pragma unroll
                         for (int i = 0; i < DP / 16; i++) {
-                            const f32x4 with = mma<F16>(only(vv[i], sc), p, o[n][i]);
+                            const f32x4 with = mma<F16>(only(w[i], sc), p, o[n][i]);
                             if (row == c) o[n][i] = with;
                         }
                     }
                 }
+            }
             }
         }
         fence_meta();                                            /* what was read is here */
@@ -488,7 +563,7 @@ __device__ __forceinline__ bool item_of(const kv_geom& g, const kv_seqs& s, cons
 }
 
 /* a workgroup's split of an item, of its rows from s0 on: its four waves a quarter of the steps each, joined over LDS; the sums to their rows where there is one split, else to a.part */
-template <int DP, int F16, int NT, bool HELD>
+template <int DP, int F16, int E8, int NT, bool HELD>
 __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, const kv_att& a, const uint32_t item, const kv_item& it, const uint32_t s0, const uint32_t split, float* lds, bool& gone)
 {
     using namespace bam;
@@ -519,7 +594,9 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
 #pragma unroll
         for (int j = 0; j < DP / 32; j++) {
             q[n][j] = u32x4{0, 0, 0, 0};
-            if (has && (4u * j + grp) * 8u < D) q[n][j] = a.aligned ? load_piece<true>(from + (4u * j + grp) * 8u) : load_piece<false>(from + (4u * j + grp) * 8u);
+            /* the eight numbers of the lane's operand of keys: in 8 bits, two products share a piece of sixteen */
+            const uint32_t c = E8 ? (4u * (j / 2) + grp) * 16u + (j & 1) * 8u : (4u * j + grp) * 8u;
+            if (has && c < D) q[n][j] = a.aligned ? load_piece<true>(from + c) : load_piece<false>(from + c);
         }
         m[n] = -INFINITY;
         l[n] = 0;
@@ -527,7 +604,7 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
         for (int i = 0; i < DP / 16; i++) o[n][i] = f32x4{0, 0, 0, 0};
     }
     uint32_t n_access = 0, n_hit = 0;
-    const bool ok = kv_steps<DP, F16, NT, HELD>(g, s, a, sp, it.seq, it.head, w0, w1, q, pos, o, m, l, gone, n_access, n_hit);
+    const bool ok = kv_steps<DP, F16, E8, NT, HELD>(g, s, a, sp, it.seq, it.head, w0, w1, q, pos, o, m, l, gone, n_access, n_hit);
     /* [4][R] maxima, [4][R] denominators, [R][DP] sums */
     float *const ms = lds, *const ls = lds + 4 * R, *const os = lds + 8 * R;
     uint32_t* const flag = (uint32_t*)(lds + 8 * R + R * DP);
@@ -575,7 +652,12 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
 #pragma unroll
         for (int w = 0; w < 4; w++) den += ls[w * R + r] * __builtin_amdgcn_exp2f(ms[w * R + r] - use - WEIGHT_SHIFT<F16>);
         if (gone) den = __builtin_nanf("");
-        f32x4 lo = *(const f32x4*)(os + r * DP + c), hi = *(const f32x4*)(os + r * DP + c + 4);
+        f32x4 lo, hi;
+        if constexpr (E8) {                              /* rows 16 i + 2 r and 16 i + 2 r + 1 of O^T are row r of two products */
+            const f32x4 x = *(const f32x4*)(os + r * DP + c / 32u * 32u + c % 32u / 2u), y = *(const f32x4*)(os + r * DP + c / 32u * 32u + 16u + c % 32u / 2u);
+            lo = f32x4{x[0], y[0], x[1], y[1]};
+            hi = f32x4{x[2], y[2], x[3], y[3]};
+        } else { lo = *(const f32x4*)(os + r * DP + c); hi = *(const f32x4*)(os + r * DP + c + 4); }
         if (a.splits > 1) {
             const uint64_t at = ((uint64_t)item * a.tile_rows + (s0 - it.r0) + r) * a.splits + split;
             *(f32x4*)(a.part + at * D + c) = lo;
@@ -594,14 +676,14 @@ __device__ __forceinline__ bool kv_split(const kv_geom& g, const kv_seqs& s, con
 }
 template <int DP, int NT> constexpr uint32_t split_lds() { return (8 * 16 * NT + 16 * NT * DP + 4) * 4; }
 
-template <int DP, int F16, int NT>
+template <int DP, int F16, int E8, int NT>
 __global__ __launch_bounds__(256) void k_kv_attend(const kv_geom g, const kv_seqs s, const kv_att a)
 {
     extern __shared__ float lds[];
     const uint32_t item = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
     kv_item it;
     bool gone = false, ok = true;
-    if (item_of(g, s, a, item, it)) ok = kv_split<DP, F16, NT, false>(g, s, a, item, it, it.r0, split, lds, gone);
+    if (item_of(g, s, a, item, it)) ok = kv_split<DP, F16, E8, NT, false>(g, s, a, item, it, it.r0, split, lds, gone);
     if (threadIdx.x == 0) a.left[blockIdx.x] = ok ? 0 : 1;
 }
 
@@ -629,7 +711,7 @@ template <int DP> constexpr uint32_t tile_lds() { return 2 * 2 * tile_tokens<DP>
  * cycles, to a tile and wave.  A document of 16384 tokens, 32 heads on 8 of 128 numbers: 2.12 ms, 1040 TFLOP/s of what is visible (a large product of the library's: 1218).  Rows of 32 to a
  * wave read a tile's 32 KiB of LDS in as many cycles as its products take; eight waves to a workgroup, one to a compute unit, were a tenth slower than two of four.
  */
-template <int DP, int F16, int NW, bool EXACT>
+template <int DP, int F16, int E8, int NW, bool EXACT>
 __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(const kv_geom g, const kv_seqs s, const kv_att a)
 {
     using namespace bam;
@@ -735,30 +817,84 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     uint32_t at_first = 0, at_end = 0, at_block = 0;          /* of the tile that is on its way */
     uint64_t at_holes = 0;
     const uint32_t k_lane0 = (lane & 7u) * 16u + (lane >> 3) * T * 16u, k_lane1 = (lane & 7u) * 16u + (lane >> 3 ^ 1u) * T * 16u;
+    /* 8 bits: a set of tokens (two units of one block) at a time, a piece of keys and one of values to a lane and load; in registers until the tile before is done with, then
+     * as the 16-bit numbers they stand for to where the pieces of a 16-bit cache would lie */
+    constexpr uint32_t ST = UNITS > 1 ? 16 : 8, SETS = UNITS * 8 / ST, LOADS = ST * DP / 1024;
+    [[maybe_unused]] u32x4 k_raw[E8 ? SETS * LOADS : 1], v_raw[E8 ? SETS * LOADS : 1];
+    [[maybe_unused]] uint32_t k_by[E8 ? SETS * LOADS : 1];
+    [[maybe_unused]] uint64_t v_by[E8 ? SETS * LOADS : 1];
     auto load_tile = [&](const uint32_t buf) {
-        const uint32_t to = lds0 + buf * 2u * HALF;
+        if constexpr (E8) {
 #pragma unroll
-        for (uint32_t x = 0; x < UNITS; x++) {
-            const uint32_t u = wave * UNITS + x, t = t_next + 8u * u, b = ((t >> g.tokens_log) - b_first) & 63u, in = t & (T - 1u);
-            const uint8_t* const k_at = g.base + ((uint64_t)bcast(k_slot, b) << g.page_log) + in * 16u;
-            const uint8_t* const v_at = g.base + ((uint64_t)bcast(v_slot, b) << g.page_log) + (in >> 3) * D * 16u;
+            for (uint32_t x = 0; x < SETS; x++) {
+                const uint32_t t = t_next + wave * UNITS * 8u + x * ST, b = ((t >> g.tokens_log) - b_first) & 63u, in = t & (T - 1u);
+                const __amdgpu_buffer_rsrc_t k_at = __builtin_amdgcn_make_buffer_rsrc(g.base + ((uint64_t)bcast(k_slot, b) << g.page_log), 0, 1 << g.page_log, 0x00027000);
+                const __amdgpu_buffer_rsrc_t v_at = __builtin_amdgcn_make_buffer_rsrc(g.base + ((uint64_t)bcast(v_slot, b) << g.page_log), 0, 1 << g.page_log, 0x00027000);
+                const uint8_t* const by = g.scales + bcast(need ? page - g.first_page : (uint64_t)0, b) * T;
 #pragma unroll
-            for (uint32_t i = 0; i < DP / 64; i++) {
-                /* odd units with neighbouring pieces exchanged: read by sixteen lanes from two units, they lie in different banks */
-                const uint32_t odd = UNITS % 2 ? u & 1u : x & 1u;
-                if (EXACT || (8u * i + (lane >> 3 ^ odd)) * 8u < D) to_lds(k_at, (odd ? k_lane1 : k_lane0) + i * 128u * T, to + u * DP * 16u + i * 1024u);
-                if (EXACT || 64u * i + lane < D) to_lds(v_at, (64u * i + lane) * 16u, to + HALF + u * DP * 16u + i * 1024u);
+                for (uint32_t i = 0; i < LOADS; i++) {
+                    const uint32_t p = i * 64u + lane, place = p % ST, c = p / ST, group = p / (DP / 2u), d2 = p % (DP / 2u);
+                    /* (sc1: past the vector L1; what lies past a row's end is not loaded) */
+                    const uint32_t k_off = (c * T + in + place) * 16u, v_off = (((in >> 3) + group) * (D / 2u) + d2) * 16u;
+                    k_raw[x * LOADS + i] = __builtin_amdgcn_raw_buffer_load_b128(k_at, EXACT || c * 16u < D ? k_off : 0u, 0, 16);
+                    v_raw[x * LOADS + i] = __builtin_amdgcn_raw_buffer_load_b128(v_at, EXACT || d2 * 2u < D ? v_off : 0u, 0, 16);
+                    k_by[x * LOADS + i] = by[place_in(g, in + place)];
+                    v_by[x * LOADS + i] = *(const uint64_t*)(by + T + in + group * 8u);
+                }
+            }
+        } else {
+            const uint32_t to = lds0 + buf * 2u * HALF;
+#pragma unroll
+            for (uint32_t x = 0; x < UNITS; x++) {
+                const uint32_t u = wave * UNITS + x, t = t_next + 8u * u, b = ((t >> g.tokens_log) - b_first) & 63u, in = t & (T - 1u);
+                const uint8_t* const k_at = g.base + ((uint64_t)bcast(k_slot, b) << g.page_log) + in * 16u;
+                const uint8_t* const v_at = g.base + ((uint64_t)bcast(v_slot, b) << g.page_log) + (in >> 3) * D * 16u;
+#pragma unroll
+                for (uint32_t i = 0; i < DP / 64; i++) {
+                    /* odd units with neighbouring pieces exchanged: read by sixteen lanes from two units, they lie in different banks */
+                    const uint32_t odd = UNITS % 2 ? u & 1u : x & 1u;
+                    if (EXACT || (8u * i + (lane >> 3 ^ odd)) * 8u < D) to_lds(k_at, (odd ? k_lane1 : k_lane0) + i * 128u * T, to + u * DP * 16u + i * 1024u);
+                    if (EXACT || 64u * i + lane < D) to_lds(v_at, (64u * i + lane) * 16u, to + HALF + u * DP * 16u + i * 1024u);
+                }
             }
         }
         at_first = t_next; at_end = t_end < sp.len ? t_end : sp.len; at_holes = holes; at_block = b_first;          /* (the last step may go on behind the table's end) */
         t_next += KT;
     };
+    [[maybe_unused]] auto put_tile = [&](const uint32_t buf) {
+        uint8_t* const to = (uint8_t*)lds + buf * 2u * HALF;
+#pragma unroll
+        for (uint32_t x = 0; x < SETS; x++)
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; i++) {
+                const uint32_t p = i * 64u + lane, place = p % ST, c = p / ST, group = p / (DP / 2u), d2 = p % (DP / 2u), n = x * LOADS + i;
+                const uint32_t unit = wave * UNITS + x * (ST / 8u), odd = (unit + (place >> 3)) & 1u;
+                const float by = scale_of(k_by[n]);
+                uint8_t* const k_to = to + (unit + (place >> 3)) * DP * 16u + (place & 7u) * 16u + c * 256u;
+                if (EXACT || c * 16u < D) {
+                    *(u32x4*)(k_to + odd * 128u) = keys_of<F16>(k_raw[n][0], k_raw[n][1], by);
+                    *(u32x4*)(k_to + (odd ^ 1u) * 128u) = keys_of<F16>(k_raw[n][2], k_raw[n][3], by);
+                }
+                float each[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) each[e] = scale_of((uint32_t)(v_by[n] >> (8 * e)) & 0xffu);
+                u32x4 a0, a1;
+                values_of<F16>(v_raw[n], each, a0, a1);
+                /* neighbouring numbers exchanged in every other sixteen: sixteen lanes that write every other piece meet all banks */
+                uint8_t* const v_to = to + HALF + ((unit + group) * DP + d2 * 2u) * 16u;
+                if (EXACT || d2 * 2u < D) {
+                    *(u32x4*)(v_to + (d2 >> 3 & 1u) * 16u) = a0;
+                    *(u32x4*)(v_to + ((d2 >> 3 & 1u) ^ 1u) * 16u) = a1;
+                }
+            }
+    };
     next_blocks();
     bool more = there;
-    if (more) { enter_next(); load_tile(0); }
+    if (more) { enter_next(); load_tile(0); if constexpr (E8) put_tile(0); }
     /* the lane's row of K among the places of 32 tokens: the one that puts the scores of tokens 8 half .. + 7 of each 16 into its accumulators */
     const uint32_t k_row = T < 16 ? (row & 0x13u) | ((row & 4u) << 1) | ((row & 8u) >> 1) : row;
     const uint32_t k_read = (k_row >> 3) * DP * 16u + (k_row & 7u) * 16u + (half ^ (k_row >> 3 & 1u)) * 128u;
+    const uint32_t v_row = E8 ? row ^ (row >> 4) : row;
     for (uint32_t buf = 0; more; buf ^= 1u) {
         fence_meta();                            /* this wave's part of the tile is in LDS, */
         __syncthreads();                         /* and everybody's; and everybody has done with the buffer that is loaded next */
@@ -787,14 +923,17 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             }
             if (ballot(odd)) ok = false;
         }
-        if (idle || (int32_t)t0 > last_pos) continue;
+        if (idle || (int32_t)t0 > last_pos) {
+            if constexpr (E8) if (more) put_tile(buf ^ 1u);
+            continue;
+        }
         /*
          * The operands from LDS are read eight ahead of the products that take them, and the order is held (sched_barrier): left to itself the compiler reads each right before
          * its product and waits for it, a hundred cycles for every 32 of the matrix unit.
          */
         constexpr uint32_t NK = DP / 16 * (KT / 32), NV = DP / 32 * (KT / 16);
         auto key_piece = [&](const uint32_t n) { return *(const u32x4*)(keys + (n / (KT / 32)) * 256u + (n % (KT / 32)) * (DP * 64u) + k_read); };
-        auto value_piece = [&](const uint32_t n) { return *(const u32x4*)(values + ((2u * (n / (DP / 32)) + half) * DP + 32u * (n % (DP / 32)) + row) * 16u); };
+        auto value_piece = [&](const uint32_t n) { return *(const u32x4*)(values + ((2u * (n / (DP / 32)) + half) * DP + 32u * (n % (DP / 32)) + v_row) * 16u); };
         f32x16 x[KT / 32];
 #pragma unroll
         for (uint32_t mt = 0; mt < KT / 32; mt++)
@@ -868,6 +1007,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (E8) if (more) put_tile(buf ^ 1u);
     }
     fence_meta();
     look_again();
@@ -913,7 +1053,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
  * unit has.  One token over 200, heads of 64: 7.4 and 4.5 us of two launches, 7.6 of this one (10.2 a pass for 12.6); over 8000, of 128: 18.5 a pass for 20.0; 7 sequences of 3000
  * 22.2 for 23.9; 60000 and more: the same.  Heads of 256 would spill (5 % slower over 60000), and keep two launches.
  */
-template <int DP, int F16, int NT>
+template <int DP, int F16, int E8, int NT>
 __global__ __launch_bounds__(256) void k_kv_attend_once(const kv_geom g, const kv_seqs s, const kv_att a)
 {
     extern __shared__ float lds[];
@@ -921,14 +1061,14 @@ __global__ __launch_bounds__(256) void k_kv_attend_once(const kv_geom g, const k
     kv_item it;
     bool gone = false;
     if (!item_of(g, s, a, item, it)) return;
-    if (kv_split<DP, F16, NT, false>(g, s, a, item, it, it.r0, split, lds, gone)) return;
+    if (kv_split<DP, F16, E8, NT, false>(g, s, a, item, it, it.r0, split, lds, gone)) return;
     __syncthreads();
     gone = false;
-    kv_split<DP, F16, NT, true>(g, s, a, item, it, it.r0, split, lds, gone);
+    kv_split<DP, F16, E8, NT, true>(g, s, a, item, it, it.r0, split, lds, gone);
 }
 
 /* what the first launch left, with its pages held; ends at once where that is nothing */
-template <int DP, int F16, int NT>
+template <int DP, int F16, int E8, int NT>
 __global__ __launch_bounds__(256) void k_kv_rest(const kv_geom g, const kv_seqs s, const kv_att a)
 {
     extern __shared__ float lds[];
@@ -941,7 +1081,7 @@ __global__ __launch_bounds__(256) void k_kv_rest(const kv_geom g, const kv_seqs 
         if (!a.left[x] || !item_of(g, s, a, (uint32_t)(x / a.splits), it)) continue;
         for (uint32_t s0 = it.r0; s0 < it.r1; s0 += 16u * NT) {
             bool gone = false;
-            kv_split<DP, F16, NT, true>(g, s, a, (uint32_t)(x / a.splits), it, s0, (uint32_t)(x % a.splits), lds, gone);
+            kv_split<DP, F16, E8, NT, true>(g, s, a, (uint32_t)(x / a.splits), it, s0, (uint32_t)(x % a.splits), lds, gone);
             __syncthreads();
         }
     }
@@ -1015,64 +1155,6 @@ __global__ __launch_bounds__(256) void k_kv_join(const kv_geom g, const kv_seqs 
 // launches
 // ---------------------------------------------------------------------------
 
-/* steps of 32 tokens that a tile of `rows` rows can have to look at, of sequences of up to max_len tokens */
-uint64_t most_steps(const uint64_t max_len, const uint64_t new_tokens, const uint32_t window, const uint32_t sinks)
-{
-    const uint64_t all = (max_len + 31) / 32;
-    if (!window) return all;
-    const uint64_t seen = (window + new_tokens + 31) / 32 + 1 + (sinks + 31ull) / 32;
-    return seen < all ? seen : all;
-}
-
-kv_plan plan_of(const bam_kv_t* kv, const uint64_t n_seqs, const uint64_t max_new, const uint32_t q_heads, const uint64_t max_len, const uint32_t window, const uint32_t sinks)
-{
-    kv_plan p{};
-    const uint64_t group = q_heads / kv->g.heads, rows = max_new * group;
-    p.nt = rows <= 16 ? 1 : 2;
-    p.waves = rows <= 32 ? 0 : rows <= 64 ? 2 : 4;
-    p.rows = p.waves ? 32 * p.waves : 16 * p.nt;
-    const uint64_t R = p.rows;
-    p.tiles = (uint32_t)((rows + R - 1) / R);
-    p.items = n_seqs * p.tiles * kv->g.heads;
-    const uint64_t steps = most_steps(max_len, (R + group - 1) / group + 1, window, sinks);
-    /*
-     * Workgroups: as many as keep the memory busy, and no more, since each has its latencies before its first token and behind its last, and its split is written and
-     * read again.  Few rows, four waves: one to a compute unit where a step of 32 tokens is 16 KiB, two where it is 8.  32 heads on 8 of 128 numbers, one token each, with
-     * a workgroup for 512 / 256 of the device: 8 sequences of up to 8000 tokens 51 / 45 us, one of 262121 179 / 167; heads of 64 numbers, 32 sequences of
-     * up to 4000, 1024 / 512 / 256: 30 / 28 / 34.
-     */
-    uint64_t splits = (kv->g.dim <= 64 ? 512 : 256) / p.items;
-    /*
-     * Tiles of rows: as many workgroups as the LDS of the compute units has room for, but no splits where there is one to each already.  The same heads, with
-     * splits for 1024 / 512 / 256 workgroups whatever there is: 1000 new tokens (256 tiles) 41 / 40 / 32 us, 500 after 32500 (128 tiles) 325 / 309 / 377;
-     * 10 after 16000 of eight sequences (64 tiles of two waves) 99 / 94 / 101; heads of 64 numbers, the same 45 / 59.
-     */
-    if (p.waves) splits = p.items >= 256 ? 1 : (kv->g.dim <= 64 ? 2048 / p.waves : 512) / p.items;
-    /*
-     * The shortest split: 16 steps, and 8 where that makes no more than 32 splits, whose join is short; for few rows only above 1024 tokens, below them the join costs more than
-     * is gained, and 32 for tiles that half the compute units have one of.  At least 32 / 16 / 8 steps: 10 new tokens of 2000 34 / 24 / 19 us, of 16000
-     * 35 / 26 / 28 (63 splits), 500 of 600 (128 tiles) 24 / 27 / 31; one token of 600, heads of 64, - / 13 / 15, of 2500 - / 14 / 13, heads of 256 - / 31 / 24.
-     */
-    uint64_t most = (steps + 15) / 16;
-    if (p.waves && p.items >= 128) most = (steps + 31) / 32;
-    else if (most < 32 && (p.waves || steps > 32)) most = (steps + 7) / 8 < 32 ? (steps + 7) / 8 : 32;
-    if (splits > most) splits = most;
-    if (splits > 256) splits = 256;
-    if (splits < 1) splits = 1;
-    p.steps = (uint32_t)((steps + splits - 1) / splits + 3) & ~3u;
-    if (p.steps < 4) p.steps = 4;
-    p.splits = (uint32_t)((steps + p.steps - 1) / p.steps);
-    if (p.splits < 1) p.splits = 1;
-    auto place = [&](uint64_t bytes) { const uint64_t at = p.bytes; p.bytes += (bytes + 255) & ~255ull; return at; };
-    p.left_at = place(p.items * p.splits);
-    if (p.splits > 1) {
-        p.m_at = place(p.items * R * p.splits * 4);
-        p.l_at = place(p.items * R * p.splits * 4);
-        p.part_at = place(p.items * R * p.splits * kv->g.dim * 4);
-    }
-    return p;
-}
-
 /* a kernel and not a memset: the stream may be captured */
 __global__ void k_kv_all_left(uint8_t* left, const uint64_t n)
 {
@@ -1080,7 +1162,7 @@ __global__ void k_kv_all_left(uint8_t* left, const uint64_t n)
     if (i < n) left[i] = 1;
 }
 
-template <int DP, int F16, int NT>
+template <int DP, int F16, int E8, int NT>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan& p, hipStream_t st)
 {
     constexpr uint32_t lds = split_lds<DP, NT>(), lds_tiles = tile_lds<DP>();
@@ -1096,18 +1178,18 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     a.tile_rows = p.rows;
     const dim3 grid((uint32_t)all);
     if (once) {
-        if constexpr (DP <= 128) hipLaunchKernelGGL((k_kv_attend_once<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
+        if constexpr (DP <= 128) hipLaunchKernelGGL((k_kv_attend_once<DP, F16, E8, NT>), grid, dim3(256), lds, st, kv->g, s, a);
     } else {
         if (!kv->unheld) hipLaunchKernelGGL(k_kv_all_left, dim3((uint32_t)((all + 255) / 256)), dim3(256), 0, st, a.left, all);
-        else if (!p.waves) hipLaunchKernelGGL((k_kv_attend<DP, F16, NT>), grid, dim3(256), lds, st, kv->g, s, a);
+        else if (!p.waves) hipLaunchKernelGGL((k_kv_attend<DP, F16, E8, NT>), grid, dim3(256), lds, st, kv->g, s, a);
         else if constexpr (NT == 2) {
             const bool exact = kv->g.dim == DP;
-            if (p.waves == 2 && exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, true>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
-            else if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 2, false>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
-            else if (exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, true>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
-            else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, 4, false>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+            if (p.waves == 2 && exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, E8, 2, true>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
+            else if (p.waves == 2) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, E8, 2, false>), grid, dim3(128), lds_tiles, st, kv->g, s, a);
+            else if (exact) hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, E8, 4, true>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
+            else hipLaunchKernelGGL((k_kv_attend_tiles<DP, F16, E8, 4, false>), grid, dim3(256), lds_tiles, st, kv->g, s, a);
         }
-        hipLaunchKernelGGL((k_kv_rest<DP, F16, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
+        hipLaunchKernelGGL((k_kv_rest<DP, F16, E8, NT>), dim3((uint32_t)groups), dim3(256), lds, st, kv->g, s, a);
     }
     if (p.splits == 1) return;
     constexpr int LPR = DP / 4;
@@ -1115,18 +1197,18 @@ void launch_attend(const bam_kv_t* kv, const kv_seqs& s, kv_att a, const kv_plan
     if (p.splits >= 16) hipLaunchKernelGGL((k_kv_join<LPR, F16, true>), dim3((uint32_t)((rows + rpw - 1) / rpw)), dim3(256), 0, st, kv->g, s, a);
     else hipLaunchKernelGGL((k_kv_join<LPR, F16, false>), dim3((uint32_t)((rows + 4 * rpw - 1) / (4 * rpw))), dim3(256), 0, st, kv->g, s, a);
 }
-template <int DP, int F16>
+template <int DP, int F16, int E8>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st)
 {
-    if (p.nt == 1) launch_attend<DP, F16, 1>(kv, s, a, p, st);
-    else launch_attend<DP, F16, 2>(kv, s, a, p, st);
+    if (p.nt == 1) launch_attend<DP, F16, E8, 1>(kv, s, a, p, st);
+    else launch_attend<DP, F16, E8, 2>(kv, s, a, p, st);
 }
-template <int F16>
+template <int F16, int E8>
 void launch_attend(const bam_kv_t* kv, const kv_seqs& s, const kv_att& a, const kv_plan& p, hipStream_t st)
 {
-    if (kv->g.dim <= 64) launch_attend<64, F16>(kv, s, a, p, st);
-    else if (kv->g.dim <= 128) launch_attend<128, F16>(kv, s, a, p, st);
-    else launch_attend<256, F16>(kv, s, a, p, st);
+    if (kv->g.dim <= 64) launch_attend<64, F16, E8>(kv, s, a, p, st);
+    else if (kv->g.dim <= 128) launch_attend<128, F16, E8>(kv, s, a, p, st);
+    else launch_attend<256, F16, E8>(kv, s, a, p, st);
 }
 
 } // namespace

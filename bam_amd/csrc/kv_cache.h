@@ -5,6 +5,9 @@
 // which the matrix instructions take them:
 //   keys    piece (c, t) at (c * T + place(t)) * 16: numbers 8c .. 8c+7 of token t             c < dim / 8
 //   values  piece (t, d) at (t * dim + d) * 16: number d of tokens 8t .. 8t+7           t < T / 8
+// and in 8 bits (T rows of `dim` bytes fit a page, sixteen at least)
+//   keys    piece (c, t) at (c * T + place(t)) * 16: numbers 16c .. 16c+15 of token t           c < dim / 16
+//   values  piece (t, x) at (t * dim/2 + x) * 16: numbers 2x and 2x+1 of token 8t, of 8t+1, ..       t < T / 8
 // place(t) is t with its bits 2 and 3 exchanged (t itself where a page holds eight tokens).  What neighbouring lanes of a wave load lies next to each other, and
 // is an operand as it stands: with the scores taken as S^T = K Q^T and the output as O^T = V^T P^T, a lane's accumulators of the scores are its
 // part of P^T if the rows of K come in that order.
@@ -25,11 +28,12 @@ struct kv_geom {
     uint8_t* base;
     uint64_t first_page, n_blocks;
     uint32_t heads, dim, tokens, tokens_log, page_log;
+    uint8_t* scales;                    /* 8 bits: powers of two of the rows, [pages of the cache][tokens], each 127 more than it is; 16 bits: NULL */
 };
 struct bam_kv {
     bam_array_t* a;
     kv_geom g;
-    int f16;
+    int f16, e8;                        /* e8: 8 bits in the pages */
     uint64_t cache_pages;
     bool unheld;                        /* reads of resident pages without a reference are switched on */
 };
@@ -116,6 +120,47 @@ template <bool ALIGNED> __device__ __forceinline__ u32x4 load_piece(const uint16
     return x;
 }
 
+// ---- the cache in 8 bits ----
+/*
+ * A row y (a token's keys of a head, or its values) is kept as e4m3 numbers (a sign, four bits of exponent, three of mantissa; the largest is 448) and a power of two: k is
+ * the least whole number with max |y| <= 448 * 2^k, between the bounds below, and what is kept of a number is y / 2^k rounded to the nearest, ties to even.
+ * A power of two and not max |y| / 448: what a row stands for is then exact in the 16-bit types (4 significant bits, and a range that the bounds keep inside theirs; in
+ * float16 but for what is smaller than that type's steps of 2^-24), so the matrix unit takes it without a second rounding; and a number of 4 significant bits is no nearer for another
+ * scale.  For the same reason there is no need of e5m2's range.
+ * Bounds: 448 * 2^k is over the type's largest for the upper one; the lower one keeps 2^(k - 9), the smallest step, a normal number (bfloat16), or the type's smallest numbers
+ * whole (float16).  A number of 1.9375 and more times the type's largest power of two would be rounded up past the type: it is kept as 1.875 times that, less than a step of an
+ * eighth away.  What is not finite is kept as NaN, and has no part in k.
+ */
+template <int F16> constexpr int32_t LEAST_POWER = F16 ? -24 : -110;
+template <int F16> constexpr int32_t MOST_POWER = F16 ? 8 : 120;
+template <int F16> constexpr float MOST_KEPT = F16 ? 1.875f * 0x1p15f : 1.875f * 0x1p127f;
+/* largest of the numbers of magnitude |x|, those that are not finite left out */
+__device__ __forceinline__ float larger_finite(const float a, const float x) { const float m = fabsf(x); return m < INFINITY ? fmaxf(a, m) : a; }
+/* 127 + k for a largest number of a */
+template <int F16> __device__ __forceinline__ uint32_t power_of(const float a)
+{
+    const uint32_t bits = __builtin_bit_cast(uint32_t, fminf(a, MOST_KEPT<F16>));
+    const int32_t k = (int32_t)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return 127u + (uint32_t)(k < LEAST_POWER<F16> ? LEAST_POWER<F16> : k > MOST_POWER<F16> ? MOST_POWER<F16> : k);
+}
+__device__ __forceinline__ float scale_of(const uint32_t power) { return __builtin_bit_cast(float, power << 23); }
+__device__ __forceinline__ float inverse_of(const uint32_t power) { return __builtin_bit_cast(float, (254u - power) << 23); }
+template <int F16> __device__ __forceinline__ float for8(const float y, const float inverse)
+{
+    return fabsf(y) < INFINITY ? fminf(fmaxf(y, -MOST_KEPT<F16>), MOST_KEPT<F16>) * inverse : __builtin_nanf("");
+}
+/* two numbers in the low or the high half of a word */
+template <int F16, bool HIGH> __device__ __forceinline__ uint32_t to8(const uint32_t word, const float a, const float b, const float inverse)
+{
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(for8<F16>(a, inverse), for8<F16>(b, inverse), (int)word, HIGH);
+}
+/* two numbers of the low or the high half of a word, times a power of two, in 16 bits */
+template <int F16, bool HIGH> __device__ __forceinline__ uint32_t from8(const uint32_t word, const float scale)
+{
+    if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, scale, HIGH));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, HIGH));
+}
+
 // ---------------------------------------------------------------------------
 // pages held for the length of a visit
 // ---------------------------------------------------------------------------
@@ -190,7 +235,8 @@ __device__ __forceinline__ void count_accesses(const kv_geom& g, const uint32_t 
 }
 
 // ---------------------------------------------------------------------------
-// rows into the cache and out of it// ---------------------------------------------------------------------------
+// rows into the cache and out of it
+// ---------------------------------------------------------------------------
 
 /* the angles of eight neighbouring numbers of a row; lanes whose numbers are not turned load some, and do not use them */
 struct kv_turn { f32x4 c[2], s[2]; };
@@ -221,13 +267,14 @@ __device__ __forceinline__ kv_turn turn_of(const kv_rows& io, const uint32_t pie
  * Eight neighbouring numbers of a row per lane, LPR lanes to a row: x * rsqrt(mean x^2 + eps) * w, then the rotation of the pairs (i, i + rot/2), or
  * (2i, 2i+1), i < rot/2, by the angles of the row's position; in 32 bits, rounded once.  A position past the tables gives NaN.
  */
-template <int LPR, int F16>
-__device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geom& g, u32x4 x, const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
+template <int F16> __device__ __forceinline__ void in_32_bits(const u32x4 x, float (&f)[8])
 {
-    if (!norm && !io.rot) return x;
-    float f[8];
 #pragma unroll
     for (int i = 0; i < 4; i++) { const uint32_t y = x[i]; f[2 * i] = from16<F16>(y & 0xffffu); f[2 * i + 1] = from16<F16>(y >> 16); }
+}
+template <int LPR, int F16>
+__device__ __forceinline__ void norm_and_rotate(const kv_rows& io, const kv_geom& g, float (&f)[8], const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
+{
     if (norm) {
         float ss = 0;                            /* (pieces past the row's end are zero) */
 #pragma unroll
@@ -262,9 +309,27 @@ __device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geo
             }
         }
     }
+}
+template <int LPR, int F16>
+__device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geom& g, u32x4 x, const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
+{
+    if (!norm && !io.rot) return x;
+    float f[8];
+    in_32_bits<F16>(x, f);
+    norm_and_rotate<LPR, F16>(io, g, f, norm, w, t, piece);
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = to16<F16>(f[2 * i], f[2 * i + 1]);
     return x;
+}
+/* the power of two of a row whose numbers LPR lanes have */
+template <int LPR, int F16> __device__ __forceinline__ uint32_t power_of_row(const float (&f)[8])
+{
+    float a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a = larger_finite(a, f[i]);
+#pragma unroll
+    for (int o = LPR / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
+    return power_of<F16>(a);
 }
 
 /*
@@ -274,7 +339,7 @@ __device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geo
  *   Bound by memory where there are many rows: 19 459 rows of 32 heads on 8 of 128 numbers, normed and turned, 480 MB in 124 us (3.9 TB/s), 160 MB out again in 43; a wave for
  * each four rows took 288 and 112 (each looked its sequence up for 1 KiB).  Few rows: the chain of looks, table, references, rows, 6 to 7 us.
  */
-template <int LPR, int F16, bool WRITE, bool ALIGNED>
+template <int LPR, int F16, int E8, bool WRITE, bool ALIGNED>
 __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
 {
     using namespace bam;
@@ -329,6 +394,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
         const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), seq = bcast(p.seq, j), row = (uint32_t)first_row + j;
         uint64_t page = 0;
         const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, head, page);
+        uint8_t* const powers = g.scales + (page - g.first_page) * g.tokens;      /* of the block's keys, and of its values behind them (only used where the block is there) */
         const uint32_t run_first = pos & (g.tokens - 1u), block_first = pos - run_first, run_end = rest < g.tokens - run_first ? run_first + rest : g.tokens;
         const uint32_t groups = io.piece / 8u, pairs = g.dim / 2u;
         /* a piece: `cnt` tokens from `in_block` of the block on; `none`: rows out are `fill` in place of keys (1), of values (2) */
@@ -344,12 +410,18 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
             if (keys || (none & 1u)) {
                 u32x4 x[TRIPS];
                 const uint32_t r0 = l / LPR;
-                uint8_t* const at = keys + (uint64_t)(col / 8u) * g.tokens * 16u;
+                /* in 8 bits the lane has one half of a piece */
+                uint8_t* const at = E8 ? keys + (uint64_t)(col / 16u) * g.tokens * 16u + (col & 8u) : keys + (uint64_t)(col / 8u) * g.tokens * 16u;
 #pragma unroll
                 for (uint32_t e = 0; e < TRIPS; e++) {
                     const uint32_t r = r0 + e * RPW < cnt ? r0 + e * RPW : 0u;
                     if constexpr (WRITE) x[e] = load_piece<ALIGNED>(k_rows + (int64_t)r * io.k_row + col);
-                    else x[e] = none & 1u ? u32x4{fill, fill, fill, fill} : ld_payload((const u32x4*)(at + place_in(g, in_block + r) * 16u));
+                    else if (none & 1u) x[e] = u32x4{fill, fill, fill, fill};
+                    else if constexpr (E8) {
+                        const uint64_t y = ld_payload((const uint64_t*)(at + place_in(g, in_block + r) * 16u));
+                        const float by = scale_of(powers[in_block + r]);
+                        x[e] = u32x4{from8<F16, false>((uint32_t)y, by), from8<F16, true>((uint32_t)y, by), from8<F16, false>((uint32_t)(y >> 32), by), from8<F16, true>((uint32_t)(y >> 32), by)};
+                    } else x[e] = ld_payload((const u32x4*)(at + place_in(g, in_block + r) * 16u));
                 }
                 u32x4 w{0, 0, 0, 0};
                 if (WRITE && io.k_norm) w = load_piece<true>(io.k_norm + col);
@@ -359,18 +431,46 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                     const uint32_t r = r0 + e * RPW;
                     if constexpr (WRITE) {
                         const kv_turn t = turn_of(io, piece, pos + off + (r < cnt ? r : 0u));
-                        x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.k_norm != nullptr, w, t, piece);
-                        if (r < cnt && in_row) st16_sys(at + place_in(g, in_block + r) * 16u, x[e]);
+                        if constexpr (E8) {
+                            float f[8];
+                            in_32_bits<F16>(in_row ? x[e] : u32x4{0, 0, 0, 0}, f);
+                            norm_and_rotate<LPR, F16>(io, g, f, io.k_norm != nullptr, w, t, piece);
+                            const uint32_t power = power_of_row<LPR, F16>(f);
+                            const float by = inverse_of(power);
+                            const uint32_t lo = to8<F16, true>(to8<F16, false>(0, f[0], f[1], by), f[2], f[3], by), hi = to8<F16, true>(to8<F16, false>(0, f[4], f[5], by), f[6], f[7], by);
+                            if (r < cnt && in_row) {
+                                __hip_atomic_store((uint64_t*)(at + place_in(g, in_block + r) * 16u), (uint64_t)hi << 32 | lo, __ATOMIC_RELAXED, BAM_SYSTEM);
+                                if (piece == 0) powers[in_block + r] = (uint8_t)power;
+                            }
+                        } else {
+                            x[e] = norm_and_rotate<LPR, F16>(io, g, in_row ? x[e] : u32x4{0, 0, 0, 0}, io.k_norm != nullptr, w, t, piece);
+                            if (r < cnt && in_row) st16_sys(at + place_in(g, in_block + r) * 16u, x[e]);
+                        }
                     } else if (r < cnt && in_row) *(u32x4*)(k_rows + (int64_t)r * io.k_row + col) = x[e];
                 }
             }
             if (values || (none & 2u)) {
+                /* in 8 bits: the powers of two of the rows first, those of the sixteen tokens that the piece is of */
+                [[maybe_unused]] uint32_t power[16];
+                if constexpr (E8 && WRITE) {
+#pragma unroll
+                    for (uint32_t e = 0; e < TRIPS; e++) {
+                        const int32_t r = (int32_t)(l / LPR + e * RPW) - piece_first;
+                        const bool mine = r >= 0 && r < (int32_t)cnt;
+                        float f[8];
+                        in_32_bits<F16>(load_piece<ALIGNED>(v_rows + (int64_t)(mine ? r : 0) * io.v_row + col), f);
+                        const uint32_t x = power_of_row<LPR, F16>(f);
+                        if (mine && piece == 0) powers[g.tokens + in_block + r] = (uint8_t)x;
+#pragma unroll
+                        for (uint32_t i = 0; i < RPW; i++) power[e * RPW + i] = (uint32_t)__builtin_amdgcn_readlane((int)x, (int)(i * LPR));
+                    }
+                }
 #pragma unroll
                 for (uint32_t e = 0; e < DT; e++) {
                     const uint32_t y = e * 64u + l, group = y / pairs, d = y % pairs * 2u;
                     const int32_t tok = (int32_t)(group * 8u) - piece_first;
                     if (group >= groups || tok + 8 <= 0 || tok >= (int32_t)cnt) continue;
-                    uint8_t* const at = values + ((uint64_t)((in_block + tok) >> 3) * g.dim + d) * 16u;
+                    uint8_t* const at = E8 ? values + ((uint64_t)((in_block + tok) >> 3) * pairs + d / 2u) * 16u : values + ((uint64_t)((in_block + tok) >> 3) * g.dim + d) * 16u;
                     uint16_t* const rows = v_rows + d;
                     const bool full = tok >= 0 && tok + 8 <= (int32_t)cnt;
                     if constexpr (WRITE) {
@@ -381,7 +481,23 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                             const uint16_t* const from = rows + r * io.v_row;
                             z[t] = ALIGNED ? *(const uint32_t*)from : (uint32_t)from[0] | ((uint32_t)from[1] << 16);
                         }
-                        if (full) {
+                        if constexpr (E8) {
+                            u32x4 y;
+#pragma unroll
+                            for (int t = 0; t < 4; t++) {
+                                const uint32_t a = z[2 * t], b = z[2 * t + 1];
+                                const uint32_t w = to8<F16, false>(0, from16<F16>(a & 0xffffu), from16<F16>(a >> 16), inverse_of(group ? power[8 + 2 * t] : power[2 * t]));
+                                y[t] = to8<F16, true>(w, from16<F16>(b & 0xffffu), from16<F16>(b >> 16), inverse_of(group ? power[8 + 2 * t + 1] : power[2 * t + 1]));
+                            }
+                            if (full) st16_sys(at, y);
+                            else {
+#pragma unroll
+                                for (int32_t t = 0; t < 8; t++) {
+                                    const uint32_t w = y[t / 2];
+                                    if (tok + t >= 0 && tok + t < (int32_t)cnt) __hip_atomic_store((uint16_t*)at + t, (uint16_t)(t & 1 ? w >> 16 : w), __ATOMIC_RELAXED, BAM_SYSTEM);
+                                }
+                            }
+                        } else if (full) {
                             u32x4 lo, hi;
 #pragma unroll
                             for (int t = 0; t < 4; t++) {
@@ -397,6 +513,20 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                                     __hip_atomic_store((uint16_t*)at + t, (uint16_t)z[t], __ATOMIC_RELAXED, BAM_SYSTEM);
                                     __hip_atomic_store((uint16_t*)at + 8 + t, (uint16_t)(z[t] >> 16), __ATOMIC_RELAXED, BAM_SYSTEM);
                                 }
+                        }
+                    } else if constexpr (E8) {
+                        u32x4 y{0, 0, 0, 0};
+                        uint64_t by = 0;
+                        if (!(none & 2u)) {
+                            y = ld_payload((const u32x4*)at);
+                            by = *(const uint64_t*)(powers + g.tokens + in_block + tok);
+                        }
+#pragma unroll
+                        for (int32_t t = 0; t < 8; t++) {
+                            const float scale = scale_of((uint32_t)(by >> (8 * t)) & 0xffu);
+                            const uint32_t w = y[t / 2];
+                            const uint32_t x = none & 2u ? fill : t & 1 ? from8<F16, true>(w, scale) : from8<F16, false>(w, scale);
+                            if (full || (tok + t >= 0 && tok + t < (int32_t)cnt)) *(uint32_t*)(rows + (tok + t) * io.v_row) = x;
                         }
                     } else {
                         u32x4 lo{fill, fill, fill, fill}, hi = lo;
@@ -429,7 +559,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
     }
 }
 
-template <bool WRITE>
+template <int E8, bool WRITE>
 void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t st)
 {
     const uint32_t lpr = kv->g.dim <= 64 ? 8 : kv->g.dim <= 128 ? 16 : 32, rpw = 64 / lpr;
@@ -442,8 +572,8 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
     if (waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
     const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
 #define KV_ROWS(LPR, AL) \
-    if (kv->f16) hipLaunchKernelGGL((k_kv_rows<LPR, 1, WRITE, AL>), grid, block, 0, st, kv->g, s, io); \
-    else hipLaunchKernelGGL((k_kv_rows<LPR, 0, WRITE, AL>), grid, block, 0, st, kv->g, s, io)
+    if (kv->f16) hipLaunchKernelGGL((k_kv_rows<LPR, 1, E8, WRITE, AL>), grid, block, 0, st, kv->g, s, io); \
+    else hipLaunchKernelGGL((k_kv_rows<LPR, 0, E8, WRITE, AL>), grid, block, 0, st, kv->g, s, io)
     if (WRITE && !io.aligned) { if (lpr == 8) { KV_ROWS(8, !WRITE); } else if (lpr == 16) { KV_ROWS(16, !WRITE); } else { KV_ROWS(32, !WRITE); } }
     else if (lpr == 8) { KV_ROWS(8, true); } else if (lpr == 16) { KV_ROWS(16, true); } else { KV_ROWS(32, true); }
 #undef KV_ROWS

@@ -34,9 +34,13 @@ class KVCache:
     `table[b, i]` is the block of its tokens i * block_tokens and on; rows starts[b] .. starts[b+1]-1 of the packed inputs are its newest tokens
     (starts None: one new token each).  They are queued on the current stream.  A block number outside the cache is not read or written.  There are no gradients: tensors
     that require them are refused where gradients are being recorded.
+
+    stored: what the pages hold.  None: numbers of `dtype`.  torch.float8_e4m3fn: half as many bytes, each row (a token's keys of a head, or its values) as eight-bit numbers of
+    four significant bits and a power of two; keys are normed and turned in 32 bits and rounded once, to that.  The powers of two are `scales`, a byte for each row in device memory
+    (uint8 [n_blocks, n_heads, 2, block_tokens]: keys, values): given, or made here.  A cache that is opened again over pages that hold something needs the scales that go with them.
     """
 
-    def __init__(self, array, n_heads, head_dim, dtype=torch.bfloat16, first_page=0, n_blocks=None, _owned=()):
+    def __init__(self, array, n_heads, head_dim, dtype=torch.bfloat16, first_page=0, n_blocks=None, _owned=(), stored=None, scales=None):
         self.L = _lib.load()
         self.h = c_vp()
         self._owned = list(_owned)
@@ -44,11 +48,30 @@ class KVCache:
             raise BamError("KVCache: dtype must be torch.bfloat16 or torch.float16")
         if n_blocks is None:
             raise BamError("KVCache: n_blocks must be given")
+        if stored not in (None, dtype, torch.float8_e4m3fn):
+            raise BamError("KVCache: stored must be None (numbers of dtype) or torch.float8_e4m3fn")
+        eight = stored is torch.float8_e4m3fn
+        if scales is not None and not eight:
+            raise BamError("KVCache: scales go with stored=torch.float8_e4m3fn")
         self.array = array
         self._index = array.device
         self.device = torch.device("cuda", array.device)
-        self.n_heads, self.head_dim, self.dtype = n_heads, head_dim, dtype
-        _chk(self.L.bam_kv_create(ctypes.byref(self.h), array.h, first_page, n_blocks, n_heads, head_dim, _TYPES[dtype]), "bam_kv_create")
+        self.n_heads, self.head_dim, self.dtype, self.stored = n_heads, head_dim, dtype, torch.float8_e4m3fn if eight else dtype
+        what = (ctypes.byref(self.h), array.h, first_page, n_blocks, n_heads, head_dim, _TYPES[dtype])
+        if eight:
+            if head_dim < 1 or n_blocks < 1 or n_heads < 1:
+                raise BamError("KVCache: n_blocks, n_heads and head_dim must be at least 1")
+            shape = (n_blocks, n_heads, 2, 1 << max(0, (array.ranges[0].cache.info()["page_size"] // head_dim).bit_length() - 1))
+            if scales is None:
+                scales = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+                # rows that are appended on another stream come after this
+                torch.cuda.current_stream(self.device).synchronize()
+            elif scales.shape != shape or scales.dtype is not torch.uint8 or scales.get_device() != self._index or not scales.is_contiguous():
+                raise BamError(f"KVCache: scales must be contiguous {list(shape)} in uint8 on {self.device}")
+            _chk(self.L.bam_kv_create_e4m3(*what, scales.data_ptr(), scales.numel()), "bam_kv_create_e4m3")
+        else:
+            _chk(self.L.bam_kv_create(*what), "bam_kv_create")
+        self.scales = scales
         out = (c_u64 * 4)()
         _chk(self.L.bam_kv_info(self.h, out), "bam_kv_info")
         self.block_tokens, self.n_blocks, self.pages_per_block, self.page_size = list(out)
@@ -200,9 +223,9 @@ class KVCache:
             pass
 
 
-def make_kv_cache(ctrl, n_blocks, n_heads, head_dim, page_size=4096, cache_pages=None, dtype=torch.bfloat16, device=0, disk_offset_bytes=0, max_range=64):
+def make_kv_cache(ctrl, n_blocks, n_heads, head_dim, page_size=4096, cache_pages=None, dtype=torch.bfloat16, device=0, disk_offset_bytes=0, max_range=64, stored=None, scales=None):
     """Page cache + one range + array + key-value cache of n_blocks blocks, stored from byte disk_offset_bytes (page aligned).  cache_pages: slots of the page cache (all
-    pages of the blocks unless given, and 64 at least)."""
+    pages of the blocks unless given, and 64 at least).  stored, scales: what the pages hold (KVCache)."""
     if disk_offset_bytes < 0 or page_size <= 0 or disk_offset_bytes % page_size:
         raise BamError("make_kv_cache: disk_offset_bytes must be the beginning of a page")
     n_pages = 2 * n_blocks * n_heads
@@ -212,7 +235,7 @@ def make_kv_cache(ctrl, n_blocks, n_heads, head_dim, page_size=4096, cache_pages
         elems = n_pages * page_size // 8
         made.insert(0, Range(0, elems, disk_offset_bytes // page_size, n_pages, 0, page_size, made[0], device))
         made.insert(0, Array(elems, disk_offset_bytes, [made[0]], device))
-        return KVCache(made[0], n_heads, head_dim, dtype, 0, n_blocks, _owned=made)
+        return KVCache(made[0], n_heads, head_dim, dtype, 0, n_blocks, _owned=made, stored=stored, scales=scales)
     except BaseException:
         # not left to the collector: the error may be kept for longer than the controller lives
         for x in made:

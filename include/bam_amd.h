@@ -445,6 +445,17 @@ double bam_target_ceiling_iops(uint64_t ns_bytes, uint32_t lba_bytes, int backin
  * The calls are queued on `stream` and do not wait; they may be captured into a graph.  A handle keeps nothing from call to call.  The array outlives it. */
 int bam_kv_create(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t n_blocks, uint32_t n_heads, uint32_t dim /* a multiple of 16, at most 256 */,
                   int f16 /* 0: bfloat16, 1: float16 */);
+/*
+ * The same with 8 bits to a number in the pages: half the pages, bytes and reads from the store for the same tokens.  What goes in and comes out has the type that f16 names.  A row
+ * (a token's keys of a head, or its values), worked out in 32 bits and not rounded before, is kept as e4m3 numbers (finite ones up to 448) and a power of two: k is the least whole number for which
+ * its largest magnitude is at most 448 * 2^k, from -110 to 120 (bfloat16) or -24 to 8 (float16); y is kept as y / 2^k rounded to the nearest, ties to even, and stands for that times 2^k,
+ * exactly so in the 16-bit type (in float16, numbers below 2^-14 come out as multiples of 2^-24).  Magnitudes above 1.875 times the type's largest power of two (2^127, 2^15) are kept as that, and what is not finite as NaN, which has no part in k.
+ * T is the largest power of two for which T rows of `dim` bytes fit a page, 16 at least.  Of keys, piece c * T + place(t) has numbers 16c .. 16c+15 of token t; of values, piece
+ * t * dim/2 + x has numbers 2x and 2x+1 of token 8t, of token 8t+1, and so on.
+ * d_scales: 2 * n_blocks * n_heads * T bytes of device memory, the caller's, aligned to 16, for as long as the handle lives: k + 127 of each row, in the order of the pages.  What was appended is
+ * in the pages and there: a cache that is opened again over the same pages needs both.
+ */
+int bam_kv_create_e4m3(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t n_blocks, uint32_t n_heads, uint32_t dim, int f16, uint8_t* d_scales, uint64_t scales_bytes);
 void bam_kv_destroy(bam_kv_t* kv);
 /* out[0] tokens to a block, [1] blocks, [2] pages to a block, [3] bytes of a page */
 int bam_kv_info(bam_kv_t* kv, uint64_t* out);
