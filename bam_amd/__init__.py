@@ -9,4 +9,5 @@ CPU fallback: without the built library every call raises.
 from ._lib import load, load_host, LibraryMissing  # noqa: F401
 from .host import Target, Controller, PageCache, Range, Array, Range32, Array32, sssp, sssp_float, vectoradd, BamError  # noqa: F401
 from .kv import KVCache, make_kv_cache  # noqa: F401
+from .beam import beam_select  # noqa: F401
 from . import gen  # noqa: F401

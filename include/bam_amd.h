@@ -510,6 +510,29 @@ typedef struct bam_kv_attend {
 int bam_kv_attend_bytes(bam_kv_t* kv, uint64_t n_seqs, uint64_t max_new, uint32_t q_heads, uint64_t max_len, uint32_t window, uint32_t sinks, uint64_t* bytes);
 int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream);
 
+/* ---- beam search's selection ----
+ * n_requests of n_beams beams each (up to 1024), with a row of `vocab` logits to a beam, logits_row numbers from row to row (request r's beam i is row r * n_beams + i; type: 0 bfloat16,
+ * 1 float16, 2 float32), and d_scores[r * scores_row + i] the sum of log-probabilities of what beam i has so far.  Out of all continuations of a request's beams by a token, whose sums are
+ * score[i] + logit[i][v] - log(sum over u of exp(logit[i][u])), the `width` (up to 256) with the largest: d_sums, d_beams (the row, r * n_beams + i) and d_tokens, [n_requests][width] each, the largest
+ * first, equal ones in the order of i * vocab + v.  Logarithms and sums are taken in 64 bits, exponentials in 32.  A token whose logit is minus infinity has minus infinity.  All tokens of a beam whose score is not finite have that score, and
+ * those of a beam whose logits have no logarithm of a sum (NaN or infinity among them, none above minus infinity) have NaN, which comes last.
+ * d_work: bam_beam_select_bytes(...) bytes for the length of the call.  Queued on `stream`; it may be captured into a graph. */
+typedef struct bam_beam_select {
+    uint64_t n_requests, n_beams, vocab;
+    const void* d_logits;
+    int64_t logits_row;
+    const float* d_scores;
+    int64_t scores_row;
+    float* d_sums;
+    int32_t *d_beams, *d_tokens;
+    void* d_work;
+    uint64_t work_bytes;
+    uint32_t width;
+    int32_t type;
+} bam_beam_select_t;
+int bam_beam_select_bytes(uint64_t n_requests, uint64_t n_beams, uint64_t vocab, uint32_t width, int type, uint64_t* bytes);
+int bam_beam_select(const bam_beam_select_t* what, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
