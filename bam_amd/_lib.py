@@ -83,6 +83,7 @@ SIGNATURES = {
     "bam_kv_read": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp]),
     "bam_kv_attend_bytes": (c_int, [c_vp, c_u64, c_u64, c_u32, c_u64, c_u32, c_u32, P(c_u64)]),
     "bam_kv_attend": (c_int, [c_vp, c_vp, c_vp]),
+    "bam_kv_reorder": (c_int, [c_vp, c_vp, c_vp]),
     "bam_beam_select_bytes": (c_int, [c_u64, c_u64, c_u64, c_u32, c_int, P(c_u64)]),
     "bam_beam_select": (c_int, [c_vp, c_vp]),
     "bam_bfs_frontier": (c_int, [c_vp, c_vp, c_u64, c_u64, c_vp, P(c_u32), c_vp]),

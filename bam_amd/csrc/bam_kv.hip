@@ -120,6 +120,150 @@ int create(const char* name, bam_kv_t** out, bam_array_t* a, const uint64_t firs
     BAM_API_END
 }
 
+/* ---- the sequences that go on behind a choice of beams ---- */
+struct kv_order {
+    const int32_t *parents, *lens, *table;
+    int64_t stride;
+    uint32_t width, n_old, n_new;
+    const int32_t* spare;
+    int32_t *lens_out, *table_out, *spare_out;
+    int32_t *freed, *copies;            /* [n_old], [n_new]: the last blocks that nobody goes on with; whether a child has one of its own */
+};
+constexpr uint32_t ORDER_OLD = 4096, ORDER_PIECES = 512;      /* old sequences that are looked at at a time; pieces of each page that a wave has in LDS, */
+static_assert(ORDER_OLD * 4 == 2 * ORDER_PIECES * 16, "in the same LDS");
+/* the last block of old sequence p, if it is there and not full; `rest` tokens in it */
+__device__ __forceinline__ bool last_block(const kv_geom& g, const kv_order& o, const uint32_t p, uint32_t& block, uint32_t& rest)
+{
+    const int32_t len = o.lens[p];
+    const uint32_t i = (uint32_t)len >> g.tokens_log;
+    rest = (uint32_t)len & (g.tokens - 1u);
+    if (len <= 0 || !rest || i >= o.width) return false;
+    block = (uint32_t)o.table[(int64_t)p * o.stride + i];
+    return block < g.n_blocks;
+}
+
+/*
+ * Workgroup 0, one wave: the spare blocks that are left.  The others, a wave each: head h of child i, whose last block is copied where an earlier child has the parent's; head 0 writes
+ * the child's length and row of blocks besides.  Whether there is an earlier child each wave finds by itself, in the parents in front of its own: one launch, nobody waits for anybody.
+ *   A page is copied by way of LDS, 8 KiB at a time, by one wave: nothing is held while the other page is waited for, and the new page needs no read (kv_cache.h, visit).  Only
+ * pieces that have tokens move.
+ */
+template <int F16>
+__global__ __launch_bounds__(64) void k_kv_reorder(const kv_geom g, const kv_order o)
+{
+    using namespace bam;
+    __shared__ u32x4 room[2 * ORDER_PIECES];
+    const uint32_t lane = threadIdx.x;
+    if (blockIdx.x == 0) {
+        int32_t* const first_child = (int32_t*)room;
+        uint32_t n_freed = 0;
+        for (uint32_t base = 0; base < o.n_old; base += ORDER_OLD) {
+            const uint32_t here = o.n_old - base < ORDER_OLD ? o.n_old - base : ORDER_OLD;
+            for (uint32_t x = lane; x < here; x += 64u) first_child[x] = 0x7fffffff;
+            __syncthreads();
+            for (uint32_t i = lane; i < o.n_new; i += 64u) {
+                const uint32_t p = (uint32_t)o.parents[i] - base;
+                if (p < here) atomicMin(&first_child[p], (int32_t)i);
+            }
+            __syncthreads();
+            for (uint32_t i = lane; i < o.n_new; i += 64u) {
+                const uint32_t p = (uint32_t)o.parents[i] - base;
+                uint32_t block, rest;
+                if (p < here) o.copies[i] = first_child[p] != (int32_t)i && last_block(g, o, base + p, block, rest);
+                else if (base == 0 && (uint32_t)o.parents[i] >= o.n_old) o.copies[i] = 0;
+            }
+            for (uint32_t x = 0; x < here; x += 64u) {
+                uint32_t block = 0, rest;
+                const bool is = x + lane < here && first_child[x + lane] == 0x7fffffff && last_block(g, o, base + x + lane, block, rest);
+                const uint64_t m = ballot(is);
+                if (is) __hip_atomic_store(&o.freed[n_freed + popc(m & ((1ull << lane) - 1u))], (int32_t)block, __ATOMIC_RELAXED, BAM_AGENT);
+                n_freed += popc(m);
+            }
+            __syncthreads();
+        }
+        wait_stores();
+        uint32_t n_copies = 0;
+        for (uint32_t x = 0; x < o.n_new; x += 64u) {
+            const bool in = x + lane < o.n_new, is = in && o.copies[x + lane];      /* (this lane's own) */
+            const uint64_t m = ballot(is);
+            const uint32_t rank = n_copies + popc(m & ((1ull << lane) - 1u));
+            if (in) o.spare_out[x + lane] = !is ? o.spare[x + lane] : rank < n_freed ? __hip_atomic_load(&o.freed[rank], __ATOMIC_RELAXED, BAM_AGENT) : -1;
+            n_copies += popc(m);
+        }
+        return;
+    }
+    const uint32_t i = (blockIdx.x - 1u) / g.heads, head = (blockIdx.x - 1u) % g.heads;
+    const int32_t parent = o.parents[i];
+    const uint32_t p = (uint32_t)parent;
+    if (p >= o.n_old) {
+        if (head) return;
+        for (uint32_t x = lane; x < o.width; x += 64u) o.table_out[(uint64_t)i * o.width + x] = -1;
+        if (lane == 0) o.lens_out[i] = 0;
+        return;
+    }
+    uint32_t block = 0, rest = 0;
+    bool copy = false;
+    if (last_block(g, o, p, block, rest))
+        for (uint32_t x = 0; x < i && !copy; x += 256u) {
+            bool same = false;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) { const uint32_t y = x + e * 64u + lane; same |= y < i && o.parents[y < i ? y : i] == parent; }
+            copy = ballot(same) != 0;
+        }
+    const uint32_t own = copy ? (uint32_t)o.spare[i] : block;
+    if (head == 0) {
+        const int32_t len = o.lens[p];
+        const uint32_t n = len > 0 ? ((uint32_t)len + g.tokens - 1u) >> g.tokens_log : 0u, last = copy ? n - 1u : 0xffffffffu;
+        for (uint32_t x = lane; x < o.width; x += 64u) o.table_out[(uint64_t)i * o.width + x] = x >= n ? -1 : x == last ? (int32_t)own : o.table[(int64_t)p * o.stride + x];
+        if (lane == 0) o.lens_out[i] = len;
+    }
+    if (!copy || own >= g.n_blocks) return;
+    const uint64_t from = ((uint64_t)block * g.heads + head) * 2u, to = ((uint64_t)own * g.heads + head) * 2u;      /* pages of the cache */
+    const bool e8 = g.scales != nullptr;
+    if (e8)
+        for (uint32_t t = lane; t < rest; t += 64u) {
+            const uint8_t k = g.scales[from * g.tokens + t], v = g.scales[(from + 1u) * g.tokens + t];
+            g.scales[to * g.tokens + t] = k;
+            g.scales[(to + 1u) * g.tokens + t] = v;
+        }
+    /* pieces of a page, of eight tokens' values; those of `rest` tokens */
+    const uint32_t pieces = g.tokens * g.dim / (e8 ? 16u : 8u), eight = e8 ? g.dim / 2u : g.dim, v_pieces = (rest + 7u) / 8u * eight;
+    const u32x4 lost = e8 ? u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu} : F16 ? u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u} : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    for (uint32_t x0 = 0; x0 < pieces; x0 += ORDER_PIECES) {
+        auto wanted = [&](const uint32_t part, const uint32_t x) { return part ? x < v_pieces : x < pieces && place_in(g, x & (g.tokens - 1u)) < rest; };
+        auto load = [&](const uint32_t part, const uint8_t* const page) {
+            const uint8_t* at[8];
+            u32x4 y[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) { const uint32_t x = x0 + e * 64u + lane; at[e] = page + (wanted(part, x) ? (uint64_t)x * 16u : 0u); }
+            load_pieces(at, y);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) room[part * ORDER_PIECES + e * 64u + lane] = y[e];
+        };
+        auto store = [&](const uint32_t part, uint8_t* const page) {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) {
+                const uint32_t x = x0 + e * 64u + lane;
+                if (wanted(part, x)) st16_sys(page + (uint64_t)x * 16u, room[part * ORDER_PIECES + e * 64u + lane]);
+            }
+        };
+        const uint32_t none = visit<false>(g, g.first_page + from, false, false, [&](uint8_t* keys, uint8_t* values) {
+            if (keys) load(0, keys);
+            if (values) load(1, values);
+        });
+        if (__builtin_expect(none != 0, 0))
+            for (uint32_t x = lane; x < ORDER_PIECES; x += 64u) {
+                if (none & 1u) room[x] = lost;
+                if (none & 2u) room[ORDER_PIECES + x] = lost;
+            }
+        /* (behind the first part, the page holds what this call has put there) */
+        visit<true>(g, g.first_page + to, x0 == 0, true, [&](uint8_t* keys, uint8_t* values) {
+            if (keys) store(0, keys);
+            if (values) store(1, values);
+        });
+    }
+}
+
 } // namespace
 
 extern "C" {
@@ -221,6 +365,28 @@ int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream)
     if (kv->e8) kv8_attend(kv, seqs_of(w.seqs), a, p, (hipStream_t)stream);
     else if (kv->f16) launch_attend<1, 0>(kv, seqs_of(w.seqs), a, p, (hipStream_t)stream);
     else launch_attend<0, 0>(kv, seqs_of(w.seqs), a, p, (hipStream_t)stream);
+    hip_err_chk(hipGetLastError());
+    BAM_API_END
+}
+
+int bam_kv_reorder(bam_kv_t* kv, const bam_kv_reorder_t* what, void* stream)
+{
+    if (!kv || !what) return fail(EINVAL, "bam_kv_reorder: null argument");
+    const bam_kv_reorder_t& w = *what;
+    if (!w.n_new) return 0;
+    if (!w.d_parents || !w.d_lens || !w.d_table || !w.d_spare || !w.d_lens_out || !w.d_table_out || !w.d_spare_out || !w.d_work) return fail(EINVAL, "bam_kv_reorder: null argument");
+    if (!w.n_old || w.n_old > 0x7fffffffull || w.n_new > 0x7ffffffeull / kv->g.heads) return fail(EINVAL, "bam_kv_reorder: no old sequences, or more sequences than 31 bits count");
+    if (w.table_width == 0 || w.table_width > 0x7fffffffull || w.table_stride < 0) return fail(EINVAL, "bam_kv_reorder: table of no width, or with its rows in reverse");
+    if (w.table_width > 0x7ffffc00ull >> kv->g.tokens_log) return fail(EINVAL, "bam_kv_reorder: the table has room for more positions than 31 bits count");
+    if (((uintptr_t)w.d_work & 3) || w.work_bytes / 4 < w.n_old + w.n_new) return fail(EINVAL, "bam_kv_reorder: the workspace must be aligned, and have 4 bytes for each sequence");
+    BAM_API_BEGIN
+    kv_order o{};
+    o.parents = w.d_parents; o.lens = w.d_lens; o.table = w.d_table; o.stride = w.table_stride; o.width = (uint32_t)w.table_width; o.n_old = (uint32_t)w.n_old; o.n_new = (uint32_t)w.n_new;
+    o.spare = w.d_spare; o.lens_out = w.d_lens_out; o.table_out = w.d_table_out; o.spare_out = w.d_spare_out;
+    o.freed = (int32_t*)w.d_work; o.copies = o.freed + w.n_old;
+    const dim3 grid(1u + o.n_new * kv->g.heads);
+    if (kv->f16) hipLaunchKernelGGL(k_kv_reorder<1>, grid, dim3(64), 0, (hipStream_t)stream, kv->g, o);
+    else hipLaunchKernelGGL(k_kv_reorder<0>, grid, dim3(64), 0, (hipStream_t)stream, kv->g, o);
     hip_err_chk(hipGetLastError());
     BAM_API_END
 }

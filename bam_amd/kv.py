@@ -18,6 +18,7 @@ _SEQS = "QQPPPqQ"
 _READ = struct.Struct("@" + _SEQS)
 _APPEND = struct.Struct("@" + _SEQS + "Pqq" * 3 + "PPPPPQIIfi")
 _ATTEND = struct.Struct("@" + _SEQS + "PqqPPPQQQIIIf")
+_REORDER = struct.Struct("@QQPPPqQPPPPPQ")
 
 
 def _packed(layout, *fields):
@@ -207,6 +208,26 @@ class KVCache:
                            hq, window, sinks, self.head_dim ** -0.5 if scale is None else scale)
             _chk(self.L.bam_kv_attend(self.h, what, _stream()), "bam_kv_attend")
         return (out, lse) if return_lse else out
+
+    def reorder(self, parents, lens, table, spare):
+        """The sequences that go on behind a choice of beams: new sequence i continues old sequence parents[i] (int32, in any order, as often as it is named).  Returns (lens, table, spare) of the
+        new ones.  Full blocks are shared; a last block that is not full (of one old sequence each) goes to the first of the parent's children, and each other one gets a copy of its tokens in block
+        spare[i], a block of nobody else's (int32, one for each new sequence; -1, or one that the cache does not have: the child's last tokens are not there).  spare comes back with those blocks replaced:
+        in the order of the children, by the last blocks, not full ones, of old sequences that nobody continues, and by -1 where there are no more.  A parent that is not there gives a sequence of no
+        tokens.  In the new table, blocks without tokens are -1."""
+        n = parents.shape[0] if len(parents.shape) == 1 else -1
+        for t, what in ((parents, "parents"), (spare, "spare")):
+            if t.shape != (n,) or t.dtype is not torch.int32 or t.get_device() != self._index or (n > 1 and t.stride()[0] != 1):
+                raise BamError(f"KVCache: {what} must be contiguous int32, one number for each new sequence, on {self.device}")
+        n_old = lens.shape[0] if len(lens.shape) == 1 else -1
+        _, _, _, lens_at, table_at, stride, width = self._seqs(n_old, lens, table, None)
+        new_lens, new_spare = torch.empty(2, n, dtype=torch.int32, device=self.device)
+        new_table, work = torch.empty(n, width, dtype=torch.int32, device=self.device), torch.empty(n_old + n, dtype=torch.int32, device=self.device)
+        if n:
+            what = _REORDER.pack(n_old, n, parents.data_ptr(), lens_at, table_at, stride, width, spare.data_ptr(), new_lens.data_ptr(), new_table.data_ptr(), new_spare.data_ptr(),
+                                 work.data_ptr(), 4 * (n_old + n))
+            _chk(self.L.bam_kv_reorder(self.h, what, _stream()), "bam_kv_reorder")
+        return new_lens, new_table, new_spare
 
     def close(self):
         if self.h:

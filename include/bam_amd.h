@@ -509,6 +509,25 @@ typedef struct bam_kv_attend {
 } bam_kv_attend_t;
 int bam_kv_attend_bytes(bam_kv_t* kv, uint64_t n_seqs, uint64_t max_new, uint32_t q_heads, uint64_t max_len, uint32_t window, uint32_t sinks, uint64_t* bytes);
 int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream);
+/*
+ * Behind a choice of beams, the sequences that go on: new sequence i continues old sequence d_parents[i], in any order and as often as it is named.  d_lens_out[i] is the parent's length and row i
+ * of d_table_out ([n_new][table_width], next to each other) its row of blocks, -1 from the first block on that has no token.  Blocks that are full are shared.  A last block that is not goes to the first of the
+ * parent's children; each other one gets a copy of its tokens in block d_spare[i] (a block of nobody else's; -1, or one that the cache does not have: the child's last tokens are not
+ * there), and d_spare_out[i] is then, in the order of the children, the next of the last blocks, not full ones, of old sequences that nobody continues, -1 where there are no more;
+ * otherwise d_spare[i].  A parent that is not there gives a sequence of no tokens.  A last block that is not full belongs to one old sequence.  Copies whose pages
+ * could not be had read as NaN.  The outputs overlap none of the inputs.  d_work: 4 * (n_old + n_new) bytes for the length of the call.
+ */
+typedef struct bam_kv_reorder {
+    uint64_t n_old, n_new;
+    const int32_t *d_parents, *d_lens, *d_table;
+    int64_t table_stride;
+    uint64_t table_width;
+    const int32_t* d_spare;
+    int32_t *d_lens_out, *d_table_out, *d_spare_out;
+    void* d_work;
+    uint64_t work_bytes;
+} bam_kv_reorder_t;
+int bam_kv_reorder(bam_kv_t* kv, const bam_kv_reorder_t* what, void* stream);
 
 /* ---- beam search's selection ----
  * n_requests of n_beams beams each (up to 1024), with a row of `vocab` logits to a beam, logits_row numbers from row to row (request r's beam i is row r * n_beams + i; type: 0 bfloat16,
