@@ -817,30 +817,44 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     uint32_t at_first = 0, at_end = 0, at_block = 0;          /* of the tile that is on its way */
     uint64_t at_holes = 0;
     const uint32_t k_lane0 = (lane & 7u) * 16u + (lane >> 3) * T * 16u, k_lane1 = (lane & 7u) * 16u + (lane >> 3 ^ 1u) * T * 16u;
-    /* 8 bits: a set of tokens (two units of one block) at a time, a piece of keys and one of values to a lane and load; in registers until the tile before is done with, then
-     * as the 16-bit numbers they stand for to where the pieces of a 16-bit cache would lie */
-    constexpr uint32_t ST = UNITS > 1 ? 16 : 8, SETS = UNITS * 8 / ST, LOADS = ST * DP / 1024;
-    [[maybe_unused]] u32x4 k_raw[E8 ? SETS * LOADS : 1], v_raw[E8 ? SETS * LOADS : 1];
-    [[maybe_unused]] uint32_t k_by[E8 ? SETS * LOADS : 1];
-    [[maybe_unused]] uint64_t v_by[E8 ? SETS * LOADS : 1];
+    /*
+     * 8 bits: a set of tokens (two units of one block, or one) at a time, a piece of keys and one of values to a lane and load.  They go to where a part of the 16-bit numbers that they
+     * stand for will lie, and are taken from there, and the numbers put there, when the tile before is done with (put_tile): each wave in its own units, so nobody else is waited for, and no registers
+     * are held meanwhile (held, they made the queries spill: 500 new tokens after 32500, 610 us).  What of a place depends on the lane does not depend on the load; the rest, and the powers
+     * of two of the values where a load is of one group of eight tokens, are scalars.
+     */
+    constexpr uint32_t ST = UNITS > 1 ? 16 : 8, SETS = UNITS * 8 / ST, LOADS = ST * DP / 1024, CPL = 64 / ST, GROUPS = ST / 8, GL = DP > 64 ? DP / 128 : 1;      /* CPL: pieces of a token's keys to a load; GL: loads to a group of eight tokens' values */
+    constexpr bool ONE = DP > 64;
+    [[maybe_unused]] uint32_t k_by[E8 ? SETS : 1];
+    [[maybe_unused]] uint64_t v_by[E8 ? SETS * GROUPS : 1];
     auto load_tile = [&](const uint32_t buf) {
         if constexpr (E8) {
+            const uint32_t to = lds0 + buf * 2u * HALF + wave * UNITS * DP * 16u;
+            uint32_t l_ = lane;                  /* (worked out anew for each tile, not kept) */
+            asm volatile("" : "+v"(l_));
+            const uint32_t k_place = l_ % ST, k_piece = l_ / ST, v_group = ONE ? 0u : l_ / 32u, v_pair = ONE ? l_ : l_ % 32u;
+            const uint32_t k_off = (k_piece * T + k_place) * 16u, v_off = (v_group * (D / 2u) + v_pair) * 16u;
 #pragma unroll
             for (uint32_t x = 0; x < SETS; x++) {
-                const uint32_t t = t_next + wave * UNITS * 8u + x * ST, b = ((t >> g.tokens_log) - b_first) & 63u, in = t & (T - 1u);
-                const __amdgpu_buffer_rsrc_t k_at = __builtin_amdgcn_make_buffer_rsrc(g.base + ((uint64_t)bcast(k_slot, b) << g.page_log), 0, 1 << g.page_log, 0x00027000);
-                const __amdgpu_buffer_rsrc_t v_at = __builtin_amdgcn_make_buffer_rsrc(g.base + ((uint64_t)bcast(v_slot, b) << g.page_log), 0, 1 << g.page_log, 0x00027000);
-                const uint8_t* const by = g.scales + bcast(need ? page - g.first_page : (uint64_t)0, b) * T;
+                const uint32_t t = t_next + wave * UNITS * 8u + x * ST, b = ((t >> g.tokens_log) - b_first) & 63u, in = t & (T - 1u), unit = to + x * GROUPS * DP * 16u;
+                const uint8_t* const k_at = g.base + ((uint64_t)bcast(k_slot, b) << g.page_log) + in * 16u;
+                const uint8_t* const v_at = g.base + ((uint64_t)bcast(v_slot, b) << g.page_log) + (in >> 3) * (D / 2u) * 16u;
+                const uint64_t by = (uint64_t)(uintptr_t)g.scales + bcast(need ? page - g.first_page : (uint64_t)0, b) * T;
 #pragma unroll
                 for (uint32_t i = 0; i < LOADS; i++) {
-                    const uint32_t p = i * 64u + lane, place = p % ST, c = p / ST, group = p / (DP / 2u), d2 = p % (DP / 2u);
-                    /* (sc1: past the vector L1; what lies past a row's end is not loaded) */
-                    const uint32_t k_off = (c * T + in + place) * 16u, v_off = (((in >> 3) + group) * (D / 2u) + d2) * 16u;
-                    k_raw[x * LOADS + i] = __builtin_amdgcn_raw_buffer_load_b128(k_at, EXACT || c * 16u < D ? k_off : 0u, 0, 16);
-                    v_raw[x * LOADS + i] = __builtin_amdgcn_raw_buffer_load_b128(v_at, EXACT || d2 * 2u < D ? v_off : 0u, 0, 16);
-                    k_by[x * LOADS + i] = by[place_in(g, in + place)];
-                    v_by[x * LOADS + i] = *(const uint64_t*)(by + T + in + group * 8u);
+                    if (EXACT || (i * CPL + k_piece) * 16u < D) to_lds(k_at, k_off + i * CPL * T * 16u, unit + i * 1024u);
+                    if constexpr (ONE) {
+                        if (EXACT || ((i % GL) * 64u + v_pair) * 2u < D) to_lds(v_at, v_off + (i / GL * (D / 2u) + (i % GL) * 64u) * 16u, unit + HALF + i / GL * DP * 16u + (i % GL) * 1024u);
+                    } else {
+#pragma unroll
+                        for (uint32_t n = 0; n < 2; n++) if (v_group == n && (EXACT || v_pair * 2u < D)) to_lds(v_at, v_off, unit + HALF + n * (DP * 16u - 512u));
+                    }
                 }
+                k_by[x] = ((const uint8_t*)by)[place_in(g, in + k_place)];
+                if constexpr (ONE) {
+#pragma unroll
+                    for (uint32_t n = 0; n < GROUPS; n++) v_by[x * GROUPS + n] = *(const __attribute__((address_space(4))) uint64_t*)(by + T + in + n * 8u);
+                } else v_by[x * GROUPS] = *(const uint64_t*)(by + T + in + v_group * 8u);
             }
         } else {
             const uint32_t to = lds0 + buf * 2u * HALF;
@@ -862,31 +876,44 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
         t_next += KT;
     };
     [[maybe_unused]] auto put_tile = [&](const uint32_t buf) {
-        uint8_t* const to = (uint8_t*)lds + buf * 2u * HALF;
+        uint8_t* const to = (uint8_t*)lds + buf * 2u * HALF + wave * UNITS * DP * 16u;
+        fence_meta();                            /* the wave's loads are in LDS */
+        uint32_t l_ = lane;
+        asm volatile("" : "+v"(l_));
+        const uint32_t k_place = l_ % ST, k_piece = l_ / ST, v_group = ONE ? 0u : l_ / 32u, v_pair = ONE ? l_ : l_ % 32u;
 #pragma unroll
-        for (uint32_t x = 0; x < SETS; x++)
+        for (uint32_t x = 0; x < SETS; x++) {
+            uint8_t* const unit = to + x * GROUPS * DP * 16u;
+            u32x4 k_raw[LOADS], v_raw[LOADS];
 #pragma unroll
             for (uint32_t i = 0; i < LOADS; i++) {
-                const uint32_t p = i * 64u + lane, place = p % ST, c = p / ST, group = p / (DP / 2u), d2 = p % (DP / 2u), n = x * LOADS + i;
-                const uint32_t unit = wave * UNITS + x * (ST / 8u), odd = (unit + (place >> 3)) & 1u;
-                const float by = scale_of(k_by[n]);
-                uint8_t* const k_to = to + (unit + (place >> 3)) * DP * 16u + (place & 7u) * 16u + c * 256u;
-                if (EXACT || c * 16u < D) {
-                    *(u32x4*)(k_to + odd * 128u) = keys_of<F16>(k_raw[n][0], k_raw[n][1], by);
-                    *(u32x4*)(k_to + (odd ^ 1u) * 128u) = keys_of<F16>(k_raw[n][2], k_raw[n][3], by);
+                k_raw[i] = *(const u32x4*)(unit + i * 1024u + l_ * 16u);
+                v_raw[i] = *(const u32x4*)(unit + HALF + (ONE ? i / GL * DP * 16u + (i % GL) * 1024u + l_ * 16u : v_group * DP * 16u + v_pair * 16u));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      /* all lanes have theirs before one writes */
+            const uint32_t odd = (wave * UNITS + (k_place >> 3)) & 1u;
+            const float by = scale_of(k_by[x]);
+            uint8_t* const k_to = unit + (k_place >> 3) * DP * 16u + (k_place & 7u) * 16u + k_piece * 256u;
+            uint8_t* const v_to = unit + HALF + v_group * DP * 16u + v_pair * 32u;
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; i++) {
+                if (EXACT || (i * CPL + k_piece) * 16u < D) {
+                    *(u32x4*)(k_to + i * CPL * 256u + odd * 128u) = keys_of<F16>(k_raw[i][0], k_raw[i][1], by);
+                    *(u32x4*)(k_to + i * CPL * 256u + (odd ^ 1u) * 128u) = keys_of<F16>(k_raw[i][2], k_raw[i][3], by);
                 }
                 float each[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) each[e] = scale_of((uint32_t)(v_by[n] >> (8 * e)) & 0xffu);
+                for (int e = 0; e < 8; e++) each[e] = scale_of((uint32_t)(v_by[x * GROUPS + (ONE ? i / GL : 0)] >> (8 * e)) & 0xffu);
                 u32x4 a0, a1;
-                values_of<F16>(v_raw[n], each, a0, a1);
+                values_of<F16>(v_raw[i], each, a0, a1);
                 /* neighbouring numbers exchanged in every other sixteen: sixteen lanes that write every other piece meet all banks */
-                uint8_t* const v_to = to + HALF + ((unit + group) * DP + d2 * 2u) * 16u;
-                if (EXACT || d2 * 2u < D) {
-                    *(u32x4*)(v_to + (d2 >> 3 & 1u) * 16u) = a0;
-                    *(u32x4*)(v_to + ((d2 >> 3 & 1u) ^ 1u) * 16u) = a1;
+                uint8_t* const at = v_to + (i / GL * DP + i % GL * 128u) * 16u;
+                if (EXACT || ((i % GL) * 64u + v_pair) * 2u < D) {
+                    *(u32x4*)(at + (v_pair >> 3 & 1u) * 16u) = a0;
+                    *(u32x4*)(at + ((v_pair >> 3 & 1u) ^ 1u) * 16u) = a1;
                 }
             }
+        }
     };
     next_blocks();
     bool more = there;
@@ -923,10 +950,8 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             }
             if (ballot(odd)) ok = false;
         }
-        if (idle || (int32_t)t0 > last_pos) {
-            if constexpr (E8) if (more) put_tile(buf ^ 1u);
-            continue;
-        }
+        do {
+        if (idle || (int32_t)t0 > last_pos) break;
         /*
          * The operands from LDS are read eight ahead of the products that take them, and the order is held (sched_barrier): left to itself the compiler reads each right before
          * its product and waits for it, a hundred cycles for every 32 of the matrix unit.
@@ -1007,6 +1032,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        } while (false);
         if constexpr (E8) if (more) put_tile(buf ^ 1u);
     }
     fence_meta();
