@@ -47,7 +47,7 @@ def beam_select(logits, scores, width=None):
         if len(_bytes) > 4096:
             _bytes.clear()
         need = _bytes[key] = b.value
-    if torch.cuda.current_device() != index:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return _select(L, logits, scores, row, score_row, beams, width, kind, need)
     return _select(L, logits, scores, row, score_row, beams, width, kind, need)
@@ -55,12 +55,11 @@ def beam_select(logits, scores, width=None):
 
 def _select(L, logits, scores, row, score_row, beams, width, kind, need):
     device = logits.device
-    sums = torch.empty(beams[0], width, dtype=torch.float32, device=device)
-    # from torch's allocator, which keeps the workspace for this stream, or for the graph that is being captured
-    chosen, work = torch.empty(2, beams[0], width, dtype=torch.int32, device=device), torch.empty(need, dtype=torch.uint8, device=device)
+    # (one tensor and its parts take less than three.)  The workspace is from torch's allocator, which keeps it for this stream, or for the graph that is being captured
+    out, work = torch.empty((3, beams[0], width), dtype=torch.int32, device=device), torch.empty(need, dtype=torch.uint8, device=device)
     if beams[0]:
-        at = chosen.data_ptr()
-        what = _SELECT.pack(beams[0], beams[1], logits.shape[1], logits.data_ptr(), row, scores.data_ptr(), score_row, sums.data_ptr(), at, at + 4 * beams[0] * width,
-                            work.data_ptr(), need, width, kind)
+        at, each = out.data_ptr(), 4 * beams[0] * width
+        what = _SELECT.pack(beams[0], beams[1], logits.shape[1], logits.data_ptr(), row, scores.data_ptr(), score_row, at, at + each, at + 2 * each, work.data_ptr(), need, width, kind)
         _chk(L.bam_beam_select(what, c_vp(_raw_stream(device.index))), "bam_beam_select")
-    return sums, chosen[0], chosen[1]
+    sums, chosen, tokens = out.unbind(0)
+    return sums.view(torch.float32), chosen, tokens

@@ -28,9 +28,9 @@ kv_plan plan_of(const bam_kv_t* kv, const uint64_t n_seqs, const uint64_t max_ne
      * Workgroups: as many as keep the memory busy, and no more, since each has its latencies before its first token and behind its last, and its split is written and
      * read again.  Few rows, four waves: one to a compute unit where a step of 32 tokens is 16 KiB, two where it is 8.  32 heads on 8 of 128 numbers, one token each, with
      * a workgroup for 512 / 256 of the device: 8 sequences of up to 8000 tokens 51 / 45 us, one of 262121 179 / 167; heads of 64 numbers, 32 sequences of
-     * up to 4000, 1024 / 512 / 256: 30 / 28 / 34.
+     * up to 4000, 1024 / 512 / 256: 30 / 28 / 34.  In 8 bits, 512 / 256: 8 of 8000 33 / 37, 24 of 9000 87 / 116, one of 262121 97 / 111; heads of 256 numbers, 8 of 8000, 63 / 54.
      */
-    uint64_t splits = (kv->g.dim <= 64 ? 512 : 256) / p.items;
+    uint64_t splits = (kv->g.dim <= 64 || (kv->e8 && kv->g.dim <= 128) ? 512 : 256) / p.items;
     /*
      * Tiles of rows: as many workgroups as the LDS of the compute units has room for, but no splits where there is one to each already.  The same heads, with
      * splits for 1024 / 512 / 256 workgroups whatever there is: 1000 new tokens (256 tiles) 41 / 40 / 32 us, 500 after 32500 (128 tiles) 325 / 309 / 377;

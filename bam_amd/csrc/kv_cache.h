@@ -54,27 +54,40 @@ struct kv_rows {
     float eps;
     uint32_t window, piece;             /* rows that a wave looks for beginnings of runs among, and the most rows it takes at a time */
     uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes */
+    uint32_t by_head;                   /* waves in the order of the heads, each one's windows side by side */
 };
 
 namespace {
 
-// sequence of row i
-__device__ __forceinline__ uint32_t seq_of(const kv_seqs& s, const uint32_t i)
+// sequence of row i, which is one of [lo, hi): the last that starts at or before it
+__device__ __forceinline__ uint32_t seq_of(const kv_seqs& s, const uint32_t i, uint32_t lo, uint32_t hi)
 {
     if (!s.starts) return i;
-    uint32_t lo = 0, hi = s.n;          /* the last sequence that starts at or before row i */
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
         if (s.starts[mid] <= (int32_t)i) lo = mid; else hi = mid;
     }
     return lo;
 }
+/* the same for a row that is the whole wave's: 64 places are looked at at a time (a look takes a microsecond of what a small call takes; 512 sequences are two looks and not nine) */
+__device__ __forceinline__ uint32_t seq_of_wave(const kv_seqs& s, const uint32_t i)
+{
+    if (!s.starts) return i;
+    uint32_t lo = 0, hi = s.n;
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 63u) / 64u, at = lo + step * bam::lane();
+        const uint64_t m = bam::ballot(at < hi && s.starts[at < hi ? at : lo] <= (int32_t)i) | 1ull;
+        lo += step * (63u - (uint32_t)__builtin_clzll(m));
+        hi = hi - lo < step ? hi : lo + step;
+    }
+    return lo;
+}
 // a row's place: sequence, position, rows of its sequence from it on (those that there are: starts may say more than `rows`), position of its sequence's first new
 // row; false where the row has none (no such sequence, before the first position, past the table)
 struct kv_place { uint32_t seq, pos, rest, first; };
-__device__ __forceinline__ bool place_of(const kv_seqs& s, const kv_geom& g, const uint32_t i, kv_place& p)
+__device__ __forceinline__ bool place_of(const kv_seqs& s, const kv_geom& g, const uint32_t i, const uint32_t lo, const uint32_t hi, kv_place& p)
 {
-    p.seq = seq_of(s, i);
+    p.seq = seq_of(s, i, lo, hi);
     if (p.seq >= s.n) return false;
     const int32_t end = s.starts ? s.starts[p.seq + 1] : (int32_t)i + 1;
     int32_t begin = s.starts ? s.starts[p.seq] : (int32_t)i;
@@ -352,7 +365,8 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
         const uint32_t per = (io.q_heads + io.q_heads_each - 1) / io.q_heads_each, i = wave / per, h0 = wave % per * io.q_heads_each;
         const uint32_t h1 = h0 + io.q_heads_each < io.q_heads ? h0 + io.q_heads_each : io.q_heads;
         kv_place p{0, 0, 0, 0};
-        const bool known = place_of(s, g, i, p);
+        const uint32_t seq = seq_of_wave(s, i);
+        const bool known = place_of(s, g, i, seq, seq + 1u, p);
         const kv_turn t = turn_of(io, piece, known ? p.pos : 0xffffffffu);
         u32x4 w{0, 0, 0, 0};
         if (io.q_norm) w = load_piece<true>(io.q_norm + col);
@@ -375,12 +389,24 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
         }
         return;
     }
-    const uint32_t n = wave - (WRITE ? io.q_waves : 0u), head = n % g.heads;
-    const uint64_t first_row = (uint64_t)(n / g.heads) * io.window;
+    const uint32_t n = wave - (WRITE ? io.q_waves : 0u), windows = (s.rows + io.window - 1u) / io.window, head = io.by_head ? n / windows : n % g.heads;
+    const uint64_t first_row = (uint64_t)(io.by_head ? n % windows : n / g.heads) * io.window;
+    if (head >= g.heads) return;
     if (first_row >= s.rows) return;
     kv_place p{0, 0, 0, 0};
     const uint32_t mine = (uint32_t)first_row + lane;
-    const bool has = lane < io.window && mine < s.rows && place_of(s, g, mine, p);
+    /* the sequence of the first row, and from the beginnings of the 64 behind it, loaded at once, those of the others */
+    const uint32_t first_seq = seq_of_wave(s, (uint32_t)first_row);
+    uint32_t lo = first_seq, hi = first_seq + 1u;
+    if (s.starts && io.window > 1u) {
+        const int32_t begin = first_seq + 1u + lane < s.n ? s.starts[first_seq + 1u + lane] : 0x7fffffff;
+        uint32_t k = 0;
+#pragma unroll
+        for (uint32_t x = 32; x; x >>= 1) k += __shfl(begin, (int)(k + x - 1u)) <= (int32_t)mine ? x : 0u;
+        lo += k;
+        hi = k == 63u ? s.n : lo + 1u;
+    }
+    const bool has = lane < io.window && mine < s.rows && place_of(s, g, mine, lo, hi, p);
     const bool begins = has && ((p.pos & (g.tokens - 1u)) == 0 || p.pos == p.first || (s.starts && s.starts[p.seq] == (int32_t)mine));
     if constexpr (!WRITE) {
         /* rows without a place come out as zeros */
@@ -390,10 +416,13 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                 ((uint16_t*)io.v)[(int64_t)(first_row + first_lane(m)) * io.v_row + (int64_t)head * io.v_head + d] = 0;
             }
     }
+    uint64_t its_page = 0;                       /* where a lane's run begins */
+    const bool is_there = begins && page_of_block(g, s, p.seq, p.pos >> g.tokens_log, head, its_page);
+    const uint64_t theres = ballot(is_there);
     for (uint64_t m = ballot(begins); m; m &= m - 1) {
-        const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), seq = bcast(p.seq, j), row = (uint32_t)first_row + j;
-        uint64_t page = 0;
-        const bool there = page_of_block(g, s, seq, pos >> g.tokens_log, head, page);
+        const uint32_t j = first_lane(m), pos = bcast(p.pos, j), rest = bcast(p.rest, j), row = (uint32_t)first_row + j;
+        const uint64_t page = bcast(its_page, j);
+        const bool there = (theres >> j) & 1u;
         uint8_t* const powers = g.scales + (page - g.first_page) * g.tokens;      /* of the block's keys, and of its values behind them (only used where the block is there) */
         const uint32_t run_first = pos & (g.tokens - 1u), block_first = pos - run_first, run_end = rest < g.tokens - run_first ? run_first + rest : g.tokens;
         const uint32_t groups = io.piece / 8u, pairs = g.dim / 2u;
@@ -567,7 +596,18 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
     io.q_heads_each = io.q && (uint64_t)s.rows * io.q_heads > 16384 ? 8 * rpw : rpw;
     io.q_waves = io.q ? (uint32_t)((io.q_heads + io.q_heads_each - 1) / io.q_heads_each * s.rows) : 0;
     io.piece = kv->g.tokens < 16 ? 8 : 16;
-    io.window = s.starts && s.rows / s.n >= 8 ? (kv->g.tokens < 64 ? kv->g.tokens : 64) : 1;
+    /*
+     * A wave goes through the runs of its window one after the other: no larger than leaves a wave to each place of the device.  Rows of the last blocks of 512 sequences, 1 to 31 tokens each and eight
+     * heads, windows of 32 / 16 / 8 / 4 rows: 52 / 51 / 44 / 50 us; 13 rows of four sequences, 32 / 1: 16 / 8.5.
+     */
+    const uint32_t rows_each = s.starts ? s.rows / s.n : 0;
+    io.window = rows_each >= 8 ? (kv->g.tokens < 64 ? kv->g.tokens : 64) : rows_each >= 4 ? 4 : rows_each >= 2 ? 2 : 1;
+    while (io.window > 1 && (uint64_t)s.rows / io.window * kv->g.heads < 4096) io.window /= 2;
+    /*
+     * Windows that are smaller than runs: by heads.  In the order of the rows, the heads of those in which a run begins would lie side by side in a few workgroups, and those on the same compute
+     * units.  512 sequences of 4 new rows, eight heads, a wave to a row: in the order of the rows 41 us, by heads 19; (four rows to a wave 12.5); 100 of 16, two rows to a wave, 27 and 14.
+     */
+    io.by_head = io.window < (rows_each < kv->g.tokens ? rows_each : kv->g.tokens);
     const uint64_t waves = (uint64_t)io.q_waves + (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads;
     if (waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
     const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
