@@ -243,8 +243,8 @@ template <int F16> __device__ __forceinline__ void values_of(const u32x4 x, cons
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t w = x[i], y = from8<F16, false>(w, by[2 * i]), z = from8<F16, true>(w, by[2 * i + 1]);
-        a[i] = (y & 0xffffu) | (z << 16);
-        b[i] = (y >> 16) | (z & 0xffff0000u);
+        a[i] = __builtin_amdgcn_perm(z, y, 0x05040100u);         /* the low halves, and the high ones: an instruction each, four with masks */
+        b[i] = __builtin_amdgcn_perm(z, y, 0x07060302u);
     }
 }
 
@@ -454,12 +454,15 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
             }
             const bool hole = (holes >> vb) & 1u;
             bool slow = false;
-            [[maybe_unused]] uint32_t any8 = 0xffu;
             if (!whole) {
                 /* values of tokens that no row sees may be anything: none of it may meet the zeros of P */
-                const uint32_t any = any8 = hole ? 0u : seen_of_eight((int32_t)vt, sp.last_pos, low_of(a, sp.first_pos), (int32_t)a.sinks);
+                const uint32_t any = hole ? 0u : seen_of_eight((int32_t)vt, sp.last_pos, low_of(a, sp.first_pos), (int32_t)a.sinks);
 #pragma unroll
                 for (int i = h * VP; i < (h + 1) * VP; i++) vv[i] = only(vv[i], any);      /* (in 8 bits: the numbers of a token are 16 bits here too) */
+                if constexpr (E8) {                      /* and powers of two that may be anything are 2^0 */
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v_by[h] = (any >> e) & 1u ? v_by[h] : (v_by[h] & ~(0xffull << (8 * e))) | 127ull << (8 * e);
+                }
                 if (sp.first_pos != sp.last_pos) {
                     bool odd = false;
 #pragma unroll
@@ -470,12 +473,12 @@ __device__ __forceinline__ bool kv_steps(const kv_geom& g, const kv_seqs& s, con
                     if (!HELD && slow) return false;             /* row by row, in the launch that holds its pages: the sums of this one stay where they are */
                 }
             }
-            /* the values as operands: in 8 bits with each token's power of two, or with one where no row sees it (what stands there may be anything) */
+            /* the values as operands: in 8 bits with each token's power of two */
             u32x4 w[DP / 16];
             if constexpr (E8) {
                 float by[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) by[e] = (any8 >> e) & 1u ? scale_of((uint32_t)(v_by[h] >> (8 * e)) & 0xffu) : 1.0f;
+                for (int e = 0; e < 8; e++) by[e] = scale_of((uint32_t)(v_by[h] >> (8 * e)) & 0xffu);
 #pragma unroll
                 for (int i = 0; i < VP; i++) values_of<F16>(vv[h * VP + i], by, w[2 * i], w[2 * i + 1]);
             } else {
