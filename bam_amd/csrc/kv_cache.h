@@ -53,7 +53,8 @@ struct kv_rows {
     uint32_t positions, q_heads, rot, pairs, aligned;      /* aligned: q, k, v in whole pieces of 16 bytes */
     float eps;
     uint32_t window, piece;             /* rows that a wave looks for beginnings of runs among, and the most rows it takes at a time */
-    uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes */
+    uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes; waves that do */
+    uint32_t kv_waves;                  /* the others, which come first: the work of each takes longer */
     uint32_t by_head;                   /* waves in the order of the heads, each one's windows side by side */
 };
 
@@ -361,8 +362,9 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
     const uint32_t sub = lane / LPR, piece = lane % LPR;
     const bool in_row = piece * 8u < g.dim;
     const uint32_t col = in_row ? piece * 8u : 0u;           /* lanes past the row's end load its beginning, and count as zeros */
-    if (WRITE && wave < io.q_waves) {
-        const uint32_t per = (io.q_heads + io.q_heads_each - 1) / io.q_heads_each, i = wave / per, h0 = wave % per * io.q_heads_each;
+    if (WRITE && wave >= io.kv_waves) {
+        if (wave - io.kv_waves >= io.q_waves) return;
+        const uint32_t per = (io.q_heads + io.q_heads_each - 1) / io.q_heads_each, i = (wave - io.kv_waves) / per, h0 = (wave - io.kv_waves) % per * io.q_heads_each;
         const uint32_t h1 = h0 + io.q_heads_each < io.q_heads ? h0 + io.q_heads_each : io.q_heads;
         kv_place p{0, 0, 0, 0};
         const uint32_t seq = seq_of_wave(s, i);
@@ -389,7 +391,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
         }
         return;
     }
-    const uint32_t n = wave - (WRITE ? io.q_waves : 0u), windows = (s.rows + io.window - 1u) / io.window, head = io.by_head ? n / windows : n % g.heads;
+    const uint32_t n = wave, windows = (s.rows + io.window - 1u) / io.window, head = io.by_head ? n / windows : n % g.heads;
     const uint64_t first_row = (uint64_t)(io.by_head ? n % windows : n / g.heads) * io.window;
     if (head >= g.heads) return;
     if (first_row >= s.rows) return;
@@ -608,7 +610,8 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
      * units.  512 sequences of 4 new rows, eight heads, a wave to a row: in the order of the rows 41 us, by heads 19; (four rows to a wave 12.5); 100 of 16, two rows to a wave, 27 and 14.
      */
     io.by_head = io.window < (rows_each < kv->g.tokens ? rows_each : kv->g.tokens);
-    const uint64_t waves = (uint64_t)io.q_waves + (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads;
+    const uint64_t kv_waves = (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads, waves = io.q_waves + kv_waves;
+    io.kv_waves = (uint32_t)kv_waves;
     if (waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
     const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
 #define KV_ROWS(LPR, AL) \
