@@ -54,7 +54,7 @@ struct kv_rows {
     float eps;
     uint32_t window, piece;             /* rows that a wave looks for beginnings of runs among, and the most rows it takes at a time */
     uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes; waves that do */
-    uint32_t kv_waves;                  /* the others, which come first: the work of each takes longer */
+    uint32_t kv_blocks, among;          /* workgroups for keys and values, which are spread among so many from the first on */
     uint32_t by_head;                   /* waves in the order of the heads, each one's windows side by side */
 };
 
@@ -350,21 +350,30 @@ template <int LPR, int F16> __device__ __forceinline__ uint32_t power_of_row(con
  * A wave takes some heads of queries of one row, or one head's keys and values of the runs of rows that begin among io.window rows: a run is the new rows of
  * a sequence in one block, gone through in pieces of up to io.piece tokens (eight or sixteen that begin at a multiple of that).  A page's rows all belong to one
  * wave: a page that holds new rows only is not read, and one that a second wave found gone again would come without the rows of the first.
- *   Bound by memory where there are many rows: 19 459 rows of 32 heads on 8 of 128 numbers, normed and turned, 480 MB in 124 us (3.9 TB/s), 160 MB out again in 43; a wave for
- * each four rows took 288 and 112 (each looked its sequence up for 1 KiB).  Few rows: the chain of looks, table, references, rows, 6 to 7 us.
+ *   Bound by memory where there are many rows: 19 459 rows of 32 heads on 8 of 128 numbers, normed and turned, 480 MB in 118 us (4.1 TB/s), 160 MB out again in 55, in 8 bits
+ * 440 MB in 123 and 120 MB in 43; a wave for each four rows took 288 and 112 (each looked its sequence up for 1 KiB).  Few rows: the chain of looks, table, references, rows, 6 to 7 us.
  */
 template <int LPR, int F16, int E8, bool WRITE, bool ALIGNED>
 __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
 {
     using namespace bam;
     constexpr uint32_t RPW = 64 / LPR, TRIPS = 16 / RPW, DT = LPR / 8;           /* trips of a piece's keys; of its values: a trip is 64 times two numbers of eight tokens */
-    const uint32_t wave = first(blockIdx.x * 4u + threadIdx.x / 64u), lane = bam::lane();
+    const uint32_t lane = bam::lane();
+    uint32_t its_block = blockIdx.x;
+    bool queries = false;
+    if constexpr (WRITE) {
+        auto in_front = [&](const uint32_t b) { return b < io.among ? (uint32_t)((uint64_t)b * io.kv_blocks / io.among) : io.kv_blocks; };
+        const uint32_t before = in_front(blockIdx.x), behind = in_front(blockIdx.x + 1u);
+        queries = before == behind;
+        its_block = queries ? blockIdx.x - before : before;
+    }
+    const uint32_t wave = first(its_block * 4u + threadIdx.x / 64u);
     const uint32_t sub = lane / LPR, piece = lane % LPR;
     const bool in_row = piece * 8u < g.dim;
     const uint32_t col = in_row ? piece * 8u : 0u;           /* lanes past the row's end load its beginning, and count as zeros */
-    if (WRITE && wave >= io.kv_waves) {
-        if (wave - io.kv_waves >= io.q_waves) return;
-        const uint32_t per = (io.q_heads + io.q_heads_each - 1) / io.q_heads_each, i = (wave - io.kv_waves) / per, h0 = (wave - io.kv_waves) % per * io.q_heads_each;
+    if (WRITE && queries) {
+        if (wave >= io.q_waves) return;
+        const uint32_t per = (io.q_heads + io.q_heads_each - 1) / io.q_heads_each, i = wave / per, h0 = wave % per * io.q_heads_each;
         const uint32_t h1 = h0 + io.q_heads_each < io.q_heads ? h0 + io.q_heads_each : io.q_heads;
         kv_place p{0, 0, 0, 0};
         const uint32_t seq = seq_of_wave(s, i);
@@ -610,10 +619,18 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
      * units.  512 sequences of 4 new rows, eight heads, a wave to a row: in the order of the rows 41 us, by heads 19; (four rows to a wave 12.5); 100 of 16, two rows to a wave, 27 and 14.
      */
     io.by_head = io.window < (rows_each < kv->g.tokens ? rows_each : kv->g.tokens);
-    const uint64_t kv_waves = (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads, waves = io.q_waves + kv_waves;
-    io.kv_waves = (uint32_t)kv_waves;
-    if (waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
-    const dim3 grid((uint32_t)((waves + 3) / 4)), block(256);
+    const uint64_t kv_waves = (uint64_t)((s.rows + io.window - 1) / io.window) * kv->g.heads;
+    if (io.q_waves + kv_waves > 0x7fffffffull) throw std::runtime_error("more rows of heads than one launch takes");
+    io.kv_blocks = (uint32_t)((kv_waves + 3) / 4);
+    const dim3 grid(io.kv_blocks + (io.q_waves + 3) / 4), block(256);
+    /*
+     * Few rows: keys and values first, whose waves work longest.  Many: their workgroups among the queries', not behind them, where they would be left to finish alone, but what is written last is what
+     * the caches have for who reads it next.  19 459 rows of 32 heads on 8 of 128 numbers into the cache and out again, keys and values first / over three quarters of the launch / evenly / last: in 8 bits
+     * 119 + 52 / 123 + 43 / 134 + 40 / 134 + 37 us, in 16 bits 119 + 65 / 117 + 61 / 118 + 55 / 130 + 47; one row in 8 bits 8.4 + 5 / - / 9.1 + 5.
+     */
+    io.among = io.kv_blocks;
+    const uint32_t most = E8 ? grid.x / 4 * 3 : grid.x;
+    if (grid.x > 1024 && io.among < most) io.among = most;
 #define KV_ROWS(LPR, AL) \
     if (kv->f16) hipLaunchKernelGGL((k_kv_rows<LPR, 1, E8, WRITE, AL>), grid, block, 0, st, kv->g, s, io); \
     else hipLaunchKernelGGL((k_kv_rows<LPR, 0, E8, WRITE, AL>), grid, block, 0, st, kv->g, s, io)
