@@ -146,6 +146,8 @@ __device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, const uint32_t 
  * (bound_of).  The loads that have such numbers are put in LDS, and looked at again by as many threads; what is found goes into `room`.  For the chunks behind the first the same bound holds.  Where
  * the candidates do not fit (numbers in an order that gives a few threads all the large ones), those that did give a higher bound.  The next chunk is on its way meanwhile.
  * Exponentials are of differences to the thread's largest so far (differences first: the type's lowest value times log2 e is out of range); LOADS * 4 or 8 of them are added up in 32 bits, the rest in 64.
+ *   Many rows: bound by memory, 768 of 150001 in float32 94 us (4.9 TB/s, what a copy reaches; 104 with loads that are kept in the caches); 128 of 128000 in bfloat16 14 us, two thirds of it the launch and the
+ * latencies of the first loads, the bound and the last list.  Few: latencies, 5.6 us for 4 rows of 32000.
  */
 template <int TYPE, uint32_t LOADS>
 __global__ __launch_bounds__(BEAM_THREADS, 4) void k_beam_rows(const beam_args a)
@@ -340,7 +342,8 @@ __device__ __forceinline__ double log_of(const double x)
  * A request: the beams' logarithms of sums of exponentials, and the best of what the pieces left, by a bound as in k_beam_rows.  Sums are compared in 64 bits:
  * the beams' own sums are rounded to 32, what is added to them is not, and of two beams that differ in their last place the right one is taken.
  *   Up to eight candidates to a thread are in registers before the sums are known, and the first bound is of the upper halves of the sums, with candidate q of piece l in group q * (pieces | 1) + l: pieces'
- * candidates come in order, so neighbouring ones in one group would leave most groups without a good one.
+ * candidates come in order, so neighbouring ones in one group would leave most groups without a good one (16 beams, 2048 candidates, 32 wanted: 55 us for 14).
+ *   Latencies: 4.4 to 5 us for up to 1024 candidates, of which an empty kernel behind another takes 4; 6.9 for 2560 of 48 requests.
  */
 template <uint32_t THREADS>
 __global__ __launch_bounds__(THREADS) void k_beam_join(const beam_args a)

@@ -986,7 +986,8 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) void k_kv_attend_tiles(c
     /*
      * 8 bits: a set of tokens (two units of one block, or one) at a time, a piece of keys and one of values to a lane and load.  They go to where a part of the 16-bit numbers that they
      * stand for will lie, and are taken from there, and the numbers put there, when the tile before is done with (put_tile): each wave in its own units, so nobody else is waited for, and no registers
-     * are held meanwhile (held, they made the queries spill: 500 new tokens after 32500, 610 us).  What of a place depends on the lane does not depend on the load; the rest, and the powers
+     * are held meanwhile (held, they made the queries spill: 500 new tokens after 32500, 610 us, and 310 so, where a 16-bit cache
+     * takes 290).  What of a place depends on the lane does not depend on the load; the rest, and the powers
      * of two of the values where a load is of one group of eight tokens, are scalars.
      */
     constexpr uint32_t ST = UNITS > 1 ? 16 : 8, SETS = UNITS * 8 / ST, LOADS = ST * DP / 1024, CPL = 64 / ST, GROUPS = ST / 8, GL = DP > 64 ? DP / 128 : 1;      /* CPL: pieces of a token's keys to a load; GL: loads to a group of eight tokens' values */
