@@ -36,12 +36,12 @@ def beam_select(logits, scores, width=None):
         raise BamError("beam_select: there are no gradients: detach what requires them, or call under torch.no_grad()")
     if width is None:
         width = beams[1]
+    if type(width) is not int or not 1 <= width <= 256:
+        raise BamError("beam_select: width must be a number from 1 to 256")
     key = (*beams, shape[1], width, kind)
     need = _bytes.get(key)
     L = _lib.load()
     if need is None:
-        if not isinstance(width, int) or not 1 <= width <= 256:
-            raise BamError("beam_select: width must be a number from 1 to 256")
         b = c_u64(0)
         _chk(L.bam_beam_select_bytes(*key, ctypes.byref(b)), "bam_beam_select_bytes")
         if len(_bytes) > 4096:

@@ -12,6 +12,7 @@ from . import _lib
 from .host import Array, BamError, PageCache, Range, _chk, _stream, c_u64, c_vp
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 # the structs of include/bam_amd.h, packed at once: a call takes 3 us less than with a ctypes argument for each field
 _SEQS = "QQPPPqQ"
@@ -79,6 +80,12 @@ class KVCache:
         self._bytes = {}
 
     # ---- checks: each property of a tensor is asked for once, they are what a small call takes on the host ----
+
+    def _queue(self):
+        """the current stream: kernels go to the device that is current, which has to be the one that the cache's memory is on"""
+        if _current() != self._index:
+            raise BamError(f"KVCache: the current device must be {self.device}: call under torch.cuda.device")
+        return _stream()
 
     def _no_grad(self, t, what):
         if t.requires_grad and torch.is_grad_enabled():
@@ -165,7 +172,7 @@ class KVCache:
             raise BamError("KVCache: cos and sin go together")
         what = _packed(_APPEND, *seqs, k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, *q_args, self._weights(q_norm, "q_norm"), self._weights(k_norm, "k_norm"),
                        *angles, q_heads, rot, eps, rotary == "pairs")
-        _chk(self.L.bam_kv_append(self.h, what, _stream()), "bam_kv_append")
+        _chk(self.L.bam_kv_append(self.h, what, self._queue()), "bam_kv_append")
         return out if q is not None else None
 
     def read(self, n_rows, lens, table, starts=None):
@@ -175,7 +182,7 @@ class KVCache:
         seqs = self._seqs(n_rows, lens, table, starts)
         k = torch.empty(n_rows, self.n_heads, self.head_dim, dtype=self.dtype, device=self.device)
         v = torch.empty_like(k)
-        _chk(self.L.bam_kv_read(self.h, _packed(_READ, *seqs), k.data_ptr(), v.data_ptr(), _stream()), "bam_kv_read")
+        _chk(self.L.bam_kv_read(self.h, _packed(_READ, *seqs), k.data_ptr(), v.data_ptr(), self._queue()), "bam_kv_read")
         return k, v
 
     def attend(self, q, lens, table, starts=None, max_new=None, max_len=None, scale=None, window=0, sinks=0, out=None, return_lse=False):
@@ -206,7 +213,7 @@ class KVCache:
             work = torch.empty(need, dtype=torch.uint8, device=self.device)
             what = _packed(_ATTEND, *seqs, q.data_ptr(), row, head, out.data_ptr(), 0 if lse is None else lse.data_ptr(), work.data_ptr(), need, max_new, max_len,
                            hq, window, sinks, self.head_dim ** -0.5 if scale is None else scale)
-            _chk(self.L.bam_kv_attend(self.h, what, _stream()), "bam_kv_attend")
+            _chk(self.L.bam_kv_attend(self.h, what, self._queue()), "bam_kv_attend")
         return (out, lse) if return_lse else out
 
     def reorder(self, parents, lens, table, spare):
@@ -226,7 +233,7 @@ class KVCache:
         if n:
             what = _REORDER.pack(n_old, n, parents.data_ptr(), lens_at, table_at, stride, width, spare.data_ptr(), new_lens.data_ptr(), new_table.data_ptr(), new_spare.data_ptr(),
                                  work.data_ptr(), 4 * (n_old + n))
-            _chk(self.L.bam_kv_reorder(self.h, what, _stream()), "bam_kv_reorder")
+            _chk(self.L.bam_kv_reorder(self.h, what, self._queue()), "bam_kv_reorder")
         return new_lens, new_table, new_spare
 
     def close(self):
