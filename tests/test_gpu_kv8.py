@@ -348,3 +348,22 @@ def test_refusals(bam):
         kv = bam.KVCache(a, 1, 128, n_blocks=16, stored=torch.bfloat16)
         assert kv.scales is None and kv.block_tokens == 16
         kv.close()
+
+
+@pytest.mark.parametrize("dtype,dim,page", [("bf16", 144, 4096), ("f16", 176, 8192), ("bf16", 192, 16384), ("f16", 240, 4096), ("bf16", 112, 4096), ("f16", 48, 1024), ("bf16", 256, 4096), ("f16", 80, 4096), ("bf16", 96, 8192), ("f16", 64, 1024)])
+@pytest.mark.parametrize("group,news", [(1, [1, 1, 1]), (5, [4, 1, 3]), (2, [25, 3, 17]), (3, [30, 41, 2])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (37, 5)])
+def test_other_head_sizes(bam, dtype, dim, page, group, news, window, sinks):
+    """one row and few, tiles of two waves (33 to 64 rows of a head of keys) and of four, blocks of 16 tokens and more"""
+    import torch
+    lens, heads = [200, 133, 90], 2
+    gen = torch.Generator().manual_seed(dim)
+    with Cache8(bam, 100, heads, dim, dtype, page) as c:
+        table = _table(lens, c.t, 100)
+        c.fill(lens, table)
+        q = torch.randn(sum(news), heads * group, dim, generator=gen).to(c.dtype)
+        want, tol, lse = c.want(q, lens, news, table, window, sinks)
+        got, got_lse = c.kv.attend(q.cuda(), _i32(lens), table.cuda(), starts=_starts(news), max_new=max(news), window=window, sinks=sinks, return_lse=True)
+        _near(got, want, tol)
+        _near(got_lse, lse, 2.0 ** -16 * (1 + lse.abs()))
+        assert not c.rig.c.aborted()
