@@ -52,6 +52,7 @@ struct kv_rows {
     const float *cos, *sin;
     uint32_t positions, q_heads, rot, pairs, aligned;      /* aligned: q, k, v in whole pieces of 16 bytes */
     float eps;
+    double of_dim;                      /* 1 / dim */
     uint32_t window, piece;             /* rows that a wave looks for beginnings of runs among, and the most rows it takes at a time */
     uint32_t q_heads_each, q_waves;     /* heads of queries that a wave takes; waves that do */
     uint32_t kv_blocks, among;          /* workgroups for keys and values, which are spread among so many from the first on */
@@ -335,6 +336,69 @@ __device__ __forceinline__ u32x4 norm_and_rotate(const kv_rows& io, const kv_geo
     for (int i = 0; i < 4; i++) x[i] = to16<F16>(f[2 * i], f[2 * i + 1]);
     return x;
 }
+/* to 32 bits so that what is rounded to fewer next comes out as if from the 64: towards zero, and the last bit set where something was cut off */
+__device__ __forceinline__ float to_odd(const double x)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)b;
+    return (float)__builtin_bit_cast(double, (b & ~0xffffffffull) | (((lo & 0x1fffffffu) + 0x1fffffffu | lo) & 0xe0000000u));
+}
+/*
+ * The same for what goes into 8 bits, with the sums and the turned numbers in 64 bits: a step of 8 bits is a sixteenth of a number, and one that lies within the error of the arithmetic of a border between
+ * two of them comes out a whole step off (of 20 million, 32 in 32 bits, 11 with 64 that were rounded to 32 on the way, none like this; 6 us of 124).  What is multiplied in 32 bits is exact: 16-bit
+ * numbers and weights, the numbers scaled by a power of two near one over their mean size.
+ */
+template <int LPR, int F16>
+__device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const u32x4 x, float (&f)[8], const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
+{
+    in_32_bits<F16>(x, f);
+    if (!norm && !io.rot) return;
+    double by = 1;
+    if (norm) {
+        double ss = 0;                           /* (pieces past the row's end are zero) */
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss = __builtin_fma((double)f[i], (double)f[i], ss);
+#pragma unroll
+        for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
+        const double v = ss * io.of_dim + (double)io.eps;
+        /* v = u 4^e with u from one to four, and so not at the ends of a float's range; 1 / sqrt(u) in 32 bits, and a step of Newton's (zero, infinity and NaN without) */
+        const int e = v > 0 && v < __builtin_inf() ? (int)(((__builtin_bit_cast(uint64_t, v) >> 52) + 1u) >> 1) - 512 : 0;
+        const double u = ldexp(v, -2 * e), first = (double)rsqrtf((float)u);
+        by = u > 0 && u < __builtin_inf() ? __builtin_fma(0.5 * first, __builtin_fma(-u * first, first, 1.0), first) : first;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t y = w[i];
+            f[2 * i] = ldexpf(f[2 * i], -e) * from16<F16>(y & 0xffffu);
+            f[2 * i + 1] = ldexpf(f[2 * i + 1], -e) * from16<F16>(y >> 16);
+        }
+    }
+    const uint32_t pieces = io.rot / 8, hp = pieces / 2;
+    const bool turns = piece < pieces;
+    if (io.rot && io.pairs) {
+        if (turns) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const double a = f[2 * i], b = f[2 * i + 1], c = t.c[0][i], sn = t.s[0][i];
+                f[2 * i] = to_odd(by * (a * c - b * sn));
+                f[2 * i + 1] = to_odd(by * (b * c + a * sn));
+            }
+            return;
+        }
+    } else if (io.rot) {
+        const uint32_t from = (bam::lane() & ~(uint32_t)(LPR - 1)) + (turns ? (piece < hp ? piece + hp : piece - hp) : piece);
+        const float sign = piece < hp ? -1.0f : 1.0f;
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = __shfl(f[i], (int)from);
+        if (turns) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = to_odd(by * ((double)f[i] * (double)t.c[i / 4][i % 4] + (double)(sign * o[i]) * (double)t.s[i / 4][i % 4]));
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = to_odd(by * (double)f[i]);
+}
 /* the power of two of a row whose numbers LPR lanes have */
 template <int LPR, int F16> __device__ __forceinline__ uint32_t power_of_row(const float (&f)[8])
 {
@@ -351,7 +415,7 @@ template <int LPR, int F16> __device__ __forceinline__ uint32_t power_of_row(con
  * a sequence in one block, gone through in pieces of up to io.piece tokens (eight or sixteen that begin at a multiple of that).  A page's rows all belong to one
  * wave: a page that holds new rows only is not read, and one that a second wave found gone again would come without the rows of the first.
  *   Bound by memory where there are many rows: 19 459 rows of 32 heads on 8 of 128 numbers, normed and turned, 480 MB in 118 us (4.1 TB/s), 160 MB out again in 55, in 8 bits
- * 440 MB in 123 and 120 MB in 43; a wave for each four rows took 288 and 112 (each looked its sequence up for 1 KiB).  Few rows: the chain of looks, table, references, rows, 6 to 7 us.
+ * 440 MB in 130 and 120 MB in 42; a wave for each four rows took 288 and 112 (each looked its sequence up for 1 KiB).  Few rows: the chain of looks, table, references, rows, 6 to 7 us.
  */
 template <int LPR, int F16, int E8, bool WRITE, bool ALIGNED>
 __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom g, const kv_seqs s, const kv_rows io)
@@ -473,8 +537,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                         const kv_turn t = turn_of(io, piece, pos + off + (r < cnt ? r : 0u));
                         if constexpr (E8) {
                             float f[8];
-                            in_32_bits<F16>(in_row ? x[e] : u32x4{0, 0, 0, 0}, f);
-                            norm_and_rotate<LPR, F16>(io, g, f, io.k_norm != nullptr, w, t, piece);
+                            norm_and_rotate_for_8<LPR, F16>(io, in_row ? x[e] : u32x4{0, 0, 0, 0}, f, io.k_norm != nullptr, w, t, piece);
                             const uint32_t power = power_of_row<LPR, F16>(f);
                             const float by = inverse_of(power);
                             const uint32_t lo = to8<F16, true>(to8<F16, false>(0, f[0], f[1], by), f[2], f[3], by), hi = to8<F16, true>(to8<F16, false>(0, f[4], f[5], by), f[6], f[7], by);
@@ -607,6 +670,7 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
     io.q_heads_each = io.q && (uint64_t)s.rows * io.q_heads > 16384 ? 8 * rpw : rpw;
     io.q_waves = io.q ? (uint32_t)((io.q_heads + io.q_heads_each - 1) / io.q_heads_each * s.rows) : 0;
     io.piece = kv->g.tokens < 16 ? 8 : 16;
+    io.of_dim = 1.0 / kv->g.dim;
     /*
      * A wave goes through the runs of its window one after the other: no larger than leaves a wave to each place of the device.  Rows of the last blocks of 512 sequences, 1 to 31 tokens each and eight
      * heads, windows of 32 / 16 / 8 / 4 rows: 52 / 51 / 44 / 50 us; 13 rows of four sequences, 32 / 1: 16 / 8.5.
@@ -626,7 +690,7 @@ void launch_rows(const bam_kv_t* kv, const kv_seqs& s, kv_rows io, hipStream_t s
     /*
      * Few rows: keys and values first, whose waves work longest.  Many: their workgroups among the queries', not behind them, where they would be left to finish alone, but what is written last is what
      * the caches have for who reads it next.  19 459 rows of 32 heads on 8 of 128 numbers into the cache and out again, keys and values first / over three quarters of the launch / evenly / last: in 8 bits
-     * 119 + 52 / 123 + 43 / 134 + 40 / 134 + 37 us, in 16 bits 119 + 65 / 117 + 61 / 118 + 55 / 130 + 47; one row in 8 bits 8.4 + 5 / - / 9.1 + 5.
+     * 119 + 52 / 123 + 43 / 134 + 40 / 134 + 37 us, in 16 bits 119 + 65 / 117 + 61 / 118 + 55 / 130 + 47; one row in 8 bits 8.4 + 5 / - / 9.1 + 5 (8 bits with sums in 32, which take 6 us less).
      */
     io.among = io.kv_blocks;
     const uint32_t most = E8 ? grid.x / 4 * 3 : grid.x;

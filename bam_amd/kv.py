@@ -38,7 +38,7 @@ class KVCache:
     that require them are refused where gradients are being recorded.
 
     stored: what the pages hold.  None: numbers of `dtype`.  torch.float8_e4m3fn: half as many bytes, each row (a token's keys of a head, or its values) as eight-bit numbers of
-    four significant bits and a power of two; keys are normed and turned in 32 bits and rounded once, to that.  The powers of two are `scales`, a byte for each row in device memory
+    four significant bits and a power of two; keys are normed and turned in 64 bits and rounded once, to that.  The powers of two are `scales`, a byte for each row in device memory
     (uint8 [n_blocks, n_heads, 2, block_tokens]: keys, values): given, or made here.  A cache that is opened again over pages that hold something needs the scales that go with them.
     """
 

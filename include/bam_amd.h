@@ -447,7 +447,7 @@ int bam_kv_create(bam_kv_t** out, bam_array_t* a, uint64_t first_page, uint64_t 
                   int f16 /* 0: bfloat16, 1: float16 */);
 /*
  * The same with 8 bits to a number in the pages: half the pages, bytes and reads from the store for the same tokens.  What goes in and comes out has the type that f16 names.  A row
- * (a token's keys of a head, or its values), worked out in 32 bits and not rounded before, is kept as e4m3 numbers (finite ones up to 448) and a power of two: k is the least whole number for which
+ * (a token's keys of a head, or its values), its keys normed and turned in 64 bits and not rounded before, is kept as e4m3 numbers (finite ones up to 448) and a power of two: k is the least whole number for which
  * its largest magnitude is at most 448 * 2^k, from -110 to 120 (bfloat16) or -24 to 8 (float16); y is kept as y / 2^k rounded to the nearest, ties to even, and stands for that times 2^k,
  * exactly so in the 16-bit type (in float16, numbers below 2^-14 come out as multiples of 2^-24).  Magnitudes above 1.875 times the type's largest power of two (2^127, 2^15) are kept as that, and what is not finite as NaN, which has no part in k.
  * T is the largest power of two for which T rows of `dim` bytes fit a page, 16 at least.  Of keys, piece c * T + place(t) has numbers 16c .. 16c+15 of token t; of values, piece

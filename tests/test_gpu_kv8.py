@@ -1,9 +1,8 @@
 """The key-value cache in 8 bits: rows in and out, and attention over it, against the definition in 64 bits on the CPU.
 
 What is kept of a row is worked out here in 64 bits without the eight-bit type: k the least whole number for which the row's largest is at most 448 * 2^k, numbers as
-multiples of an eighth of their own power of two (of 2^-9 below 2^-6).  Values go in as they are, so what comes out has to be that, bit for bit.  Keys are normed and turned in 32 bits
-first: a number that lies next to a border of two codes may take the other one, and a largest that lies next to 448 * 2^k the other k, so they are off by half a step (2^-4 of
-the number, or 2^-10 * 2^k) of the larger k, and 2^-18 of the terms that were added up.  Attention goes over what the cache holds, by the bounds of test_gpu_kv.
+multiples of an eighth of their own power of two (of 2^-9 below 2^-6).  Values go in as they are, and keys are normed and turned in 64 bits, so what comes out has to be that, number for number
+(test_keys_are_rounded_once); beside the number itself it is off by half a step (2^-4 of the number, or 2^-10 * 2^k), for which test_rows_in_and_out leaves 2^-17 of the terms that were added up besides.  Attention goes over what the cache holds, by the bounds of test_gpu_kv.
 """
 import numpy as np
 import pytest
@@ -132,6 +131,26 @@ def test_rows_in_and_out(bam, dtype, dim, heads, q_heads, page, rot, style, norm
             _same(old_k, torch.stack([c.k[int(table[b, p // c.t]), :, p % c.t] for b, p in rows]))
             _same(old_v, torch.stack([c.v[int(table[b, p // c.t]), :, p % c.t] for b, p in rows]))
         assert not c.rig.c.aborted()
+
+
+@pytest.mark.parametrize("dtype,dim,page,rot,style,norm", [("bf16", 128, 4096, 128, "half", True), ("bf16", 64, 4096, 32, "pairs", True), ("f16", 256, 4096, 256, "half", True), ("f16", 80, 4096, 64, "half", False),
+                                                           ("bf16", 96, 8192, 0, "half", True), ("f16", 16, 512, 16, "pairs", True)])
+def test_keys_are_rounded_once(bam, dtype, dim, page, rot, style, norm):
+    """what is kept of a key is what the definition in 64 bits rounds to, number for number: of rows of all sizes, and rows that are tiny beside eps.  (Borders of two codes that 64 bits miss by their
+    own error of some 2^-50 are not met.)"""
+    import torch
+    gen = torch.Generator().manual_seed(dim)
+    n, dt, eps = 700, _type(dtype), 2.0 ** -17
+    with Cache8(bam, 2 + n // (1 << ((page // dim).bit_length() - 1)), 1, dim, dtype, page) as c:
+        table = _table([n], c.t, c.n_blocks)
+        k = (torch.randn(n, 1, dim, generator=gen) * torch.exp2(torch.randint(-9, 9, (n, 1, 1), generator=gen).float())).to(dt)
+        w = (1 + 0.2 * torch.randn(dim, generator=gen)).to(dt) if norm else None
+        angle = torch.rand(n, rot // 2, generator=gen) * 6.28
+        cos, sin = (angle.cos(), angle.sin()) if rot else (None, None)
+        c.kv.append(k.cuda(), k.cuda(), _i32([n]), table.cuda(), starts=_starts([n]), k_norm=None if w is None else w.cuda(), eps=eps, cos=cos.cuda() if rot else None, sin=sin.cuda() if rot else None, rotary=style)
+        got, _ = c.kv.read(n, _i32([n]), table.cuda(), starts=_starts([n]))
+        want = torch.stack([_rotated(k[i, 0], w, i, cos, sin, style, eps)[0] for i in range(n)])
+        _same(got[:, 0], _kept(want, dtype))
 
 
 # ---------------------------------------------------------------- attention
