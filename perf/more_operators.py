@@ -308,12 +308,13 @@ def prepare(case, seed):
         assert s["cache"].block_tokens == t
         if old_k.shape[0]:
             s["cache"].append(old_k, old_v, _i32(before), s["table"], starts=_starts(before))
+        # the pages that the call writes to are in the cache too, as for a program that has used these blocks before; what they hold is not what the call puts there
         if case["op"] == "append":
-            # the pages of the new tokens are in the cache too, as for a program that has used these blocks before
-            s["cache"].append(s["k"], s["v"], s["lens"], s["table"], starts=s["starts"])
+            s["cache"].append(s["v"], s["k"], s["lens"], s["table"], starts=s["starts"])
         if case["op"] == "reorder":
-            # and those of the spare blocks
-            s["cache"].reorder(s["parents"], s["lens"], s["table"], s["spare"])
+            n = s["spare"].numel()
+            rows = old_k[:1].expand(n * t, -1, -1)
+            s["cache"].append(rows, rows, _i32([t] * n), s["spare"][:, None], starts=_starts([t] * n))
         torch.cuda.synchronize()
         return s
     kind = torch.uint8 if eight else dt
