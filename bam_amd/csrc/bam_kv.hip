@@ -220,15 +220,14 @@ __global__ __launch_bounds__(64) void k_kv_reorder(const kv_geom g, const kv_ord
     if (!copy || own >= g.n_blocks) return;
     const uint64_t from = ((uint64_t)block * g.heads + head) * 2u, to = ((uint64_t)own * g.heads + head) * 2u;      /* pages of the cache */
     const bool e8 = g.scales != nullptr;
-    if (e8)
-        for (uint32_t t = lane; t < rest; t += 64u) {
-            const uint8_t k = g.scales[from * g.tokens + t], v = g.scales[(from + 1u) * g.tokens + t];
-            g.scales[to * g.tokens + t] = k;
-            g.scales[(to + 1u) * g.tokens + t] = v;
-        }
     /* pieces of a page, of eight tokens' values; those of `rest` tokens */
     const uint32_t pieces = g.tokens * g.dim / (e8 ? 16u : 8u), eight = e8 ? g.dim / 2u : g.dim, v_pieces = (rest + 7u) / 8u * eight;
     const u32x4 lost = e8 ? u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu} : F16 ? u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u} : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    /* the powers of two of the rows, while their page is held: of one that could not be had (`not_had`, as visit has it), neither the numbers nor their powers change, then or later */
+    uint32_t not_had = 0;
+    auto powers = [&](const uint32_t part) {
+        for (uint32_t t = lane; t < rest; t += 64u) g.scales[(to + part) * g.tokens + t] = g.scales[(from + part) * g.tokens + t];
+    };
     for (uint32_t x0 = 0; x0 < pieces; x0 += ORDER_PIECES) {
         auto wanted = [&](const uint32_t part, const uint32_t x) { return part ? x < v_pieces : x < pieces && place_in(g, x & (g.tokens - 1u)) < rest; };
         auto load = [&](const uint32_t part, const uint8_t* const page) {
@@ -257,9 +256,13 @@ __global__ __launch_bounds__(64) void k_kv_reorder(const kv_geom g, const kv_ord
                 if (none & 2u) room[ORDER_PIECES + x] = lost;
             }
         /* (behind the first part, the page holds what this call has put there) */
-        visit<true>(g, g.first_page + to, x0 == 0, true, [&](uint8_t* keys, uint8_t* values) {
-            if (keys) store(0, keys);
-            if (values) store(1, values);
+        not_had |= visit<true>(g, g.first_page + to, x0 == 0, true, [&](uint8_t* keys, uint8_t* values) {
+            if (e8 && x0 == 0) {
+                if (keys) powers(0);
+                if (values) powers(1);
+            }
+            if (keys && !(not_had & 1u)) store(0, keys);
+            if (values && !(not_had & 2u)) store(1, values);
         });
     }
 }

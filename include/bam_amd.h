@@ -514,8 +514,9 @@ int bam_kv_attend(bam_kv_t* kv, const bam_kv_attend_t* what, void* stream);
  * of d_table_out ([n_new][table_width], next to each other) its row of blocks, -1 from the first block on that has no token.  Blocks that are full are shared.  A last block that is not goes to the first of the
  * parent's children; each other one gets a copy of its tokens in block d_spare[i] (a block of nobody else's; -1, or one that the cache does not have: the child's last tokens are not
  * there), and d_spare_out[i] is then, in the order of the children, the next of the last blocks, not full ones, of old sequences that nobody continues, -1 where there are no more;
- * otherwise d_spare[i].  A parent that is not there gives a sequence of no tokens.  A last block that is not full belongs to one old sequence.  Copies whose pages
- * could not be had read as NaN.  The outputs overlap none of the inputs.  d_work: 4 * (n_old + n_new) bytes for the length of the call.
+ * otherwise d_spare[i].  A parent that is not there gives a sequence of no tokens.  A last block that is not full belongs to one old sequence.  Where the wait for a page is
+ * given up, a copy of a page that could not be had reads as NaN, and what should have gone to a page that could not be had is dropped: the spare block then holds there what it held.  The outputs
+ * overlap none of the inputs.  d_work: 4 * (n_old + n_new) bytes for the length of the call.
  */
 typedef struct bam_kv_reorder {
     uint64_t n_old, n_new;
