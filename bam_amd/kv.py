@@ -73,7 +73,7 @@ class KVCache:
             _chk(self.L.bam_kv_create_e4m3(*what, scales.data_ptr(), scales.numel()), "bam_kv_create_e4m3")
         else:
             _chk(self.L.bam_kv_create(*what), "bam_kv_create")
-        self.scales = scales
+        self.scales, self._scales_on = scales, set()
         out = (c_u64 * 4)()
         _chk(self.L.bam_kv_info(self.h, out), "bam_kv_info")
         self.block_tokens, self.n_blocks, self.pages_per_block, self.page_size = list(out)
@@ -85,7 +85,12 @@ class KVCache:
         """the current stream: kernels go to the device that is current, which has to be the one that the cache's memory is on"""
         if _current() != self._index:
             raise BamError(f"KVCache: the current device must be {self.device}: call under torch.cuda.device")
-        return _stream()
+        stream = _stream()
+        if self.scales is not None and stream.value not in self._scales_on:
+            # a handle may go while its calls are queued: once told, torch's allocator gives the memory to nobody else before what this stream has by then is done
+            self.scales.record_stream(torch.cuda.current_stream(self.device))
+            self._scales_on.add(stream.value)
+        return stream
 
     def _no_grad(self, t, what):
         if t.requires_grad and torch.is_grad_enabled():
