@@ -345,26 +345,35 @@ __device__ __forceinline__ float to_odd(const double x)
 }
 /*
  * The same for what goes into 8 bits, with the sums and the turned numbers in 64 bits: a step of 8 bits is a sixteenth of a number, and one that lies within the error of the arithmetic of a border between
- * two of them comes out a whole step off (of 20 million, 32 in 32 bits, 11 with 64 that were rounded to 32 on the way, none like this; 6 us of 124).  What is multiplied in 32 bits is exact: 16-bit
+ * two of them comes out a whole step off (of 20 million, 32 in 32 bits, 11 with 64 that were rounded to 32 on the way, none like this; 9 us of 127).  On the borders themselves are rows of one
+ * magnitude, which the norm makes plus or minus the weights: with a factor that is 2^-45 off, always downwards, a third of them went to the wrong side.  What is multiplied in 32 bits is exact: 16-bit
  * numbers and weights, the numbers scaled by a power of two near one over their mean size.
  */
 template <int LPR, int F16>
-__device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const u32x4 x, float (&f)[8], const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
+__device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const uint32_t dim, const u32x4 x, float (&f)[8], const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
 {
     in_32_bits<F16>(x, f);
     if (!norm && !io.rot) return;
-    double by = 1;
+    double by = 1, more = 0;
+    auto normed = [&](const double y) { return to_odd(__builtin_fma(by, y, more * y)); };      /* (by + more) y, rounded to 64 bits once */
     if (norm) {
         double ss = 0;                           /* (pieces past the row's end are zero) */
 #pragma unroll
         for (int i = 0; i < 8; i++) ss = __builtin_fma((double)f[i], (double)f[i], ss);
 #pragma unroll
         for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
-        const double v = ss * io.of_dim + (double)io.eps;
-        /* v = u 4^e with u from one to four, and so not at the ends of a float's range; 1 / sqrt(u) in 32 bits, and a step of Newton's (zero, infinity and NaN without) */
+        /* (the quotient by the head's dimension, whose reciprocal is rounded where it is no power of two) */
+        const double mean = ss * io.of_dim, rest = __builtin_fma(-mean, (double)dim, ss), v = (rest - rest == 0 ? __builtin_fma(rest, io.of_dim, mean) : mean) + (double)io.eps;
+        /* v = u 4^e with u from one to four, and so not at the ends of a float's range; 1 / sqrt(u) in 32 bits, a step of Newton's, 2^-45 off, and what a second one adds, kept beside it (zero, infinity and NaN
+         * without) */
         const int e = v > 0 && v < __builtin_inf() ? (int)(((__builtin_bit_cast(uint64_t, v) >> 52) + 1u) >> 1) - 512 : 0;
         const double u = ldexp(v, -2 * e), first = (double)rsqrtf((float)u);
-        by = u > 0 && u < __builtin_inf() ? __builtin_fma(0.5 * first, __builtin_fma(-u * first, first, 1.0), first) : first;
+        by = first;
+        if (u > 0 && u < __builtin_inf()) {
+            by = __builtin_fma(0.5 * first, __builtin_fma(-u * first, first, 1.0), first);
+            const double h = u * by, cut = __builtin_fma(u, by, -h);
+            more = 0.5 * by * (__builtin_fma(-h, by, 1.0) - cut * by);
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t y = w[i];
@@ -379,8 +388,8 @@ __device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const u
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const double a = f[2 * i], b = f[2 * i + 1], c = t.c[0][i], sn = t.s[0][i];
-                f[2 * i] = to_odd(by * (a * c - b * sn));
-                f[2 * i + 1] = to_odd(by * (b * c + a * sn));
+                f[2 * i] = normed(a * c - b * sn);
+                f[2 * i + 1] = normed(b * c + a * sn);
             }
             return;
         }
@@ -392,12 +401,12 @@ __device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const u
         for (int i = 0; i < 8; i++) o[i] = __shfl(f[i], (int)from);
         if (turns) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] = to_odd(by * ((double)f[i] * (double)t.c[i / 4][i % 4] + (double)(sign * o[i]) * (double)t.s[i / 4][i % 4]));
+            for (int i = 0; i < 8; i++) f[i] = normed((double)f[i] * (double)t.c[i / 4][i % 4] + (double)(sign * o[i]) * (double)t.s[i / 4][i % 4]);
             return;
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = to_odd(by * (double)f[i]);
+    for (int i = 0; i < 8; i++) f[i] = normed((double)f[i]);
 }
 /* the power of two of a row whose numbers LPR lanes have */
 template <int LPR, int F16> __device__ __forceinline__ uint32_t power_of_row(const float (&f)[8])
@@ -537,7 +546,7 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                         const kv_turn t = turn_of(io, piece, pos + off + (r < cnt ? r : 0u));
                         if constexpr (E8) {
                             float f[8];
-                            norm_and_rotate_for_8<LPR, F16>(io, in_row ? x[e] : u32x4{0, 0, 0, 0}, f, io.k_norm != nullptr, w, t, piece);
+                            norm_and_rotate_for_8<LPR, F16>(io, g.dim, in_row ? x[e] : u32x4{0, 0, 0, 0}, f, io.k_norm != nullptr, w, t, piece);
                             const uint32_t power = power_of_row<LPR, F16>(f);
                             const float by = inverse_of(power);
                             const uint32_t lo = to8<F16, true>(to8<F16, false>(0, f[0], f[1], by), f[2], f[3], by), hi = to8<F16, true>(to8<F16, false>(0, f[4], f[5], by), f[6], f[7], by);
