@@ -14,6 +14,9 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 /* the most that are wanted, and beams; places for candidates of a workgroup */
 constexpr uint32_t BEAM_WIDTH = 256, BEAM_BEAMS = 1024, BEAM_ROOM = 2048;
 constexpr uint32_t BEAM_THREADS = 256, BEAM_NOTED = 256;      /* BEAM_NOTED: loads that are kept in LDS */
+/* the most candidates of a request: a piece to a beam, or several (plan_of) */
+constexpr uint32_t BEAM_CANDIDATES = BEAM_BEAMS * BEAM_WIDTH, BEAM_CANDIDATES_OF_PIECES = 8192;
+static_assert(BEAM_CANDIDATES < 1u << 22 && BEAM_CANDIDATES_OF_PIECES <= BEAM_CANDIDATES, "k_beam_join divides their numbers in 32-bit floating point");
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct beam_args {
@@ -382,8 +385,8 @@ __global__ __launch_bounds__(THREADS) void k_beam_join(const beam_args a)
         if (lane == 0) { offset[i] = by; largest[i] = most; }
     }
     __syncthreads();
-    /* candidate c; (numbers below 2^22 are divided exactly this way) */
-    auto beam_of = [&](const uint32_t c) { return all < 1u << 22 ? (uint32_t)(((float)c + 0.5f) * of_each) : c / each; };
+    /* candidate c; (numbers below 2^22 are divided exactly this way, and there are no more than BEAM_CANDIDATES) */
+    auto beam_of = [&](const uint32_t c) { return (uint32_t)(((float)c + 0.5f) * of_each); };
     auto place_of = [&](const uint32_t c, const uint64_t k) {
         const uint32_t i = beam_of(c), j = c - i * each;
         const double by = offset[i];
@@ -400,7 +403,7 @@ __global__ __launch_bounds__(THREADS) void k_beam_join(const beam_args a)
     };
     const bool few = all <= HELD * THREADS;
     auto note = [&](const uint32_t c, const beam_place& p) {
-        const uint32_t l = all < 1u << 22 ? (uint32_t)(((float)c + 0.5f) * of_width) : c / a.width;
+        const uint32_t l = (uint32_t)(((float)c + 0.5f) * of_width);
         if (p.sum) atomicMax(&halves[((c - l * a.width) * (pieces | 1u) + l) & (groups - 1u)], high(p.sum));
     };
     if (few) {
@@ -505,7 +508,8 @@ beam_plan plan_of(const uint64_t requests, const uint64_t beams, const uint64_t 
     const uint64_t rows = requests * beams, load = BEAM_THREADS * (type == 2 ? 4 : 8);
     uint64_t splits = (1024 + rows - 1) / rows;
     if (splits < (vocab + 32 * load - 1) / (32 * load)) splits = (vocab + 32 * load - 1) / (32 * load);
-    if (splits > 8192 / (beams * width)) splits = 8192 / (beams * width) ? 8192 / (beams * width) : 1;
+    const uint64_t most = BEAM_CANDIDATES_OF_PIECES / (beams * width);
+    if (splits > most) splits = most ? most : 1;
     if (splits > (vocab + load - 1) / load) splits = (vocab + load - 1) / load;
     p.per = (uint32_t)(((vocab + splits - 1) / splits + 15) / 16 * 16);
     p.splits = (uint32_t)((vocab + p.per - 1) / p.per);
@@ -549,7 +553,7 @@ int bam_beam_select(const bam_beam_select_t* what, void* stream)
     const beam_plan p = plan_of(w.n_requests, w.n_beams, w.vocab, w.width, w.type);
     if (w.work_bytes < p.bytes) return fail(EINVAL, "bam_beam_select: the workspace is smaller than bam_beam_select_bytes says");
     const uint64_t rows = w.n_requests * w.n_beams, all = w.n_beams * p.splits * w.width;
-    if (rows * p.splits > 0x7fffffffull || all > 0x7fffffffull) return fail(EINVAL, "bam_beam_select: more workgroups or candidates than 31 bits count");
+    if (rows * p.splits > 0x7fffffffull) return fail(EINVAL, "bam_beam_select: more workgroups than 31 bits count");
     beam_args a{};
     a.logits = w.d_logits; a.row = w.logits_row; a.scores = w.d_scores; a.score_row = w.scores_row;
     a.requests = (uint32_t)w.n_requests; a.beams = (uint32_t)w.n_beams; a.vocab = (uint32_t)w.vocab; a.width = w.width; a.splits = p.splits; a.per = p.per;
