@@ -19,7 +19,8 @@ def beam_select(logits, scores, width=None):
     """The best continuations of each request's beams: (sums, beams, tokens), [requests, width] each, in float32, int32 and int32, the largest sum first.
 
     logits: [requests * beams, vocab] in bfloat16, float16 or float32, a request's beams one after the other; scores: [requests, beams] in float32, the sum of log-probabilities of each
-    beam so far.  sum = score + logit - log(sum(exp(logits of the beam))); `beams` are rows of logits.  Equal sums: the lower beam first, then the lower token.  width: beams unless given,
+    beam so far.  sum = score + logit - log(sum(exp(logits of the beam))); `beams` are rows of logits.  Equal sums: the lower beam first, then the lower token.  Tokens of a beam are
+    in the order of sums in 64 bits, those of different beams where their sums differ by more than 2^-18 (exponentials are taken in 32 bits).  width: beams unless given,
     256 at most.  A beam whose score is minus infinity has no finite continuation; one with NaN or infinity among its logits, or nothing above minus infinity, has NaN, which comes last.
     There are no gradients: tensors that require them are refused where gradients are being recorded.  Queued on the current stream of the tensors' device."""
     shape, beams = logits.shape, scores.shape

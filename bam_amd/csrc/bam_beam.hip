@@ -342,8 +342,9 @@ __device__ __forceinline__ double log_of(const double x)
 }
 
 /*
- * A request: the beams' logarithms of sums of exponentials, and the best of what the pieces left, by a bound as in k_beam_rows.  Sums are compared in 64 bits:
- * the beams' own sums are rounded to 32, what is added to them is not, and of two beams that differ in their last place the right one is taken.
+ * A request: the beams' logarithms of sums of exponentials, and the best of what the pieces left, by a bound as in k_beam_rows.  Sums are compared in 64 bits and not rounded to 32 before.  They are
+ * as near as the exponentials under them, which k_beam_rows takes, and adds up by the chunk, in 32: within 2^-19.  Beams whose sums differ by more than twice that come in the right order; a beam's own
+ * tokens, which have that error in common, where 64 bits tell them apart; and beams of the same differences and scores have the same sums.
  *   Up to eight candidates to a thread are in registers before the sums are known, and the first bound is of the upper halves of the sums, with candidate q of piece l in group q * (pieces | 1) + l: pieces'
  * candidates come in order, so neighbouring ones in one group would leave most groups without a good one (16 beams, 2048 candidates, 32 wanted: 55 us for 14).
  *   Latencies: 4.4 to 5 us for up to 1024 candidates, of which an empty kernel behind another takes 4; 6.9 for 2560 of 48 requests.

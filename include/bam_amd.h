@@ -534,7 +534,8 @@ int bam_kv_reorder(bam_kv_t* kv, const bam_kv_reorder_t* what, void* stream);
  * n_requests of n_beams beams each (up to 1024), with a row of `vocab` logits to a beam, logits_row numbers from row to row (request r's beam i is row r * n_beams + i; type: 0 bfloat16,
  * 1 float16, 2 float32), and d_scores[r * scores_row + i] the sum of log-probabilities of what beam i has so far.  Out of all continuations of a request's beams by a token, whose sums are
  * score[i] + logit[i][v] - log(sum over u of exp(logit[i][u])), the `width` (up to 256) with the largest: d_sums, d_beams (the row, r * n_beams + i) and d_tokens, [n_requests][width] each, the largest
- * first, equal ones in the order of i * vocab + v.  Logarithms and sums are taken in 64 bits, exponentials in 32.  A token whose logit is minus infinity has minus infinity.  All tokens of a beam whose score is not finite have that score, and
+ * first, equal ones in the order of i * vocab + v.  Exponentials are taken, and up to 64 of them added up, in 32 bits, the rest and logarithms in 64: before it is rounded, a beam's offset is within 2^-19, so beams
+ * whose sums lie closer than twice that may come in another order (a beam's own tokens have that in common, and come in the order of sums in 64 bits).  A token whose logit is minus infinity has minus infinity.  All tokens of a beam whose score is not finite have that score, and
  * those of a beam whose logits have no logarithm of a sum (NaN or infinity among them, none above minus infinity) have NaN, which comes last.
  * d_work: bam_beam_select_bytes(...) bytes for the length of the call.  Queued on `stream`; it may be captured into a graph. */
 typedef struct bam_beam_select {
