@@ -8,7 +8,7 @@ import struct
 import torch
 
 from . import _lib
-from .host import BamError, _chk, _raw_stream, c_u64, c_vp
+from .host import BamError, _chk, _current, _stream, c_u64
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SELECT = struct.Struct("@QQQPqPqPPPPQIi")          # bam_beam_select_t
@@ -48,7 +48,7 @@ def beam_select(logits, scores, width=None):
         if len(_bytes) > 4096:
             _bytes.clear()
         need = _bytes[key] = b.value
-    if torch._C._cuda_getDevice() != index:
+    if _current() != index:
         with torch.cuda.device(index):
             return _select(L, logits, scores, row, score_row, beams, width, kind, need)
     return _select(L, logits, scores, row, score_row, beams, width, kind, need)
@@ -61,6 +61,6 @@ def _select(L, logits, scores, row, score_row, beams, width, kind, need):
     if beams[0]:
         at, each = out.data_ptr(), 4 * beams[0] * width
         what = _SELECT.pack(beams[0], beams[1], logits.shape[1], logits.data_ptr(), row, scores.data_ptr(), score_row, at, at + each, at + 2 * each, work.data_ptr(), need, width, kind)
-        _chk(L.bam_beam_select(what, c_vp(_raw_stream(device.index))), "bam_beam_select")
+        _chk(L.bam_beam_select(what, _stream()), "bam_beam_select")
     sums, chosen, tokens = out.unbind(0)
     return sums.view(torch.float32), chosen, tokens

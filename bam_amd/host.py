@@ -16,6 +16,7 @@ import torch
 from . import _lib
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) if hasattr(torch._C, "_cuda_getDevice") else None
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 c_u64, c_u32, c_vp = ctypes.c_uint64, ctypes.c_uint32, ctypes.c_void_p
 MASK64 = (1 << 64) - 1

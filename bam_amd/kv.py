@@ -9,10 +9,9 @@ import struct
 import torch
 
 from . import _lib
-from .host import Array, BamError, PageCache, Range, _chk, _stream, c_u64, c_vp
+from .host import Array, BamError, PageCache, Range, _chk, _current, _stream, c_u64, c_vp
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
-_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 # the structs of include/bam_amd.h, packed at once: a call takes 3 us less than with a ctypes argument for each field
 _SEQS = "QQPPPqQ"
