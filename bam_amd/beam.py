@@ -6,9 +6,10 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .host import BamError, _chk, _current, _stream, c_u64
+from .host import BamError, _chk, _current, _stream, _wants_gradients, c_u64
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SELECT = struct.Struct("@QQQPqPqPPPPQIi")          # bam_beam_select_t
@@ -22,7 +23,7 @@ def beam_select(logits, scores, width=None):
     beam so far.  sum = score + logit - log(sum(exp(logits of the beam))); `beams` are rows of logits.  Equal sums: the lower beam first, then the lower token.  Tokens of a beam are
     in the order of sums in 64 bits, those of different beams where their sums differ by more than 2^-18 (exponentials are taken in 32 bits).  width: beams unless given,
     256 at most.  A beam whose score is minus infinity has no finite continuation; one with NaN or infinity among its logits, or nothing above minus infinity, has NaN, which comes last.
-    There are no gradients: tensors that require them are refused where gradients are being recorded.  Queued on the current stream of the tensors' device."""
+    There are no gradients: tensors that require them are refused where gradients are being recorded, and those with a tangent (forward_ad).  Queued on the current stream of the tensors' device."""
     shape, beams = logits.shape, scores.shape
     kind, index = _TYPES.get(logits.dtype), logits.get_device()
     if kind is None or len(shape) != 2 or index < 0:
@@ -33,8 +34,8 @@ def beam_select(logits, scores, width=None):
     score_row, next_score = scores.stride()
     if (one != 1 and shape[1] > 1) or (next_score != 1 and beams[1] > 1):
         raise BamError("beam_select: the numbers of a row must be next to each other")
-    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
-        raise BamError("beam_select: there are no gradients: detach what requires them, or call under torch.no_grad()")
+    if (logits.requires_grad or scores.requires_grad or forward_ad._current_level >= 0) and (_wants_gradients(logits) or _wants_gradients(scores)):
+        raise BamError("beam_select: there are no gradients: detach what requires them or has a tangent, or call under torch.no_grad()")
     if width is None:
         width = beams[1]
     if type(width) is not int or not 1 <= width <= 256:

@@ -12,6 +12,7 @@ import errno
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -50,6 +51,11 @@ def _stream():
     if _raw_stream is not None and torch.cuda.is_initialized():
         return c_vp(_raw_stream(torch._C._cuda_getDevice()))
     return c_vp(torch.cuda.current_stream().cuda_stream)
+
+
+def _wants_gradients(t):
+    """whether torch would carry gradients through what is done with the tensor: backwards, or forwards (a tangent, within forward_ad.dual_level)"""
+    return (t.requires_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None)
 
 
 class Target:

@@ -7,9 +7,10 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .host import Array, BamError, PageCache, Range, _chk, _current, _stream, c_u64, c_vp
+from .host import Array, BamError, PageCache, Range, _chk, _current, _stream, _wants_gradients, c_u64, c_vp
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -34,7 +35,7 @@ class KVCache:
     The calls below share how sequences are given, all on the device in int32: `lens[b]` counts the tokens of sequence b, the new ones among them;
     `table[b, i]` is the block of its tokens i * block_tokens and on; rows starts[b] .. starts[b+1]-1 of the packed inputs are its newest tokens
     (starts None: one new token each).  They are queued on the current stream.  A block number outside the cache is not read or written.  There are no gradients: tensors
-    that require them are refused where gradients are being recorded.
+    that require them are refused where gradients are being recorded, and those with a tangent (forward_ad).  The cache's device has to be the current one.
 
     stored: what the pages hold.  None: numbers of `dtype`.  torch.float8_e4m3fn: half as many bytes, each row (a token's keys of a head, or its values) as eight-bit numbers of
     four significant bits and a power of two; keys are normed and turned in 64 bits and rounded once, to that.  The powers of two are `scales`, a byte for each row in device memory
@@ -92,8 +93,8 @@ class KVCache:
         return stream
 
     def _no_grad(self, t, what):
-        if t.requires_grad and torch.is_grad_enabled():
-            raise BamError(f"KVCache: {what} requires gradients and there are none: detach it, or call under torch.no_grad()")
+        if (t.requires_grad or forward_ad._current_level >= 0) and _wants_gradients(t):
+            raise BamError(f"KVCache: {what} requires gradients or has a tangent, and there are none: detach it, or call under torch.no_grad()")
 
     def _rows(self, t, what, heads=None):
         """(rows, heads, row stride, head stride) of a tensor of rows"""
