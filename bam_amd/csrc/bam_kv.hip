@@ -146,7 +146,7 @@ __device__ __forceinline__ bool last_block(const kv_geom& g, const kv_order& o, 
  * Workgroup 0, one wave: the spare blocks that are left.  The others, a wave each: head h of child i, whose last block is copied where an earlier child has the parent's; head 0 writes
  * the child's length and row of blocks besides.  Whether there is an earlier child each wave finds by itself, in the parents in front of its own: one launch, nobody waits for anybody.
  *   A page is copied by way of LDS, 8 KiB at a time, by one wave: nothing is held while the other page is waited for, and the new page needs no read (kv_cache.h, visit).  Only
- * pieces that have tokens move.  4 beams 6.7 us, the launch and a chain of looks, references and stores; 512 sequences of which 256 are copied, eight heads, pages of 8 KiB, 22 us (33 MB).
+ * pieces that have tokens move.  4 beams 7.1 us, the launch and a chain of looks, references and stores; 512 sequences of which 256 are copied, eight heads, pages of 8 KiB, 22 us (33 MB).
  */
 template <int F16>
 __global__ __launch_bounds__(64) void k_kv_reorder(const kv_geom g, const kv_order o)
@@ -225,8 +225,11 @@ __global__ __launch_bounds__(64) void k_kv_reorder(const kv_geom g, const kv_ord
     const u32x4 lost = e8 ? u32x4{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu} : F16 ? u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u} : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
     /* the powers of two of the rows, while their page is held: of one that could not be had (`not_had`, as visit has it), neither the numbers nor their powers change, then or later */
     uint32_t not_had = 0;
+    const bool has = e8 && lane < rest;
+    const uint8_t its[2] = {has ? g.scales[from * g.tokens + lane] : (uint8_t)0, has ? g.scales[(from + 1u) * g.tokens + lane] : (uint8_t)0};      /* (of the first 64 tokens: on their way while the source is looked for) */
     auto powers = [&](const uint32_t part) {
-        for (uint32_t t = lane; t < rest; t += 64u) g.scales[(to + part) * g.tokens + t] = g.scales[(from + part) * g.tokens + t];
+        if (has) g.scales[(to + part) * g.tokens + lane] = its[part];
+        for (uint32_t t = lane + 64u; t < rest; t += 64u) g.scales[(to + part) * g.tokens + t] = g.scales[(from + part) * g.tokens + t];
     };
     for (uint32_t x0 = 0; x0 < pieces; x0 += ORDER_PIECES) {
         auto wanted = [&](const uint32_t part, const uint32_t x) { return part ? x < v_pieces : x < pieces && place_in(g, x & (g.tokens - 1u)) < rest; };

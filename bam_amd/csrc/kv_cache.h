@@ -345,7 +345,7 @@ __device__ __forceinline__ float to_odd(const double x)
 }
 /*
  * The same for what goes into 8 bits, with the sums and the turned numbers in 64 bits: a step of 8 bits is a sixteenth of a number, and one that lies within the error of the arithmetic of a border between
- * two of them comes out a whole step off (of 20 million, 32 in 32 bits, 11 with 64 that were rounded to 32 on the way, none like this; 9 us of 127).  On the borders themselves are rows of one
+ * two of them comes out a whole step off (of 20 million, 32 in 32 bits, 11 with 64 that were rounded to 32 on the way, none like this; 8 us of 126).  On the borders themselves are rows of one
  * magnitude, which the norm makes plus or minus the weights: with a factor that is 2^-45 off, always downwards, a third of them went to the wrong side.  What is multiplied in 32 bits is exact: 16-bit
  * numbers and weights, the numbers scaled by a power of two near one over their mean size.
  */
