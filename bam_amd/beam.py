@@ -9,7 +9,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .host import BamError, _chk, _current, _stream, _wants_gradients, c_u64
+from .host import BamError, _chk, _current, _raw_stream, _stream, _wants_gradients, c_u64, c_vp
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SELECT = struct.Struct("@QQQPqPqPPPPQIi")          # bam_beam_select_t
@@ -62,6 +62,7 @@ def _select(L, logits, scores, row, score_row, beams, width, kind, need):
     if beams[0]:
         at, each = out.data_ptr(), 4 * beams[0] * width
         what = _SELECT.pack(beams[0], beams[1], logits.shape[1], logits.data_ptr(), row, scores.data_ptr(), score_row, at, at + each, at + 2 * each, work.data_ptr(), need, width, kind)
-        _chk(L.bam_beam_select(what, _stream()), "bam_beam_select")
+        # (the device is up, there are tensors on it: _stream asks for that first, 0.2 us)
+        _chk(L.bam_beam_select(what, c_vp(_raw_stream(device.index)) if _raw_stream is not None else _stream()), "bam_beam_select")
     sums, chosen, tokens = out.unbind(0)
     return sums.view(torch.float32), chosen, tokens
