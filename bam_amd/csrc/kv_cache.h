@@ -151,23 +151,24 @@ template <int F16> constexpr int32_t MOST_POWER = F16 ? 8 : 120;
 template <int F16> constexpr float MOST_KEPT = F16 ? 1.875f * 0x1p15f : 1.875f * 0x1p127f;
 /* largest of the numbers of magnitude |x|, those that are not finite left out */
 __device__ __forceinline__ float larger_finite(const float a, const float x) { const float m = fabsf(x); return m < INFINITY ? fmaxf(a, m) : a; }
-/* 127 + k for a largest number of a */
-template <int F16> __device__ __forceinline__ uint32_t power_of(const float a)
-{
-    const uint32_t bits = __builtin_bit_cast(uint32_t, fminf(a, MOST_KEPT<F16>));
-    const int32_t k = (int32_t)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return 127u + (uint32_t)(k < LEAST_POWER<F16> ? LEAST_POWER<F16> : k > MOST_POWER<F16> ? MOST_POWER<F16> : k);
-}
 __device__ __forceinline__ float scale_of(const uint32_t power) { return __builtin_bit_cast(float, power << 23); }
 __device__ __forceinline__ float inverse_of(const uint32_t power) { return __builtin_bit_cast(float, (254u - power) << 23); }
-template <int F16> __device__ __forceinline__ float for8(const float y, const float inverse)
+/* 127 + k for a largest number of a 2^down (numbers that are larger than the type's largest are in 32 bits with a power of two less) */
+template <int F16> __device__ __forceinline__ uint32_t power_of(const float a, const uint32_t down)
 {
-    return fabsf(y) < INFINITY ? fminf(fmaxf(y, -MOST_KEPT<F16>), MOST_KEPT<F16>) * inverse : __builtin_nanf("");
+    const uint32_t bits = __builtin_bit_cast(uint32_t, fminf(a, MOST_KEPT<F16> * inverse_of(127u + down)));
+    const int32_t k = (int32_t)(bits >> 23) + (int32_t)down - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return 127u + (uint32_t)(k < LEAST_POWER<F16> ? LEAST_POWER<F16> : k > MOST_POWER<F16> ? MOST_POWER<F16> : k);
+}
+/* a number, the largest that is kept, and 2^-k, the first two 2^-down of what they are and the last 2^down of it */
+__device__ __forceinline__ float for8(const float y, const float most, const float inverse)
+{
+    return fabsf(y) < INFINITY ? fminf(fmaxf(y, -most), most) * inverse : __builtin_nanf("");
 }
 /* two numbers in the low or the high half of a word */
-template <int F16, bool HIGH> __device__ __forceinline__ uint32_t to8(const uint32_t word, const float a, const float b, const float inverse)
+template <int F16, bool HIGH> __device__ __forceinline__ uint32_t to8(const uint32_t word, const float a, const float b, const float inverse, const float most = MOST_KEPT<F16>)
 {
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(for8<F16>(a, inverse), for8<F16>(b, inverse), (int)word, HIGH);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(for8(a, most, inverse), for8(b, most, inverse), (int)word, HIGH);
 }
 /* two numbers of the low or the high half of a word, times a power of two, in 16 bits */
 template <int F16, bool HIGH> __device__ __forceinline__ uint32_t from8(const uint32_t word, const float scale)
@@ -345,16 +346,19 @@ __device__ __forceinline__ float to_odd(const double x)
 }
 /*
  * The same for what goes into 8 bits, with the sums and the turned numbers in 64 bits: a step of 8 bits is a sixteenth of a number, and one that lies within the error of the arithmetic of a border between
- * two of them comes out a whole step off (of 20 million, 32 in 32 bits, 11 with 64 that were rounded to 32 on the way, none like this; 8 us of 126).  On the borders themselves are rows of one
+ * two of them comes out a whole step off (of 20 million, 32 in 32 bits, 11 with 64 that were rounded to 32 on the way, none like this; 9 us of 127).  On the borders themselves are rows of one
  * magnitude, which the norm makes plus or minus the weights: with a factor that is 2^-45 off, always downwards, a third of them went to the wrong side.  What is multiplied in 32 bits is exact: 16-bit
  * numbers and weights, the numbers scaled by a power of two near one over their mean size.
+ *   What comes out is 2^-5 of the row, which is in range whatever the weights are (a number is at most sqrt(256) of the mean size, sqrt(2) of that turned): a normed key past the type's largest number is kept as
+ * that and not as NaN.  The 5 is returned; 0 where there is nothing to do, and the row is as it was.
  */
 template <int LPR, int F16>
-__device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const uint32_t dim, const u32x4 x, float (&f)[8], const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
+__device__ __forceinline__ uint32_t norm_and_rotate_for_8(const kv_rows& io, const uint32_t dim, const u32x4 x, float (&f)[8], const bool norm, const u32x4 w, const kv_turn& t, const uint32_t piece)
 {
+    constexpr int DOWN = 5;
     in_32_bits<F16>(x, f);
-    if (!norm && !io.rot) return;
-    double by = 1, more = 0;
+    if (!norm && !io.rot) return 0;
+    double by = 1.0 / (1 << DOWN), more = 0;
     auto normed = [&](const double y) { return to_odd(__builtin_fma(by, y, more * y)); };      /* (by + more) y, rounded to 64 bits once */
     if (norm) {
         double ss = 0;                           /* (pieces past the row's end are zero) */
@@ -377,8 +381,8 @@ __device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const u
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const uint32_t y = w[i];
-            f[2 * i] = ldexpf(f[2 * i], -e) * from16<F16>(y & 0xffffu);
-            f[2 * i + 1] = ldexpf(f[2 * i + 1], -e) * from16<F16>(y >> 16);
+            f[2 * i] = ldexpf(f[2 * i], -e - DOWN) * from16<F16>(y & 0xffffu);
+            f[2 * i + 1] = ldexpf(f[2 * i + 1], -e - DOWN) * from16<F16>(y >> 16);
         }
     }
     const uint32_t pieces = io.rot / 8, hp = pieces / 2;
@@ -391,7 +395,7 @@ __device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const u
                 f[2 * i] = normed(a * c - b * sn);
                 f[2 * i + 1] = normed(b * c + a * sn);
             }
-            return;
+            return DOWN;
         }
     } else if (io.rot) {
         const uint32_t from = (bam::lane() & ~(uint32_t)(LPR - 1)) + (turns ? (piece < hp ? piece + hp : piece - hp) : piece);
@@ -402,21 +406,22 @@ __device__ __forceinline__ void norm_and_rotate_for_8(const kv_rows& io, const u
         if (turns) {
 #pragma unroll
             for (int i = 0; i < 8; i++) f[i] = normed((double)f[i] * (double)t.c[i / 4][i % 4] + (double)(sign * o[i]) * (double)t.s[i / 4][i % 4]);
-            return;
+            return DOWN;
         }
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) f[i] = normed((double)f[i]);
+    return DOWN;
 }
 /* the power of two of a row whose numbers LPR lanes have */
-template <int LPR, int F16> __device__ __forceinline__ uint32_t power_of_row(const float (&f)[8])
+template <int LPR, int F16> __device__ __forceinline__ uint32_t power_of_row(const float (&f)[8], const uint32_t down = 0)
 {
     float a = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) a = larger_finite(a, f[i]);
 #pragma unroll
     for (int o = LPR / 2; o; o >>= 1) a = fmaxf(a, __shfl_xor(a, o));
-    return power_of<F16>(a);
+    return power_of<F16>(a, down);
 }
 
 /*
@@ -546,10 +551,10 @@ __global__ __launch_bounds__(256, LPR < 32 ? 4 : 3) void k_kv_rows(const kv_geom
                         const kv_turn t = turn_of(io, piece, pos + off + (r < cnt ? r : 0u));
                         if constexpr (E8) {
                             float f[8];
-                            norm_and_rotate_for_8<LPR, F16>(io, g.dim, in_row ? x[e] : u32x4{0, 0, 0, 0}, f, io.k_norm != nullptr, w, t, piece);
-                            const uint32_t power = power_of_row<LPR, F16>(f);
-                            const float by = inverse_of(power);
-                            const uint32_t lo = to8<F16, true>(to8<F16, false>(0, f[0], f[1], by), f[2], f[3], by), hi = to8<F16, true>(to8<F16, false>(0, f[4], f[5], by), f[6], f[7], by);
+                            const uint32_t down = norm_and_rotate_for_8<LPR, F16>(io, g.dim, in_row ? x[e] : u32x4{0, 0, 0, 0}, f, io.k_norm != nullptr, w, t, piece);
+                            const uint32_t power = power_of_row<LPR, F16>(f, down);
+                            const float by = inverse_of(power - down), most = MOST_KEPT<F16> * inverse_of(127u + down);
+                            const uint32_t lo = to8<F16, true>(to8<F16, false>(0, f[0], f[1], by, most), f[2], f[3], by, most), hi = to8<F16, true>(to8<F16, false>(0, f[4], f[5], by, most), f[6], f[7], by, most);
                             if (r < cnt && in_row) {
                                 __hip_atomic_store((uint64_t*)(at + place_in(g, in_block + r) * 16u), (uint64_t)hi << 32 | lo, __ATOMIC_RELAXED, BAM_SYSTEM);
                                 if (piece == 0) powers[in_block + r] = (uint8_t)power;

@@ -55,3 +55,29 @@ def test_norms_of_what_is_not_finite_and_of_nothing(bam, dtype, dim, eps):
         got, _ = k.kv.read(12, *at, starts=_starts([12]))
         want = torch.stack([_rotated(x[i, 0], w, i, None, None, "half", eps)[0] for i in range(12)])
         _same(got[:, 0], _kept(want, dtype))
+
+
+@pytest.mark.parametrize("dim,page", [(128, 4096), (256, 4096), (80, 4096), (16, 512)])
+@pytest.mark.parametrize("dtype,top", [("bf16", 2.0 ** 127), ("bf16", 2.0 ** -112), ("f16", 2.0 ** 15), ("f16", 2.0 ** -14)])
+@pytest.mark.parametrize("rot", [0, 16])
+def test_weights_at_the_ends_of_the_range(bam, dtype, top, dim, page, rot):
+    """normed keys past the type's largest number are kept as the largest that is, and weights near its ends do not lose or overflow on the way: rows of one magnitude, and with a few large numbers"""
+    import torch
+    gen = torch.Generator().manual_seed(dim)
+    n, dt = 64, _type(dtype)
+    x = torch.randn(n, 1, dim, generator=gen).sign()
+    x[16:32] *= torch.exp2(torch.randint(-3, 4, (16, 1, dim), generator=gen).float())
+    x[32:48] = torch.randn(16, 1, dim, generator=gen)
+    x[48:, :, 1:] = 0                               # sqrt(dim) times the mean size, and nothing
+    x = x.to(dt)
+    w = ((1 + torch.randint(0, 127, (dim,), generator=gen) / 128) * top).to(dt)
+    angle = torch.rand(n, rot // 2, generator=gen) * 6.28
+    with Cache8(bam, 2 + n // 16, 1, dim, dtype, page) as k:
+        table = _table([n], k.t, k.n_blocks).cuda()
+        at = (_i32([n]), table)
+        k.kv.append(x.cuda(), x.cuda(), *at, starts=_starts([n]), k_norm=w.cuda(), eps=0.0, cos=angle.cos().cuda() if rot else None, sin=angle.sin().cuda() if rot else None)
+        got, _ = k.kv.read(n, *at, starts=_starts([n]))
+        cos, sin = (angle.cos(), angle.sin()) if rot else (None, None)
+        want = torch.stack([_rotated(x[i, 0], w, i, cos, sin, "half", 0.0)[0] for i in range(n)])
+        assert bool(torch.isfinite(want).all())
+        _same(got[:, 0], _kept(want, dtype))
